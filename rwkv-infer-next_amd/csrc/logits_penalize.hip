@@ -1,0 +1,151 @@
+// logits_penalize.hip -- penalties, biases and grammar masks on logits (include/logits.h), one pass over the logits.
+//
+// A workgroup owns 2048 columns of one sequence, eight to a thread, for all T positions: the columns' counts are read once and
+// carried from position to position, each draft adding one where it falls.  A bias list belongs to a whole row: every workgroup
+// picks the entries of its columns out of it, 256 at a time, in their order (so equal ids add up in order), and the thread that
+// owns the column adds them.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "logits.h"
+#include "logits_device.h"
+
+namespace lg {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kColumns = kThreads * 8;
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void penalize_kernel(const logits_penalize_args p, uint32_t segments) {
+    __shared__ int64_t found_id[kThreads];
+    __shared__ float found_value[kThreads];
+    __shared__ int wave_found[kThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t b = blockIdx.x / segments, first = (int64_t)(blockIdx.x % segments) * kColumns, v0 = first + 8 * tid;
+    const int n = v0 >= p.V ? 0 : p.V - v0 < 8 ? (int)(p.V - v0) : 8;
+    const bool reports = p.status && first == 0 && tid == 0;  // one thread a sequence
+
+    const float rep = p.repetition ? p.repetition[b] : p.repetition_all;
+    const float pres = p.presence ? p.presence[b] : p.presence_all;
+    const float freq = p.frequency ? p.frequency[b] : p.frequency_all;
+    const bool penalised = rep != 1.f || pres != 0.f || freq != 0.f;
+
+    float c[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = 0.f;
+    if (p.counts) {
+        const int64_t s = p.slots ? p.slots[b] : b;
+        if (s < 0 || s >= p.counts_rows) {
+            if (reports) atomicOr(p.status, LOGITS_STATUS_ROW);
+        } else if (penalised) {
+            load8<LOGITS_F32>(p.counts, s * p.counts_stride + v0, n, 0.f, c);
+            if (p.counts_dtype == LOGITS_COUNTS_I32)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) c[j] = (float)__float_as_int(c[j]);
+        }
+    }
+
+    float bias[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bias[j] = 0.f;
+    for (int i0 = 0; i0 < p.n_bias; i0 += kThreads) {
+        const int i = i0 + tid;
+        const int64_t id = i < p.n_bias ? p.bias_ids[b * p.bias_stride + i] : -1;
+        if (p.status && first == 0 && id >= p.V) atomicOr(p.status, LOGITS_STATUS_TOKEN);
+        const bool mine = id >= first && id < first + kColumns && id < p.V;
+        const uint64_t all = __ballot(mine);
+        if (lane == 0) wave_found[wave] = __popcll(all);
+        __syncthreads();
+        int at = __popcll(all & ((1ull << lane) - 1)), total = 0;
+#pragma unroll
+        for (int w = 0; w < kThreads / 64; ++w) {
+            if (w < wave) at += wave_found[w];
+            total += wave_found[w];
+        }
+        if (mine) {
+            found_id[at] = id - v0 + 8 * tid;  // the column within the workgroup's
+            found_value[at] = p.bias_values[b * p.bias_stride + i];
+        }
+        __syncthreads();
+        for (int e = 0; e < total; ++e) {
+            const int at8 = (int)found_id[e] - 8 * tid;
+            const float add = found_value[e];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (at8 == j) bias[j] += add;
+        }
+        __syncthreads();
+    }
+
+    const char* in = static_cast<const char*>(p.logits) + b * p.in_seq_stride * element_bytes(DT);
+    char* out = static_cast<char*>(p.out) + b * p.out_seq_stride * element_bytes(p.out_dtype);
+    for (int t = 0; t < p.T; ++t) {
+        if (t > 0 && p.drafts) {
+            const int64_t id = p.drafts[b * p.drafts_stride + t - 1];
+            if (reports && id >= p.V) atomicOr(p.status, LOGITS_STATUS_TOKEN);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (id == v0 + j) c[j] += 1.f;
+        }
+        uint32_t allowed = 0xFF;
+        if (p.mask) {
+            const int64_t row = b * p.T + t, m = p.mask_row ? p.mask_row[row] : row;
+            if (m >= p.mask_rows) {
+                if (reports) atomicOr(p.status, LOGITS_STATUS_ROW);
+            } else if (m >= 0 && n > 0) {
+                allowed = reinterpret_cast<const uint8_t*>(p.mask + m * p.mask_stride)[v0 >> 3];
+            }
+        }
+        float x[8];
+        load8<DT>(in + t * p.in_pos_stride * element_bytes(DT), v0, n, 0.f, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (penalised && c[j] > 0.f) x[j] = (x[j] > 0.f ? x[j] / rep : x[j] * rep) - (freq * c[j] + pres);
+            x[j] += bias[j];
+            if (!(allowed >> j & 1)) x[j] = -__builtin_inff();
+        }
+        store8(out + t * p.out_pos_stride * element_bytes(p.out_dtype), p.out_dtype, v0, n, x);
+    }
+}
+
+bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+}  // namespace
+}  // namespace lg
+
+extern "C" {
+
+size_t logits_penalize_args_size(void) { return sizeof(logits_penalize_args); }
+
+int logits_penalize(const logits_penalize_args* a, void* stream) {
+    if (!a) return WKV7_ERR_NULL;
+    if (a->B < 0 || a->T < 0 || a->V < 1 || a->n_bias < 0) return WKV7_ERR_SHAPE;
+    if (a->in_dtype < LOGITS_BF16 || a->in_dtype > LOGITS_F32 || a->out_dtype < LOGITS_BF16 || a->out_dtype > LOGITS_F32 ||
+        (a->counts && a->counts_dtype != LOGITS_COUNTS_I32 && a->counts_dtype != LOGITS_COUNTS_F32))
+        return WKV7_ERR_ARG;
+    if (a->B == 0 || a->T == 0) return WKV7_OK;
+    if (!a->logits || !a->out || (a->n_bias && (!a->bias_ids || !a->bias_values))) return WKV7_ERR_NULL;
+    if (a->counts && (a->counts_rows < 0 || a->counts_stride < a->V)) return WKV7_ERR_SHAPE;
+    if (a->drafts && a->T > 1 && a->B > 1 && a->drafts_stride < a->T - 1) return WKV7_ERR_SHAPE;
+    if (a->n_bias && a->B > 1 && a->bias_stride < a->n_bias) return WKV7_ERR_SHAPE;
+    if (a->mask && (a->mask_rows < 0 || a->mask_stride < ((int64_t)a->V + 31) / 32)) return WKV7_ERR_SHAPE;
+    if (!lg::aligned(a->logits, lg::element_bytes(a->in_dtype)) || !lg::aligned(a->out, lg::element_bytes(a->out_dtype)) ||
+        !lg::aligned(a->counts, 4) || !lg::aligned(a->mask, 4))
+        return WKV7_ERR_ALIGN;
+    const int64_t segments = ((int64_t)a->V + lg::kColumns - 1) / lg::kColumns;
+    if (segments * a->B > 0xFFFFFF) return WKV7_ERR_SHAPE;  // 256 threads each: below 2^32 work-items
+    logits_penalize_args p = *a;
+    if (!p.counts && !p.drafts) p.repetition = p.presence = p.frequency = nullptr, p.repetition_all = 1.f, p.presence_all = p.frequency_all = 0.f;
+    const dim3 grid((unsigned)(segments * a->B)), block(lg::kThreads);
+    const auto s = static_cast<hipStream_t>(stream);
+    if (a->in_dtype == LOGITS_BF16)
+        hipLaunchKernelGGL((lg::penalize_kernel<LOGITS_BF16>), grid, block, 0, s, p, (uint32_t)segments);
+    else if (a->in_dtype == LOGITS_F16)
+        hipLaunchKernelGGL((lg::penalize_kernel<LOGITS_F16>), grid, block, 0, s, p, (uint32_t)segments);
+    else
+        hipLaunchKernelGGL((lg::penalize_kernel<LOGITS_F32>), grid, block, 0, s, p, (uint32_t)segments);
+    return static_cast<int>(hipGetLastError());
+}
+
+}  // extern "C"

@@ -1,4 +1,4 @@
-"""ctypes binding of librwkv7_hip.so (the C ABI declared in include/wkv7.h and include/w6a16.h) and of
+"""ctypes binding of librwkv7_hip.so (the C ABI declared in include/wkv7.h, w6a16.h, w4a16.h and logits.h) and of
 librwkv7_noalloc.so (include/wkv7_noalloc.h, loaded only on request by load_noalloc).
 
 The library must have been built (rwkv_next_amd._build / __graft_entry__.build()).  There is no fallback: if the
@@ -53,6 +53,18 @@ W6A16_OUT_F16 = 1
 W6A16_OUT_F32 = 2
 W6A16_IN_BF16 = 0
 W6A16_IN_F16 = 1
+W4A16_EXPORTED = ("w4a16_args_size", "w4a16_packed_size", "w4a16_pack", "w4a16_dequantize", "w4a16_matmul")
+W4A16_BF16 = 0
+W4A16_F16 = 1
+W4A16_F32 = 2
+LOGITS_EXPORTED = ("logits_penalize_args_size", "logits_sample_args_size", "logits_penalize", "logits_sample")
+LOGITS_BF16 = 0
+LOGITS_F16 = 1
+LOGITS_F32 = 2
+LOGITS_COUNTS_I32 = 0
+LOGITS_COUNTS_F32 = 1
+LOGITS_STATUS_ROW = 256
+LOGITS_STATUS_TOKEN = 512
 MAX_MOVES = 1024
 
 _vp = ctypes.c_void_p
@@ -114,6 +126,48 @@ class W6a16Args(ctypes.Structure):
         ("B", ctypes.c_int32), ("M", ctypes.c_int32), ("N", ctypes.c_int32), ("K", ctypes.c_int32),
         ("group_k", ctypes.c_int32), ("split_k", ctypes.c_int32), ("out_dtype", ctypes.c_int32),
         ("format", ctypes.c_int32), ("a_dtype", ctypes.c_int32),
+    ]
+
+
+class W4a16Args(ctypes.Structure):
+    """Mirror of `w4a16_args` (include/w4a16.h)."""
+    _fields_ = [
+        ("a", _vp), ("a_row_stride", ctypes.c_int64), ("weight", _vp), ("scales", _vp), ("out", _vp),
+        ("out_row_stride", ctypes.c_int64),
+        ("M", ctypes.c_int32), ("N", ctypes.c_int32), ("K", ctypes.c_int32), ("group_k", ctypes.c_int32),
+        ("a_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32),
+    ]
+
+
+class PenalizeArgs(ctypes.Structure):
+    """Mirror of `logits_penalize_args` (include/logits.h)."""
+    _fields_ = [
+        ("logits", _vp), ("in_seq_stride", ctypes.c_int64), ("in_pos_stride", ctypes.c_int64),
+        ("out", _vp), ("out_seq_stride", ctypes.c_int64), ("out_pos_stride", ctypes.c_int64),
+        ("counts", _vp), ("counts_stride", ctypes.c_int64), ("counts_rows", ctypes.c_int64), ("slots", _vp),
+        ("repetition", _vp), ("presence", _vp), ("frequency", _vp),
+        ("drafts", _vp), ("drafts_stride", ctypes.c_int64),
+        ("bias_ids", _vp), ("bias_values", _vp), ("bias_stride", ctypes.c_int64),
+        ("mask", _vp), ("mask_stride", ctypes.c_int64), ("mask_rows", ctypes.c_int64), ("mask_row", _vp),
+        ("status", _vp),
+        ("repetition_all", ctypes.c_float), ("presence_all", ctypes.c_float), ("frequency_all", ctypes.c_float),
+        ("B", ctypes.c_int32), ("T", ctypes.c_int32), ("V", ctypes.c_int32), ("n_bias", ctypes.c_int32),
+        ("in_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32), ("counts_dtype", ctypes.c_int32),
+    ]
+
+
+class SampleArgs(ctypes.Structure):
+    """Mirror of `logits_sample_args` (include/logits.h)."""
+    _fields_ = [
+        ("logits", _vp), ("seq_stride", ctypes.c_int64), ("pos_stride", ctypes.c_int64),
+        ("noise", _vp), ("noise_seq_stride", ctypes.c_int64), ("noise_pos_stride", ctypes.c_int64),
+        ("temperature", _vp), ("top_k", _vp), ("top_p", _vp), ("min_p", _vp),
+        ("token", _vp), ("logprob", _vp),
+        ("counts", _vp), ("counts_stride", ctypes.c_int64), ("counts_rows", ctypes.c_int64), ("slots", _vp),
+        ("status", _vp),
+        ("temperature_all", ctypes.c_float), ("top_p_all", ctypes.c_float), ("min_p_all", ctypes.c_float),
+        ("top_k_all", ctypes.c_int32), ("B", ctypes.c_int32), ("T", ctypes.c_int32), ("V", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("counts_dtype", ctypes.c_int32),
     ]
 
 
@@ -179,6 +233,22 @@ def load(path: str = LIB_PATH):
     lib.w6a16_pack.argtypes = [_vp, _vp, _vp, i32, i32, i32, i32, i64, i64, i64, _vp, _vp, _vp]
     lib.w6a16_dequantize_packed.restype = ctypes.c_int
     lib.w6a16_dequantize_packed.argtypes = [_vp, _vp, _vp, i32, i32, i32, i32, i64, i32, _vp]
+    psz = ctypes.POINTER(ctypes.c_size_t)
+    lib.w4a16_args_size.restype = ctypes.c_size_t
+    lib.w4a16_packed_size.restype = ctypes.c_int
+    lib.w4a16_packed_size.argtypes = [i32, i32, i32, psz, psz]
+    lib.w4a16_pack.restype = ctypes.c_int
+    lib.w4a16_pack.argtypes = [_vp, _vp, i32, i32, i32, _vp, _vp, _vp]
+    lib.w4a16_dequantize.restype = ctypes.c_int
+    lib.w4a16_dequantize.argtypes = [_vp, _vp, _vp, i32, i32, i32, i32, _vp]
+    lib.w4a16_matmul.restype = ctypes.c_int
+    lib.w4a16_matmul.argtypes = [ctypes.POINTER(W4a16Args), _vp]
+    lib.logits_penalize_args_size.restype = ctypes.c_size_t
+    lib.logits_sample_args_size.restype = ctypes.c_size_t
+    lib.logits_penalize.restype = ctypes.c_int
+    lib.logits_penalize.argtypes = [ctypes.POINTER(PenalizeArgs), _vp]
+    lib.logits_sample.restype = ctypes.c_int
+    lib.logits_sample.argtypes = [ctypes.POINTER(SampleArgs), _vp]
     if lib.wkv7_abi_version() != WKV7_ABI_VERSION:
         raise ImportError(f"{path}: ABI version {lib.wkv7_abi_version()} != {WKV7_ABI_VERSION}")
     if lib.wkv7_args_size() != ctypes.sizeof(Wkv7Args):
@@ -187,6 +257,10 @@ def load(path: str = LIB_PATH):
         raise ImportError(f"{path}: wkv7_args field offsets {args_layout(lib)} != binding {binding_layout()}")
     if lib.w6a16_args_size() != ctypes.sizeof(W6a16Args):
         raise ImportError(f"{path}: sizeof(w6a16_args) {lib.w6a16_args_size()} != binding {ctypes.sizeof(W6a16Args)}")
+    for size, mirror in ((lib.w4a16_args_size(), W4a16Args), (lib.logits_penalize_args_size(), PenalizeArgs),
+                         (lib.logits_sample_args_size(), SampleArgs)):
+        if size != ctypes.sizeof(mirror):
+            raise ImportError(f"{path}: {mirror.__name__} has {size} bytes, binding {ctypes.sizeof(mirror)}")
     _lib = lib
     return lib
 

@@ -1,0 +1,263 @@
+"""From logits to tokens on the HIP kernels of include/logits.h: what the reference's sampler and its speculative step do with
+torch operations (rwkv_next/sampler.py:1-81, rwkv_next/spec.py:35-84).
+
+    penalize_logits(logits, ...)        penalties for repeated tokens, per-request biases, grammar masks
+    sample_logits(logits, noise, ...)   temperature, top-k, top-p, min-p, and a draw by given noise
+    next_tokens(x, head, noise, ...)    a decode step's end: head product, penalties, draw, the drawn tokens counted
+
+Logits are (B, V), one token for each sequence, or (B, T, V), T positions of a block of drafted tokens, in bfloat16, float16 or
+float32.  A per-sequence parameter is a tensor of B entries on the logits' device, or one number for all.  Every call runs on the
+current stream, no host sync, and can be recorded into a HIP graph; `status` (wkv7.new_status) reports indices that the kernels
+left out (check_status names them).
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+from ._workspace import on_device, stream_handle
+from .int4_gemm import Int4Packed, int4_matmul
+
+_DTYPES = {torch.bfloat16: _lib.LOGITS_BF16, torch.float16: _lib.LOGITS_F16, torch.float32: _lib.LOGITS_F32}
+_COUNTS = {torch.int32: _lib.LOGITS_COUNTS_I32, torch.float32: _lib.LOGITS_COUNTS_F32}
+
+
+def _shape(logits):
+    """(B, T, V, sequence stride, position stride) of (B, V) or (B, T, V) logits."""
+    if logits.dtype not in _DTYPES:
+        raise TypeError(f"logits must be bfloat16, float16 or float32 (got {logits.dtype})")
+    if logits.device.type != "cuda":
+        raise ValueError(f"logits must be on a GPU (got {logits.device})")
+    if logits.dim() == 2:
+        B, V = logits.shape
+        return B, 1, V, logits.stride(0), 0
+    if logits.dim() != 3:
+        raise ValueError(f"logits must be (B, V) or (B, T, V) (got {tuple(logits.shape)})")
+    return (*logits.shape, logits.stride(0), logits.stride(1))
+
+
+def _on(t, dev, name):
+    if t.device != dev:
+        raise ValueError(f"{name} must be on {dev} (got {t.device})")
+
+
+def _per_sequence(x, dtype, B, dev, name):
+    """(pointer, scalar) of a parameter: a tensor of B entries, or a number."""
+    if not isinstance(x, torch.Tensor):
+        return None, x
+    _on(x, dev, name)
+    if x.dtype != dtype or x.dim() != 1 or x.shape[0] != B or not (x.is_contiguous() or B == 1):
+        raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor of {B} entries "
+                         f"(got {x.dtype} {tuple(x.shape)})")
+    return x.data_ptr(), 0
+
+
+def _rows(x, dtype, lead, least, dev, name):
+    """A tensor of rows of at least `least` contiguous elements whose leading sizes are `lead`: its row stride."""
+    _on(x, dev, name)
+    if x.dtype != dtype or tuple(x.shape[:-1]) != lead or x.shape[-1] < least or x.stride(-1) != 1:
+        raise ValueError(f"{name} must be a {dtype} {(*lead, least)} tensor with contiguous rows "
+                         f"(got {x.dtype} {tuple(x.shape)}, strides {x.stride()})")
+    return x.stride(0) if lead[0] > 1 else max(x.stride(0), x.shape[-1])
+
+
+def _overlaps(t):
+    """Whether rows of a (B, V) or (B, T, V) tensor with contiguous rows may share memory."""
+    least = t.shape[-1]
+    for stride, size in sorted((s, n) for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+        if stride < least:
+            return True
+        least = stride * (size - 1) + least
+    return False
+
+
+def _counts(counts, slots, B, V, dev):
+    """(pointer, row stride, rows, type, slots' pointer) of a count table (S, V)."""
+    if counts is None:
+        if slots is not None:
+            raise ValueError("slots without counts")
+        return None, 0, 0, 0, None
+    _on(counts, dev, "counts")
+    if counts.dtype not in _COUNTS or counts.dim() != 2 or counts.shape[1] != V or counts.stride(1) != 1 or \
+            (counts.shape[0] > 1 and counts.stride(0) < V):
+        raise ValueError(f"counts must be an int32 or float32 (S, {V}) tensor with contiguous rows "
+                         f"(got {counts.dtype} {tuple(counts.shape)}, strides {counts.stride()})")
+    if slots is None and counts.shape[0] < B:
+        raise ValueError(f"counts has {counts.shape[0]} rows for {B} sequences (or pass slots)")
+    return (counts.data_ptr(), max(counts.stride(0), V), counts.shape[0], _COUNTS[counts.dtype],
+            None if slots is None else _per_sequence(slots, torch.int64, B, dev, "slots")[0])
+
+
+def _status(status, dev):
+    if status is None:
+        return None
+    _on(status, dev, "status")
+    if status.dtype != torch.int32 or status.numel() < 1:
+        raise ValueError("status must be an int32 tensor (new_status)")
+    return status.data_ptr()
+
+
+def penalize_logits(logits, *, counts=None, slots=None, repetition=1.0, presence=0.0, frequency=0.0, drafts=None,
+                    bias_ids=None, bias_values=None, mask=None, mask_rows=None, out=None, status=None):
+    """Per sequence b, position t and token v, with x the logit and c = counts[slots[b], v] + the number of drafts[b, :t] that
+    are v:
+
+        c > 0:  x = (x / repetition if x > 0 else x * repetition) - (frequency * c + presence)
+        x += bias_values[b, i] for every i with bias_ids[b, i] == v, in their order
+        x = -inf where the mask's bit of v is 0
+
+    in fp32, rounded once.  Returns a new tensor of the logits' type, or fills and returns `out` (any of the three types;
+    `logits` itself for an update in place).
+
+    counts (S, V) int32 or float32, row slots[b] (int64; row b without slots) of sequence b; the reference's penalty table.
+    drafts (B, >= T - 1) int64: the tokens fed at positions 1 .. T - 1, not yet in `counts` (negative: none).
+    bias_ids (B, P) int64 (negative: an unused place), bias_values (B, P) float32.
+    mask int32, ceil(V / 32) words to a row, bit v % 32 of word v / 32 set where v is allowed: one row for each row of the logits
+    ((B, words) or (B, T, words)), or a table (R, words) with mask_rows int64 in the shape of the rows (negative: no mask).
+    """
+    B, T, V, seq_stride, pos_stride = _shape(logits)
+    dev = logits.device
+    if B and T and V and logits.stride(-1) != 1:
+        if out is logits:
+            raise ValueError("logits must have contiguous rows to be changed in place")
+        logits = logits.contiguous()
+        _, _, _, seq_stride, pos_stride = _shape(logits)
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    elif out is not logits:
+        _on(out, dev, "out")
+        if out.shape != logits.shape or out.dtype not in _DTYPES or (out.numel() and out.stride(-1) != 1):
+            raise ValueError(f"out must be bfloat16, float16 or float32 {tuple(logits.shape)} with contiguous rows "
+                             f"(got {out.dtype} {tuple(out.shape)}, strides {out.stride()})")
+        if out.data_ptr() == logits.data_ptr() and out.numel() and (
+                out.dtype != logits.dtype or out.stride() != logits.stride()):
+            raise ValueError("out over the logits must have their type and strides")
+    if not (B and T and V):
+        return out
+    if _overlaps(out):
+        raise ValueError(f"out must not share memory between its rows (strides {out.stride()})")
+    lead = (B,) if logits.dim() == 2 else (B, T)
+    ct, ct_stride, ct_rows, ct_type, slots_p = _counts(counts, slots, B, V, dev)
+    rep_p, rep = _per_sequence(repetition, torch.float32, B, dev, "repetition")
+    pres_p, pres = _per_sequence(presence, torch.float32, B, dev, "presence")
+    freq_p, freq = _per_sequence(frequency, torch.float32, B, dev, "frequency")
+    if rep_p is None and not rep > 0:
+        raise ValueError(f"repetition must be positive (got {rep})")
+    dr_p = dr_stride = 0
+    if drafts is not None and T > 1:
+        dr_stride = _rows(drafts, torch.int64, (B,), T - 1, dev, "drafts")
+        dr_p = drafts.data_ptr()
+    bi_p = bv_p = bias_stride = n_bias = 0
+    if (bias_ids is None) != (bias_values is None):
+        raise ValueError("bias_ids and bias_values go together")
+    if bias_ids is not None and bias_ids.numel():
+        n_bias = bias_ids.shape[-1]
+        bias_stride = _rows(bias_ids, torch.int64, (B,), n_bias, dev, "bias_ids")
+        if _rows(bias_values, torch.float32, (B,), n_bias, dev, "bias_values") != bias_stride or \
+                bias_values.shape != bias_ids.shape:
+            bias_ids, bias_values = bias_ids.contiguous(), bias_values[..., :n_bias].contiguous()
+            bias_stride = n_bias
+        bi_p, bv_p = bias_ids.data_ptr(), bias_values.data_ptr()
+    m_p = m_stride = m_rows = mr_p = 0
+    if mask is not None:
+        words = (V + 31) // 32
+        if mask_rows is None:
+            m_stride = _rows(mask, torch.int32, lead, words, dev, "mask")
+            m_rows = B * T
+            if len(lead) == 2:  # rows of (b, t) one after another
+                if not mask.is_contiguous():
+                    mask = mask.contiguous()
+                m_stride = mask.shape[-1]
+        else:
+            _on(mask_rows, dev, "mask_rows")
+            if mask_rows.dtype != torch.int64 or tuple(mask_rows.shape) != lead or not mask_rows.is_contiguous():
+                raise ValueError(f"mask_rows must be a contiguous int64 {lead} tensor "
+                                 f"(got {mask_rows.dtype} {tuple(mask_rows.shape)})")
+            if mask.dim() != 2:
+                raise ValueError("mask must be a table (R, words) where mask_rows is given")
+            m_rows = mask.shape[0]
+            m_stride = _rows(mask, torch.int32, (m_rows,), words, dev, "mask") if m_rows else words
+            mr_p = mask_rows.data_ptr()
+        m_p = mask.data_ptr()
+        if not m_rows:
+            m_p = 0
+    elif mask_rows is not None:
+        raise ValueError("mask_rows without a mask")
+    if out.dim() == 2:
+        out_seq, out_pos = out.stride(0), 0
+    else:
+        out_seq, out_pos = out.stride(0), out.stride(1)
+    args = _lib.PenalizeArgs(
+        logits.data_ptr(), seq_stride, pos_stride, out.data_ptr(), out_seq, out_pos, ct, ct_stride, ct_rows, slots_p,
+        rep_p, pres_p, freq_p, dr_p or None, dr_stride, bi_p or None, bv_p or None, bias_stride, m_p or None, m_stride,
+        m_rows, mr_p or None, _status(status, dev), rep, pres, freq, B, T, V, n_bias, _DTYPES[logits.dtype],
+        _DTYPES[out.dtype], ct_type)  # in the order of the fields
+    with on_device(dev):
+        _lib.check(_lib.load().logits_penalize(args, stream_handle(dev)))
+    return out
+
+
+def sample_logits(logits, noise=None, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, counts=None, slots=None,
+                  status=None):
+    """(tokens int64, log-probabilities float32), each (B,) or (B, T): one token for each row of the logits.
+
+    With d = (max - x) / temperature and w = exp(-d), tokens are ordered by (d, index).  Kept are the first top_k (all where
+    top_k <= 0), of those the smallest prefix whose weights reach top_p of their sum (all where top_p >= 1), of those the ones
+    with w >= min_p; the first always.  The token is the kept one with the largest w / noise, the lowest index of equals: with
+    noise of the exponential distribution (torch.empty_like(logits, dtype=torch.float32).exponential_()) a draw by the kept
+    weights.  Rows with a temperature of 0, and all rows without noise, take the largest logit.  The log-probability is that of
+    the row's softmax at its temperature, before the filters (at a temperature of 1 in greedy rows).
+
+    NaN counts as -inf, and tokens of -inf are never chosen; a row of nothing else gives -1 and -inf.  A row's result depends on
+    that row alone.  noise float32 in the logits' shape; top_k int32 where it is a tensor, the other parameters float32.
+    counts (S, V) int32 or float32 with slots, for (B, V) logits: counts[slots[b], token] += 1, the next step's penalties.
+    """
+    B, T, V, seq_stride, pos_stride = _shape(logits)
+    dev = logits.device
+    if V < 1:
+        raise ValueError("logits without a token to choose")
+    if logits.stride(-1) != 1 and V > 1:
+        logits = logits.contiguous()
+        _, _, _, seq_stride, pos_stride = _shape(logits)
+    lead = logits.shape[:-1]
+    token = torch.empty(lead, dtype=torch.int64, device=dev)
+    logprob = torch.empty(lead, dtype=torch.float32, device=dev)
+    nz = nz_seq = nz_pos = None
+    if noise is not None:
+        _on(noise, dev, "noise")
+        if noise.dtype != torch.float32 or noise.shape != logits.shape:
+            raise ValueError(f"noise must be float32 {tuple(logits.shape)} (got {noise.dtype} {tuple(noise.shape)})")
+        if noise.stride(-1) != 1 and V > 1:
+            noise = noise.contiguous()
+        nz, nz_seq, nz_pos = noise.data_ptr(), noise.stride(0), noise.stride(1) if noise.dim() == 3 else 0
+    t_p, t = _per_sequence(temperature, torch.float32, B, dev, "temperature")
+    k_p, k = _per_sequence(top_k, torch.int32, B, dev, "top_k")
+    p_p, p = _per_sequence(top_p, torch.float32, B, dev, "top_p")
+    m_p, m = _per_sequence(min_p, torch.float32, B, dev, "min_p")
+    if counts is not None and logits.dim() != 2:
+        raise ValueError("counts are kept for (B, V) logits: a block's accepted tokens are known only later")
+    ct, ct_stride, ct_rows, ct_type, slots_p = _counts(counts, slots, B, V, dev)
+    if not (B and T):
+        return token, logprob
+    args = _lib.SampleArgs(
+        logits.data_ptr(), seq_stride, pos_stride, nz, nz_seq or 0, nz_pos or 0, t_p, k_p, p_p, m_p, token.data_ptr(),
+        logprob.data_ptr(), ct, ct_stride, ct_rows, slots_p, _status(status, dev), t, p, m,
+        max(-1, min(int(k), 2 ** 31 - 1)), B, T, V, _DTYPES[logits.dtype], ct_type)  # in the order of the fields
+    with on_device(dev):
+        _lib.check(_lib.load().logits_sample(args, stream_handle(dev)))
+    return token, logprob
+
+
+def next_tokens(x, head: Int4Packed, noise=None, *, counts=None, slots=None, repetition=1.0, presence=0.0,
+                frequency=0.0, bias_ids=None, bias_values=None, mask=None, mask_rows=None, temperature=1.0, top_k=0,
+                top_p=1.0, min_p=0.0, status=None):
+    """The end of a decode step: the output head's product with the last hidden states x (B, C) in fp32, the penalties, the
+    draw, and the drawn tokens counted in `counts`.  Returns (tokens, log-probabilities), each (B,).  Arguments as in
+    int4_matmul, penalize_logits and sample_logits; the whole can be recorded into a HIP graph."""
+    if x.dim() != 2:
+        raise ValueError(f"x must be (B, C), the hidden state of one token for each sequence (got {tuple(x.shape)})")
+    logits = int4_matmul(x, head, out_dtype=torch.float32)
+    penalize_logits(logits, counts=counts, slots=slots, repetition=repetition, presence=presence, frequency=frequency,
+                    bias_ids=bias_ids, bias_values=bias_values, mask=mask, mask_rows=mask_rows, out=logits, status=status)
+    return sample_logits(logits, noise, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, counts=counts,
+                         slots=slots, status=status)

@@ -355,11 +355,13 @@ STATUS_REASONS = {_lib.WKV7_STATUS_H0_SLOT: "initial-state slot index outside th
                                                "sequence stores or reads its state): the result depends on timing",
                   _lib.WKV7_STATUS_SEGMENT_WAIT: "the segmented prefill gave up waiting for a segment hand-off: "
                                                  "the results are wrong and the stream's workspace flags must be "
-                                                 "zeroed (reset_workspaces())"}
+                                                 "zeroed (reset_workspaces())",
+                  _lib.LOGITS_STATUS_ROW: "a slot outside the count table, or a mask row past the masks",
+                  _lib.LOGITS_STATUS_TOKEN: "a draft or bias token outside the vocabulary"}
 
 
 def check_status(status: torch.Tensor) -> None:
-    """Raise ValueError naming every WKV7_STATUS_* bit set in `status` (synchronises the host: call it outside
+    """Raise ValueError naming every WKV7_STATUS_* or LOGITS_STATUS_* bit set in `status` (synchronises the host: call it outside
     graph capture and the hot loop)."""
     bits = int(status.reshape(-1)[0].item())
     if bits:
