@@ -86,6 +86,8 @@ typedef struct logits_sample_args {
     int64_t counts_stride, counts_rows;
     const int64_t *slots;                    /* NULL (row b has counts row b), or [B] */
     int32_t *status;                         /* NULL, or one device word */
+    void *workspace;                         /* logits_sample_workspace_size bytes, 256-byte aligned */
+    size_t workspace_bytes;
     float temperature_all, top_p_all, min_p_all;
     int32_t top_k_all;
     int32_t B, T, V;
@@ -95,6 +97,11 @@ typedef struct logits_sample_args {
 /* sizeof the structs as compiled into the library (bindings check their layout against them). */
 size_t logits_penalize_args_size(void);
 size_t logits_sample_args_size(void);
+
+/* Bytes of workspace that logits_sample needs.  They must be zero before the workspace's first use; every completed call
+ * leaves them zero, so one workspace serves any number of calls of any shapes one after another (stream order).  Calls that
+ * can run at the same time need different workspaces. */
+int logits_sample_workspace_size(const logits_sample_args *args, size_t *bytes);
 
 int logits_penalize(const logits_penalize_args *args, void *stream);
 int logits_sample(const logits_sample_args *args, void *stream);

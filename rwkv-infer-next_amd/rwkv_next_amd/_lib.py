@@ -57,7 +57,8 @@ W4A16_EXPORTED = ("w4a16_args_size", "w4a16_packed_size", "w4a16_pack", "w4a16_d
 W4A16_BF16 = 0
 W4A16_F16 = 1
 W4A16_F32 = 2
-LOGITS_EXPORTED = ("logits_penalize_args_size", "logits_sample_args_size", "logits_penalize", "logits_sample")
+LOGITS_EXPORTED = ("logits_penalize_args_size", "logits_sample_args_size", "logits_sample_workspace_size",
+                   "logits_penalize", "logits_sample")
 LOGITS_BF16 = 0
 LOGITS_F16 = 1
 LOGITS_F32 = 2
@@ -165,6 +166,7 @@ class SampleArgs(ctypes.Structure):
         ("token", _vp), ("logprob", _vp),
         ("counts", _vp), ("counts_stride", ctypes.c_int64), ("counts_rows", ctypes.c_int64), ("slots", _vp),
         ("status", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
         ("temperature_all", ctypes.c_float), ("top_p_all", ctypes.c_float), ("min_p_all", ctypes.c_float),
         ("top_k_all", ctypes.c_int32), ("B", ctypes.c_int32), ("T", ctypes.c_int32), ("V", ctypes.c_int32),
         ("dtype", ctypes.c_int32), ("counts_dtype", ctypes.c_int32),
@@ -247,6 +249,8 @@ def load(path: str = LIB_PATH):
     lib.logits_sample_args_size.restype = ctypes.c_size_t
     lib.logits_penalize.restype = ctypes.c_int
     lib.logits_penalize.argtypes = [ctypes.POINTER(PenalizeArgs), _vp]
+    lib.logits_sample_workspace_size.restype = ctypes.c_int
+    lib.logits_sample_workspace_size.argtypes = [ctypes.POINTER(SampleArgs), psz]
     lib.logits_sample.restype = ctypes.c_int
     lib.logits_sample.argtypes = [ctypes.POINTER(SampleArgs), _vp]
     if lib.wkv7_abi_version() != WKV7_ABI_VERSION:

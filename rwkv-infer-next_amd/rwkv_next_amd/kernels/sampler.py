@@ -12,10 +12,12 @@ left out (check_status names them).
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from .. import _lib
-from ._workspace import on_device, stream_handle
+from ._workspace import on_device, stream_handle, stream_workspace
 from .int4_gemm import Int4Packed, int4_matmul
 
 _DTYPES = {torch.bfloat16: _lib.LOGITS_BF16, torch.float16: _lib.LOGITS_F16, torch.float32: _lib.LOGITS_F32}
@@ -197,6 +199,22 @@ def penalize_logits(logits, *, counts=None, slots=None, repetition=1.0, presence
     return out
 
 
+_WORKSPACES: dict = {}  # (device index, stream handle) -> [buffer, zeroed in stream order, capture id]
+_BYTES: dict = {}       # rows -> bytes of workspace
+
+
+def _workspace(rows, V, dev):
+    """The zeroed workspace of the current stream (include/logits.h, logits_sample_workspace_size).  Every byte that a call
+    uses has to be zero, so the buffer is asked for twice: a larger call does not find room that was never cleared."""
+    n = _BYTES.get(rows)
+    if n is None:
+        size = ctypes.c_size_t(0)
+        _lib.check(_lib.load().logits_sample_workspace_size(_lib.SampleArgs(B=rows, T=1, V=V), ctypes.byref(size)))
+        n = _BYTES[rows] = int(size.value)
+    with on_device(dev):
+        return stream_workspace(_WORKSPACES, dev, 2 * n, n)
+
+
 def sample_logits(logits, noise=None, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, counts=None, slots=None,
                   status=None):
     """(tokens int64, log-probabilities float32), each (B,) or (B, T): one token for each row of the logits.
@@ -239,9 +257,11 @@ def sample_logits(logits, noise=None, *, temperature=1.0, top_k=0, top_p=1.0, mi
     ct, ct_stride, ct_rows, ct_type, slots_p = _counts(counts, slots, B, V, dev)
     if not (B and T):
         return token, logprob
+    ws = _workspace(B * T, V, dev)
     args = _lib.SampleArgs(
         logits.data_ptr(), seq_stride, pos_stride, nz, nz_seq or 0, nz_pos or 0, t_p, k_p, p_p, m_p, token.data_ptr(),
-        logprob.data_ptr(), ct, ct_stride, ct_rows, slots_p, _status(status, dev), t, p, m,
+        logprob.data_ptr(), ct, ct_stride, ct_rows, slots_p, _status(status, dev),
+        ws.data_ptr(), ws.numel(), t, p, m,
         max(-1, min(int(k), 2 ** 31 - 1)), B, T, V, _DTYPES[logits.dtype], ct_type)  # in the order of the fields
     with on_device(dev):
         _lib.check(_lib.load().logits_sample(args, stream_handle(dev)))
