@@ -98,9 +98,10 @@ typedef struct logits_sample_args {
 size_t logits_penalize_args_size(void);
 size_t logits_sample_args_size(void);
 
-/* Bytes of workspace that logits_sample needs.  They must be zero before the workspace's first use; every completed call
- * leaves them zero, so one workspace serves any number of calls of any shapes one after another (stream order).  Calls that
- * can run at the same time need different workspaces. */
+/* Bytes of workspace that logits_sample needs, 256-byte aligned.  The first LOGITS_SAMPLE_STATE_BYTES must be zero before the
+ * workspace's first use; every completed call leaves them zero and writes nothing else into them, so one workspace serves any
+ * number of calls of any shapes one after another (stream order).  Calls that can run at the same time need different ones. */
+#define LOGITS_SAMPLE_STATE_BYTES 6422528
 int logits_sample_workspace_size(const logits_sample_args *args, size_t *bytes);
 
 int logits_penalize(const logits_penalize_args *args, void *stream);

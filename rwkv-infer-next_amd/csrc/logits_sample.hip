@@ -1,80 +1,88 @@
-// logits_sample.hip -- the choice of a token from each row of logits (include/logits.h), in three launches:
+// logits_sample.hip -- the choice of a token from each row of logits (include/logits.h), in four launches:
 //
-//   max     segments of 8192 elements, a workgroup each: the row's maximum and its lowest index
+//   max     a row's segments, a workgroup each: the row's maximum and its lowest index
 //   weigh   the same segments: with d = (max - x) / T, w = exp(-d) the sum of w; in rows without top-k and top-p the draw among
 //           their elements; in the others a histogram over d in steps of 1/32, of the tokens' number and of their weights
-//   choose  a workgroup a row: where the histogram reaches the wanted number or weight the threshold lies in that bin; one pass
-//           over the row gathers the bin in LDS (and draws among the tokens before it); sorted by (d, index) and scanned, it gives
-//           the last kept token
+//   gather  the same segments: where the histogram reaches the wanted number or weight, the last kept token is in that bin.  The
+//           tokens before it are kept, and drawn among; the bin's own (top-k: all up to its end) go into the row's list
+//   choose  a workgroup a row: the last kept token of the list, by histograms over ever finer parts of (d, index), and the draw
 //
-// A row's maximum must be known before its weights are, and its weights before a threshold: hence the launches.  Sums are
-// of whole numbers of 2^-40, so no order of the atomics shows in a result.  A bin of more tokens than the list in LDS holds (equal
-// logits, or a top-k of thousands) goes the long way: the workgroup cuts it into 1024 parts by (d, index), again and again.
+// A row's maximum must be known before its weights, its weights before a threshold, and the threshold before the draw: hence the
+// launches; no row and no list is sorted.  Sums that decide are of whole numbers of 2^-40: no order of the atomics shows in a
+// result.  A bin of more tokens than the list holds (equal logits, a top-k of thousands) goes the long way: its row's workgroup
+// cuts the row itself into finer parts.
+//
+// d is kept as 32 d (bins are its whole part), which the scaling by a power of two leaves as exact as d.
 #include <hip/hip_runtime.h>
+#include <float.h>
 #include <stdint.h>
+
+#include <algorithm>
 
 #include "logits.h"
 #include "logits_device.h"
+#include "wkv7_launch.h"
 
 namespace lg {
 namespace {
 
-constexpr int kThreads = 1024;     // of the choosing workgroup
-constexpr int kWaves = kThreads / 64;
-constexpr int kSegThreads = 256;   // of a segment's workgroup
-constexpr int kSegPieces = 4;      // eight elements each to a thread
-constexpr int kSegment = kSegThreads * kSegPieces * 8;
-constexpr int kRowsAtOnce = 512;   // rows of one set of launches: the workspace holds as many
-constexpr int kBins = 1024;        // one per thread
-constexpr float kPerUnit = 32.f;   // bins to a unit of d; the last one holds all from 1023/32 on
-constexpr int kGather = 4096;      // tokens of a bin that are sorted in LDS
+constexpr int kThreads = 1024;     // of the choosing workgroup, one per bin
+constexpr int kSegThreads = 256;   // of a segment's workgroup: 8 elements, or 4 x 8, to a thread
+constexpr int kBins = 1024;        // the last one holds all from 1023/32 on
+constexpr float kPerUnit = 32.f;   // bins to a unit of d
+constexpr int kList = 4096;        // tokens that a row's list holds
+constexpr int kOwn = kList / kThreads;
+constexpr int kRowsAtOnce = 512;   // rows of one set of launches
 constexpr float kOne = 1099511627776.f;  // 2^40: a weight of 1
 constexpr uint32_t kInfBits = 0x7F800000u;
+constexpr float kExp2PerBin = -1.44269504088896341f / kPerUnit;  // w = 2^(32 d * this)
 
-// A row's part of the workspace: all zero between calls.
+// A row's part of the workspace: all zero between calls.  The rows' lists, which need not be, follow the kRowsAtOnce of them.
 struct RowState {
-    unsigned long long max_key;     // order_bits(max) << 32 | ~index
-    unsigned long long total;       // sum of the weights
-    unsigned long long won;         // order of w / noise << 32 | ~index, rows without top-k and top-p
-    unsigned long long unused[29];
+    unsigned long long max_key;  // order_bits(max) << 32 | ~index
+    unsigned long long total;    // sum of the weights
+    unsigned long long won;      // the draw so far: w / noise as an integer << 32 | ~index
+    uint32_t gathered;           // entries of the list
+    uint32_t unused[57];
     unsigned long long weight[kBins];
     uint32_t count[kBins];
 };
-
-struct Shared {
-    uint64_t list[kGather];
-    uint64_t weight[kBins];
-    uint32_t count[kBins];
-    uint64_t wave[kWaves];
-    uint64_t found, base;
-    uint32_t gathered, bin;
-};
+static_assert(sizeof(RowState) * kRowsAtOnce == LOGITS_SAMPLE_STATE_BYTES, "include/logits.h");
 
 __device__ __forceinline__ uint64_t shuffle(uint64_t x, int from) {
     const uint32_t lo = __shfl((int)(uint32_t)x, from), hi = __shfl((int)(uint32_t)(x >> 32), from);
     return (uint64_t)hi << 32 | lo;
 }
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint64_t plus(uint64_t a, uint64_t b) { return a + b; }
 
 template <typename F>
 __device__ __forceinline__ uint64_t wave_reduce(uint64_t x, F&& f) {
     for (int o = 32; o; o >>= 1) x = f(x, shuffle(x, (threadIdx.x & 63) ^ o));
     return x;
 }
-template <typename F>
-__device__ __forceinline__ uint64_t block_reduce(Shared& s, uint64_t x, F&& f) {
+
+template <int THREADS>
+struct Scratch {
+    uint64_t wave[THREADS / 64];
+    uint64_t base, found;
+    uint32_t bin, n;
+};
+
+template <int THREADS, typename F>
+__device__ __forceinline__ uint64_t block_reduce(Scratch<THREADS>& s, uint64_t x, F&& f) {
     x = wave_reduce(x, f);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s.wave[threadIdx.x >> 6] = x;
     __syncthreads();
     x = s.wave[0];
-    for (int w = 1; w < kWaves; ++w) x = f(x, s.wave[w]);
+    for (int w = 1; w < THREADS / 64; ++w) x = f(x, s.wave[w]);
     return x;
 }
-__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint64_t plus(uint64_t a, uint64_t b) { return a + b; }
 
 // The sum over the threads before this one.
-__device__ __forceinline__ uint64_t block_before(Shared& s, uint64_t x) {
+template <int THREADS>
+__device__ __forceinline__ uint64_t block_before(Scratch<THREADS>& s, uint64_t x) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint64_t sum = x;
     for (int o = 1; o < 64; o <<= 1) {
@@ -89,12 +97,39 @@ __device__ __forceinline__ uint64_t block_before(Shared& s, uint64_t x) {
     return before;
 }
 
+// The first bin at whose end the running sum reaches `target`, the sum before it and the tokens in it; kBins where none does.  A
+// thread has kBins / THREADS bins: their sums and numbers.
+template <int THREADS>
+__device__ __forceinline__ uint32_t reaching_bin(Scratch<THREADS>& s, const uint64_t (&sums)[kBins / THREADS],
+                                                 const uint32_t (&counts)[kBins / THREADS], uint64_t target, uint64_t& base,
+                                                 uint32_t& n) {
+    if (threadIdx.x == 0) s.bin = kBins, s.base = 0, s.n = 0;
+    uint64_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < kBins / THREADS; ++j) mine += sums[j];
+    uint64_t before = block_before(s, mine);  // its barriers order the first line
+#pragma unroll
+    for (int j = 0; j < kBins / THREADS; ++j) {
+        if (before < target && before + sums[j] >= target)
+            s.bin = threadIdx.x * (kBins / THREADS) + j, s.base = before, s.n = counts[j];
+        before += sums[j];
+    }
+    __syncthreads();
+    const uint32_t b = s.bin;
+    base = s.base, n = s.n;
+    __syncthreads();
+    return b;
+}
+
 // What a row's passes need to know of it.
 struct Row {
     const void* x;
     int V;
-    float max, inv;  // inv = 1 / temperature
+    float max, inv;  // inv = 32 / temperature
 };
+
+// A logit as the kernels take it: NaN as -infinity, infinity as the largest number (so that no difference is NaN).
+__device__ __forceinline__ float logit(float x) { return fminf(fmaxf(x, -__builtin_inff()), FLT_MAX); }
 
 // Bits of a float that order as the numbers do (-0 as 0), and back.
 __device__ __forceinline__ uint32_t order_bits(float x) {
@@ -103,133 +138,27 @@ __device__ __forceinline__ uint32_t order_bits(float x) {
 }
 __device__ __forceinline__ float from_order(uint32_t u) { return __uint_as_float(u >> 31 ? u & 0x7FFFFFFFu : ~u); }
 
-// (max - x) / temperature; 0 for the maximum (an infinite one too), infinity for -infinity.
-__device__ __forceinline__ float distance(const Row& r, float x) {
-    const float d = (r.max - x) * r.inv;
-    return x == r.max ? 0.f : d >= 0.f ? d : __builtin_inff();
-}
-__device__ __forceinline__ float weight(float d) { return __builtin_amdgcn_exp2f(d * -1.44269504088896341f); }
+__device__ __forceinline__ float distance(const Row& r, float x) { return (r.max - x) * r.inv; }  // 32 d >= 0
+__device__ __forceinline__ float weight(float d32) { return __builtin_amdgcn_exp2f(d32 * kExp2PerBin); }
 __device__ __forceinline__ uint64_t whole(float w) { return (uint64_t)(w * kOne); }
-__device__ __forceinline__ uint32_t bin_of(float d) { return (uint32_t)(int)fminf(d * kPerUnit, (float)(kBins - 1)); }
+// The first 32 d past a bin; every finite one lies before the last bin's.
+__device__ __forceinline__ float end_of_bin(uint32_t b) { return b >= kBins - 1 ? __builtin_inff() : (float)(b + 1); }
 
-// f(index, x) for every element of the row, NaN as -infinity; four 8-element pieces of it in flight to a thread.
-template <int DT, typename F>
-__device__ __forceinline__ void each(const Row& r, F&& f) {
-    constexpr int kAhead = 4;
-    for (int64_t i0 = 8 * (int64_t)threadIdx.x; i0 < r.V; i0 += (int64_t)kAhead * kThreads * 8) {
-        float x[kAhead][8];
-#pragma unroll
-        for (int a = 0; a < kAhead; ++a) {
-            const int64_t i = i0 + (int64_t)a * kThreads * 8;
-            load8<DT>(r.x, i, i >= r.V ? 0 : r.V - i < 8 ? (int)(r.V - i) : 8, -__builtin_inff(), x[a]);
-        }
-#pragma unroll
-        for (int a = 0; a < kAhead; ++a)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float v = x[a][j];
-                f((uint32_t)(i0 + (int64_t)a * kThreads * 8 + j), v == v ? v : -__builtin_inff());
-            }
-    }
-}
-
-__device__ __forceinline__ uint64_t key_of(float d, uint32_t i) { return (uint64_t)__float_as_uint(d) << 32 | i; }
+__device__ __forceinline__ uint64_t key_of(float d32, uint32_t i) { return (uint64_t)__float_as_uint(d32) << 32 | i; }
 __device__ __forceinline__ float d_of(uint64_t key) { return __uint_as_float((uint32_t)(key >> 32)); }
-
-// Sorts list[0 .. n-1] upwards; the threads' own, n <= kGather.
-__device__ void sort_list(Shared& s, uint32_t n) {
-    uint32_t size = 64;
-    while (size < n) size *= 2;
-    for (uint32_t i = n + threadIdx.x; i < size; i += kThreads) s.list[i] = ~0ull;
-    for (uint32_t k = 2; k <= size; k *= 2)
-        for (uint32_t j = k / 2; j; j /= 2) {
-            __syncthreads();
-            for (uint32_t e = threadIdx.x; e < size / 2; e += kThreads) {
-                const uint32_t a = (e & ~(j - 1)) * 2 + (e & (j - 1)), b = a + j;
-                const uint64_t x = s.list[a], y = s.list[b];
-                if ((x > y) == ((a & k) == 0)) s.list[a] = y, s.list[b] = x;
-            }
-        }
-    __syncthreads();
-}
-
-// The key of the last token of the smallest prefix, in the order of keys up to `limit`, whose number (COUNT) or weight reaches
-// `target`; `limit` where all together do not.  Tokens without weight in 64 bits (d infinite) are in no prefix.
-template <int DT, bool COUNT>
-__device__ uint64_t last_kept(Shared& s, const Row& r, uint64_t limit, uint64_t target) {
-    const int tid = threadIdx.x;
-    uint64_t lo = 0, hi = (uint64_t)kInfBits << 32, base = 0;  // keys of the part that is searched
-    int shift = -1;                                             // -1: by bins of d
-    for (;;) {
-        s.count[tid] = 0;
-        s.weight[tid] = 0;
-        if (tid == 0) s.bin = kBins, s.gathered = 0;
-        __syncthreads();
-        each<DT>(r, [&](uint32_t i, float x) {
-            const float d = distance(r, x);
-            const uint64_t key = key_of(d, i);
-            if (key >= lo && key < hi && key <= limit) {
-                const uint32_t b = shift < 0 ? bin_of(d) : (uint32_t)((key - lo) >> shift);
-                atomicAdd(&s.count[b], 1u);
-                if (!COUNT) atomicAdd((unsigned long long*)&s.weight[b], (unsigned long long)whole(weight(d)));
-            }
-        });
-        __syncthreads();
-        const uint64_t mine = COUNT ? s.count[tid] : s.weight[tid], before = base + block_before(s, mine);
-        if (before < target && before + mine >= target) s.bin = tid, s.base = before;  // one thread at most
-        __syncthreads();
-        const uint32_t b = s.bin;
-        if (b == kBins) return limit;
-        const uint32_t n = s.count[b];
-        base = s.base;
-        if (shift < 0) {
-            lo = (uint64_t)__float_as_uint((float)b / kPerUnit) << 32;
-            if (b < kBins - 1) hi = (uint64_t)__float_as_uint((float)(b + 1) / kPerUnit) << 32;
-        } else {
-            lo += (uint64_t)b << shift;
-            hi = min(hi, lo + (1ull << shift));
-        }
-        __syncthreads();
-        if (n <= kGather) break;
-        shift = 0;
-        while (((hi - lo - 1) >> shift) >= kBins) ++shift;
-    }
-    each<DT>(r, [&](uint32_t i, float x) {
-        const uint64_t key = key_of(distance(r, x), i);
-        if (key >= lo && key < hi && key <= limit) {
-            const uint32_t at = atomicAdd(&s.gathered, 1u);
-            if (at < kGather) s.list[at] = key;  // as many as were counted, unless someone writes the logits meanwhile
-        }
-    });
-    __syncthreads();
-    const uint32_t n = min(s.gathered, (uint32_t)kGather);
-    sort_list(s, n);
-    if (COUNT) return s.list[min((uint32_t)(target - base - 1), (uint32_t)kGather - 1)];
-    uint64_t w[kGather / kThreads], sum = 0;
-#pragma unroll
-    for (int j = 0; j < kGather / kThreads; ++j) {
-        const uint32_t e = tid * (kGather / kThreads) + j;
-        w[j] = e < n ? whole(weight(d_of(s.list[e]))) : 0;
-        sum += w[j];
-    }
-    uint64_t before = base + block_before(s, sum);
-#pragma unroll
-    for (int j = 0; j < kGather / kThreads; ++j) {
-        if (before < target && before + w[j] >= target) s.found = s.list[tid * (kGather / kThreads) + j];
-        before += w[j];
-    }
-    __syncthreads();
-    return s.found;
-}
 
 // A row's parameters, the same in every launch.
 struct Choice {
     int64_t b, t;
     Row row;
     const float* noise;
-    int k;              // 0: no top-k
+    int k;                  // 0: no top-k
     float top_p, min_p;
     bool greedy, searches;  // searches: top-k or top-p
+    __device__ uint64_t want(uint64_t sum) const {  // the weight that a top-p prefix has to reach
+        const double x = (double)top_p * (double)sum;
+        return x >= 1.0 ? (uint64_t)ceil(x) : 1;
+    }
 };
 
 template <int DT>
@@ -241,7 +170,7 @@ __device__ __forceinline__ Choice choice_of(const logits_sample_args& p, int64_t
     c.row.x = static_cast<const char*>(p.logits) + (c.b * p.seq_stride + c.t * p.pos_stride) * element_bytes(DT);
     c.row.V = p.V;
     c.row.max = 0.f;
-    c.row.inv = temperature > 0.f ? fminf(fmaxf(1.f / temperature, 1e-30f), 3e38f) : 1.f;
+    c.row.inv = kPerUnit * (temperature > 0.f ? fminf(fmaxf(1.f / temperature, 1e-25f), 1e30f) : 1.f);
     c.noise = p.noise + c.b * p.noise_seq_stride + c.t * p.noise_pos_stride;
     c.k = p.top_k ? p.top_k[c.b] : p.top_k_all;
     if (c.k < 0 || c.k >= p.V) c.k = 0;
@@ -251,34 +180,38 @@ __device__ __forceinline__ Choice choice_of(const logits_sample_args& p, int64_t
     return c;
 }
 
-// This thread's pieces of a segment, NaN as -infinity; fill past the row.
-template <int DT>
-__device__ __forceinline__ void load_segment(const Row& r, int64_t first, float (&x)[kSegPieces][8]) {
+__device__ __forceinline__ int piece(int64_t i, int V) { return i >= V ? 0 : V - i < 8 ? (int)(V - i) : 8; }
+
+// This thread's pieces of a segment; -infinity past the row.
+template <int DT, int PIECES>
+__device__ __forceinline__ void load_segment(const Row& r, int64_t first, float (&x)[PIECES][8]) {
 #pragma unroll
-    for (int a = 0; a < kSegPieces; ++a) {
+    for (int a = 0; a < PIECES; ++a) {
         const int64_t i = first + (a * kSegThreads + threadIdx.x) * 8;
-        load8<DT>(r.x, i, i >= r.V ? 0 : r.V - i < 8 ? (int)(r.V - i) : 8, -__builtin_inff(), x[a]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[a][j] = x[a][j] == x[a][j] ? x[a][j] : -__builtin_inff();
+        load8<DT>(r.x, i, piece(i, r.V), -__builtin_inff(), x[a]);
     }
+#pragma unroll
+    for (int a = 0; a < PIECES; ++a)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[a][j] = logit(x[a][j]);
 }
 
-template <int DT>
+template <int DT, int PIECES>
 __global__ __launch_bounds__(kSegThreads) void max_kernel(const logits_sample_args p, int64_t row0, uint32_t segments,
                                                           RowState* states) {
     const uint32_t at = blockIdx.x / segments;
-    const int64_t first = (int64_t)(blockIdx.x % segments) * kSegment;
+    const int64_t first = (int64_t)(blockIdx.x % segments) * (kSegThreads * PIECES * 8);
     const Choice c = choice_of<DT>(p, row0 + at);
-    float x[kSegPieces][8];
-    load_segment<DT>(c.row, first, x);
+    float x[PIECES][8];
+    load_segment<DT, PIECES>(c.row, first, x);
     float m = x[0][0];
 #pragma unroll
-    for (int a = 0; a < kSegPieces; ++a)
+    for (int a = 0; a < PIECES; ++a)
 #pragma unroll
         for (int j = 0; j < 8; ++j) m = fmaxf(m, x[a][j]);
     uint32_t where = 0;
 #pragma unroll
-    for (int a = kSegPieces - 1; a >= 0; --a)
+    for (int a = PIECES - 1; a >= 0; --a)
 #pragma unroll
         for (int j = 7; j >= 0; --j)
             if (x[a][j] == m) where = (uint32_t)(first + (a * kSegThreads + threadIdx.x) * 8 + j);
@@ -286,77 +219,57 @@ __global__ __launch_bounds__(kSegThreads) void max_kernel(const logits_sample_ar
     if ((threadIdx.x & 63) == 0) atomicMax(&states[at].max_key, (unsigned long long)key);
 }
 
-// The noise of eight elements from i on, where any of them may be drawn.
-__device__ __forceinline__ void load_noise(const float* noise, int64_t i, int V, bool any, float (&e)[8]) {
-    load8<LOGITS_F32>(noise, i, !any || i >= V ? 0 : V - i < 8 ? (int)(V - i) : 8, 1.f, e);
-}
-
-// The better of a draw so far and of element i: the largest w / noise, NaN never; indexes come upwards, so the first of equals
-// stays.
+// The better of a draw so far and of element i: the largest w / noise, NaN never; where indexes come upwards the first of equals
+// stays.  The reciprocal is the hardware's (1 ulp): both sides of a comparison have it.
 __device__ __forceinline__ void draw(float w, float noise, uint32_t i, float& best, uint32_t& where) {
-    const float score = w / noise;
+    const float score = w * __builtin_amdgcn_rcpf(noise);
     if (score > best) best = score, where = i;
 }
 __device__ __forceinline__ uint64_t draw_key(float best, uint32_t where) {  // 0: nothing drawn
     return best > 0.f ? (uint64_t)__float_as_uint(best) << 32 | (uint32_t)~where : 0;
 }
 
-template <int DT>
+template <int DT, int PIECES>
 __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_args p, int64_t row0, uint32_t segments,
                                                             RowState* states) {
     __shared__ uint64_t weights[kBins];
     __shared__ uint32_t counts[kBins];
     const int tid = threadIdx.x;
     const uint32_t at = blockIdx.x / segments;
-    const int64_t first = (int64_t)(blockIdx.x % segments) * kSegment;
+    const int64_t first = (int64_t)(blockIdx.x % segments) * (kSegThreads * PIECES * 8);
     RowState& state = states[at];
     Choice c = choice_of<DT>(p, row0 + at);
-    float x[kSegPieces][8];
-    load_segment<DT>(c.row, first, x);
+    float x[PIECES][8];
+    load_segment<DT, PIECES>(c.row, first, x);
     c.row.max = from_order((uint32_t)(state.max_key >> 32));
     if (c.row.max == -__builtin_inff()) return;
     const bool draws = !c.greedy && !c.searches, weighs = c.top_p < 1.f;
+    float total = 0.f;
     if (c.searches) {
         for (int b = tid; b < kBins; b += kSegThreads) weights[b] = 0, counts[b] = 0;
         __syncthreads();
-    }
-    uint64_t total = 0, far_weight = 0;
-    uint32_t far = 0, where = 0;
-    float best = 0.f;
+        uint64_t far_weight = 0;  // a long tail's tokens all fall into the last bin: added up in registers
+        uint32_t far = 0;
 #pragma unroll
-    for (int a = 0; a < kSegPieces; ++a) {
-        const int64_t i = first + (a * kSegThreads + tid) * 8;
-        float e[8];
-        if (draws) load_noise(c.noise, i, p.V, true, e);
+        for (int a = 0; a < PIECES; ++a)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float d = distance(c.row, x[a][j]), w = weight(d);
-            const uint64_t u = whole(w);
-            total += u;
-            if (draws && w >= c.min_p && w > 0.f) draw(w, e[j], (uint32_t)(i + j), best, where);
-            if (c.searches && d < __builtin_inff()) {
-                const uint32_t b = bin_of(d);
-                if (b == kBins - 1) {  // a long tail's tokens all fall here: counted in registers
-                    ++far, far_weight += u;
+            for (int j = 0; j < 8; ++j) {
+                const float d = distance(c.row, x[a][j]), w = weight(d);
+                total += w;
+                if (d >= (float)(kBins - 1)) {
+                    far += d < __builtin_inff();
+                    far_weight += whole(w);
                 } else {
+                    const uint32_t b = (uint32_t)fmaxf(d, 0.f);
                     atomicAdd(&counts[b], 1u);
-                    if (weighs) atomicAdd((unsigned long long*)&weights[b], (unsigned long long)u);
+                    if (weighs) atomicAdd((unsigned long long*)&weights[b], (unsigned long long)whole(w));
                 }
             }
-        }
-    }
-    total = wave_reduce(total, plus);
-    if ((tid & 63) == 0) atomicAdd(&state.total, (unsigned long long)total);
-    if (draws) {
-        const uint64_t key = wave_reduce(draw_key(best, where), larger);
-        if ((tid & 63) == 0 && key) atomicMax(&state.won, (unsigned long long)key);
-    }
-    if (c.searches) {
         far_weight = wave_reduce(far_weight, plus);
-        const uint64_t n = wave_reduce((uint64_t)far, plus);
+        const uint32_t n = (uint32_t)wave_reduce((uint64_t)far, plus);
         if ((tid & 63) == 0 && n) {
-            atomicAdd(&counts[kBins - 1], (uint32_t)n);
-            if (weighs) atomicAdd((unsigned long long*)&weights[kBins - 1], (unsigned long long)far_weight);
+            atomicAdd(&counts[kBins - 1], n);
+            atomicAdd((unsigned long long*)&weights[kBins - 1], (unsigned long long)far_weight);
         }
         __syncthreads();
         for (int b = tid; b < kBins; b += kSegThreads)
@@ -364,152 +277,292 @@ __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_
                 atomicAdd(&state.count[b], counts[b]);
                 if (weighs && weights[b]) atomicAdd(&state.weight[b], (unsigned long long)weights[b]);
             }
+    } else {
+        float best = 0.f;
+        uint32_t where = 0;
+        float e[PIECES][8];
+        if (draws)
+#pragma unroll
+            for (int a = 0; a < PIECES; ++a) {
+                const int64_t i = first + (a * kSegThreads + tid) * 8;
+                load8<LOGITS_F32>(c.noise, i, piece(i, p.V), 1.f, e[a]);
+            }
+#pragma unroll
+        for (int a = 0; a < PIECES; ++a)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float w = weight(distance(c.row, x[a][j]));
+                total += w;
+                if (draws && w >= c.min_p && w > 0.f)
+                    draw(w, e[a][j], (uint32_t)(first + (a * kSegThreads + tid) * 8 + j), best, where);
+            }
+        if (draws) {
+            const uint64_t key = wave_reduce(draw_key(best, where), larger);
+            if ((tid & 63) == 0 && key) atomicMax(&state.won, (unsigned long long)key);
+        }
+    }
+    const uint64_t sum = wave_reduce(whole(total), plus);
+    if ((tid & 63) == 0) atomicAdd(&state.total, (unsigned long long)sum);
+}
+
+// Where a row's threshold lies, from its histogram: the 32 d from which and before which tokens are candidates for it (those
+// before d_lo are kept), how many the candidates are, the number or weight that is to be reached, and what of it lies before d_lo.
+struct Part {
+    float d_lo, d_hi;
+    uint64_t target, base;
+    uint32_t n;
+};
+
+template <int THREADS>
+__device__ __forceinline__ Part part_of(Scratch<THREADS>& s, const Choice& c, const RowState& state) {
+    constexpr int kEach = kBins / THREADS;
+    uint32_t counts[kEach], n;
+    uint64_t sums[kEach], all = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        counts[j] = state.count[threadIdx.x * kEach + j];
+        sums[j] = c.k > 0 ? counts[j] : state.weight[threadIdx.x * kEach + j];
+        all += sums[j];
+    }
+    Part part;
+    if (c.k > 0) {  // all tokens up to the bin's end (where less than k can be drawn at all, all of those)
+        part.target = (uint64_t)c.k;
+        const uint32_t b = reaching_bin(s, sums, counts, part.target, part.base, n);
+        part.d_lo = 0.f, part.d_hi = end_of_bin(b);
+        if (b == kBins) part.base = block_reduce(s, all, plus), n = 0;
+        part.n = (uint32_t)part.base + n;
+        part.base = 0;
+    } else {
+        part.target = c.want(block_reduce(s, all, plus));
+        const uint32_t b = reaching_bin(s, sums, counts, part.target, part.base, n);
+        part.d_lo = b > 0 ? end_of_bin(b - 1) : 0.f, part.d_hi = end_of_bin(b);
+        part.n = n;
+    }
+    return part;
+}
+
+template <int DT, int PIECES>
+__global__ __launch_bounds__(kSegThreads) void gather_kernel(const logits_sample_args p, int64_t row0, uint32_t segments,
+                                                             RowState* states, uint64_t* lists) {
+    __shared__ Scratch<kSegThreads> s;
+    const int tid = threadIdx.x;
+    const uint32_t at = blockIdx.x / segments;
+    const int64_t first = (int64_t)(blockIdx.x % segments) * (kSegThreads * PIECES * 8);
+    RowState& state = states[at];
+    Choice c = choice_of<DT>(p, row0 + at);
+    if (!c.searches) return;
+    float x[PIECES][8];
+    load_segment<DT, PIECES>(c.row, first, x);
+    const uint64_t max_key = state.max_key;
+    const uint32_t top = ~(uint32_t)max_key;
+    c.row.max = from_order((uint32_t)(max_key >> 32));
+    if (c.row.max == -__builtin_inff()) return;
+    const Part part = part_of(s, c, state);
+    if (part.n > kList) return;  // the choosing workgroup's work
+
+    float nearest[PIECES];  // of each piece
+#pragma unroll
+    for (int a = 0; a < PIECES; ++a) {
+        float m = x[a][0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) m = fmaxf(m, x[a][j]);
+        nearest[a] = distance(c.row, m);
+    }
+    float best = 0.f;
+    uint32_t where = 0, mine = 0;
+    if (c.k <= 0) {  // kept for sure
+        float e[PIECES][8];
+#pragma unroll
+        for (int a = 0; a < PIECES; ++a) {
+            const int64_t i = first + (a * kSegThreads + tid) * 8;
+            load8<LOGITS_F32>(c.noise, i, nearest[a] < part.d_lo ? piece(i, p.V) : 0, 1.f, e[a]);
+        }
+#pragma unroll
+        for (int a = 0; a < PIECES; ++a)
+            if (nearest[a] < part.d_lo)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t i = (uint32_t)(first + (a * kSegThreads + tid) * 8 + j);
+                    const float d = distance(c.row, x[a][j]), w = weight(d);
+                    if (d < part.d_lo && w > 0.f && (w >= c.min_p || i == top)) draw(w, e[a][j], i, best, where);
+                }
+    }
+#pragma unroll
+    for (int a = 0; a < PIECES; ++a)
+        if (nearest[a] < part.d_hi)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float d = distance(c.row, x[a][j]);
+                mine += d >= part.d_lo && d < part.d_hi;
+            }
+    const uint64_t key = wave_reduce(draw_key(best, where), larger);
+    if ((tid & 63) == 0 && key) atomicMax(&state.won, (unsigned long long)key);
+    uint32_t to = (uint32_t)block_before(s, mine);
+    if (tid == kSegThreads - 1) s.n = to + mine ? atomicAdd(&state.gathered, to + mine) : 0;
+    __syncthreads();
+    to += s.n;
+    uint64_t* const list = lists + (int64_t)at * kList;
+#pragma unroll
+    for (int a = 0; a < PIECES; ++a)
+        if (nearest[a] < part.d_hi)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float d = distance(c.row, x[a][j]);
+                if (d >= part.d_lo && d < part.d_hi) {
+                    // as many as were counted, unless someone writes the logits meanwhile
+                    if (to < kList) list[to] = key_of(d, (uint32_t)(first + (a * kSegThreads + tid) * 8 + j));
+                    ++to;
+                }
+            }
+}
+
+struct Shared {
+    uint64_t weight[kBins];
+    uint32_t count[kBins];
+    Scratch<kThreads> scratch;
+};
+
+// f(index, 32 d) for every element of the row; four 8-element pieces in flight to a thread.
+template <int DT, typename F>
+__device__ __forceinline__ void each(const Row& r, F&& f) {
+    constexpr int kAhead = 4;
+    for (int64_t i0 = 8 * (int64_t)threadIdx.x; i0 < r.V; i0 += (int64_t)kAhead * kThreads * 8) {
+        float x[kAhead][8];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const int64_t i = i0 + (int64_t)a * kThreads * 8;
+            load8<DT>(r.x, i, piece(i, r.V), -__builtin_inff(), x[a]);
+        }
+#pragma unroll 1
+        for (int a = 0; a < kAhead; ++a) {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = a == 0 ? x[0][j] : a == 1 ? x[1][j] : a == 2 ? x[2][j] : x[3][j];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                f((uint32_t)(i0 + (int64_t)a * kThreads * 8 + j), distance(r, logit(y[j])));
+        }
     }
 }
 
-// The first bin at whose end the running sum of `mine` reaches `target`, and the sum before it; kBins where none does.
-__device__ __forceinline__ uint32_t reaching_bin(Shared& s, uint64_t mine, uint64_t target, uint64_t& base) {
-    if (threadIdx.x == 0) s.bin = kBins, s.base = 0;
-    const uint64_t before = block_before(s, mine);  // its barriers order the line above
-    if (before < target && before + mine >= target) s.bin = threadIdx.x, s.base = before;
-    __syncthreads();
-    const uint32_t b = s.bin;
-    base = s.base;
-    __syncthreads();
-    return b;
-}
-
-// Keys of d below a bin's end; every finite d for the last bin.
-__device__ __forceinline__ uint64_t end_of_bin(uint32_t b) {
-    return b >= kBins - 1 ? (uint64_t)kInfBits << 32 : (uint64_t)__float_as_uint((float)(b + 1) / kPerUnit) << 32;
-}
-
-constexpr int kOwn = kGather / kThreads;  // entries of the sorted list to a thread
-
-// Draws among what top-k, top-p and min-p keep.  `total`: the row's sum of weights; `top`: its most likely token, which min-p
-// always keeps.  Returns draw_key of the chosen, 0 for none.
-template <int DT>
-__device__ uint64_t draw_kept(Shared& s, const Choice& c, RowState& state, uint64_t total, uint32_t top) {
+// The key of the last token of the smallest prefix, in the order of keys, whose number (COUNT) or weight reaches `target`, among
+// the tokens of `all(f)` (f(key) for each) with keys in [lo, hi), `base` of it lying before lo; `none` where all do not reach it.
+// Parts of keys are cut into 1024 until the part in which the target is reached has one token.
+template <bool COUNT, typename All>
+__device__ uint64_t last_kept(Shared& s, All&& all, uint64_t lo, uint64_t hi, uint64_t base, uint64_t target, uint64_t none) {
     const int tid = threadIdx.x;
-    const Row& r = c.row;
-    const uint32_t count = state.count[tid];
-    const uint64_t weights = state.weight[tid];
+    for (;;) {
+        int shift = 0;
+        while (((hi - lo - 1) >> shift) >= kBins) ++shift;
+        s.count[tid] = 0;
+        s.weight[tid] = 0;
+        __syncthreads();
+        all([&](uint64_t key) {
+            if (key >= lo && key < hi) {
+                const uint32_t b = (uint32_t)((key - lo) >> shift);
+                atomicAdd(&s.count[b], 1u);
+                if (!COUNT) atomicAdd((unsigned long long*)&s.weight[b], (unsigned long long)whole(weight(d_of(key))));
+            }
+        });
+        __syncthreads();
+        const uint32_t counts[1] = {s.count[tid]};
+        const uint64_t sums[1] = {COUNT ? counts[0] : s.weight[tid]};
+        uint64_t before;
+        uint32_t n;
+        const uint32_t b = reaching_bin(s.scratch, sums, counts, target - base, before, n);
+        if (b == kBins) return none;
+        base += before;
+        lo += (uint64_t)b << shift;
+        const uint64_t end = lo + (1ull << shift);
+        hi = end < hi ? end : hi;
+        if (n <= 1 || shift == 0) break;
+    }
+    if (hi - lo == 1) return lo;
+    all([&](uint64_t key) {
+        if (key >= lo && key < hi) s.scratch.found = key;
+    });
+    __syncthreads();
+    const uint64_t found = s.scratch.found;
+    __syncthreads();
+    return found;
+}
+
+constexpr uint64_t kEveryKey = (uint64_t)kInfBits << 32;  // past every token that can be drawn
+
+// The choice in a row with top-k or top-p, as draw_key; `won`: the draw among the tokens that the gathering workgroups kept.
+template <int DT>
+__device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const uint64_t* list, uint32_t top, uint64_t won) {
+    const int tid = threadIdx.x;
+    const Part part = part_of(s.scratch, c, state);
+    const uint32_t n = min(state.gathered, (uint32_t)kList);
+    __syncthreads();
     state.count[tid] = 0;
     state.weight[tid] = 0;
     float best = 0.f;
     uint32_t where = 0;
-    const auto want = [&](uint64_t sum) {  // the weight that a top-p prefix has to reach
-        const double x = (double)c.top_p * (double)sum;
-        return x >= 1.0 ? (uint64_t)ceil(x) : 1;
-    };
 
-    uint64_t base = 0, lo = 0, hi;
-    bool listed = false;  // the list holds every candidate (top-k), not the threshold's bin alone
-    uint32_t n;
-    if (c.k > 0) {
-        const uint32_t b = reaching_bin(s, count, (uint64_t)c.k, base);
-        // fewer than k tokens can be drawn at all: all of them are candidates
-        n = (uint32_t)block_reduce(s, (uint32_t)tid <= b ? count : 0, plus);
-        hi = end_of_bin(b);
-        base = 0;
-        listed = true;
-    } else {
-        const uint32_t b = reaching_bin(s, weights, want(total), base);
-        n = (uint32_t)block_reduce(s, (uint32_t)tid == b ? count : 0, plus);
-        if (b == kBins) n = kGather + 1;  // not reached: only if someone writes the logits meanwhile
-        hi = end_of_bin(b);
-        lo = b > 0 && b < kBins ? end_of_bin(b - 1) : 0;
-    }
-
-    if (n > kGather) {  // the long way
-        uint64_t limit = ((uint64_t)kInfBits << 32) - 1;
-        if (c.k > 0) limit = last_kept<DT, true>(s, r, limit, (uint64_t)c.k);
+    if (part.n > kList) {  // the long way
+        uint64_t limit = kEveryKey - 1;
+        const auto all = [&](auto&& f) {
+            each<DT>(c.row, [&](uint32_t i, float d) {
+                const uint64_t key = key_of(d, i);
+                if (key <= limit) f(key);
+            });
+        };
+        if (c.k > 0) limit = last_kept<true>(s, all, 0, kEveryKey, 0, (uint64_t)c.k, limit);
         if (c.top_p < 1.f) {
             uint64_t sum = 0;
-            each<DT>(r, [&](uint32_t i, float x) {
-                const float d = distance(r, x);
-                if (key_of(d, i) <= limit) sum += whole(weight(d));
-            });
-            limit = last_kept<DT, false>(s, r, limit, want(block_reduce(s, sum, plus)));
+            all([&](uint64_t key) { sum += whole(weight(d_of(key))); });
+            limit = last_kept<false>(s, all, 0, kEveryKey, 0, c.want(block_reduce(s.scratch, sum, plus)), limit);
         }
-        each<DT>(r, [&](uint32_t i, float x) {
-            const float d = distance(r, x), w = weight(d);
-            if (key_of(d, i) <= limit && w > 0.f && (w >= c.min_p || i == top)) draw(w, c.noise[i], i, best, where);
+        all([&](uint64_t key) {
+            const float w = weight(d_of(key));
+            const uint32_t i = (uint32_t)key;
+            if (w > 0.f && (w >= c.min_p || i == top)) draw(w, c.noise[i], i, best, where);
         });
-        return block_reduce(s, draw_key(best, where), larger);
+        return block_reduce(s.scratch, draw_key(best, where), larger);
     }
 
-    if (tid == 0) s.gathered = 0;
-    __syncthreads();
-    const float d_lo = d_of(lo), d_hi = d_of(hi);  // whole bins: d alone decides
-    for (int64_t i0 = 8 * (int64_t)tid; i0 < r.V; i0 += 4 * (int64_t)kThreads * 8) {
-        float x[4][8], e[4][8];
+    uint64_t key[kOwn];
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            const int64_t i = i0 + (int64_t)a * kThreads * 8;
-            load8<DT>(r.x, i, i >= r.V ? 0 : r.V - i < 8 ? (int)(r.V - i) : 8, -__builtin_inff(), x[a]);
+    for (int j = 0; j < kOwn; ++j) key[j] = tid + j * kThreads < n ? list[tid + j * kThreads] : ~0ull;
+    float noise[kOwn];  // of all candidates, asked for before it is known which are kept
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) noise[j] = key[j] != ~0ull ? c.noise[min((uint32_t)key[j], (uint32_t)c.row.V - 1)] : 1.f;
+    uint64_t limit = kEveryKey - 1;
+    const auto all = [&](auto&& f) {
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j)
+            if (key[j] <= limit) f(key[j]);
+    };
+    const uint64_t lo = (uint64_t)__float_as_uint(part.d_lo) << 32, hi = (uint64_t)__float_as_uint(part.d_hi) << 32;
+    if (c.k > 0) {
+        if (n > (uint32_t)c.k) limit = last_kept<true>(s, all, lo, hi, 0, (uint64_t)c.k, limit);
+        if (c.top_p < 1.f) {
+            uint64_t sum = 0;
+            all([&](uint64_t k) { sum += whole(weight(d_of(k))); });
+            limit = last_kept<false>(s, all, lo, hi, 0, c.want(block_reduce(s.scratch, sum, plus)), limit);
         }
-        bool any[4];
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            float m = x[a][0];
-#pragma unroll
-            for (int j = 1; j < 8; ++j) m = fmaxf(m, x[a][j]);
-            const float d = distance(r, m);
-            any[a] = d < d_hi;
-            load_noise(c.noise, i0 + (int64_t)a * kThreads * 8, r.V, d < d_lo, e[a]);
-        }
-#pragma unroll
-        for (int a = 0; a < 4; ++a)
-            if (any[a])
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t i = (uint32_t)(i0 + (int64_t)a * kThreads * 8 + j);
-                    const float v = x[a][j];
-                    const float d = v == v ? distance(r, v) : __builtin_inff();
-                    if (d < d_lo) {
-                        const float w = weight(d);
-                        if (w > 0.f && (w >= c.min_p || i == top)) draw(w, e[a][j], i, best, where);
-                    } else if (d < d_hi) {
-                        const uint32_t g = atomicAdd(&s.gathered, 1u);
-                        if (g < kGather) s.list[g] = key_of(d, i);  // as many as were counted, unless someone writes the logits
-                    }
-                }
+    } else {
+        limit = last_kept<false>(s, all, lo, hi, part.base, part.target, limit);
     }
-    __syncthreads();
-    n = min(s.gathered, (uint32_t)kGather);
-    sort_list(s, n);
-    if (listed) n = min(n, (uint32_t)c.k);
-    uint64_t key[kOwn], w[kOwn], sum = 0;
 #pragma unroll
-    for (int j = 0; j < kOwn; ++j) {
-        const uint32_t e = tid * kOwn + j;
-        key[j] = e < n ? s.list[e] : ~0ull;
-        w[j] = e < n ? whole(weight(d_of(key[j]))) : 0;
-        sum += w[j];
-    }
-    uint64_t target = ~0ull;
-    if (c.top_p < 1.f) target = want(listed ? block_reduce(s, sum, plus) : total);
-    uint64_t before = base + block_before(s, sum);
-#pragma unroll
-    for (int j = 0; j < kOwn; ++j) {
-        if (key[j] != ~0ull && before < target) {
-            const float x = weight(d_of(key[j]));
+    for (int j = 0; j < kOwn; ++j)
+        if (key[j] <= limit) {
+            const float w = weight(d_of(key[j]));
             const uint32_t i = (uint32_t)key[j];
-            if (x > 0.f && (x >= c.min_p || i == top)) {
-                const float score = x / c.noise[i];  // in the list's order: of equals the lowest index
+            if (w > 0.f && (w >= c.min_p || i == top)) {
+                const float score = w * __builtin_amdgcn_rcpf(noise[j]);
                 if (score > best || (score == best && score > 0.f && i < where)) best = score, where = i;
             }
         }
-        before += w[j];
-    }
-    return block_reduce(s, draw_key(best, where), larger);
+    return larger(won, block_reduce(s.scratch, draw_key(best, where), larger));
 }
 
 template <int DT>
-__global__ __launch_bounds__(kThreads) void choose_kernel(const logits_sample_args p, int64_t row0, RowState* states) {
+__global__ __launch_bounds__(kThreads) void choose_kernel(const logits_sample_args p, int64_t row0, RowState* states,
+                                                          const uint64_t* lists) {
     __shared__ Shared s;
-    const int tid = threadIdx.x;
     const int64_t row = row0 + blockIdx.x;
     RowState& state = states[blockIdx.x];
     Choice c = choice_of<DT>(p, row);
@@ -518,16 +571,18 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(const logits_sample_ar
     uint32_t token = ~(uint32_t)max_key;
     c.row.max = from_order((uint32_t)(max_key >> 32));
     const bool none = c.row.max == -__builtin_inff();  // nothing is allowed
-    if (c.searches && !none) won = draw_kept<DT>(s, c, state, total, token);
+    if (c.searches && !none) won = choose<DT>(s, c, state, lists + (int64_t)blockIdx.x * kList, token, won);
     if (won) token = ~(uint32_t)won;  // else greedy, or no noise was a number: the most likely token
     __syncthreads();
-    if (tid == 0) {
+    if (threadIdx.x == 0) {
         state.max_key = state.total = state.won = 0;
+        state.gathered = 0;
         p.token[row] = none ? -1 : (int64_t)token;
         if (p.logprob) {
             float x[8];
-            load8<DT>(c.row.x, token, 1, 0.f, x);
-            p.logprob[row] = none ? c.row.max : -distance(c.row, x[0]) - logf((float)total * (1.f / kOne));
+            load8<DT>(c.row.x, none ? 0 : token, 1, 0.f, x);
+            p.logprob[row] =
+                none ? c.row.max : -distance(c.row, logit(x[0])) * (1.f / kPerUnit) - logf((float)total * (1.f / kOne));
         }
         if (p.counts && !none) {
             const int64_t slot = p.slots ? p.slots[c.b] : c.b;
@@ -542,20 +597,32 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(const logits_sample_ar
     }
 }
 
-template <int DT>
+template <int DT, int PIECES>
 hipError_t launch(const logits_sample_args& a, hipStream_t s) {
-    const int64_t rows = (int64_t)a.B * a.T;
-    const uint32_t segments = (uint32_t)(((int64_t)a.V + kSegment - 1) / kSegment);
+    constexpr int kSegment = kSegThreads * PIECES * 8;
+    const int64_t rows = (int64_t)a.B * a.T, segments = ((int64_t)a.V + kSegment - 1) / kSegment;
     RowState* const states = static_cast<RowState*>(a.workspace);
-    for (int64_t row0 = 0; row0 < rows; row0 += kRowsAtOnce) {
-        const uint32_t n = (uint32_t)(rows - row0 < kRowsAtOnce ? rows - row0 : kRowsAtOnce);
-        hipLaunchKernelGGL((max_kernel<DT>), dim3(n * segments), dim3(kSegThreads), 0, s, a, row0, segments, states);
-        hipLaunchKernelGGL((weigh_kernel<DT>), dim3(n * segments), dim3(kSegThreads), 0, s, a, row0, segments, states);
-        hipLaunchKernelGGL((choose_kernel<DT>), dim3(n), dim3(kThreads), 0, s, a, row0, states);
+    uint64_t* const lists = reinterpret_cast<uint64_t*>(static_cast<char*>(a.workspace) + LOGITS_SAMPLE_STATE_BYTES);
+    const int64_t at_once = std::min<int64_t>(kRowsAtOnce, 0xFFFFFF / segments);  // 256 threads each: below 2^32 work-items
+    for (int64_t row0 = 0; row0 < rows; row0 += at_once) {
+        const int64_t n = std::min(rows - row0, at_once);
+        const dim3 grid((unsigned)(n * segments)), block(kSegThreads);
+        const uint32_t seg = (uint32_t)segments;
+        hipLaunchKernelGGL((max_kernel<DT, PIECES>), grid, block, 0, s, a, row0, seg, states);
+        hipLaunchKernelGGL((weigh_kernel<DT, PIECES>), grid, block, 0, s, a, row0, seg, states);
+        hipLaunchKernelGGL((gather_kernel<DT, PIECES>), grid, block, 0, s, a, row0, seg, states, lists);
+        hipLaunchKernelGGL((choose_kernel<DT>), dim3((unsigned)n), dim3(kThreads), 0, s, a, row0, states, lists);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
+}
+
+// Short segments while long ones would leave CUs without two workgroups.
+template <int DT>
+hipError_t launch(const logits_sample_args& a, hipStream_t s) {
+    const int64_t long_ones = (int64_t)a.B * a.T * (((int64_t)a.V + 8191) / 8192);
+    return long_ones < 2 * wkv7::device_cu_count() ? launch<DT, 1>(a, s) : launch<DT, 4>(a, s);
 }
 
 bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -570,8 +637,8 @@ size_t logits_sample_args_size(void) { return sizeof(logits_sample_args); }
 int logits_sample_workspace_size(const logits_sample_args* a, size_t* bytes) {
     if (!a || !bytes) return WKV7_ERR_NULL;
     if (a->B < 0 || a->T < 0 || a->V < 1) return WKV7_ERR_SHAPE;
-    const int64_t rows = (int64_t)a->B * a->T;
-    *bytes = sizeof(lg::RowState) * (size_t)(rows < lg::kRowsAtOnce ? rows : lg::kRowsAtOnce);
+    const int64_t rows = std::min<int64_t>((int64_t)a->B * a->T, lg::kRowsAtOnce);
+    *bytes = LOGITS_SAMPLE_STATE_BYTES + (size_t)rows * lg::kList * sizeof(uint64_t);
     return WKV7_OK;
 }
 
@@ -584,13 +651,13 @@ int logits_sample(const logits_sample_args* a, void* stream) {
     if (a->B == 0 || a->T == 0) return WKV7_OK;
     if (!a->logits || !a->token) return WKV7_ERR_NULL;
     if (a->counts && (a->counts_rows < 0 || a->counts_stride < a->V)) return WKV7_ERR_SHAPE;
-    if (!lg::aligned(a->logits, lg::element_bytes(a->dtype)) || !lg::aligned(a->noise, 4) || !lg::aligned(a->counts, 4))
+    if (!lg::aligned(a->logits, lg::element_bytes(a->dtype)) || !lg::aligned(a->noise, 4) || !lg::aligned(a->counts, 4) ||
+        !lg::aligned(a->workspace, 256))
         return WKV7_ERR_ALIGN;
     size_t bytes = 0;
     const int rc = logits_sample_workspace_size(a, &bytes);
     if (rc != WKV7_OK) return rc;
     if (!a->workspace || a->workspace_bytes < bytes) return WKV7_ERR_WORKSPACE;
-    if (!lg::aligned(a->workspace, 256)) return WKV7_ERR_ALIGN;
     const auto s = static_cast<hipStream_t>(stream);
     if (a->dtype == LOGITS_BF16) return static_cast<int>(lg::launch<LOGITS_BF16>(*a, s));
     if (a->dtype == LOGITS_F16) return static_cast<int>(lg::launch<LOGITS_F16>(*a, s));

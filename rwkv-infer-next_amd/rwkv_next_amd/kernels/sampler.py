@@ -204,15 +204,14 @@ _BYTES: dict = {}       # rows -> bytes of workspace
 
 
 def _workspace(rows, V, dev):
-    """The zeroed workspace of the current stream (include/logits.h, logits_sample_workspace_size).  Every byte that a call
-    uses has to be zero, so the buffer is asked for twice: a larger call does not find room that was never cleared."""
+    """The workspace of the current stream (include/logits.h, logits_sample_workspace_size); see
+    `_workspace.stream_workspace`."""
     n = _BYTES.get(rows)
     if n is None:
         size = ctypes.c_size_t(0)
         _lib.check(_lib.load().logits_sample_workspace_size(_lib.SampleArgs(B=rows, T=1, V=V), ctypes.byref(size)))
         n = _BYTES[rows] = int(size.value)
-    with on_device(dev):
-        return stream_workspace(_WORKSPACES, dev, 2 * n, n)
+    return stream_workspace(_WORKSPACES, dev, n, _lib.LOGITS_SAMPLE_STATE_BYTES)
 
 
 def sample_logits(logits, noise=None, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, counts=None, slots=None,
@@ -257,7 +256,8 @@ def sample_logits(logits, noise=None, *, temperature=1.0, top_k=0, top_p=1.0, mi
     ct, ct_stride, ct_rows, ct_type, slots_p = _counts(counts, slots, B, V, dev)
     if not (B and T):
         return token, logprob
-    ws = _workspace(B * T, V, dev)
+    with on_device(dev):
+        ws = _workspace(B * T, V, dev)
     args = _lib.SampleArgs(
         logits.data_ptr(), seq_stride, pos_stride, nz, nz_seq or 0, nz_pos or 0, t_p, k_p, p_p, m_p, token.data_ptr(),
         logprob.data_ptr(), ct, ct_stride, ct_rows, slots_p, _status(status, dev),
