@@ -71,7 +71,9 @@ typedef struct logits_penalize_args {
  * largest logit's lowest index.  NaN counts as -infinity, and tokens of -infinity are never chosen: a row of nothing else gives
  * -1 and a log-probability of -infinity.
  * logprob = -d - log(sum of w over the row), before the filters, with a temperature of 1 in greedy rows.
- * Sums that decide which tokens are kept are exact sums of whole numbers of 2^-40: no order of atomics changes a result. */
+ * What is added up by atomics are whole numbers (of 2^-20 of a bin's weights, of 2^-40): their order changes no result.
+ * V is at most LOGITS_SAMPLE_MAX_V. */
+#define LOGITS_SAMPLE_MAX_V 2097152
 typedef struct logits_sample_args {
     const void *logits;                      /* [B][T][V] */
     int64_t seq_stride, pos_stride;          /* elements */
@@ -101,7 +103,7 @@ size_t logits_sample_args_size(void);
 /* Bytes of workspace that logits_sample needs, 256-byte aligned.  The first LOGITS_SAMPLE_STATE_BYTES must be zero before the
  * workspace's first use; every completed call leaves them zero and writes nothing else into them, so one workspace serves any
  * number of calls of any shapes one after another (stream order).  Calls that can run at the same time need different ones. */
-#define LOGITS_SAMPLE_STATE_BYTES 6422528
+#define LOGITS_SAMPLE_STATE_BYTES 4325376
 int logits_sample_workspace_size(const logits_sample_args *args, size_t *bytes);
 
 int logits_penalize(const logits_penalize_args *args, void *stream);

@@ -1,18 +1,20 @@
 // logits_sample.hip -- the choice of a token from each row of logits (include/logits.h), in four launches:
 //
 //   max     a row's segments, a workgroup each: the row's maximum and its lowest index
-//   weigh   the same segments: with d = (max - x) / T, w = exp(-d) the sum of w; in rows without top-k and top-p the draw among
-//           their elements; in the others a histogram over d in steps of 1/32, of the tokens' number and of their weights
+//   weigh   the same segments: with d = (max - x) / T, w = exp(-d), in rows without top-k and top-p the sum of w and the draw
+//           among their elements; in the others a histogram over d in steps of 1/32, of the tokens' number and of their weights
 //   gather  the same segments: where the histogram reaches the wanted number or weight, the last kept token is in that bin.  The
 //           tokens before it are kept, and drawn among; the bin's own (top-k: all up to its end) go into the row's list
 //   choose  a workgroup a row: the last kept token of the list, by histograms over ever finer parts of (d, index), and the draw
 //
 // A row's maximum must be known before its weights, its weights before a threshold, and the threshold before the draw: hence the
-// launches; no row and no list is sorted.  Sums that decide are of whole numbers of 2^-40: no order of the atomics shows in a
-// result.  A bin of more tokens than the list holds (equal logits, a top-k of thousands) goes the long way: its row's workgroup
-// cuts the row itself into finer parts.
+// launches; no row and no list is sorted.  What atomics add up are whole numbers, so their order shows in no result.  A bin of
+// more tokens than the list holds (equal logits, a top-k of thousands) goes the long way: its row's workgroup cuts the row itself
+// into finer parts.
 //
-// d is kept as 32 d (bins are its whole part), which the scaling by a power of two leaves as exact as d.
+// d is kept as 32 d (bins are its whole part), which the scaling by a power of two leaves as exact as d.  A bin's weights are
+// added up as whole numbers of 2^-20 of the weight at its start, beside its tokens' number in one 64-bit word: one atomic to a
+// token.  Vector instructions bound the segments' kernels, not memory.
 #include <hip/hip_runtime.h>
 #include <float.h>
 #include <stdint.h>
@@ -26,7 +28,7 @@
 namespace lg {
 namespace {
 
-constexpr int kThreads = 1024;     // of the choosing workgroup, one per bin
+constexpr int kThreads = 512;      // of the choosing workgroup
 constexpr int kSegThreads = 256;   // of a segment's workgroup: 8 elements, or 4 x 8, to a thread
 constexpr int kBins = 1024;        // the last one holds all from 1023/32 on
 constexpr float kPerUnit = 32.f;   // bins to a unit of d
@@ -36,6 +38,9 @@ constexpr int kRowsAtOnce = 512;   // rows of one set of launches
 constexpr float kOne = 1099511627776.f;  // 2^40: a weight of 1
 constexpr uint32_t kInfBits = 0x7F800000u;
 constexpr float kExp2PerBin = -1.44269504088896341f / kPerUnit;  // w = 2^(32 d * this)
+// A bin's word: its tokens' number above their weights, each below 2^20 + 1 times the bin's first: 2^21 tokens at most.
+constexpr int kWeightBits = 20, kCountAt = 42;
+static_assert(LOGITS_SAMPLE_MAX_V == 1 << 21 && kCountAt > kWeightBits + 21 && kCountAt + 22 <= 64, "");
 
 // A row's part of the workspace: all zero between calls.  The rows' lists, which need not be, follow the kRowsAtOnce of them.
 struct RowState {
@@ -44,8 +49,7 @@ struct RowState {
     unsigned long long won;      // the draw so far: w / noise as an integer << 32 | ~index
     uint32_t gathered;           // entries of the list
     uint32_t unused[57];
-    unsigned long long weight[kBins];
-    uint32_t count[kBins];
+    unsigned long long bins[kBins];
 };
 static_assert(sizeof(RowState) * kRowsAtOnce == LOGITS_SAMPLE_STATE_BYTES, "include/logits.h");
 
@@ -80,43 +84,50 @@ __device__ __forceinline__ uint64_t block_reduce(Scratch<THREADS>& s, uint64_t x
     return x;
 }
 
-// The sum over the threads before this one.
-template <int THREADS>
-__device__ __forceinline__ uint64_t block_before(Scratch<THREADS>& s, uint64_t x) {
+// The sum over the threads before this one, always added in the same order.
+template <int THREADS, typename T>
+__device__ __forceinline__ T block_before(Scratch<THREADS>& s, T x) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint64_t sum = x;
+    T sum = x;
     for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t y = shuffle(sum, (lane - o) & 63);
+        const T y = __builtin_bit_cast(T, shuffle(__builtin_bit_cast(uint64_t, sum), (lane - o) & 63));
         if (lane >= o) sum += y;
     }
+    T before = __builtin_bit_cast(T, shuffle(__builtin_bit_cast(uint64_t, sum), (lane - 1) & 63));
+    if (lane == 0) before = T(0);
     __syncthreads();
-    if (lane == 63) s.wave[wave] = sum;
+    if (lane == 63) s.wave[wave] = __builtin_bit_cast(uint64_t, sum);
     __syncthreads();
-    uint64_t before = sum - x;
-    for (int w = 0; w < wave; ++w) before += s.wave[w];
-    return before;
+    T others = T(0);
+    for (int w = 0; w < wave; ++w) others += __builtin_bit_cast(T, s.wave[w]);
+    return others + before;
 }
 
-// The first bin at whose end the running sum reaches `target`, the sum before it and the tokens in it; kBins where none does.  A
-// thread has kBins / THREADS bins: their sums and numbers.
-template <int THREADS>
-__device__ __forceinline__ uint32_t reaching_bin(Scratch<THREADS>& s, const uint64_t (&sums)[kBins / THREADS],
-                                                 const uint32_t (&counts)[kBins / THREADS], uint64_t target, uint64_t& base,
-                                                 uint32_t& n) {
+// The first of kBins bins at whose end the running sum reaches `target`, with the sum before it (s.base) and its `counts` (s.n);
+// kBins where none does.  A thread has kBins / THREADS of them.
+template <int THREADS, typename T>
+__device__ __forceinline__ uint32_t reaching_bin(Scratch<THREADS>& s, const T (&sums)[kBins / THREADS],
+                                                 const uint32_t (&counts)[kBins / THREADS], T target, T& base, uint32_t& n) {
     if (threadIdx.x == 0) s.bin = kBins, s.base = 0, s.n = 0;
-    uint64_t mine = 0;
+    T mine = sums[0];
 #pragma unroll
-    for (int j = 0; j < kBins / THREADS; ++j) mine += sums[j];
-    uint64_t before = block_before(s, mine);  // its barriers order the first line
+    for (int j = 1; j < kBins / THREADS; ++j) mine += sums[j];
+    T before = block_before(s, mine);  // its barriers order the first line
 #pragma unroll
     for (int j = 0; j < kBins / THREADS; ++j) {
-        if (before < target && before + sums[j] >= target)
-            s.bin = threadIdx.x * (kBins / THREADS) + j, s.base = before, s.n = counts[j];
+        // sums before two neighbours may be rounded apart in floating point: the lowest bin of those that fit
+        if (before < target && before + sums[j] >= target) atomicMin(&s.bin, threadIdx.x * (kBins / THREADS) + j);
         before += sums[j];
     }
     __syncthreads();
     const uint32_t b = s.bin;
-    base = s.base, n = s.n;
+#pragma unroll
+    for (int j = kBins / THREADS - 1; j >= 0; --j) {
+        before -= sums[j];
+        if (b == threadIdx.x * (kBins / THREADS) + j) s.base = __builtin_bit_cast(uint64_t, before), s.n = counts[j];
+    }
+    __syncthreads();
+    base = __builtin_bit_cast(T, s.base), n = s.n;
     __syncthreads();
     return b;
 }
@@ -141,6 +152,11 @@ __device__ __forceinline__ float from_order(uint32_t u) { return __uint_as_float
 __device__ __forceinline__ float distance(const Row& r, float x) { return (r.max - x) * r.inv; }  // 32 d >= 0
 __device__ __forceinline__ float weight(float d32) { return __builtin_amdgcn_exp2f(d32 * kExp2PerBin); }
 __device__ __forceinline__ uint64_t whole(float w) { return (uint64_t)(w * kOne); }
+// A weight in its bin's units, and the unit.
+__device__ __forceinline__ uint32_t in_bin(float d32) {
+    return (uint32_t)__builtin_amdgcn_exp2f(fmaf(__builtin_amdgcn_fractf(d32), kExp2PerBin, (float)kWeightBits));
+}
+__device__ __forceinline__ double unit_of_bin(uint32_t b) { return (double)weight((float)b) * (1.0 / (1 << kWeightBits)); }
 // The first 32 d past a bin; every finite one lies before the last bin's.
 __device__ __forceinline__ float end_of_bin(uint32_t b) { return b >= kBins - 1 ? __builtin_inff() : (float)(b + 1); }
 
@@ -155,7 +171,7 @@ struct Choice {
     int k;                  // 0: no top-k
     float top_p, min_p;
     bool greedy, searches;  // searches: top-k or top-p
-    __device__ uint64_t want(uint64_t sum) const {  // the weight that a top-p prefix has to reach
+    __device__ uint64_t want(uint64_t sum) const {  // the weight that a top-p prefix has to reach, of whole()s
         const double x = (double)top_p * (double)sum;
         return x >= 1.0 ? (uint64_t)ceil(x) : 1;
     }
@@ -232,8 +248,7 @@ __device__ __forceinline__ uint64_t draw_key(float best, uint32_t where) {  // 0
 template <int DT, int PIECES>
 __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_args p, int64_t row0, uint32_t segments,
                                                             RowState* states) {
-    __shared__ uint64_t weights[kBins];
-    __shared__ uint32_t counts[kBins];
+    __shared__ uint64_t bins[kBins];
     const int tid = threadIdx.x;
     const uint32_t at = blockIdx.x / segments;
     const int64_t first = (int64_t)(blockIdx.x % segments) * (kSegThreads * PIECES * 8);
@@ -243,42 +258,28 @@ __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_
     load_segment<DT, PIECES>(c.row, first, x);
     c.row.max = from_order((uint32_t)(state.max_key >> 32));
     if (c.row.max == -__builtin_inff()) return;
-    const bool draws = !c.greedy && !c.searches, weighs = c.top_p < 1.f;
-    float total = 0.f;
     if (c.searches) {
-        for (int b = tid; b < kBins; b += kSegThreads) weights[b] = 0, counts[b] = 0;
+        for (int b = tid; b < kBins; b += kSegThreads) bins[b] = 0;
         __syncthreads();
-        uint64_t far_weight = 0;  // a long tail's tokens all fall into the last bin: added up in registers
-        uint32_t far = 0;
+        uint32_t far = 0;  // a long tail's tokens all fall into the last bin: counted in registers, their weights (e^-32) left out
 #pragma unroll
         for (int a = 0; a < PIECES; ++a)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float d = distance(c.row, x[a][j]), w = weight(d);
-                total += w;
-                if (d >= (float)(kBins - 1)) {
+                const float d = distance(c.row, x[a][j]);
+                if (d < (float)(kBins - 1))
+                    atomicAdd((unsigned long long*)&bins[(uint32_t)fmaxf(d, 0.f)], 1ull << kCountAt | in_bin(d));
+                else
                     far += d < __builtin_inff();
-                    far_weight += whole(w);
-                } else {
-                    const uint32_t b = (uint32_t)fmaxf(d, 0.f);
-                    atomicAdd(&counts[b], 1u);
-                    if (weighs) atomicAdd((unsigned long long*)&weights[b], (unsigned long long)whole(w));
-                }
             }
-        far_weight = wave_reduce(far_weight, plus);
-        const uint32_t n = (uint32_t)wave_reduce((uint64_t)far, plus);
-        if ((tid & 63) == 0 && n) {
-            atomicAdd(&counts[kBins - 1], n);
-            atomicAdd((unsigned long long*)&weights[kBins - 1], (unsigned long long)far_weight);
-        }
+        far = (uint32_t)wave_reduce((uint64_t)far, plus);
+        if ((tid & 63) == 0 && far) atomicAdd((unsigned long long*)&bins[kBins - 1], (unsigned long long)far << kCountAt);
         __syncthreads();
         for (int b = tid; b < kBins; b += kSegThreads)
-            if (counts[b]) {
-                atomicAdd(&state.count[b], counts[b]);
-                if (weighs && weights[b]) atomicAdd(&state.weight[b], (unsigned long long)weights[b]);
-            }
+            if (bins[b]) atomicAdd(&state.bins[b], (unsigned long long)bins[b]);
     } else {
-        float best = 0.f;
+        const bool draws = !c.greedy;
+        float total = 0.f, best = 0.f;
         uint32_t where = 0;
         float e[PIECES][8];
         if (draws)
@@ -300,43 +301,63 @@ __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_
             const uint64_t key = wave_reduce(draw_key(best, where), larger);
             if ((tid & 63) == 0 && key) atomicMax(&state.won, (unsigned long long)key);
         }
+        const uint64_t sum = wave_reduce(whole(total), plus);
+        if ((tid & 63) == 0) atomicAdd(&state.total, (unsigned long long)sum);
     }
-    const uint64_t sum = wave_reduce(whole(total), plus);
-    if ((tid & 63) == 0) atomicAdd(&state.total, (unsigned long long)sum);
 }
 
-// Where a row's threshold lies, from its histogram: the 32 d from which and before which tokens are candidates for it (those
-// before d_lo are kept), how many the candidates are, the number or weight that is to be reached, and what of it lies before d_lo.
+// Where a row's last kept token lies, from its histogram: in bin [from, to) of 32 d, where the prefix that ends with it has to
+// reach `target` tokens (top-k) or units of the bin (top-p) beside what lies before the bin.  The candidates' list begins at d_lo:
+// with top-k at 0, since top-p looks at them all again; with top-p alone at the bin, what lies before it being kept.
 struct Part {
-    float d_lo, d_hi;
-    uint64_t target, base;
-    uint32_t n;
+    float d_lo, from, to;
+    uint64_t target;
+    uint32_t n;    // candidates
+    double total;  // of the row's weights
 };
 
 template <int THREADS>
-__device__ __forceinline__ Part part_of(Scratch<THREADS>& s, const Choice& c, const RowState& state) {
+__device__ __forceinline__ Part part_of(Scratch<THREADS>& s, const Choice& c, const RowState& state, bool wants_total) {
     constexpr int kEach = kBins / THREADS;
     uint32_t counts[kEach], n;
-    uint64_t sums[kEach], all = 0;
+    uint64_t numbers[kEach];
+    double sums[kEach], all = 0;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-        counts[j] = state.count[threadIdx.x * kEach + j];
-        sums[j] = c.k > 0 ? counts[j] : state.weight[threadIdx.x * kEach + j];
+        const uint32_t b = threadIdx.x * kEach + j;
+        const uint64_t word = state.bins[b];
+        numbers[j] = counts[j] = (uint32_t)(word >> kCountAt);
+        sums[j] = (double)(word & ((1ull << kCountAt) - 1)) * unit_of_bin(b);
         all += sums[j];
     }
     Part part;
-    if (c.k > 0) {  // all tokens up to the bin's end (where less than k can be drawn at all, all of those)
-        part.target = (uint64_t)c.k;
-        const uint32_t b = reaching_bin(s, sums, counts, part.target, part.base, n);
-        part.d_lo = 0.f, part.d_hi = end_of_bin(b);
-        if (b == kBins) part.base = block_reduce(s, all, plus), n = 0;
-        part.n = (uint32_t)part.base + n;
-        part.base = 0;
+    part.total = 0;
+    if (c.k <= 0 || wants_total) {  // the last thread's sum before it and its own are the row's
+        const double before = block_before(s, all);
+        if (threadIdx.x == THREADS - 1) s.base = __builtin_bit_cast(uint64_t, before + all);
+        __syncthreads();
+        part.total = __builtin_bit_cast(double, s.base);
+        __syncthreads();
+    }
+    if (c.k > 0) {
+        uint64_t base;
+        const uint32_t b = reaching_bin(s, numbers, counts, (uint64_t)c.k, base, n);
+        if (b == kBins) {  // less than k tokens can be drawn at all: all of them are candidates
+            uint64_t mine = 0;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) mine += numbers[j];
+            base = block_reduce(s, mine, plus);
+        }
+        part.from = b > 0 ? end_of_bin(b - 1) : 0.f, part.to = end_of_bin(b), part.d_lo = 0.f;
+        part.target = (uint64_t)c.k - (b == kBins ? 0 : base);
+        part.n = (uint32_t)base + n;
     } else {
-        part.target = c.want(block_reduce(s, all, plus));
-        const uint32_t b = reaching_bin(s, sums, counts, part.target, part.base, n);
-        part.d_lo = b > 0 ? end_of_bin(b - 1) : 0.f, part.d_hi = end_of_bin(b);
-        part.n = n;
+        double base;
+        const uint32_t b = reaching_bin(s, sums, counts, fmax((double)c.top_p * part.total, 1e-300), base, n);
+        part.from = b > 0 ? end_of_bin(b - 1) : 0.f, part.to = end_of_bin(b), part.d_lo = part.from;
+        const double rest = ceil(((double)c.top_p * part.total - base) / unit_of_bin(b));
+        part.target = rest >= 1.0 ? (uint64_t)rest : 1;
+        part.n = b == kBins ? kList + 1 : n;  // past all bins only if someone writes the logits meanwhile
     }
     return part;
 }
@@ -357,20 +378,21 @@ __global__ __launch_bounds__(kSegThreads) void gather_kernel(const logits_sample
     const uint32_t top = ~(uint32_t)max_key;
     c.row.max = from_order((uint32_t)(max_key >> 32));
     if (c.row.max == -__builtin_inff()) return;
-    const Part part = part_of(s, c, state);
+    const Part part = part_of(s, c, state, false);
     if (part.n > kList) return;  // the choosing workgroup's work
 
-    float nearest[PIECES];  // of each piece
+    float nearest[PIECES];  // x becomes 32 d, nearest a piece's smallest
 #pragma unroll
     for (int a = 0; a < PIECES; ++a) {
-        float m = x[a][0];
 #pragma unroll
-        for (int j = 1; j < 8; ++j) m = fmaxf(m, x[a][j]);
-        nearest[a] = distance(c.row, m);
+        for (int j = 0; j < 8; ++j) x[a][j] = distance(c.row, x[a][j]);
+        nearest[a] = x[a][0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) nearest[a] = fminf(nearest[a], x[a][j]);
     }
     float best = 0.f;
-    uint32_t where = 0, mine = 0;
-    if (c.k <= 0) {  // kept for sure
+    uint32_t where = 0;
+    if (part.d_lo > 0.f) {  // kept for sure
         float e[PIECES][8];
 #pragma unroll
         for (int a = 0; a < PIECES; ++a) {
@@ -383,37 +405,35 @@ __global__ __launch_bounds__(kSegThreads) void gather_kernel(const logits_sample
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const uint32_t i = (uint32_t)(first + (a * kSegThreads + tid) * 8 + j);
-                    const float d = distance(c.row, x[a][j]), w = weight(d);
-                    if (d < part.d_lo && w > 0.f && (w >= c.min_p || i == top)) draw(w, e[a][j], i, best, where);
+                    const float w = weight(x[a][j]);
+                    if (x[a][j] < part.d_lo && w > 0.f && (w >= c.min_p || i == top)) draw(w, e[a][j], i, best, where);
                 }
+        const uint64_t key = wave_reduce(draw_key(best, where), larger);
+        if ((tid & 63) == 0 && key) atomicMax(&state.won, (unsigned long long)key);
     }
+    // bits of non-negative floats order as they do
+    const uint32_t from = __float_as_uint(part.d_lo), span = __float_as_uint(part.to) - from;
+    uint32_t hits = 0;  // a bit for each of the 8 PIECES elements, the first the highest
 #pragma unroll
     for (int a = 0; a < PIECES; ++a)
-        if (nearest[a] < part.d_hi)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float d = distance(c.row, x[a][j]);
-                mine += d >= part.d_lo && d < part.d_hi;
-            }
-    const uint64_t key = wave_reduce(draw_key(best, where), larger);
-    if ((tid & 63) == 0 && key) atomicMax(&state.won, (unsigned long long)key);
-    uint32_t to = (uint32_t)block_before(s, mine);
+        for (int j = 0; j < 8; ++j) hits = hits + hits + (__float_as_uint(x[a][j]) - from < span);
+    const uint32_t mine = __popc(hits);
+    uint32_t to = (uint32_t)block_before(s, (uint64_t)mine);
     if (tid == kSegThreads - 1) s.n = to + mine ? atomicAdd(&state.gathered, to + mine) : 0;
     __syncthreads();
     to += s.n;
     uint64_t* const list = lists + (int64_t)at * kList;
-#pragma unroll
-    for (int a = 0; a < PIECES; ++a)
-        if (nearest[a] < part.d_hi)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float d = distance(c.row, x[a][j]);
-                if (d >= part.d_lo && d < part.d_hi) {
-                    // as many as were counted, unless someone writes the logits meanwhile
-                    if (to < kList) list[to] = key_of(d, (uint32_t)(first + (a * kSegThreads + tid) * 8 + j));
-                    ++to;
-                }
-            }
+    while (hits) {  // few: read again rather than picked out of registers
+        const int bit = 31 - __clz(hits), e = 8 * PIECES - 1 - bit;
+        hits ^= 1u << bit;
+        const int64_t i = first + ((e >> 3) * kSegThreads + tid) * 8 + (e & 7);
+        float y[8];
+        load8<DT>(c.row.x, i, 1, 0.f, y);
+        // as many as were counted, unless someone writes the logits meanwhile
+        if (to < kList) list[to] = key_of(distance(c.row, logit(y[0])), (uint32_t)i);
+        ++to;
+    }
 }
 
 struct Shared {
@@ -445,39 +465,56 @@ __device__ __forceinline__ void each(const Row& r, F&& f) {
     }
 }
 
-// The key of the last token of the smallest prefix, in the order of keys, whose number (COUNT) or weight reaches `target`, among
-// the tokens of `all(f)` (f(key) for each) with keys in [lo, hi), `base` of it lying before lo; `none` where all do not reach it.
-// Parts of keys are cut into 1024 until the part in which the target is reached has one token.
-template <bool COUNT, typename All>
-__device__ uint64_t last_kept(Shared& s, All&& all, uint64_t lo, uint64_t hi, uint64_t base, uint64_t target, uint64_t none) {
+enum Measure { kNumber, kUnits, kWhole };  // of a prefix: its tokens, their weights in their bin's units, or in whole()s
+
+// The key of the last token of the smallest prefix, in the order of keys, whose measure reaches `target`, among the tokens of
+// `all(f)` (f(key) for each) with keys in [lo, hi); `none` where all do not reach it.  [lo, hi) is cut into 1024 parts, first
+// (BINS) by bins of d, until the part in which the target is reached has one token.
+template <Measure M, bool BINS, typename All>
+__device__ uint64_t last_kept(Shared& s, All&& all, uint64_t lo, uint64_t hi, uint64_t target, uint64_t none) {
+    constexpr int kEach = kBins / kThreads;
     const int tid = threadIdx.x;
+    bool bins = BINS;
     for (;;) {
-        int shift = 0;
-        while (((hi - lo - 1) >> shift) >= kBins) ++shift;
-        s.count[tid] = 0;
-        s.weight[tid] = 0;
+        const uint64_t last = hi - lo - 1;
+        const int shift = max(0, 54 - (int)__clzll(last | 1));  // last >> shift < kBins
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) s.count[tid * kEach + j] = 0, s.weight[tid * kEach + j] = 0;
         __syncthreads();
         all([&](uint64_t key) {
             if (key >= lo && key < hi) {
-                const uint32_t b = (uint32_t)((key - lo) >> shift);
+                const float d = d_of(key);
+                const uint32_t b = bins ? (uint32_t)fminf(d, (float)(kBins - 1)) : (uint32_t)((key - lo) >> shift);
                 atomicAdd(&s.count[b], 1u);
-                if (!COUNT) atomicAdd((unsigned long long*)&s.weight[b], (unsigned long long)whole(weight(d_of(key))));
+                if (M != kNumber)
+                    atomicAdd((unsigned long long*)&s.weight[b],
+                              (unsigned long long)(M == kUnits ? in_bin(d) : whole(weight(d))));
             }
         });
         __syncthreads();
-        const uint32_t counts[1] = {s.count[tid]};
-        const uint64_t sums[1] = {COUNT ? counts[0] : s.weight[tid]};
-        uint64_t before;
-        uint32_t n;
-        const uint32_t b = reaching_bin(s.scratch, sums, counts, target - base, before, n);
+        uint32_t counts[kEach], n;
+        uint64_t sums[kEach], before;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            counts[j] = s.count[tid * kEach + j];
+            sums[j] = M == kNumber ? counts[j] : s.weight[tid * kEach + j];
+        }
+        const uint32_t b = reaching_bin(s.scratch, sums, counts, target, before, n);
         if (b == kBins) return none;
-        base += before;
-        lo += (uint64_t)b << shift;
-        const uint64_t end = lo + (1ull << shift);
-        hi = end < hi ? end : hi;
-        if (n <= 1 || shift == 0) break;
+        target -= before;
+        if (bins) {
+            const uint64_t from = key_of(b > 0 ? end_of_bin(b - 1) : 0.f, 0), to = key_of(end_of_bin(b), 0);
+            lo = lo > from ? lo : from;
+            hi = hi < to ? hi : to;
+            bins = false;
+        } else {
+            lo += (uint64_t)b << shift;
+            const uint64_t to = lo + (uint64_t(1) << shift);
+            hi = hi < to ? hi : to;
+        }
+        if (n <= 1 || hi - lo <= 1) break;
     }
-    if (hi - lo == 1) return lo;
+    if (hi - lo <= 1) return lo;
     all([&](uint64_t key) {
         if (key >= lo && key < hi) s.scratch.found = key;
     });
@@ -489,15 +526,16 @@ __device__ uint64_t last_kept(Shared& s, All&& all, uint64_t lo, uint64_t hi, ui
 
 constexpr uint64_t kEveryKey = (uint64_t)kInfBits << 32;  // past every token that can be drawn
 
-// The choice in a row with top-k or top-p, as draw_key; `won`: the draw among the tokens that the gathering workgroups kept.
+// The choice in a row with top-k or top-p, as draw_key; `won`: the draw among the tokens that the gathering workgroups kept;
+// `total` becomes the sum of the row's weights.
 template <int DT>
-__device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const uint64_t* list, uint32_t top, uint64_t won) {
+__device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const uint64_t* list, uint32_t top, uint64_t won,
+                           double& total) {
     const int tid = threadIdx.x;
-    const Part part = part_of(s.scratch, c, state);
     const uint32_t n = min(state.gathered, (uint32_t)kList);
-    __syncthreads();
-    state.count[tid] = 0;
-    state.weight[tid] = 0;
+    const Part part = part_of(s.scratch, c, state, true);
+    total = part.total;
+    for (int b = tid; b < kBins; b += kThreads) state.bins[b] = 0;
     float best = 0.f;
     uint32_t where = 0;
 
@@ -509,11 +547,11 @@ __device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const ui
                 if (key <= limit) f(key);
             });
         };
-        if (c.k > 0) limit = last_kept<true>(s, all, 0, kEveryKey, 0, (uint64_t)c.k, limit);
+        if (c.k > 0) limit = last_kept<kNumber, true>(s, all, 0, kEveryKey, (uint64_t)c.k, limit);
         if (c.top_p < 1.f) {
             uint64_t sum = 0;
             all([&](uint64_t key) { sum += whole(weight(d_of(key))); });
-            limit = last_kept<false>(s, all, 0, kEveryKey, 0, c.want(block_reduce(s.scratch, sum, plus)), limit);
+            limit = last_kept<kWhole, true>(s, all, 0, kEveryKey, c.want(block_reduce(s.scratch, sum, plus)), limit);
         }
         all([&](uint64_t key) {
             const float w = weight(d_of(key));
@@ -528,23 +566,26 @@ __device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const ui
     for (int j = 0; j < kOwn; ++j) key[j] = tid + j * kThreads < n ? list[tid + j * kThreads] : ~0ull;
     float noise[kOwn];  // of all candidates, asked for before it is known which are kept
 #pragma unroll
-    for (int j = 0; j < kOwn; ++j) noise[j] = key[j] != ~0ull ? c.noise[min((uint32_t)key[j], (uint32_t)c.row.V - 1)] : 1.f;
+    for (int j = 0; j < kOwn; ++j) {
+        noise[j] = 1.f;
+        if (key[j] != ~0ull) noise[j] = c.noise[min((uint32_t)key[j], (uint32_t)c.row.V - 1)];
+    }
     uint64_t limit = kEveryKey - 1;
     const auto all = [&](auto&& f) {
 #pragma unroll
         for (int j = 0; j < kOwn; ++j)
             if (key[j] <= limit) f(key[j]);
     };
-    const uint64_t lo = (uint64_t)__float_as_uint(part.d_lo) << 32, hi = (uint64_t)__float_as_uint(part.d_hi) << 32;
+    const uint64_t lo = key_of(part.from, 0), hi = key_of(part.to, 0);
     if (c.k > 0) {
-        if (n > (uint32_t)c.k) limit = last_kept<true>(s, all, lo, hi, 0, (uint64_t)c.k, limit);
+        if (n > (uint32_t)c.k) limit = last_kept<kNumber, false>(s, all, lo, hi, part.target, limit);
         if (c.top_p < 1.f) {
             uint64_t sum = 0;
             all([&](uint64_t k) { sum += whole(weight(d_of(k))); });
-            limit = last_kept<false>(s, all, lo, hi, 0, c.want(block_reduce(s.scratch, sum, plus)), limit);
+            limit = last_kept<kWhole, true>(s, all, 0, hi, c.want(block_reduce(s.scratch, sum, plus)), limit);
         }
     } else {
-        limit = last_kept<false>(s, all, lo, hi, part.base, part.target, limit);
+        limit = last_kept<kUnits, false>(s, all, lo, hi, part.target, limit);
     }
 #pragma unroll
     for (int j = 0; j < kOwn; ++j)
@@ -560,18 +601,19 @@ __device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const ui
 }
 
 template <int DT>
-__global__ __launch_bounds__(kThreads) void choose_kernel(const logits_sample_args p, int64_t row0, RowState* states,
+__global__ __launch_bounds__(kThreads, 4) void choose_kernel(const logits_sample_args p, int64_t row0, RowState* states,
                                                           const uint64_t* lists) {
     __shared__ Shared s;
     const int64_t row = row0 + blockIdx.x;
     RowState& state = states[blockIdx.x];
     Choice c = choice_of<DT>(p, row);
-    const uint64_t max_key = state.max_key, total = state.total;
+    const uint64_t max_key = state.max_key;
     uint64_t won = state.won;
+    double total = (double)state.total * (1.0 / kOne);
     uint32_t token = ~(uint32_t)max_key;
     c.row.max = from_order((uint32_t)(max_key >> 32));
     const bool none = c.row.max == -__builtin_inff();  // nothing is allowed
-    if (c.searches && !none) won = choose<DT>(s, c, state, lists + (int64_t)blockIdx.x * kList, token, won);
+    if (c.searches && !none) won = choose<DT>(s, c, state, lists + (int64_t)blockIdx.x * kList, token, won, total);
     if (won) token = ~(uint32_t)won;  // else greedy, or no noise was a number: the most likely token
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -582,7 +624,7 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(const logits_sample_ar
             float x[8];
             load8<DT>(c.row.x, none ? 0 : token, 1, 0.f, x);
             p.logprob[row] =
-                none ? c.row.max : -distance(c.row, logit(x[0])) * (1.f / kPerUnit) - logf((float)total * (1.f / kOne));
+                none ? c.row.max : -distance(c.row, logit(x[0])) * (1.f / kPerUnit) - logf((float)total);
         }
         if (p.counts && !none) {
             const int64_t slot = p.slots ? p.slots[c.b] : c.b;
@@ -636,7 +678,7 @@ size_t logits_sample_args_size(void) { return sizeof(logits_sample_args); }
 
 int logits_sample_workspace_size(const logits_sample_args* a, size_t* bytes) {
     if (!a || !bytes) return WKV7_ERR_NULL;
-    if (a->B < 0 || a->T < 0 || a->V < 1) return WKV7_ERR_SHAPE;
+    if (a->B < 0 || a->T < 0 || a->V < 1 || a->V > LOGITS_SAMPLE_MAX_V) return WKV7_ERR_SHAPE;
     const int64_t rows = std::min<int64_t>((int64_t)a->B * a->T, lg::kRowsAtOnce);
     *bytes = LOGITS_SAMPLE_STATE_BYTES + (size_t)rows * lg::kList * sizeof(uint64_t);
     return WKV7_OK;
@@ -644,7 +686,7 @@ int logits_sample_workspace_size(const logits_sample_args* a, size_t* bytes) {
 
 int logits_sample(const logits_sample_args* a, void* stream) {
     if (!a) return WKV7_ERR_NULL;
-    if (a->B < 0 || a->T < 0 || a->V < 1) return WKV7_ERR_SHAPE;
+    if (a->B < 0 || a->T < 0 || a->V < 1 || a->V > LOGITS_SAMPLE_MAX_V) return WKV7_ERR_SHAPE;
     if (a->dtype < LOGITS_BF16 || a->dtype > LOGITS_F32 ||
         (a->counts && ((a->counts_dtype != LOGITS_COUNTS_I32 && a->counts_dtype != LOGITS_COUNTS_F32) || a->T > 1)))
         return WKV7_ERR_ARG;

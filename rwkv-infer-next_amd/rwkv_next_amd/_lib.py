@@ -64,7 +64,7 @@ LOGITS_F16 = 1
 LOGITS_F32 = 2
 LOGITS_COUNTS_I32 = 0
 LOGITS_COUNTS_F32 = 1
-LOGITS_SAMPLE_STATE_BYTES = 6422528  # leading workspace region that is zero between calls
+LOGITS_SAMPLE_STATE_BYTES = 4325376  # leading workspace region that is zero between calls
 LOGITS_STATUS_ROW = 256
 LOGITS_STATUS_TOKEN = 512
 MAX_MOVES = 1024
