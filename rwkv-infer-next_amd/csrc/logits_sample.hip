@@ -53,17 +53,37 @@ struct RowState {
 };
 static_assert(sizeof(RowState) * kRowsAtOnce == LOGITS_SAMPLE_STATE_BYTES, "include/logits.h");
 
-__device__ __forceinline__ uint64_t shuffle(uint64_t x, int from) {
-    const uint32_t lo = __shfl((int)(uint32_t)x, from), hi = __shfl((int)(uint32_t)(x >> 32), from);
+// The value of the lane that DPP control CTRL selects, 0 in lanes of rows outside ROWS or without such a lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t from_lane(uint64_t x) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xF, false);
     return (uint64_t)hi << 32 | lo;
 }
 __device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint64_t plus(uint64_t a, uint64_t b) { return a + b; }
+template <typename T>
+__device__ __forceinline__ T plus(T a, T b) { return a + b; }
 
-template <typename F>
-__device__ __forceinline__ uint64_t wave_reduce(uint64_t x, F&& f) {
-    for (int o = 32; o; o >>= 1) x = f(x, shuffle(x, (threadIdx.x & 63) ^ o));
+// f over the lanes up to this one; bits 0 are f's identity.  Rows of 16 lanes by shifts, then a row's end to the rows after it
+// (without the LDS crossbar's round trips).
+template <typename T, typename F>
+__device__ __forceinline__ T wave_scan(T x, F&& f) {
+    const auto bits = [](T v) { return __builtin_bit_cast(uint64_t, v); };
+    x = f(x, __builtin_bit_cast(T, from_lane<0x111, 0xF>(bits(x))));  // row_shr:1, 2, 4, 8
+    x = f(x, __builtin_bit_cast(T, from_lane<0x112, 0xF>(bits(x))));
+    x = f(x, __builtin_bit_cast(T, from_lane<0x114, 0xF>(bits(x))));
+    x = f(x, __builtin_bit_cast(T, from_lane<0x118, 0xF>(bits(x))));
+    x = f(x, __builtin_bit_cast(T, from_lane<0x142, 0xA>(bits(x))));  // row_bcast:15 into rows 1 and 3
+    x = f(x, __builtin_bit_cast(T, from_lane<0x143, 0xC>(bits(x))));  // row_bcast:31 into rows 2 and 3
     return x;
+}
+
+// f over all lanes of the wavefront.
+template <typename T, typename F>
+__device__ __forceinline__ T wave_reduce(T x, F&& f) {
+    const uint64_t all = __builtin_bit_cast(uint64_t, wave_scan(x, f));
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)all, 63), hi = __builtin_amdgcn_readlane((int)(uint32_t)(all >> 32), 63);
+    return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
 }
 
 template <int THREADS>
@@ -73,34 +93,40 @@ struct Scratch {
     uint32_t bin, n;
 };
 
-template <int THREADS, typename F>
-__device__ __forceinline__ uint64_t block_reduce(Scratch<THREADS>& s, uint64_t x, F&& f) {
+template <int THREADS, typename T, typename F>
+__device__ __forceinline__ T block_reduce(Scratch<THREADS>& s, T x, F&& f) {
     x = wave_reduce(x, f);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) s.wave[threadIdx.x >> 6] = x;
+    if ((threadIdx.x & 63) == 0) s.wave[threadIdx.x >> 6] = __builtin_bit_cast(uint64_t, x);
     __syncthreads();
-    x = s.wave[0];
-    for (int w = 1; w < THREADS / 64; ++w) x = f(x, s.wave[w]);
+    x = __builtin_bit_cast(T, s.wave[0]);
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) x = f(x, __builtin_bit_cast(T, s.wave[w]));
     return x;
 }
 
-// The sum over the threads before this one, always added in the same order.
+// The sum over the threads before this one, always added in the same order; `all`: over all threads.
 template <int THREADS, typename T>
-__device__ __forceinline__ T block_before(Scratch<THREADS>& s, T x) {
+__device__ __forceinline__ T block_before(Scratch<THREADS>& s, T x, T& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    T sum = x;
-    for (int o = 1; o < 64; o <<= 1) {
-        const T y = __builtin_bit_cast(T, shuffle(__builtin_bit_cast(uint64_t, sum), (lane - o) & 63));
-        if (lane >= o) sum += y;
-    }
-    T before = __builtin_bit_cast(T, shuffle(__builtin_bit_cast(uint64_t, sum), (lane - 1) & 63));
-    if (lane == 0) before = T(0);
+    const T sum = wave_scan(x, plus<T>);
+    // of the lane before, in the row and at a row's start
+    uint64_t bits = from_lane<0x111, 0xF>(__builtin_bit_cast(uint64_t, sum));
+    const uint64_t bits15 = from_lane<0x142, 0xA>(__builtin_bit_cast(uint64_t, sum));
+    const uint64_t bits31 = from_lane<0x143, 0xC>(__builtin_bit_cast(uint64_t, sum));
+    if (lane == 16 || lane == 48) bits = bits15;
+    if (lane == 32) bits = bits31;
     __syncthreads();
     if (lane == 63) s.wave[wave] = __builtin_bit_cast(uint64_t, sum);
     __syncthreads();
     T others = T(0);
-    for (int w = 0; w < wave; ++w) others += __builtin_bit_cast(T, s.wave[w]);
-    return others + before;
+    all = T(0);
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+        if (w == wave) others = all;
+        all += __builtin_bit_cast(T, s.wave[w]);
+    }
+    return others + __builtin_bit_cast(T, bits);
 }
 
 // The first of kBins bins at whose end the running sum reaches `target`, with the sum before it (s.base) and its `counts` (s.n);
@@ -112,7 +138,7 @@ __device__ __forceinline__ uint32_t reaching_bin(Scratch<THREADS>& s, const T (&
     T mine = sums[0];
 #pragma unroll
     for (int j = 1; j < kBins / THREADS; ++j) mine += sums[j];
-    T before = block_before(s, mine);  // its barriers order the first line
+    T all, before = block_before(s, mine, all);  // its barriers order the first line
 #pragma unroll
     for (int j = 0; j < kBins / THREADS; ++j) {
         // sums before two neighbours may be rounded apart in floating point: the lowest bin of those that fit
@@ -272,7 +298,7 @@ __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_
                 else
                     far += d < __builtin_inff();
             }
-        far = (uint32_t)wave_reduce((uint64_t)far, plus);
+        far = (uint32_t)wave_reduce((uint64_t)far, plus<uint64_t>);
         if ((tid & 63) == 0 && far) atomicAdd((unsigned long long*)&bins[kBins - 1], (unsigned long long)far << kCountAt);
         __syncthreads();
         for (int b = tid; b < kBins; b += kSegThreads)
@@ -301,7 +327,7 @@ __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_
             const uint64_t key = wave_reduce(draw_key(best, where), larger);
             if ((tid & 63) == 0 && key) atomicMax(&state.won, (unsigned long long)key);
         }
-        const uint64_t sum = wave_reduce(whole(total), plus);
+        const uint64_t sum = wave_reduce(whole(total), plus<uint64_t>);
         if ((tid & 63) == 0) atomicAdd(&state.total, (unsigned long long)sum);
     }
 }
@@ -332,13 +358,7 @@ __device__ __forceinline__ Part part_of(Scratch<THREADS>& s, const Choice& c, co
     }
     Part part;
     part.total = 0;
-    if (c.k <= 0 || wants_total) {  // the last thread's sum before it and its own are the row's
-        const double before = block_before(s, all);
-        if (threadIdx.x == THREADS - 1) s.base = __builtin_bit_cast(uint64_t, before + all);
-        __syncthreads();
-        part.total = __builtin_bit_cast(double, s.base);
-        __syncthreads();
-    }
+    if (c.k <= 0 || wants_total) part.total = block_reduce(s, all, plus<double>);
     if (c.k > 0) {
         uint64_t base;
         const uint32_t b = reaching_bin(s, numbers, counts, (uint64_t)c.k, base, n);
@@ -346,7 +366,7 @@ __device__ __forceinline__ Part part_of(Scratch<THREADS>& s, const Choice& c, co
             uint64_t mine = 0;
 #pragma unroll
             for (int j = 0; j < kEach; ++j) mine += numbers[j];
-            base = block_reduce(s, mine, plus);
+            base = block_reduce(s, mine, plus<uint64_t>);
         }
         part.from = b > 0 ? end_of_bin(b - 1) : 0.f, part.to = end_of_bin(b), part.d_lo = 0.f;
         part.target = (uint64_t)c.k - (b == kBins ? 0 : base);
@@ -419,7 +439,8 @@ __global__ __launch_bounds__(kSegThreads) void gather_kernel(const logits_sample
 #pragma unroll
         for (int j = 0; j < 8; ++j) hits = hits + hits + (__float_as_uint(x[a][j]) - from < span);
     const uint32_t mine = __popc(hits);
-    uint32_t to = (uint32_t)block_before(s, (uint64_t)mine);
+    uint64_t all;
+    uint32_t to = (uint32_t)block_before(s, (uint64_t)mine, all);
     if (tid == kSegThreads - 1) s.n = to + mine ? atomicAdd(&state.gathered, to + mine) : 0;
     __syncthreads();
     to += s.n;
@@ -532,6 +553,9 @@ template <int DT>
 __device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const uint64_t* list, uint32_t top, uint64_t won,
                            double& total) {
     const int tid = threadIdx.x;
+    uint64_t mine[kOwn];  // asked for before it is known how many of them are there
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) mine[j] = list[tid + j * kThreads];
     const uint32_t n = min(state.gathered, (uint32_t)kList);
     const Part part = part_of(s.scratch, c, state, true);
     total = part.total;
@@ -551,7 +575,7 @@ __device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const ui
         if (c.top_p < 1.f) {
             uint64_t sum = 0;
             all([&](uint64_t key) { sum += whole(weight(d_of(key))); });
-            limit = last_kept<kWhole, true>(s, all, 0, kEveryKey, c.want(block_reduce(s.scratch, sum, plus)), limit);
+            limit = last_kept<kWhole, true>(s, all, 0, kEveryKey, c.want(block_reduce(s.scratch, sum, plus<uint64_t>)), limit);
         }
         all([&](uint64_t key) {
             const float w = weight(d_of(key));
@@ -563,7 +587,7 @@ __device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const ui
 
     uint64_t key[kOwn];
 #pragma unroll
-    for (int j = 0; j < kOwn; ++j) key[j] = tid + j * kThreads < n ? list[tid + j * kThreads] : ~0ull;
+    for (int j = 0; j < kOwn; ++j) key[j] = tid + j * kThreads < n ? mine[j] : ~0ull;
     float noise[kOwn];  // of all candidates, asked for before it is known which are kept
 #pragma unroll
     for (int j = 0; j < kOwn; ++j) {
@@ -582,7 +606,7 @@ __device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const ui
         if (c.top_p < 1.f) {
             uint64_t sum = 0;
             all([&](uint64_t k) { sum += whole(weight(d_of(k))); });
-            limit = last_kept<kWhole, true>(s, all, 0, hi, c.want(block_reduce(s.scratch, sum, plus)), limit);
+            limit = last_kept<kWhole, true>(s, all, 0, hi, c.want(block_reduce(s.scratch, sum, plus<uint64_t>)), limit);
         }
     } else {
         limit = last_kept<kUnits, false>(s, all, lo, hi, part.target, limit);
