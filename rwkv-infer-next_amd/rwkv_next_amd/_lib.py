@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 from ._build import LIB_PATH, NOALLOC_LIB_PATH
 
@@ -174,6 +175,20 @@ class SampleArgs(ctypes.Structure):
     ]
 
 
+_PACK = {_vp: "Q", ctypes.c_int64: "q", ctypes.c_size_t: "Q", ctypes.c_int32: "i", ctypes.c_float: "f"}
+
+
+def _packer(mirror):
+    """A struct.Struct that lays a call's fields out as `mirror` does: its bytes are passed as the argument struct, at a third of
+    the host time of building the ctypes structure (0 for a NULL pointer)."""
+    s = struct.Struct("@" + "".join(_PACK[t] for _, t in mirror._fields_) + "0q")
+    assert s.size == ctypes.sizeof(mirror)
+    return s.pack
+
+
+pack_w4a16, pack_penalize, pack_sample = _packer(W4a16Args), _packer(PenalizeArgs), _packer(SampleArgs)
+
+
 class Wkv7Error(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"wkv7 error {code}: {msg}")
@@ -245,15 +260,15 @@ def load(path: str = LIB_PATH):
     lib.w4a16_dequantize.restype = ctypes.c_int
     lib.w4a16_dequantize.argtypes = [_vp, _vp, _vp, i32, i32, i32, i32, _vp]
     lib.w4a16_matmul.restype = ctypes.c_int
-    lib.w4a16_matmul.argtypes = [ctypes.POINTER(W4a16Args), _vp]
+    lib.w4a16_matmul.argtypes = [_vp, _vp]  # a W4a16Args by reference, or pack_w4a16's bytes
     lib.logits_penalize_args_size.restype = ctypes.c_size_t
     lib.logits_sample_args_size.restype = ctypes.c_size_t
     lib.logits_penalize.restype = ctypes.c_int
-    lib.logits_penalize.argtypes = [ctypes.POINTER(PenalizeArgs), _vp]
+    lib.logits_penalize.argtypes = [_vp, _vp]
     lib.logits_sample_workspace_size.restype = ctypes.c_int
     lib.logits_sample_workspace_size.argtypes = [ctypes.POINTER(SampleArgs), psz]
     lib.logits_sample.restype = ctypes.c_int
-    lib.logits_sample.argtypes = [ctypes.POINTER(SampleArgs), _vp]
+    lib.logits_sample.argtypes = [_vp, _vp]
     if lib.wkv7_abi_version() != WKV7_ABI_VERSION:
         raise ImportError(f"{path}: ABI version {lib.wkv7_abi_version()} != {WKV7_ABI_VERSION}")
     if lib.wkv7_args_size() != ctypes.sizeof(Wkv7Args):

@@ -130,31 +130,34 @@ def int4_matmul(a, packed: Int4Packed, *, out_dtype=None):
     """a (..., K) bf16 or fp16 @ dequant(packed (K, N)) -> (..., N) in a.dtype, or out_dtype (bfloat16 / float16 / float32).
     An infinity or NaN in a row of `a` makes the whole row NaN."""
     weight, scales, K, N, g = packed
-    odt = a.dtype if out_dtype is None else out_dtype
-    if a.dtype not in _CODES or a.dtype == torch.float32:
-        raise TypeError(f"int4_matmul takes bfloat16 or float16 activations (got {a.dtype})")
+    adt = a.dtype
+    odt = adt if out_dtype is None else out_dtype
+    if adt is not torch.bfloat16 and adt is not torch.float16:
+        raise TypeError(f"int4_matmul takes bfloat16 or float16 activations (got {adt})")
     if odt not in _CODES:
         raise TypeError(f"int4_matmul writes bfloat16, float16 or float32 (got {odt})")
-    dev = a.device
-    if dev.type != "cuda" or weight.device != dev or scales.device != dev:
-        raise ValueError(f"int4_matmul needs a and the weight on one GPU (got {dev}, {weight.device})")
-    if a.dim() < 1 or a.shape[-1] != K:
-        raise ValueError(f"K mismatch: a is {tuple(a.shape)}, int4 weight has {K} rows")
-    if weight.dtype != torch.uint8 or scales.dtype != torch.float16 or not weight.is_contiguous() or \
+    index = a.get_device()
+    if index < 0 or weight.get_device() != index or scales.get_device() != index:
+        raise ValueError(f"int4_matmul needs a and the weight on one GPU (got {a.device}, {weight.device})")
+    shape = a.shape
+    if len(shape) < 1 or shape[-1] != K:
+        raise ValueError(f"K mismatch: a is {tuple(shape)}, int4 weight has {K} rows")
+    if weight.dtype is not torch.uint8 or scales.dtype is not torch.float16 or not weight.is_contiguous() or \
             not scales.is_contiguous() or (weight.numel(), scales.numel()) != _sizes(K, N, g):
         raise ValueError("the packed weight and scales are not prepack_int4's")
-    x = a if a.dim() == 2 else a.reshape(-1, K)
-    M = x.shape[0]
-    out = torch.empty((*a.shape[:-1], N), dtype=odt, device=dev)
+    x = a if len(shape) == 2 else a.reshape(-1, K)
+    M = x.size(0)
+    out = a.new_empty((*shape[:-1], N), dtype=odt)
     if M == 0:
         return out
-    if x.stride(1) != 1 or x.stride(0) % 8 or (x.stride(0) < K and M > 1) or x.data_ptr() % 16:
-        x = x.contiguous() if x.data_ptr() % 16 == 0 and not x.is_contiguous() else x.clone(
-            memory_format=torch.contiguous_format)
-    args = _lib.W4a16Args(x.data_ptr(), x.stride(0) if M > 1 else K, weight.data_ptr(), scales.data_ptr(),
-                          out.data_ptr(), N, M, N, K, g, _CODES[a.dtype], _CODES[odt])
-    with on_device(dev):
-        _lib.check(_lib.load().w4a16_matmul(args, stream_handle(dev)))
+    row, ptr = x.stride(0) if M > 1 else K, x.data_ptr()
+    if x.stride(1) != 1 or row % 8 or row < K or ptr % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        row, ptr = K, x.data_ptr()
+    args = _lib.pack_w4a16(ptr, row, weight.data_ptr(), scales.data_ptr(), out.data_ptr(), N, M, N, K, g, _CODES[adt],
+                           _CODES[odt])  # in the order of the fields
+    with on_device(a.device):
+        _lib.check(_lib.load().w4a16_matmul(args, stream_handle(a.device)))
     return out
 
 

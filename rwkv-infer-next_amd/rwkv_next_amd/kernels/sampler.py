@@ -25,42 +25,45 @@ _COUNTS = {torch.int32: _lib.LOGITS_COUNTS_I32, torch.float32: _lib.LOGITS_COUNT
 
 
 def _shape(logits):
-    """(B, T, V, sequence stride, position stride) of (B, V) or (B, T, V) logits."""
+    """(B, T, V, sequence stride, position stride, the last stride) of (B, V) or (B, T, V) logits."""
     if logits.dtype not in _DTYPES:
         raise TypeError(f"logits must be bfloat16, float16 or float32 (got {logits.dtype})")
-    if logits.device.type != "cuda":
+    if not logits.is_cuda:
         raise ValueError(f"logits must be on a GPU (got {logits.device})")
-    if logits.dim() == 2:
-        B, V = logits.shape
-        return B, 1, V, logits.stride(0), 0
-    if logits.dim() != 3:
+    n = logits.dim()
+    if n == 2:
+        (B, V), (seq, last) = logits.shape, logits.stride()
+        return B, 1, V, seq, 0, last
+    if n != 3:
         raise ValueError(f"logits must be (B, V) or (B, T, V) (got {tuple(logits.shape)})")
-    return (*logits.shape, logits.stride(0), logits.stride(1))
+    return (*logits.shape, *logits.stride())
 
 
 def _on(t, dev, name):
-    if t.device != dev:
+    if t.get_device() != dev.index:
         raise ValueError(f"{name} must be on {dev} (got {t.device})")
 
 
 def _per_sequence(x, dtype, B, dev, name):
-    """(pointer, scalar) of a parameter: a tensor of B entries, or a number."""
+    """(pointer, scalar) of a parameter: a tensor of B entries, or a number (pointer 0)."""
     if not isinstance(x, torch.Tensor):
-        return None, x
+        return 0, x
+    if x.dtype is dtype and x.dim() == 1 and x.size(0) == B and (B == 1 or x.stride(0) == 1) and \
+            x.get_device() == dev.index:
+        return x.data_ptr(), 0
     _on(x, dev, name)
-    if x.dtype != dtype or x.dim() != 1 or x.shape[0] != B or not (x.is_contiguous() or B == 1):
-        raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor of {B} entries "
-                         f"(got {x.dtype} {tuple(x.shape)})")
-    return x.data_ptr(), 0
+    raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor of {B} entries "
+                     f"(got {x.dtype} {tuple(x.shape)})")
 
 
 def _rows(x, dtype, lead, least, dev, name):
     """A tensor of rows of at least `least` contiguous elements whose leading sizes are `lead`: its row stride."""
     _on(x, dev, name)
-    if x.dtype != dtype or tuple(x.shape[:-1]) != lead or x.shape[-1] < least or x.stride(-1) != 1:
+    shape, stride = x.shape, x.stride()
+    if x.dtype is not dtype or shape[:-1] != lead or shape[-1] < least or (stride[-1] != 1 and shape[-1] > 1):
         raise ValueError(f"{name} must be a {dtype} {(*lead, least)} tensor with contiguous rows "
-                         f"(got {x.dtype} {tuple(x.shape)}, strides {x.stride()})")
-    return x.stride(0) if lead[0] > 1 else max(x.stride(0), x.shape[-1])
+                         f"(got {x.dtype} {tuple(shape)}, strides {stride})")
+    return stride[0] if lead[0] > 1 else max(stride[0], shape[-1])
 
 
 def _overlaps(t):
@@ -78,21 +81,25 @@ def _counts(counts, slots, B, V, dev):
     if counts is None:
         if slots is not None:
             raise ValueError("slots without counts")
-        return None, 0, 0, 0, None
+        return 0, 0, 0, 0, 0
     _on(counts, dev, "counts")
-    if counts.dtype not in _COUNTS or counts.dim() != 2 or counts.shape[1] != V or counts.stride(1) != 1 or \
-            (counts.shape[0] > 1 and counts.stride(0) < V):
+    code, shape, stride = _COUNTS.get(counts.dtype), counts.shape, counts.stride()
+    if code is None or len(shape) != 2 or shape[1] != V or (stride[1] != 1 and V > 1) or (shape[0] > 1 and stride[0] < V):
         raise ValueError(f"counts must be an int32 or float32 (S, {V}) tensor with contiguous rows "
-                         f"(got {counts.dtype} {tuple(counts.shape)}, strides {counts.stride()})")
-    if slots is None and counts.shape[0] < B:
-        raise ValueError(f"counts has {counts.shape[0]} rows for {B} sequences (or pass slots)")
-    return (counts.data_ptr(), max(counts.stride(0), V), counts.shape[0], _COUNTS[counts.dtype],
-            None if slots is None else _per_sequence(slots, torch.int64, B, dev, "slots")[0])
+                         f"(got {counts.dtype} {tuple(shape)}, strides {stride})")
+    if slots is None:
+        if shape[0] < B:
+            raise ValueError(f"counts has {shape[0]} rows for {B} sequences (or pass slots)")
+        return counts.data_ptr(), max(stride[0], V), shape[0], code, 0
+    if not isinstance(slots, torch.Tensor):
+        raise TypeError(f"slots must be an int64 tensor of {B} entries (got {type(slots).__name__})")
+    return (counts.data_ptr(), max(stride[0], V), shape[0], code,
+            _per_sequence(slots, torch.int64, B, dev, "slots")[0])
 
 
 def _status(status, dev):
     if status is None:
-        return None
+        return 0
     _on(status, dev, "status")
     if status.dtype != torch.int32 or status.numel() < 1:
         raise ValueError("status must be an int32 tensor (new_status)")
@@ -117,33 +124,36 @@ def penalize_logits(logits, *, counts=None, slots=None, repetition=1.0, presence
     mask int32, ceil(V / 32) words to a row, bit v % 32 of word v / 32 set where v is allowed: one row for each row of the logits
     ((B, words) or (B, T, words)), or a table (R, words) with mask_rows int64 in the shape of the rows (negative: no mask).
     """
-    B, T, V, seq_stride, pos_stride = _shape(logits)
-    dev = logits.device
-    if B and T and V and logits.stride(-1) != 1:
-        if out is logits:
+    B, T, V, seq_stride, pos_stride, last = _shape(logits)
+    dev, in_place = logits.device, out is logits
+    if last != 1 and V > 1:
+        if in_place:
             raise ValueError("logits must have contiguous rows to be changed in place")
         logits = logits.contiguous()
-        _, _, _, seq_stride, pos_stride = _shape(logits)
+        _, _, _, seq_stride, pos_stride, _ = _shape(logits)
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-    elif out is not logits:
-        _on(out, dev, "out")
-        if out.shape != logits.shape or out.dtype not in _DTYPES or (out.numel() and out.stride(-1) != 1):
-            raise ValueError(f"out must be bfloat16, float16 or float32 {tuple(logits.shape)} with contiguous rows "
-                             f"(got {out.dtype} {tuple(out.shape)}, strides {out.stride()})")
-        if out.data_ptr() == logits.data_ptr() and out.numel() and (
-                out.dtype != logits.dtype or out.stride() != logits.stride()):
-            raise ValueError("out over the logits must have their type and strides")
+        out_seq, out_pos = (V, 0) if logits.dim() == 2 else (T * V, V)
+    else:
+        if not in_place:
+            _on(out, dev, "out")
+            if out.shape != logits.shape or out.dtype not in _DTYPES or (out.stride(-1) != 1 and V > 1):
+                raise ValueError(f"out must be bfloat16, float16 or float32 {tuple(logits.shape)} with contiguous rows "
+                                 f"(got {out.dtype} {tuple(out.shape)}, strides {out.stride()})")
+            if out.data_ptr() == logits.data_ptr() and out.numel() and (
+                    out.dtype != logits.dtype or out.stride() != logits.stride()):
+                raise ValueError("out over the logits must have their type and strides")
+        if _overlaps(out):
+            raise ValueError(f"out must not share memory between its rows (strides {out.stride()})")
+        out_seq, out_pos = out.stride(0), out.stride(1) if out.dim() == 3 else 0
     if not (B and T and V):
         return out
-    if _overlaps(out):
-        raise ValueError(f"out must not share memory between its rows (strides {out.stride()})")
     lead = (B,) if logits.dim() == 2 else (B, T)
     ct, ct_stride, ct_rows, ct_type, slots_p = _counts(counts, slots, B, V, dev)
     rep_p, rep = _per_sequence(repetition, torch.float32, B, dev, "repetition")
     pres_p, pres = _per_sequence(presence, torch.float32, B, dev, "presence")
     freq_p, freq = _per_sequence(frequency, torch.float32, B, dev, "frequency")
-    if rep_p is None and not rep > 0:
+    if not rep_p and not rep > 0:
         raise ValueError(f"repetition must be positive (got {rep})")
     dr_p = dr_stride = 0
     if drafts is not None and T > 1:
@@ -152,48 +162,42 @@ def penalize_logits(logits, *, counts=None, slots=None, repetition=1.0, presence
     bi_p = bv_p = bias_stride = n_bias = 0
     if (bias_ids is None) != (bias_values is None):
         raise ValueError("bias_ids and bias_values go together")
-    if bias_ids is not None and bias_ids.numel():
-        n_bias = bias_ids.shape[-1]
-        bias_stride = _rows(bias_ids, torch.int64, (B,), n_bias, dev, "bias_ids")
-        if _rows(bias_values, torch.float32, (B,), n_bias, dev, "bias_values") != bias_stride or \
-                bias_values.shape != bias_ids.shape:
-            bias_ids, bias_values = bias_ids.contiguous(), bias_values[..., :n_bias].contiguous()
-            bias_stride = n_bias
+    if bias_ids is not None:
+        n_bias = bias_ids.size(-1)
+        bias_stride = _rows(bias_ids, torch.int64, (B,), 0, dev, "bias_ids")
+        value_stride = _rows(bias_values, torch.float32, (B,), 0, dev, "bias_values")
+        if bias_values.size(-1) != n_bias:
+            raise ValueError(f"bias_ids and bias_values must have one shape (got {n_bias} and {bias_values.size(-1)} places)")
+        if value_stride != bias_stride:
+            bias_ids, bias_values, bias_stride = bias_ids.contiguous(), bias_values.contiguous(), n_bias
         bi_p, bv_p = bias_ids.data_ptr(), bias_values.data_ptr()
     m_p = m_stride = m_rows = mr_p = 0
     if mask is not None:
         words = (V + 31) // 32
         if mask_rows is None:
-            m_stride = _rows(mask, torch.int32, lead, words, dev, "mask")
-            m_rows = B * T
+            m_rows, m_stride = B * T, _rows(mask, torch.int32, lead, words, dev, "mask")
             if len(lead) == 2:  # rows of (b, t) one after another
                 if not mask.is_contiguous():
                     mask = mask.contiguous()
-                m_stride = mask.shape[-1]
+                m_stride = mask.size(-1)
         else:
             _on(mask_rows, dev, "mask_rows")
-            if mask_rows.dtype != torch.int64 or tuple(mask_rows.shape) != lead or not mask_rows.is_contiguous():
+            if mask_rows.dtype is not torch.int64 or mask_rows.shape != lead or not mask_rows.is_contiguous():
                 raise ValueError(f"mask_rows must be a contiguous int64 {lead} tensor "
                                  f"(got {mask_rows.dtype} {tuple(mask_rows.shape)})")
             if mask.dim() != 2:
-                raise ValueError("mask must be a table (R, words) where mask_rows is given")
-            m_rows = mask.shape[0]
-            m_stride = _rows(mask, torch.int32, (m_rows,), words, dev, "mask") if m_rows else words
+                raise ValueError(f"mask must be a table (R, words) where mask_rows is given (got {tuple(mask.shape)})")
+            m_rows = mask.size(0)
+            m_stride = max(_rows(mask, torch.int32, (m_rows,), words, dev, "mask") if m_rows else 0, words)
             mr_p = mask_rows.data_ptr()
-        m_p = mask.data_ptr()
-        if not m_rows:
-            m_p = 0
+        m_p = mask.data_ptr() if m_rows else 0
     elif mask_rows is not None:
         raise ValueError("mask_rows without a mask")
-    if out.dim() == 2:
-        out_seq, out_pos = out.stride(0), 0
-    else:
-        out_seq, out_pos = out.stride(0), out.stride(1)
-    args = _lib.PenalizeArgs(
+    args = _lib.pack_penalize(
         logits.data_ptr(), seq_stride, pos_stride, out.data_ptr(), out_seq, out_pos, ct, ct_stride, ct_rows, slots_p,
-        rep_p, pres_p, freq_p, dr_p or None, dr_stride, bi_p or None, bv_p or None, bias_stride, m_p or None, m_stride,
-        m_rows, mr_p or None, _status(status, dev), rep, pres, freq, B, T, V, n_bias, _DTYPES[logits.dtype],
-        _DTYPES[out.dtype], ct_type)  # in the order of the fields
+        rep_p, pres_p, freq_p, dr_p, dr_stride, bi_p, bv_p, bias_stride, m_p, m_stride, m_rows, mr_p,
+        _status(status, dev), rep, pres, freq, B, T, V, n_bias, _DTYPES[logits.dtype], _DTYPES[out.dtype],
+        ct_type)  # in the order of the fields
     with on_device(dev):
         _lib.check(_lib.load().logits_penalize(args, stream_handle(dev)))
     return out
@@ -229,41 +233,40 @@ def sample_logits(logits, noise=None, *, temperature=1.0, top_k=0, top_p=1.0, mi
     that row alone.  noise float32 in the logits' shape; top_k int32 where it is a tensor, the other parameters float32.
     counts (S, V) int32 or float32 with slots, for (B, V) logits: counts[slots[b], token] += 1, the next step's penalties.
     """
-    B, T, V, seq_stride, pos_stride = _shape(logits)
+    B, T, V, seq_stride, pos_stride, last = _shape(logits)
     dev = logits.device
     if V < 1:
         raise ValueError("logits without a token to choose")
-    if logits.stride(-1) != 1 and V > 1:
+    if last != 1 and V > 1:
         logits = logits.contiguous()
-        _, _, _, seq_stride, pos_stride = _shape(logits)
-    lead = logits.shape[:-1]
-    token = torch.empty(lead, dtype=torch.int64, device=dev)
-    logprob = torch.empty(lead, dtype=torch.float32, device=dev)
-    nz = nz_seq = nz_pos = None
+        _, _, _, seq_stride, pos_stride, _ = _shape(logits)
+    three = logits.dim() == 3
+    nz = nz_seq = nz_pos = 0
     if noise is not None:
         _on(noise, dev, "noise")
-        if noise.dtype != torch.float32 or noise.shape != logits.shape:
+        if noise.dtype is not torch.float32 or noise.shape != logits.shape:
             raise ValueError(f"noise must be float32 {tuple(logits.shape)} (got {noise.dtype} {tuple(noise.shape)})")
         if noise.stride(-1) != 1 and V > 1:
             noise = noise.contiguous()
-        nz, nz_seq, nz_pos = noise.data_ptr(), noise.stride(0), noise.stride(1) if noise.dim() == 3 else 0
+        nz, nz_seq, nz_pos = noise.data_ptr(), noise.stride(0), noise.stride(1) if three else 0
     t_p, t = _per_sequence(temperature, torch.float32, B, dev, "temperature")
     k_p, k = _per_sequence(top_k, torch.int32, B, dev, "top_k")
     p_p, p = _per_sequence(top_p, torch.float32, B, dev, "top_p")
     m_p, m = _per_sequence(min_p, torch.float32, B, dev, "min_p")
-    if counts is not None and logits.dim() != 2:
+    if counts is not None and three:
         raise ValueError("counts are kept for (B, V) logits: a block's accepted tokens are known only later")
     ct, ct_stride, ct_rows, ct_type, slots_p = _counts(counts, slots, B, V, dev)
+    lead = (B, T) if three else B
+    token = torch.empty(lead, dtype=torch.int64, device=dev)
+    logprob = torch.empty(lead, dtype=torch.float32, device=dev)
     if not (B and T):
         return token, logprob
     with on_device(dev):
         ws = _workspace(B * T, V, dev)
-    args = _lib.SampleArgs(
-        logits.data_ptr(), seq_stride, pos_stride, nz, nz_seq or 0, nz_pos or 0, t_p, k_p, p_p, m_p, token.data_ptr(),
-        logprob.data_ptr(), ct, ct_stride, ct_rows, slots_p, _status(status, dev),
-        ws.data_ptr(), ws.numel(), t, p, m,
-        max(-1, min(int(k), 2 ** 31 - 1)), B, T, V, _DTYPES[logits.dtype], ct_type)  # in the order of the fields
-    with on_device(dev):
+        args = _lib.pack_sample(
+            logits.data_ptr(), seq_stride, pos_stride, nz, nz_seq, nz_pos, t_p, k_p, p_p, m_p, token.data_ptr(),
+            logprob.data_ptr(), ct, ct_stride, ct_rows, slots_p, _status(status, dev), ws.data_ptr(), ws.numel(), t, p, m,
+            max(-1, min(int(k), 2 ** 31 - 1)), B, T, V, _DTYPES[logits.dtype], ct_type)  # in the order of the fields
         _lib.check(_lib.load().logits_sample(args, stream_handle(dev)))
     return token, logprob
 
