@@ -29,9 +29,11 @@ extern "C" {
 #define W4A16_F16 1
 #define W4A16_F32 2
 
+#define W4A16_MAX_ROW_STRIDE (1 << 24)  /* elements between rows of activations */
+
 typedef struct w4a16_args {
     const uint16_t *a;       /* activations [M][K], 16-byte aligned */
-    int64_t a_row_stride;    /* elements, >= K, a multiple of 8 */
+    int64_t a_row_stride;    /* elements, >= K, a multiple of 8, at most W4A16_MAX_ROW_STRIDE */
     const void *weight;      /* w4a16_pack's layout, 16-byte aligned */
     const uint16_t *scales;  /* w4a16_pack's layout, 16-byte aligned */
     void *out;               /* [M][N], aligned to its type */

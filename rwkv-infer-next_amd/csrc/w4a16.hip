@@ -42,20 +42,32 @@ __device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
 
+// The codes' bits in an operand pair, and the pattern of (16, 16).  Kept in vector registers: v_and_or_b32 takes one constant.
+struct Patterns {
+    uint32_t mask, sixteen;
+};
+template <int AT>
+__device__ __forceinline__ Patterns patterns() {
+    Patterns p = AT == W4A16_BF16 ? Patterns{0x00780078u, 0x41804180u}   // bf16 of 16: the code's place is bit 3
+                                  : Patterns{0x03C003C0u, 0x4C004C00u};  // fp16 of 16: bit 6
+    asm("" : "+v"(p.mask), "+v"(p.sixteen));
+    return p;
+}
+
 // Eight codes (k = 2j in bits 4j.., k = 2j + 1 in bits 16 + 4j..) as eight operands of value 16 + u.
 template <int AT>
-__device__ __forceinline__ u4 operands(uint32_t w) {
+__device__ __forceinline__ u4 operands(uint32_t w, const Patterns& p) {
     u4 r;
-    if constexpr (AT == W4A16_BF16) {  // bf16 of 16: 0x4180, the code's place is bit 3
-        r[0] = ((w << 3) & 0x00780078u) | 0x41804180u;
-        r[1] = ((w >> 1) & 0x00780078u) | 0x41804180u;
-        r[2] = ((w >> 5) & 0x00780078u) | 0x41804180u;
-        r[3] = ((w >> 9) & 0x00780078u) | 0x41804180u;
-    } else {  // fp16 of 16: 0x4C00, the code's place is bit 6
-        r[0] = ((w << 6) & 0x03C003C0u) | 0x4C004C00u;
-        r[1] = ((w << 2) & 0x03C003C0u) | 0x4C004C00u;
-        r[2] = ((w >> 2) & 0x03C003C0u) | 0x4C004C00u;
-        r[3] = ((w >> 6) & 0x03C003C0u) | 0x4C004C00u;
+    if constexpr (AT == W4A16_BF16) {
+        r[0] = ((w << 3) & p.mask) | p.sixteen;
+        r[1] = ((w >> 1) & p.mask) | p.sixteen;
+        r[2] = ((w >> 5) & p.mask) | p.sixteen;
+        r[3] = ((w >> 9) & p.mask) | p.sixteen;
+    } else {
+        r[0] = ((w << 6) & p.mask) | p.sixteen;
+        r[1] = ((w << 2) & p.mask) | p.sixteen;
+        r[2] = ((w >> 2) & p.mask) | p.sixteen;
+        r[3] = ((w >> 6) & p.mask) | p.sixteen;
     }
     return r;
 }
@@ -76,7 +88,7 @@ __device__ __forceinline__ void store(void* out, int dtype, int64_t at, float x)
 // A workgroup's wavefronts take the 128-row chunks of K in turn, each with sums of its own; they are added in LDS in the
 // wavefronts' order.
 template <int AT, int MT, int NT, int SPC>
-__global__ __launch_bounds__(512) void w4a16_kernel(const Params p) {
+__global__ __launch_bounds__(512) void w4a16_strip_kernel(const Params p) {
     extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][MT * 16][NT * 16]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const uint32_t on_xcd = blockIdx.x >> 3;
@@ -105,6 +117,7 @@ __global__ __launch_bounds__(512) void w4a16_kernel(const Params p) {
         for (int t = 0; t < NT; ++t) acc[i][t] = f4{0.f, 0.f, 0.f, 0.f};
     const uint32_t one = AT == W4A16_BF16 ? 0x3F803F80u : 0x3C003C00u;
     const u4 ones = {one, one, one, one};
+    const Patterns pat = patterns<AT>();
 
     for (int c = wave; c < p.chunks; c += waves) {
         u4 w[NT], a[MT][4];
@@ -140,7 +153,7 @@ __global__ __launch_bounds__(512) void w4a16_kernel(const Params p) {
                 for (int i = 0; i < MT; ++i) d[i] = zero;
 #pragma unroll
                 for (int k = j * 4 / SPC; k < (j + 1) * 4 / SPC; ++k) {
-                    const u4 b = operands<AT>(w[t][k]);
+                    const u4 b = operands<AT>(w[t][k], pat);
 #pragma unroll
                     for (int i = 0; i < MT; ++i) d[i] = mfma<AT>(a[i][k], b, d[i]);
                 }
@@ -168,6 +181,202 @@ __global__ __launch_bounds__(512) void w4a16_kernel(const Params p) {
         const int64_t n = (int64_t)strip0 * kStrip + e % (16 * NT);
         if (row < p.M && n < p.N) store(p.out, p.out_dtype, row * p.out_row_stride + n, x);
     }
+}
+
+template <int MT, int WK>
+constexpr int kPanelStride = WK * kChunk * 2 + 16;  // bytes of a row of A's panel in LDS: 16 more, so 16 rows lie in different banks
+template <int MT, int WK>
+constexpr int kPanelBytes = 16 * MT * kPanelStride<MT, WK>;
+// A workgroup's WN WK wavefronts are WN groups of columns by WK groups of chunks: they share A, a panel of WK chunks at a time,
+// through LDS, which global loads fill by whole lines; each reads its own weights three panels deep.
+template <int AT, int MT, int NT, int SPC, int WN, int WK>
+__global__ __launch_bounds__(64 * WN * WK, 2) void w4a16_block_kernel(const Params p) {
+    constexpr int kThreads = 64 * WN * WK;
+    constexpr int kStride = kPanelStride<MT, WK>, kBuffers = 3;
+    constexpr int kSums = (WK - 1) * WN * MT * NT * 1024;
+    constexpr int kLds = kBuffers * kPanelBytes<MT, WK> > kSums ? kBuffers * kPanelBytes<MT, WK> : kSums;
+    constexpr int kPieces = 16 * MT * WK * 16 / kThreads;  // 16-byte pieces of a panel to a thread
+    static_assert(kPieces >= 1, "");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wn = wave % WN, wk = wave / WN, col = lane & 15, quad = lane >> 4;
+    const uint32_t on_xcd = blockIdx.x >> 3;
+    const uint32_t group = on_xcd / (uint32_t)p.row_groups * 8 + (blockIdx.x & 7);
+    const int row0 = (int)(on_xcd % (uint32_t)p.row_groups) * 16 * MT;
+    if (group >= (uint32_t)p.strip_groups) return;
+    const int strip0 = ((int)group * WN + wn) * NT;
+
+    const uint8_t* wp[NT];
+    const uint8_t* sp[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {  // past the last strip: that strip again, not stored
+        const int64_t s = min(strip0 + t, p.strips - 1);
+        wp[t] = wkv7::uniform_ptr(p.weight + s * p.chunks * kBlockBytes);
+        sp[t] = wkv7::uniform_ptr(reinterpret_cast<const uint8_t*>(p.scales) + s * p.chunks * (kStrip * SPC * 2));
+    }
+    const int panels = (p.chunks + WK - 1) / WK;
+
+    // A's pieces of a thread: rows past the last are that row again (not stored), columns past K zeros
+    const uint8_t* const ap = reinterpret_cast<const uint8_t*>(p.a) + (int64_t)row0 * p.a_row_stride * 2;
+    uint32_t at_a[kPieces];
+    int at_k[kPieces], at_lds[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const int e = tid + kThreads * i, row = e / (WK * 16), piece = e % (WK * 16);
+        at_a[i] = (uint32_t)min(row, p.M - 1 - row0) * (uint32_t)(p.a_row_stride * 2);
+        at_k[i] = piece * 8;
+        at_lds[i] = row * kStride + piece * 16;
+    }
+    u4 next[kPieces];
+    // No branch around a load, here and below: what lies past the end is read from the end and then not used.
+    const auto load_a = [&](int panel) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+            next[i] = *reinterpret_cast<const u4*>(ap + at_a[i] + (int64_t)min(panel * (WK * kChunk) + at_k[i], p.K - 8) * 2);
+    };
+    const auto store_a = [&](int panel, int buffer) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const bool in = panel * (WK * kChunk) + at_k[i] < p.K;
+            u4 x = next[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = in ? x[j] : 0;
+            *reinterpret_cast<u4*>(lds + buffer * kPanelBytes<MT, WK> + at_lds[i]) = x;
+        }
+    };
+    struct Weights {
+        u4 w[NT];
+        uint32_t s[NT][(SPC + 1) / 2];
+    };
+    const auto load_w = [&](int panel, Weights& w) {
+        const int64_t c = min(panel * WK + wk, p.chunks - 1);  // past the last chunk A is zero
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            w.w[t] = *reinterpret_cast<const u4*>(wp[t] + c * kBlockBytes + (uint32_t)lane * 16);
+            const uint8_t* const s = sp[t] + c * (kStrip * SPC * 2) + (uint32_t)col * (SPC * 2);
+            if constexpr (SPC == 1)
+                w.s[t][0] = *reinterpret_cast<const uint16_t*>(s);
+            else
+#pragma unroll
+                for (int j = 0; j < SPC / 2; ++j) w.s[t][j] = reinterpret_cast<const uint32_t*>(s)[j];
+        }
+    };
+
+    f4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[i][t] = f4{0.f, 0.f, 0.f, 0.f};
+    const uint32_t m24 = AT == W4A16_BF16 ? 0xC1C0C1C0u : 0xCE00CE00u;  // -24
+    const u4 minus24 = {m24, m24, m24, m24};
+    const Patterns pat = patterns<AT>();
+
+    // A chunk in parts of kSteps MFMA steps, at least two: the operands of one are read from LDS while the one before multiplies.
+    constexpr int kParts = SPC > 2 ? SPC : 2, kSteps = 4 / kParts;
+    struct Operands {
+        u4 a[MT][kSteps];
+    };
+    const auto read = [&](int buffer, int part, Operands& o) {
+        const uint8_t* const at =
+            lds + buffer * kPanelBytes<MT, WK> + col * kStride + wk * (kChunk * 2) + quad * 16 + part * (kSteps * 64);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) o.a[i][k] = *reinterpret_cast<const u4*>(at + i * (16 * kStride) + k * 64);
+    };
+    const auto multiply = [&](int part, const Operands& o, const Weights& w) {
+        f4 bias[MT];  // -24 sum a, where each strip's sum begins
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                bias[i] = mfma<AT>(o.a[i][k], minus24, k == 0 ? f4{0.f, 0.f, 0.f, 0.f} : bias[i]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int js = part * SPC / kParts;
+            const float s = f16_to_f32(SPC == 1 ? w.s[t][0] : js & 1 ? w.s[t][js / 2] >> 16 : w.s[t][js / 2] & 0xFFFFu);
+            f4 d[MT];
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                const u4 b = operands<AT>(w.w[t][part * kSteps + k], pat);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) d[i] = mfma<AT>(o.a[i][k], b, k == 0 ? bias[i] : d[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[i][t][r] = fmaf(s, d[i][r], acc[i][t][r]);
+        }
+    };
+
+    Weights w0, w1, w2;
+    Operands even, odd;
+    load_a(0);
+    load_w(0, w0);
+    load_w(1, w1);
+    store_a(0, 0);
+    load_a(1);
+    store_a(1, 1);
+    __syncthreads();
+    read(0, 0, even);
+    // Step p multiplies panel p, in LDS buffer `now`; the next panel is in LDS already, the one after it goes there.
+    const auto step = [&](int panel, int now, int next_one, int after, const Weights& w, Weights& later) {
+        load_a(panel + 2);
+        load_w(panel + 2, later);
+        __builtin_amdgcn_sched_barrier(0);  // the loads go out before the products, not beside their uses
+        wkv7::unroll<kParts>([&](auto q) {
+            constexpr int part = decltype(q)::value;
+            Operands& mine = part % 2 == 0 ? even : odd;
+            Operands& other = part % 2 == 0 ? odd : even;
+            if (part + 1 < kParts)
+                read(now, part + 1, other);
+            else
+                read(next_one, 0, other);
+            multiply(part, mine, w);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+        store_a(panel + 2, after);
+        __syncthreads();
+    };
+    int panel = 0;
+    for (; panel + 3 <= panels; panel += 3) {
+        step(panel, 0, 1, 2, w0, w2);
+        step(panel + 1, 1, 2, 0, w1, w0);
+        step(panel + 2, 2, 0, 1, w2, w1);
+    }
+    if (panel < panels) step(panel, 0, 1, 2, w0, w2);
+    if (panel + 1 < panels) step(panel + 1, 1, 2, 0, w1, w0);
+
+    // chunk groups 1 .. put their sums into LDS, group 0 adds them to its own in their order and stores
+    if constexpr (WK > 1) {
+        float* const sums = reinterpret_cast<float*>(lds);
+        if (wk > 0)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    *reinterpret_cast<f4*>(sums + ((((wk - 1) * WN + wn) * MT + i) * NT + t) * 256 + lane * 4) = acc[i][t];
+        __syncthreads();
+        if (wk > 0) return;
+        for (int g = 0; g < WK - 1; ++g)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    acc[i][t] += *reinterpret_cast<const f4*>(sums + (((g * WN + wn) * MT + i) * NT + t) * 256 + lane * 4);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = row0 + 16 * i + quad * 4 + r;
+            if (row < p.M)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const int64_t n = (int64_t)(strip0 + t) * kStrip + col;
+                    if (n < p.N) store(p.out, p.out_dtype, row * p.out_row_stride + n, acc[i][t][r]);
+                }
+        }
 }
 
 // One 16-byte piece of the packed weight a thread: lane l of (strip, chunk) holds column l % 16, and in word k the rows
@@ -222,36 +431,51 @@ bool good_weight(int32_t K, int32_t N, int32_t g) {
 }
 constexpr int64_t kMaxGrid = 0x7FFFFF;  // workgroups of one launch: with 512 threads below 2^32 work-items
 
-template <int AT, int MT, int NT>
-void launch(const Params& p, const Plan& pl, int spc, hipStream_t s) {
-    const dim3 grid((unsigned)pl.grid), block(64 * pl.waves);
-    const size_t lds = (size_t)pl.waves * MT * NT * 256 * sizeof(float);
+template <int AT, int MT, int NT, int WN, int WK>
+void launch_block(const Params& p, const Plan& pl, int spc, hipStream_t s) {
+    const dim3 grid((unsigned)pl.grid), block(64 * WN * WK);
     if (spc == 1)
-        hipLaunchKernelGGL((w4a16_kernel<AT, MT, NT, 1>), grid, block, lds, s, p);
+        hipLaunchKernelGGL((w4a16_block_kernel<AT, MT, NT, 1, WN, WK>), grid, block, 0, s, p);
     else if (spc == 2)
-        hipLaunchKernelGGL((w4a16_kernel<AT, MT, NT, 2>), grid, block, lds, s, p);
+        hipLaunchKernelGGL((w4a16_block_kernel<AT, MT, NT, 2, WN, WK>), grid, block, 0, s, p);
     else
-        hipLaunchKernelGGL((w4a16_kernel<AT, MT, NT, 4>), grid, block, lds, s, p);
+        hipLaunchKernelGGL((w4a16_block_kernel<AT, MT, NT, 4, WN, WK>), grid, block, 0, s, p);
 }
 
 template <int AT, int MT>
-void launch(const Params& p, const Plan& pl, int spc, hipStream_t s) {
-    if (pl.nt == 1)
-        launch<AT, MT, 1>(p, pl, spc, s);
-    else if (pl.nt == 2)
-        launch<AT, MT, 2>(p, pl, spc, s);
+void launch_block(const Params& p, const Plan& pl, int spc, hipStream_t s) {
+    if (pl.shape == kBlock256)
+        launch_block<AT, MT, 2, 8, 1>(p, pl, spc, s);
+    else if (pl.shape == kBlock128)
+        launch_block<AT, MT, 2, 4, 2>(p, pl, spc, s);
     else
-        launch<AT, MT, 4>(p, pl, spc, s);
+        launch_block<AT, MT, 1, 4, 2>(p, pl, spc, s);
+}
+
+template <int AT, int MT, int NT>
+void launch_strips(const Params& p, const Plan& pl, int spc, hipStream_t s) {
+    const dim3 grid((unsigned)pl.grid), block(64 * pl.waves);
+    const size_t lds = (size_t)pl.waves * MT * NT * 256 * sizeof(float);
+    if (spc == 1)
+        hipLaunchKernelGGL((w4a16_strip_kernel<AT, MT, NT, 1>), grid, block, lds, s, p);
+    else if (spc == 2)
+        hipLaunchKernelGGL((w4a16_strip_kernel<AT, MT, NT, 2>), grid, block, lds, s, p);
+    else
+        hipLaunchKernelGGL((w4a16_strip_kernel<AT, MT, NT, 4>), grid, block, lds, s, p);
 }
 
 template <int AT>
 void launch(const Params& p, const Plan& pl, int spc, hipStream_t s) {
-    if (pl.mt == 1)
-        launch<AT, 1>(p, pl, spc, s);
+    if (pl.shape != kStrips)
+        pl.mt == 2 ? launch_block<AT, 2>(p, pl, spc, s) : launch_block<AT, 4>(p, pl, spc, s);
+    else if (pl.mt == 1)
+        pl.nt == 1   ? launch_strips<AT, 1, 1>(p, pl, spc, s)
+        : pl.nt == 2 ? launch_strips<AT, 1, 2>(p, pl, spc, s)
+                     : launch_strips<AT, 1, 4>(p, pl, spc, s);
     else if (pl.mt == 2)
-        launch<AT, 2>(p, pl, spc, s);
+        launch_strips<AT, 2, 1>(p, pl, spc, s);
     else
-        launch<AT, 4>(p, pl, spc, s);
+        launch_strips<AT, 4, 1>(p, pl, spc, s);
 }
 
 }  // namespace
@@ -311,7 +535,7 @@ int w4a16_matmul(const w4a16_args* x, void* stream) {
     if (!w4::aligned(x->a, 16) || !w4::aligned(x->weight, 16) || !w4::aligned(x->scales, 16) || x->a_row_stride % 8 ||
         !w4::aligned(x->out, x->out_dtype == W4A16_F32 ? 4 : 2))
         return WKV7_ERR_ALIGN;
-    if ((x->M > 1 && (x->a_row_stride < x->K || x->out_row_stride < x->N))) return WKV7_ERR_SHAPE;
+    if ((x->M > 1 && (x->a_row_stride < x->K || x->a_row_stride > W4A16_MAX_ROW_STRIDE || x->out_row_stride < x->N))) return WKV7_ERR_SHAPE;
     const w4::Plan pl = w4::plan(x->M, x->N, x->K, wkv7::device_cu_count());
     if (pl.grid > w4::kMaxGrid) return WKV7_ERR_SHAPE;
     w4::Params p;

@@ -22,21 +22,39 @@ inline size_t scale_bytes(int32_t K, int32_t N, int32_t group_k) {
     return (size_t)(strips(N) * chunks(K)) * kStrip * scales_per_chunk(group_k) * 2;
 }
 
-// How a product runs: a workgroup computes 16 mt rows by 16 nt columns, its `waves` wavefronts share K.
+// How a product runs: by strips (a workgroup's wavefronts share K, each reading A for itself) or by blocks of 256, 128 or 64
+// columns (they share A in LDS).
+enum Shape { kStrips, kBlock256, kBlock128, kBlock64 };
 struct Plan {
-    int mt, nt, waves;
+    Shape shape;
+    int mt, nt, waves;  // 16 mt rows; kStrips: 16 nt columns, shared by `waves` wavefronts
     int64_t row_groups, strip_groups, grid;
 };
 
+inline int64_t groups(int32_t N, int columns) { return ((int64_t)N + columns - 1) / columns; }
+
+// Up to 16 rows strips, as wide as leaves every CU two workgroups: A is little, and 16 columns read it as fast as 256 (4096 x
+// 65536, one row: 28.5 us, blocks of 256 columns 36).  From 17 rows on A's share of the reading decides: the widest blocks of
+// which every CU gets one, and the narrowest while every second CU does (64 rows, K = 4096, strips / blocks: N = 65536 93 / 62 us,
+// 16384 40 / 24.3; K = 2560, N = 10240 34 / 15.6; but N = 4096, 64 blocks, 19.1 / 21.5).
 inline Plan plan(int32_t M, int32_t N, int32_t K, int cus) {
     Plan p;
     p.mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
     p.row_groups = ((int64_t)M + 16 * p.mt - 1) / (16 * p.mt);
-    p.nt = 4;
-    while (p.nt > 1 && (strips(N) + p.nt - 1) / p.nt * p.row_groups < 2 * cus) p.nt /= 2;
-    p.strip_groups = (strips(N) + p.nt - 1) / p.nt;
-    p.waves = (int)std::min<int64_t>(p.mt == 4 && p.nt == 4 ? 4 : 8, chunks(K));
-    // strip groups are dealt to the eight XCDs in turn, the row groups of one of them following each other on one XCD
+    p.nt = 1;
+    p.waves = 8;
+    p.shape = M <= 16                                          ? kStrips
+              : groups(N, 256) * p.row_groups >= cus           ? kBlock256
+              : groups(N, 128) * p.row_groups >= cus           ? kBlock128
+              : 2 * groups(N, 64) * p.row_groups >= cus        ? kBlock64
+                                                               : kStrips;
+    if (p.shape == kStrips) {
+        if (M <= 16)
+            for (p.nt = 4; p.nt > 1 && groups(N, kStrip * p.nt) < 2 * cus;) p.nt /= 2;
+        p.waves = (int)std::min<int64_t>(8, chunks(K));
+    }
+    p.strip_groups = groups(N, p.shape == kBlock256 ? 256 : p.shape == kBlock128 ? 128 : p.shape == kBlock64 ? 64 : kStrip * p.nt);
+    // column groups are dealt to the eight XCDs in turn, the row groups of one of them following each other on one XCD
     p.grid = (p.strip_groups + 7) / 8 * 8 * p.row_groups;
     return p;
 }

@@ -58,6 +58,7 @@ W4A16_EXPORTED = ("w4a16_args_size", "w4a16_packed_size", "w4a16_pack", "w4a16_d
 W4A16_BF16 = 0
 W4A16_F16 = 1
 W4A16_F32 = 2
+W4A16_MAX_ROW_STRIDE = 1 << 24
 LOGITS_EXPORTED = ("logits_penalize_args_size", "logits_sample_args_size", "logits_sample_workspace_size",
                    "logits_penalize", "logits_sample")
 LOGITS_BF16 = 0

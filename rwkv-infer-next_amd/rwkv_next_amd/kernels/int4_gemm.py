@@ -151,7 +151,7 @@ def int4_matmul(a, packed: Int4Packed, *, out_dtype=None):
     if M == 0:
         return out
     row, ptr = x.stride(0) if M > 1 else K, x.data_ptr()
-    if x.stride(1) != 1 or row % 8 or row < K or ptr % 16:
+    if x.stride(1) != 1 or row % 8 or row < K or row > _lib.W4A16_MAX_ROW_STRIDE or ptr % 16:
         x = x.clone(memory_format=torch.contiguous_format)
         row, ptr = K, x.data_ptr()
     args = _lib.pack_w4a16(ptr, row, weight.data_ptr(), scales.data_ptr(), out.data_ptr(), N, M, N, K, g, _CODES[adt],
