@@ -16,7 +16,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kColumns = kThreads * 8;
 
-template <int DT>
+// BLOCK: more than one position; the next one's logits are asked for while this one's are worked on.
+template <int DT, bool BLOCK>
 __global__ __launch_bounds__(kThreads) void penalize_kernel(const logits_penalize_args p, uint32_t segments) {
     __shared__ int64_t found_id[kThreads];
     __shared__ float found_value[kThreads];
@@ -25,6 +26,20 @@ __global__ __launch_bounds__(kThreads) void penalize_kernel(const logits_penaliz
     const int64_t b = blockIdx.x / segments, first = (int64_t)(blockIdx.x % segments) * kColumns, v0 = first + 8 * tid;
     const int n = v0 >= p.V ? 0 : p.V - v0 < 8 ? (int)(p.V - v0) : 8;
     const bool reports = p.status && first == 0 && tid == 0;  // one thread a sequence
+
+    // The first position's logits and its mask are asked for before the parameters and the biases are known: a workgroup's time is
+    // its loads', one after another.
+    const char* in = static_cast<const char*>(p.logits) + b * p.in_seq_stride * element_bytes(DT);
+    char* out = static_cast<char*>(p.out) + b * p.out_seq_stride * element_bytes(p.out_dtype);
+    float x[8];
+    load8<DT>(in, v0, n, 0.f, x);
+    const auto mask_of = [&](int t) -> uint32_t {  // eight bits; all set without a mask
+        if (!p.mask) return 0xFF;
+        const int64_t row = b * p.T + t, m = p.mask_row ? p.mask_row[row] : row;
+        if (m >= p.mask_rows && reports) atomicOr(p.status, LOGITS_STATUS_ROW);
+        return m >= 0 && m < p.mask_rows && n > 0 ? reinterpret_cast<const uint8_t*>(p.mask + m * p.mask_stride)[v0 >> 3] : 0xFF;
+    };
+    uint32_t allowed = mask_of(0);
 
     const float rep = p.repetition ? p.repetition[b] : p.repetition_all;
     const float pres = p.presence ? p.presence[b] : p.presence_all;
@@ -78,27 +93,20 @@ __global__ __launch_bounds__(kThreads) void penalize_kernel(const logits_penaliz
         __syncthreads();
     }
 
-    const char* in = static_cast<const char*>(p.logits) + b * p.in_seq_stride * element_bytes(DT);
-    char* out = static_cast<char*>(p.out) + b * p.out_seq_stride * element_bytes(p.out_dtype);
-    for (int t = 0; t < p.T; ++t) {
-        if (t > 0 && p.drafts) {
+    for (int t = 0; t < (BLOCK ? p.T : 1); ++t) {
+        if (BLOCK && t > 0 && p.drafts) {
             const int64_t id = p.drafts[b * p.drafts_stride + t - 1];
             if (reports && id >= p.V) atomicOr(p.status, LOGITS_STATUS_TOKEN);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (id == v0 + j) c[j] += 1.f;
         }
-        uint32_t allowed = 0xFF;
-        if (p.mask) {
-            const int64_t row = b * p.T + t, m = p.mask_row ? p.mask_row[row] : row;
-            if (m >= p.mask_rows) {
-                if (reports) atomicOr(p.status, LOGITS_STATUS_ROW);
-            } else if (m >= 0 && n > 0) {
-                allowed = reinterpret_cast<const uint8_t*>(p.mask + m * p.mask_stride)[v0 >> 3];
-            }
+        float next[8];
+        uint32_t next_allowed = 0xFF;
+        if (BLOCK && t + 1 < p.T) {
+            load8<DT>(in + (t + 1) * p.in_pos_stride * element_bytes(DT), v0, n, 0.f, next);
+            next_allowed = mask_of(t + 1);
         }
-        float x[8];
-        load8<DT>(in + t * p.in_pos_stride * element_bytes(DT), v0, n, 0.f, x);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             if (penalised && c[j] > 0.f) x[j] = (x[j] > 0.f ? x[j] / rep : x[j] * rep) - (freq * c[j] + pres);
@@ -106,7 +114,20 @@ __global__ __launch_bounds__(kThreads) void penalize_kernel(const logits_penaliz
             if (!(allowed >> j & 1)) x[j] = -__builtin_inff();
         }
         store8(out + t * p.out_pos_stride * element_bytes(p.out_dtype), p.out_dtype, v0, n, x);
+        if (BLOCK) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = next[j];
+            allowed = next_allowed;
+        }
     }
+}
+
+template <int DT>
+void launch(const logits_penalize_args& p, dim3 grid, uint32_t segments, hipStream_t s) {
+    if (p.T > 1)
+        hipLaunchKernelGGL((penalize_kernel<DT, true>), grid, dim3(kThreads), 0, s, p, segments);
+    else
+        hipLaunchKernelGGL((penalize_kernel<DT, false>), grid, dim3(kThreads), 0, s, p, segments);
 }
 
 bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -136,15 +157,19 @@ int logits_penalize(const logits_penalize_args* a, void* stream) {
     const int64_t segments = ((int64_t)a->V + lg::kColumns - 1) / lg::kColumns;
     if (segments * a->B > 0xFFFFFF) return WKV7_ERR_SHAPE;  // 256 threads each: below 2^32 work-items
     logits_penalize_args p = *a;
-    if (!p.counts && !p.drafts) p.repetition = p.presence = p.frequency = nullptr, p.repetition_all = 1.f, p.presence_all = p.frequency_all = 0.f;
-    const dim3 grid((unsigned)(segments * a->B)), block(lg::kThreads);
+    if (!p.counts && !p.drafts) {  // nothing is counted
+        p.repetition = p.presence = p.frequency = nullptr;
+        p.repetition_all = 1.f;
+        p.presence_all = p.frequency_all = 0.f;
+    }
+    const dim3 grid((unsigned)(segments * a->B));
     const auto s = static_cast<hipStream_t>(stream);
     if (a->in_dtype == LOGITS_BF16)
-        hipLaunchKernelGGL((lg::penalize_kernel<LOGITS_BF16>), grid, block, 0, s, p, (uint32_t)segments);
+        lg::launch<LOGITS_BF16>(p, grid, (uint32_t)segments, s);
     else if (a->in_dtype == LOGITS_F16)
-        hipLaunchKernelGGL((lg::penalize_kernel<LOGITS_F16>), grid, block, 0, s, p, (uint32_t)segments);
+        lg::launch<LOGITS_F16>(p, grid, (uint32_t)segments, s);
     else
-        hipLaunchKernelGGL((lg::penalize_kernel<LOGITS_F32>), grid, block, 0, s, p, (uint32_t)segments);
+        lg::launch<LOGITS_F32>(p, grid, (uint32_t)segments, s);
     return static_cast<int>(hipGetLastError());
 }
 
