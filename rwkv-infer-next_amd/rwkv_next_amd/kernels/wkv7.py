@@ -355,9 +355,10 @@ STATUS_REASONS = {_lib.WKV7_STATUS_H0_SLOT: "initial-state slot index outside th
                                                "sequence stores or reads its state): the result depends on timing",
                   _lib.WKV7_STATUS_SEGMENT_WAIT: "the segmented prefill gave up waiting for a segment hand-off: "
                                                  "the results are wrong and the stream's workspace flags must be "
-                                                 "zeroed (reset_workspaces())",
-                  _lib.LOGITS_STATUS_ROW: "a slot outside the count table, or a mask row past the masks",
-                  _lib.LOGITS_STATUS_TOKEN: "a draft or bias token outside the vocabulary"}
+                                                 "zeroed (reset_workspaces())"}
+# the logit operators' bits of the same word (include/logits.h)
+LOGITS_STATUS_REASONS = {_lib.LOGITS_STATUS_ROW: "a slot outside the count table, or a mask row past the masks",
+                         _lib.LOGITS_STATUS_TOKEN: "a draft or bias token outside the vocabulary"}
 
 
 def check_status(status: torch.Tensor) -> None:
@@ -365,7 +366,10 @@ def check_status(status: torch.Tensor) -> None:
     graph capture and the hot loop)."""
     bits = int(status.reshape(-1)[0].item())
     if bits:
-        raise ValueError("wkv7: " + "; ".join(m for bit, m in STATUS_REASONS.items() if bits & bit))
+        wkv7 = [m for bit, m in STATUS_REASONS.items() if bits & bit]
+        logits = [m for bit, m in LOGITS_STATUS_REASONS.items() if bits & bit]
+        raise ValueError("; ".join(f"{name}: " + "; ".join(found) for name, found in (("wkv7", wkv7), ("logits", logits))
+                                   if found))
 
 
 def check_distinct_slots(slots: torch.Tensor, num_slots: int) -> None:
