@@ -4,6 +4,10 @@
 // carried from position to position, each draft adding one where it falls.  A bias list belongs to a whole row: every workgroup
 // picks the entries of its columns out of it, 256 at a time, in their order (so equal ids add up in order), and the thread that
 // owns the column adds them.
+//
+// Bound by memory where there is enough of it: V = 65536, 64 sequences of five positions, fp32 with counts and masks, 187 MB in
+// 41.9 us = 4.5 TB/s (a large copy moves 4.9); 64 sequences bf16, 33.6 MB in 9.3 us = 3.6 TB/s, a workgroup's three dependent
+// reads counting (10.1 us before the logits were asked for first); one sequence 3.6 us, a launch.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -85,8 +85,12 @@ __device__ __forceinline__ void store(void* out, int dtype, int64_t at, float x)
         static_cast<_Float16*>(out)[at] = (_Float16)x;
 }
 
-// A workgroup's wavefronts take the 128-row chunks of K in turn, each with sums of its own; they are added in LDS in the
-// wavefronts' order.
+// Strips, for up to 16 rows and narrow products: a workgroup's wavefronts take the 128-row chunks of K in turn, each with sums of
+// its own; they are added in LDS in the wavefronts' order.  A wavefront reads A in operand order by itself: for a few rows it is
+// little, and reads of the weights are what counts.  Measured (graph replays, weights cycled past the caches): 4096 x 65536, one row
+// 30 us = 4.6 TB/s where a large copy moves 4.9, bound by memory; 4096 x 4096, one row 4.2 us and 2560 x 10240, five rows 7.2 us,
+// bound by the trips to memory of a wavefront's two to four chunks, one after another.  Asked for a chunk ahead they took twice
+// the registers, and half the wavefronts were no faster (33 and 7.8 us for the first and last).
 template <int AT, int MT, int NT, int SPC>
 __global__ __launch_bounds__(512) void w4a16_strip_kernel(const Params p) {
     extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][MT * 16][NT * 16]
@@ -187,8 +191,12 @@ template <int MT, int WK>
 constexpr int kPanelStride = WK * kChunk * 2 + 16;  // bytes of a row of A's panel in LDS: 16 more, so 16 rows lie in different banks
 template <int MT, int WK>
 constexpr int kPanelBytes = 16 * MT * kPanelStride<MT, WK>;
-// A workgroup's WN WK wavefronts are WN groups of columns by WK groups of chunks: they share A, a panel of WK chunks at a time,
-// through LDS, which global loads fill by whole lines; each reads its own weights three panels deep.
+// Blocks, from 17 rows on: a workgroup's WN WK wavefronts are WN groups of columns by WK groups of chunks.  They share A, a panel of
+// WK chunks at a time, through LDS, which loads of whole lines fill (in operand order a load of A takes four times as long, and
+// every wavefront would read all of it); weights come two panels ahead into registers.  Measured: 64 rows, 4096 x 65536 57.7 us (93 by
+// strips), 203 rows, 2560 x 8191, groups of 32 24 us (33).  In the first the matrix cores work 37 % of the time, the vector units
+// 31 % and LDS 28 %, hardly at once: two wavefronts a SIMD is what registers and 256 workgroups leave.  A two panels ahead as well,
+// and four strips a wavefront at one wavefront a SIMD, were not faster (62 to 82 us).
 template <int AT, int MT, int NT, int SPC, int WN, int WK>
 __global__ __launch_bounds__(64 * WN * WK, 2) void w4a16_block_kernel(const Params p) {
     constexpr int kThreads = 64 * WN * WK;
