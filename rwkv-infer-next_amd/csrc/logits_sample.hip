@@ -676,6 +676,8 @@ hipError_t launch(const logits_sample_args& a, hipStream_t s) {
     const int64_t rows = (int64_t)a.B * a.T, segments = ((int64_t)a.V + kSegment - 1) / kSegment;
     RowState* const states = static_cast<RowState*>(a.workspace);
     uint64_t* const lists = reinterpret_cast<uint64_t*>(static_cast<char*>(a.workspace) + LOGITS_SAMPLE_STATE_BYTES);
+    // rows' own parameters decide what the gathering kernel does; where one for all says that nothing is searched, it is left out
+    const bool searches = a.noise && (a.top_k || a.top_p || (a.top_k_all > 0 && a.top_k_all < a.V) || a.top_p_all < 1.f);
     const int64_t at_once = std::min<int64_t>(kRowsAtOnce, 0xFFFFFF / segments);  // 256 threads each: below 2^32 work-items
     for (int64_t row0 = 0; row0 < rows; row0 += at_once) {
         const int64_t n = std::min(rows - row0, at_once);
@@ -683,7 +685,7 @@ hipError_t launch(const logits_sample_args& a, hipStream_t s) {
         const uint32_t seg = (uint32_t)segments;
         hipLaunchKernelGGL((max_kernel<DT, PIECES>), grid, block, 0, s, a, row0, seg, states);
         hipLaunchKernelGGL((weigh_kernel<DT, PIECES>), grid, block, 0, s, a, row0, seg, states);
-        hipLaunchKernelGGL((gather_kernel<DT, PIECES>), grid, block, 0, s, a, row0, seg, states, lists);
+        if (searches) hipLaunchKernelGGL((gather_kernel<DT, PIECES>), grid, block, 0, s, a, row0, seg, states, lists);
         hipLaunchKernelGGL((choose_kernel<DT>), dim3((unsigned)n), dim3(kThreads), 0, s, a, row0, states, lists);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;

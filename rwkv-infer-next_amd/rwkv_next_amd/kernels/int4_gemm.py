@@ -145,9 +145,10 @@ def int4_matmul(a, packed: Int4Packed, *, out_dtype=None):
     if weight.dtype is not torch.uint8 or scales.dtype is not torch.float16 or not weight.is_contiguous() or \
             not scales.is_contiguous() or (weight.numel(), scales.numel()) != _sizes(K, N, g):
         raise ValueError("the packed weight and scales are not prepack_int4's")
+    dev = a.device
     x = a if len(shape) == 2 else a.reshape(-1, K)
     M = x.size(0)
-    out = a.new_empty((*shape[:-1], N), dtype=odt)
+    out = torch.empty(*shape[:-1], N, dtype=odt, device=dev)
     if M == 0:
         return out
     row, ptr = x.stride(0) if M > 1 else K, x.data_ptr()
@@ -156,8 +157,8 @@ def int4_matmul(a, packed: Int4Packed, *, out_dtype=None):
         row, ptr = K, x.data_ptr()
     args = _lib.pack_w4a16(ptr, row, weight.data_ptr(), scales.data_ptr(), out.data_ptr(), N, M, N, K, g, _CODES[adt],
                            _CODES[odt])  # in the order of the fields
-    with on_device(a.device):
-        _lib.check(_lib.load().w4a16_matmul(args, stream_handle(a.device)))
+    with on_device(dev):
+        _lib.check(_lib.load().w4a16_matmul(args, stream_handle(dev)))
     return out
 
 

@@ -48,8 +48,7 @@ def _per_sequence(x, dtype, B, dev, name):
     """(pointer, scalar) of a parameter: a tensor of B entries, or a number (pointer 0)."""
     if not isinstance(x, torch.Tensor):
         return 0, x
-    if x.dtype is dtype and x.dim() == 1 and x.size(0) == B and (B == 1 or x.stride(0) == 1) and \
-            x.get_device() == dev.index:
+    if x.dtype is dtype and x.shape == (B,) and x.is_contiguous() and x.get_device() == dev.index:
         return x.data_ptr(), 0
     _on(x, dev, name)
     raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor of {B} entries "
@@ -132,7 +131,7 @@ def penalize_logits(logits, *, counts=None, slots=None, repetition=1.0, presence
         logits = logits.contiguous()
         _, _, _, seq_stride, pos_stride, _ = _shape(logits)
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
         out_seq, out_pos = (V, 0) if logits.dim() == 2 else (T * V, V)
     else:
         if not in_place:
@@ -256,9 +255,12 @@ def sample_logits(logits, noise=None, *, temperature=1.0, top_k=0, top_p=1.0, mi
     if counts is not None and three:
         raise ValueError("counts are kept for (B, V) logits: a block's accepted tokens are known only later")
     ct, ct_stride, ct_rows, ct_type, slots_p = _counts(counts, slots, B, V, dev)
-    lead = (B, T) if three else B
-    token = torch.empty(lead, dtype=torch.int64, device=dev)
-    logprob = torch.empty(lead, dtype=torch.float32, device=dev)
+    if three:
+        token = torch.empty(B, T, dtype=torch.int64, device=dev)
+        logprob = torch.empty(B, T, dtype=torch.float32, device=dev)
+    else:
+        token = torch.empty(B, dtype=torch.int64, device=dev)
+        logprob = torch.empty(B, dtype=torch.float32, device=dev)
     if not (B and T):
         return token, logprob
     with on_device(dev):
