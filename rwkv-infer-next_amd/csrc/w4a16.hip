@@ -85,19 +85,20 @@ __device__ __forceinline__ void store(void* out, int dtype, int64_t at, float x)
         static_cast<_Float16*>(out)[at] = (_Float16)x;
 }
 
-// Strips, for up to 16 rows and narrow products: a workgroup's wavefronts take the 128-row chunks of K in turn, each with sums of
-// its own; they are added in LDS in the wavefronts' order.  A wavefront reads A in operand order by itself: for a few rows it is
-// little, and reads of the weights are what counts.  Measured (graph replays, weights cycled past the caches): 4096 x 65536, one row
-// 30 us = 4.6 TB/s where a large copy moves 4.9, bound by memory; 4096 x 4096, one row 4.2 us and 2560 x 10240, five rows 7.2 us,
-// bound by the trips to memory of a wavefront's two to four chunks, one after another.  Asked for a chunk ahead they took twice
-// the registers, and half the wavefronts were no faster (33 and 7.8 us for the first and last).
-template <int AT, int MT, int NT, int SPC>
+// Strips, for up to 16 rows and for narrow products of more: a workgroup's wavefronts take the 128-row chunks of K in turn, each with
+// sums of its own; they are added in LDS in the wavefronts' order.  A wavefront reads A in operand order by itself, so 16 rows of A go
+// with up to 64 columns.  Measured (graph replays, weights cycled past the caches): 4096 x 65536, one row 28.6 us = 4.8 TB/s
+// where a large copy moves 4.9, bound by memory; 4096 x 4096, one row 4.2 us and 2560 x 10240, five rows 6.5 us, bound by the
+// trips to memory of a wavefront's two to four chunks, one after another.  Asked for a chunk ahead they took twice the
+// registers, and half the wavefronts were no faster (33 and 7.8 us for the first and last).  Workgroups of 32 and 64 rows, whose
+// wavefronts use a weight's operands two and four times, were slower than more workgroups: 64 rows, 4096 x 4096 19 us against 9.2.
+template <int AT, int NT, int SPC>
 __global__ __launch_bounds__(512) void w4a16_strip_kernel(const Params p) {
-    extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][MT * 16][NT * 16]
+    extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][16][16 * NT]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const uint32_t on_xcd = blockIdx.x >> 3;
     const uint32_t group = on_xcd / (uint32_t)p.row_groups * 8 + (blockIdx.x & 7);
-    const int row0 = (int)(on_xcd % (uint32_t)p.row_groups) * 16 * MT;
+    const int row0 = (int)(on_xcd % (uint32_t)p.row_groups) * 16;
     if (group >= (uint32_t)p.strip_groups) return;
     const int strip0 = (int)group * NT, col = lane & 15, quad = lane >> 4;
 
@@ -109,22 +110,17 @@ __global__ __launch_bounds__(512) void w4a16_strip_kernel(const Params p) {
         wp[t] = p.weight + s * p.chunks * kBlockBytes + lane * 16;
         sp[t] = p.scales + (s * p.chunks * kStrip + col) * SPC;
     }
-    const uint16_t* ap[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)  // past the last row: that row again, not stored
-        ap[i] = p.a + (int64_t)min(row0 + 16 * i + col, p.M - 1) * p.a_row_stride;
+    const uint16_t* const ap = p.a + (int64_t)min(row0 + col, p.M - 1) * p.a_row_stride;  // past the last row: it again, not stored
 
-    f4 acc[MT][NT];
+    f4 acc[NT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[i][t] = f4{0.f, 0.f, 0.f, 0.f};
-    const uint32_t one = AT == W4A16_BF16 ? 0x3F803F80u : 0x3C003C00u;
-    const u4 ones = {one, one, one, one};
+    for (int t = 0; t < NT; ++t) acc[t] = f4{0.f, 0.f, 0.f, 0.f};
+    const uint32_t m24 = AT == W4A16_BF16 ? 0xC1C0C1C0u : 0xCE00CE00u;  // -24
+    const u4 minus24 = {m24, m24, m24, m24};
     const Patterns pat = patterns<AT>();
 
     for (int c = wave; c < p.chunks; c += waves) {
-        u4 w[NT], a[MT][4];
+        u4 w[NT], a[4];
         float s[NT][SPC];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -133,54 +129,37 @@ __global__ __launch_bounds__(512) void w4a16_strip_kernel(const Params p) {
             for (int j = 0; j < SPC; ++j) s[t][j] = f16_to_f32(sp[t][(int64_t)c * kStrip * SPC + j]);
         }
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int at = c * kChunk + k * 32 + quad * 8;
-                a[i][k] = u4{0, 0, 0, 0};
-                if (at < p.K) a[i][k] = *reinterpret_cast<const u4*>(ap[i] + at);
-            }
-        const f4 zero = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < 4; ++k) {
+            const int at = c * kChunk + k * 32 + quad * 8;
+            a[k] = u4{0, 0, 0, 0};
+            if (at < p.K) a[k] = *reinterpret_cast<const u4*>(ap + at);
+        }
+        constexpr int kSteps = 4 / SPC;
 #pragma unroll
         for (int j = 0; j < SPC; ++j) {
-            f4 sum[MT];
+            f4 bias = {0.f, 0.f, 0.f, 0.f};  // -24 sum a, where each strip's sum begins
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                sum[i] = zero;
-#pragma unroll
-                for (int k = j * 4 / SPC; k < (j + 1) * 4 / SPC; ++k) sum[i] = mfma<AT>(a[i][k], ones, sum[i]);
-            }
+            for (int k = 0; k < kSteps; ++k) bias = mfma<AT>(a[j * kSteps + k], minus24, bias);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                f4 d[MT];
+                f4 d = bias;
 #pragma unroll
-                for (int i = 0; i < MT; ++i) d[i] = zero;
+                for (int k = 0; k < kSteps; ++k) d = mfma<AT>(a[j * kSteps + k], operands<AT>(w[t][j * kSteps + k], pat), d);
 #pragma unroll
-                for (int k = j * 4 / SPC; k < (j + 1) * 4 / SPC; ++k) {
-                    const u4 b = operands<AT>(w[t][k], pat);
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) d[i] = mfma<AT>(a[i][k], b, d[i]);
-                }
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        acc[i][t][r] = fmaf(s[t][j], fmaf(-24.f, sum[i][r], d[i][r]), acc[i][t][r]);
+                for (int r = 0; r < 4; ++r) acc[t][r] = fmaf(s[t][j], d[r], acc[t][r]);
             }
         }
     }
 
-    float* const mine = part + wave * (MT * NT * 256);
+    float* const mine = part + wave * (NT * 256);
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) mine[(16 * i + quad * 4 + r) * (16 * NT) + 16 * t + col] = acc[i][t][r];
+        for (int r = 0; r < 4; ++r) mine[(quad * 4 + r) * (16 * NT) + 16 * t + col] = acc[t][r];
     __syncthreads();
-    for (int e = threadIdx.x; e < MT * NT * 256; e += blockDim.x) {
+    for (int e = threadIdx.x; e < NT * 256; e += blockDim.x) {
         float x = 0.f;
-        for (int v = 0; v < waves; ++v) x += part[v * (MT * NT * 256) + e];
+        for (int v = 0; v < waves; ++v) x += part[v * (NT * 256) + e];
         const int row = row0 + e / (16 * NT);
         const int64_t n = (int64_t)strip0 * kStrip + e % (16 * NT);
         if (row < p.M && n < p.N) store(p.out, p.out_dtype, row * p.out_row_stride + n, x);
@@ -460,30 +439,26 @@ void launch_block(const Params& p, const Plan& pl, int spc, hipStream_t s) {
         launch_block<AT, MT, 1, 4, 2>(p, pl, spc, s);
 }
 
-template <int AT, int MT, int NT>
+template <int AT, int NT>
 void launch_strips(const Params& p, const Plan& pl, int spc, hipStream_t s) {
     const dim3 grid((unsigned)pl.grid), block(64 * pl.waves);
-    const size_t lds = (size_t)pl.waves * MT * NT * 256 * sizeof(float);
+    const size_t lds = (size_t)pl.waves * NT * 256 * sizeof(float);
     if (spc == 1)
-        hipLaunchKernelGGL((w4a16_strip_kernel<AT, MT, NT, 1>), grid, block, lds, s, p);
+        hipLaunchKernelGGL((w4a16_strip_kernel<AT, NT, 1>), grid, block, lds, s, p);
     else if (spc == 2)
-        hipLaunchKernelGGL((w4a16_strip_kernel<AT, MT, NT, 2>), grid, block, lds, s, p);
+        hipLaunchKernelGGL((w4a16_strip_kernel<AT, NT, 2>), grid, block, lds, s, p);
     else
-        hipLaunchKernelGGL((w4a16_strip_kernel<AT, MT, NT, 4>), grid, block, lds, s, p);
+        hipLaunchKernelGGL((w4a16_strip_kernel<AT, NT, 4>), grid, block, lds, s, p);
 }
 
 template <int AT>
 void launch(const Params& p, const Plan& pl, int spc, hipStream_t s) {
     if (pl.shape != kStrips)
         pl.mt == 2 ? launch_block<AT, 2>(p, pl, spc, s) : launch_block<AT, 4>(p, pl, spc, s);
-    else if (pl.mt == 1)
-        pl.nt == 1   ? launch_strips<AT, 1, 1>(p, pl, spc, s)
-        : pl.nt == 2 ? launch_strips<AT, 1, 2>(p, pl, spc, s)
-                     : launch_strips<AT, 1, 4>(p, pl, spc, s);
-    else if (pl.mt == 2)
-        launch_strips<AT, 2, 1>(p, pl, spc, s);
     else
-        launch_strips<AT, 4, 1>(p, pl, spc, s);
+        pl.nt == 1   ? launch_strips<AT, 1>(p, pl, spc, s)
+        : pl.nt == 2 ? launch_strips<AT, 2>(p, pl, spc, s)
+                     : launch_strips<AT, 4>(p, pl, spc, s);
 }
 
 }  // namespace

@@ -22,35 +22,37 @@ inline size_t scale_bytes(int32_t K, int32_t N, int32_t group_k) {
     return (size_t)(strips(N) * chunks(K)) * kStrip * scales_per_chunk(group_k) * 2;
 }
 
-// How a product runs: by strips (a workgroup's wavefronts share K, each reading A for itself) or by blocks of 256, 128 or 64
-// columns (they share A in LDS).
+// How a product runs: by strips (16 rows by 16 nt columns to a workgroup, whose wavefronts share K, each reading A for itself) or by
+// blocks (32 or 64 rows by 256, 128 or 64 columns, whose wavefronts share A in LDS).
 enum Shape { kStrips, kBlock256, kBlock128, kBlock64 };
 struct Plan {
     Shape shape;
-    int mt, nt, waves;  // 16 mt rows; kStrips: 16 nt columns, shared by `waves` wavefronts
+    int mt, nt, waves;  // 16 mt rows; kStrips: 16 nt columns, K shared by `waves` wavefronts
     int64_t row_groups, strip_groups, grid;
 };
 
 inline int64_t groups(int32_t N, int columns) { return ((int64_t)N + columns - 1) / columns; }
 
-// Up to 16 rows strips, as wide as leaves every CU two workgroups: A is little, and 16 columns read it as fast as 256 (4096 x
-// 65536, one row: 28.5 us, blocks of 256 columns 36).  From 17 rows on A's share of the reading decides: the widest blocks of
-// which every CU gets one, and the narrowest while every second CU does (64 rows, K = 4096, strips / blocks: N = 65536 93 / 62 us,
-// 16384 40 / 24.3; K = 2560, N = 10240 34 / 15.6; but N = 4096, 64 blocks, 19.1 / 21.5).
+// Blocks once there are more than 16 rows and enough of them for every CU, the widest first: A is then read once a block.  Below
+// that, strips of 16 rows: more workgroups, and as many columns to each as leave three CUs in five one.  us, K = 4096, strips /
+// blocks: 64 rows N = 65536 97 / 62, 16384 26.6 / 24.3, 4096 9.0 / 21.5; 256 rows N = 4096 24.1 / 22.6; 203 rows, K = 2560, N = 8191
+// 30.8 / 25.2; but N = 10240 64 rows, 160 blocks, 14.3 / 16.5.  Strips of 64 / 32 / 16 columns: 64 rows, K = N = 2560 (160, 320, 640
+// workgroups) 7.1 / 8.9 / 10.8; 24 rows, N = 4096 (128, 256, 512) 8.7 / 7.7 / 10.7; one row, N = 4096 (64, 128, 256) 8.0 / 6.2 / 5.4.
 inline Plan plan(int32_t M, int32_t N, int32_t K, int cus) {
     Plan p;
-    p.mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+    const int rows = M <= 32 ? 32 : 64;
+    const int64_t blocks = ((int64_t)M + rows - 1) / rows;
+    p.shape = M <= 16                          ? kStrips
+              : groups(N, 256) * blocks >= cus ? kBlock256
+              : groups(N, 128) * blocks >= cus ? kBlock128
+              : groups(N, 64) * blocks >= cus  ? kBlock64
+                                               : kStrips;
+    p.mt = p.shape == kStrips ? 1 : rows / 16;
     p.row_groups = ((int64_t)M + 16 * p.mt - 1) / (16 * p.mt);
     p.nt = 1;
     p.waves = 8;
-    p.shape = M <= 16                                          ? kStrips
-              : groups(N, 256) * p.row_groups >= cus           ? kBlock256
-              : groups(N, 128) * p.row_groups >= cus           ? kBlock128
-              : 2 * groups(N, 64) * p.row_groups >= cus        ? kBlock64
-                                                               : kStrips;
     if (p.shape == kStrips) {
-        if (M <= 16)
-            for (p.nt = 4; p.nt > 1 && groups(N, kStrip * p.nt) < 2 * cus;) p.nt /= 2;
+        for (p.nt = 4; p.nt > 1 && 5 * groups(N, kStrip * p.nt) * p.row_groups < 3 * cus;) p.nt /= 2;
         p.waves = (int)std::min<int64_t>(8, chunks(K));
     }
     p.strip_groups = groups(N, p.shape == kBlock256 ? 256 : p.shape == kBlock128 ? 128 : p.shape == kBlock64 ? 64 : kStrip * p.nt);
