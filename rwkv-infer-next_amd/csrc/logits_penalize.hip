@@ -2,12 +2,14 @@
 //
 // A workgroup owns 2048 columns of one sequence, eight to a thread, for all T positions: the columns' counts are read once and
 // carried from position to position, each draft adding one where it falls.  A bias list belongs to a whole row: every workgroup
-// picks the entries of its columns out of it, 256 at a time, in their order (so equal ids add up in order), and the thread that
-// owns the column adds them.
+// picks the entries of its columns out of it, 256 at a time, and adds them up in LDS.  Entries of one column are added in their order:
+// of those that are left the first takes the column, adds and leaves, until none is left (mostly after one turn).  One entry after
+// another, looked at by all threads, took 33 us a call where this takes 12.4 (16 sequences of two positions, V = 1500, 300
+// biases each).
 //
 // Bound by memory where there is enough of it: V = 65536, 64 sequences of five positions, fp32 with counts and masks, 187 MB in
-// 41.9 us = 4.5 TB/s (a large copy moves 4.9); 64 sequences bf16, 33.6 MB in 9.3 us = 3.6 TB/s, a workgroup's three dependent
-// reads counting (10.1 us before the logits were asked for first); one sequence 3.6 us, a launch.
+// 42.0 us = 4.5 TB/s (a large copy moves 4.9); 64 sequences bf16, 33.6 MB in 9.7 us = 3.5 TB/s, a workgroup's three dependent
+// reads and the biases' barriers counting; one sequence 4.0 us, a launch.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -23,10 +25,9 @@ constexpr int kColumns = kThreads * 8;
 // BLOCK: more than one position; the next one's logits are asked for while this one's are worked on.
 template <int DT, bool BLOCK>
 __global__ __launch_bounds__(kThreads) void penalize_kernel(const logits_penalize_args p, uint32_t segments) {
-    __shared__ int64_t found_id[kThreads];
-    __shared__ float found_value[kThreads];
-    __shared__ int wave_found[kThreads / 64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ float sums[kColumns];
+    __shared__ uint32_t turn[kColumns];  // of the entries of a column that are left, the first one's thread
+    const int tid = threadIdx.x;
     const int64_t b = blockIdx.x / segments, first = (int64_t)(blockIdx.x % segments) * kColumns, v0 = first + 8 * tid;
     const int n = v0 >= p.V ? 0 : p.V - v0 < 8 ? (int)(p.V - v0) : 8;
     const bool reports = p.status && first == 0 && tid == 0;  // one thread a sequence
@@ -68,33 +69,26 @@ __global__ __launch_bounds__(kThreads) void penalize_kernel(const logits_penaliz
     float bias[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) bias[j] = 0.f;
-    for (int i0 = 0; i0 < p.n_bias; i0 += kThreads) {
-        const int i = i0 + tid;
-        const int64_t id = i < p.n_bias ? p.bias_ids[b * p.bias_stride + i] : -1;
-        if (p.status && first == 0 && id >= p.V) atomicOr(p.status, LOGITS_STATUS_TOKEN);
-        const bool mine = id >= first && id < first + kColumns && id < p.V;
-        const uint64_t all = __ballot(mine);
-        if (lane == 0) wave_found[wave] = __popcll(all);
-        __syncthreads();
-        int at = __popcll(all & ((1ull << lane) - 1)), total = 0;
+    if (p.n_bias > 0) {
+        for (int e = tid; e < kColumns; e += kThreads) sums[e] = 0.f, turn[e] = ~0u;
+        for (int i0 = 0; i0 < p.n_bias; i0 += kThreads) {
+            const int i = i0 + tid;
+            const int64_t id = i < p.n_bias ? p.bias_ids[b * p.bias_stride + i] : -1;
+            if (p.status && first == 0 && id >= p.V) atomicOr(p.status, LOGITS_STATUS_TOKEN);
+            bool left = id >= first && id < first + kColumns && id < p.V;
+            const int column = left ? (int)(id - first) : 0;
+            const float add = left ? p.bias_values[b * p.bias_stride + i] : 0.f;
+            while (__syncthreads_or(left)) {
+                if (left) atomicMin(&turn[column], (uint32_t)tid);
+                __syncthreads();
+                const bool mine = left && turn[column] == (uint32_t)tid;
+                if (mine) sums[column] += add, left = false;
+                __syncthreads();
+                if (mine) turn[column] = ~0u;
+            }
+        }
 #pragma unroll
-        for (int w = 0; w < kThreads / 64; ++w) {
-            if (w < wave) at += wave_found[w];
-            total += wave_found[w];
-        }
-        if (mine) {
-            found_id[at] = id - v0 + 8 * tid;  // the column within the workgroup's
-            found_value[at] = p.bias_values[b * p.bias_stride + i];
-        }
-        __syncthreads();
-        for (int e = 0; e < total; ++e) {
-            const int at8 = (int)found_id[e] - 8 * tid;
-            const float add = found_value[e];
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (at8 == j) bias[j] += add;
-        }
-        __syncthreads();
+        for (int j = 0; j < 8; ++j) bias[j] = sums[8 * tid + j];
     }
 
     for (int t = 0; t < (BLOCK ? p.T : 1); ++t) {
