@@ -4,9 +4,9 @@
 //
 // The inner sums run on the matrix cores (16x16x32, fp32 accumulation).  A code becomes an operand without a conversion: put
 // into mantissa bits 3..6 (bf16) or 6..9 (fp16) of the pattern of 16.0, it reads as exactly 16 + u, two codes to one shift and
-// one and-or.  The 24 that this is too much is taken out once per sum: a product with a tile of ones gives sum_k a[m][k] in the
-// same lanes as the result, so   sum a q = sum a (16 + u) - 24 sum a.   All three are fp32 sums of exact products; of the
-// offsets that give whole numbers 16 is the smallest, so the subtraction cancels least.
+// one and-or.  The 24 that this is too much comes off once for all columns: a product with a tile of -24 gives -24 sum_k a[m][k] in
+// the lanes of the result, where each strip's sum begins:   sum a q = -24 sum a + sum a (16 + u).   All are fp32 sums of exact
+// products; of the offsets that give whole numbers 16 is the smallest, so the difference cancels least.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
