@@ -646,18 +646,20 @@ __global__ __launch_bounds__(kThreads, 4) void choose_kernel(const logits_sample
     const bool none = c.row.max == -__builtin_inff();  // nothing is allowed
     if (c.searches && !none) won = choose<DT>(s, c, state, lists + (int64_t)blockIdx.x * kList, token, won, total);
     if (won) token = ~(uint32_t)won;  // else greedy, or no noise was a number: the most likely token
+    // A token past the row comes only out of a workspace that calls used at the same time: no memory is touched for it.
+    const bool chosen = !none && token < (uint32_t)p.V;
     __syncthreads();
     if (threadIdx.x == 0) {
         state.max_key = state.total = state.won = 0;
         state.gathered = 0;
-        p.token[row] = none ? -1 : (int64_t)token;
+        p.token[row] = chosen ? (int64_t)token : -1;
         if (p.logprob) {
             float x[8];
-            load8<DT>(c.row.x, none ? 0 : token, 1, 0.f, x);
+            load8<DT>(c.row.x, chosen ? token : 0, 1, 0.f, x);
             p.logprob[row] =
-                none ? c.row.max : -distance(c.row, logit(x[0])) * (1.f / kPerUnit) - logf((float)total);
+                chosen ? -distance(c.row, logit(x[0])) * (1.f / kPerUnit) - logf((float)total) : -__builtin_inff();
         }
-        if (p.counts && !none) {
+        if (p.counts && chosen) {
             const int64_t slot = p.slots ? p.slots[c.b] : c.b;
             if (slot < 0 || slot >= p.counts_rows) {
                 if (p.status) atomicOr(p.status, LOGITS_STATUS_ROW);

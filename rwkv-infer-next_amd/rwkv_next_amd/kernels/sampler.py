@@ -13,6 +13,7 @@ left out (check_status names them).
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import torch
 
@@ -203,6 +204,9 @@ def penalize_logits(logits, *, counts=None, slots=None, repetition=1.0, presence
 
 
 _WORKSPACES: dict = {}  # (device index, stream handle) -> [buffer, zeroed in stream order, capture id]
+# A call's launches pass a row's state on through the stream's workspace, and the library runs without Python's lock: of threads
+# on one stream one at a time looks its workspace up and launches.
+_LAUNCHES = threading.Lock()
 _BYTES: dict = {}       # rows -> bytes of workspace
 
 
@@ -229,7 +233,8 @@ def sample_logits(logits, noise=None, *, temperature=1.0, top_k=0, top_p=1.0, mi
     the row's softmax at its temperature, before the filters (at a temperature of 1 in greedy rows).
 
     NaN counts as -inf, and tokens of -inf are never chosen; a row of nothing else gives -1 and -inf.  A row's result depends on
-    that row alone.  noise float32 in the logits' shape; top_k int32 where it is a tensor, the other parameters float32.
+    that row alone.  Calls of one stream share a workspace, from any threads; graphs captured on one stream share it too, and are
+    replayed one after another, or captured on streams of their own.  noise float32 in the logits' shape; top_k int32 where it is a tensor, the other parameters float32.
     counts (S, V) int32 or float32 with slots, for (B, V) logits: counts[slots[b], token] += 1, the next step's penalties.
     """
     B, T, V, seq_stride, pos_stride, last = _shape(logits)
@@ -263,7 +268,7 @@ def sample_logits(logits, noise=None, *, temperature=1.0, top_k=0, top_p=1.0, mi
         logprob = torch.empty(B, dtype=torch.float32, device=dev)
     if not (B and T):
         return token, logprob
-    with on_device(dev):
+    with on_device(dev), _LAUNCHES:
         ws = _workspace(B * T, V, dev)
         args = _lib.pack_sample(
             logits.data_ptr(), seq_stride, pos_stride, nz, nz_seq, nz_pos, t_p, k_p, p_p, m_p, token.data_ptr(),
