@@ -43,7 +43,7 @@ extern "C" {
 typedef struct logits_penalize_args {
     const void *logits;                      /* [B][T][V] */
     int64_t in_seq_stride, in_pos_stride;    /* elements */
-    void *out;                               /* [B][T][V]; may be `logits` itself (same type and strides) */
+    void *out;                               /* [B][T][V]; `logits` itself (same type and strides), or apart from it */
     int64_t out_seq_stride, out_pos_stride;  /* elements */
     const void *counts;                      /* NULL, or [counts_rows][V] */
     int64_t counts_stride, counts_rows;      /* elements between rows */

@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes
 import threading
 
+import numpy as np
 import torch
 
 from .. import _lib
@@ -76,6 +77,27 @@ def _overlaps(t):
     return False
 
 
+def _share_memory(a, b):
+    """Whether rows of two (B, V) or (B, T, V) tensors with contiguous rows have memory in common.  Where their address ranges
+    are apart, the usual case, at the cost of a few additions; else (columns of one buffer, say) by the rows' addresses."""
+    ranges = []
+    for t in (a, b):
+        if t.numel() == 0:
+            return False
+        at = t.data_ptr()
+        ranges.append((at, at + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()))
+    if ranges[0][1] <= ranges[1][0] or ranges[1][1] <= ranges[0][0]:
+        return False
+    starts = [np.sort((t.data_ptr() + t.element_size() * sum(
+        np.arange(n, dtype=np.int64).reshape(-1, *(1,) * (t.dim() - 2 - i)) * s
+        for i, (n, s) in enumerate(zip(t.shape[:-1], t.stride()[:-1])))).reshape(-1)) for t in (a, b)]
+    rows, others = starts
+    # of the rows of b that begin before a row of a ends, the last one: does it end after that row begins?
+    before = np.searchsorted(others, rows + a.shape[-1] * a.element_size(), side="left")
+    last = others[np.maximum(before - 1, 0)] + b.shape[-1] * b.element_size()
+    return bool(((before > 0) & (last > rows)).any())
+
+
 def _counts(counts, slots, B, V, dev):
     """(pointer, row stride, rows, type, slots' pointer) of a count table (S, V)."""
     if counts is None:
@@ -116,7 +138,7 @@ def penalize_logits(logits, *, counts=None, slots=None, repetition=1.0, presence
         x = -inf where the mask's bit of v is 0
 
     in fp32, rounded once.  Returns a new tensor of the logits' type, or fills and returns `out` (any of the three types;
-    `logits` itself for an update in place).
+    `logits` itself for an update in place, else apart from the logits).
 
     counts (S, V) int32 or float32, row slots[b] (int64; row b without slots) of sequence b; the reference's penalty table.
     drafts (B, >= T - 1) int64: the tokens fed at positions 1 .. T - 1, not yet in `counts` (negative: none).
@@ -140,9 +162,10 @@ def penalize_logits(logits, *, counts=None, slots=None, repetition=1.0, presence
             if out.shape != logits.shape or out.dtype not in _DTYPES or (out.stride(-1) != 1 and V > 1):
                 raise ValueError(f"out must be bfloat16, float16 or float32 {tuple(logits.shape)} with contiguous rows "
                                  f"(got {out.dtype} {tuple(out.shape)}, strides {out.stride()})")
-            if out.data_ptr() == logits.data_ptr() and out.numel() and (
-                    out.dtype != logits.dtype or out.stride() != logits.stride()):
-                raise ValueError("out over the logits must have their type and strides")
+            if (out.data_ptr() != logits.data_ptr() or out.dtype != logits.dtype or out.stride() != logits.stride()) and \
+                    _share_memory(out, logits):
+                raise ValueError("out may share memory with the logits only as the logits themselves: at their address, of their "
+                                 "type and strides")
         if _overlaps(out):
             raise ValueError(f"out must not share memory between its rows (strides {out.stride()})")
         out_seq, out_pos = out.stride(0), out.stride(1) if out.dim() == 3 else 0

@@ -55,3 +55,25 @@ def test_threads_launch_one_after_another(library, monkeypatch):
     for t in threads:
         t.join()
     assert library.calls == 12 and library.most == 1
+
+
+def _bytes(t):
+    at = torch.arange(t.untyped_storage().nbytes() // t.element_size()).as_strided(t.shape, t.stride(), t.storage_offset())
+    return {int(i) * t.element_size() + b for i in at.reshape(-1).unique() for b in range(t.element_size())}
+
+
+def test_shared_memory_is_found():
+    """Against the bytes that two views of one buffer have; out over the logits at another place is refused, before any launch."""
+    buf = torch.zeros(4000, dtype=torch.bfloat16)
+    views = [buf.as_strided(shape, stride, at) for shape, stride in [
+        ((3, 50), (50, 1)), ((3, 50), (100, 1)), ((3, 50), (120, 1)), ((1, 50), (7, 1)), ((4, 2, 25), (100, 50, 1)), ((2, 4, 25), (25, 50, 1)),
+        ((2, 3, 50), (0, 60, 1)), ((3, 1), (9, 1)), ((2, 0, 5), (9, 5, 1))] for at in (0, 8, 50, 58, 150, 500, 2)]
+    views += [v.view(torch.float32) for v in views if v.shape[-1] % 2 == 0 and v.storage_offset() % 2 == 0 and
+              all(s % 2 == 0 for s in v.stride()[:-1])]
+    seen = set()
+    for a in views:
+        for b in views:
+            want = bool(_bytes(a) & _bytes(b))
+            seen.add(want)
+            assert sampler._share_memory(a, b) == want, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
+    assert seen == {False, True}
