@@ -230,18 +230,17 @@ _WORKSPACES: dict = {}  # (device index, stream handle) -> [buffer, zeroed in st
 # A call's launches pass a row's state on through the stream's workspace, and the library runs without Python's lock: of threads
 # on one stream one at a time looks its workspace up and launches.
 _LAUNCHES = threading.Lock()
-_BYTES: dict = {}       # rows -> bytes of workspace
+_BYTES: list = []  # of the workspace, once it is known
 
 
-def _workspace(rows, V, dev):
-    """The workspace of the current stream (include/logits.h, logits_sample_workspace_size); see
-    `_workspace.stream_workspace`."""
-    n = _BYTES.get(rows)
-    if n is None:
+def _workspace(dev):
+    """The workspace of the current stream, see `_workspace.stream_workspace`: 20 MiB, which serve any number of rows (as many as a
+    set of launches takes).  One of a call's own rows alone would be replaced, and kept for captured graphs, whenever they grow."""
+    if not _BYTES:
         size = ctypes.c_size_t(0)
-        _lib.check(_lib.load().logits_sample_workspace_size(_lib.SampleArgs(B=rows, T=1, V=V), ctypes.byref(size)))
-        n = _BYTES[rows] = int(size.value)
-    return stream_workspace(_WORKSPACES, dev, n, _lib.LOGITS_SAMPLE_STATE_BYTES)
+        _lib.check(_lib.load().logits_sample_workspace_size(_lib.SampleArgs(B=2 ** 31 - 1, T=1, V=1), ctypes.byref(size)))
+        _BYTES.append(int(size.value))
+    return stream_workspace(_WORKSPACES, dev, _BYTES[0], _lib.LOGITS_SAMPLE_STATE_BYTES)
 
 
 def sample_logits(logits, noise=None, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, counts=None, slots=None,
@@ -292,7 +291,7 @@ def sample_logits(logits, noise=None, *, temperature=1.0, top_k=0, top_p=1.0, mi
     if not (B and T):
         return token, logprob
     with on_device(dev), _LAUNCHES:
-        ws = _workspace(B * T, V, dev)
+        ws = _workspace(dev)
         args = _lib.pack_sample(
             logits.data_ptr(), seq_stride, pos_stride, nz, nz_seq, nz_pos, t_p, k_p, p_p, m_p, token.data_ptr(),
             logprob.data_ptr(), ct, ct_stride, ct_rows, slots_p, _status(status, dev), ws.data_ptr(), ws.numel(), t, p, m,

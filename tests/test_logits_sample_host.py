@@ -1,7 +1,9 @@
 """sample_logits between its arguments and the library, without a GPU: tensors' sizes and strides are real, the library is a stand-in."""
 import contextlib
+import ctypes
 import threading
 import time
+import types
 
 import pytest
 
@@ -48,7 +50,7 @@ def library(monkeypatch):
 
 def test_threads_launch_one_after_another(library, monkeypatch):
     """A call's launches follow each other on the stream: two threads' calls do not mix them."""
-    monkeypatch.setattr(sampler, "_workspace", lambda rows, V, dev: torch.zeros(8))
+    monkeypatch.setattr(sampler, "_workspace", lambda *_: torch.zeros(8))
     threads = [threading.Thread(target=lambda: [sampler.sample_logits(_Logits(2, 8)) for _ in range(3)]) for _ in range(4)]
     for t in threads:
         t.start()
@@ -77,3 +79,28 @@ def test_shared_memory_is_found():
             seen.add(want)
             assert sampler._share_memory(a, b) == want, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
     assert seen == {False, True}
+
+
+def test_one_workspace_serves_any_number_of_rows(monkeypatch):
+    """Calls of ever more rows ask for the same bytes: nothing is replaced, and so nothing kept beside it."""
+    asked = set()
+
+    def note(cache, dev, nbytes, zero_bytes):
+        asked.add((nbytes, zero_bytes))
+        return torch.zeros(8)
+
+    monkeypatch.setattr(sampler, "stream_workspace", note)
+    monkeypatch.setattr(sampler, "on_device", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(sampler, "stream_handle", lambda dev: 0)
+    real, size = sampler._lib.load(), ctypes.c_size_t(0)
+    monkeypatch.setattr(sampler._lib, "load", lambda: types.SimpleNamespace(
+        logits_sample=lambda args, stream: 0, logits_sample_workspace_size=real.logits_sample_workspace_size))
+    for rows in (1, 132, 133, 134, 511, 512, 513, 5000):
+        sampler.sample_logits(_Logits(rows, 3))
+        sampler.sample_logits(_Logits(rows, 2, 3))
+    assert len(asked) == 1
+    nbytes, zero = asked.pop()
+    assert zero == sampler._lib.LOGITS_SAMPLE_STATE_BYTES
+    for rows in (1, 512, 10 ** 6):
+        args = sampler._lib.SampleArgs(B=rows, T=3, V=100)
+        assert real.logits_sample_workspace_size(ctypes.byref(args), ctypes.byref(size)) == 0 and size.value <= nbytes < 32 << 20
