@@ -49,6 +49,13 @@ def capture_id(stream: int) -> int:
     return int(cid.value)
 
 
+def retire(cache: dict) -> None:
+    """Takes every workspace out of `cache`, so that the next calls get new, zeroed ones; they are kept alive, since a captured
+    graph may still address them."""
+    _RETIRED.extend(entry[0] for entry in cache.values())
+    cache.clear()
+
+
 def stream_workspace(cache: dict, device, nbytes: int, zero_bytes: int):
     """The workspace of the current stream on `device` from `cache`, at least `nbytes` long, whose first `zero_bytes`
     are zero in stream order when the call that requested it runs.

@@ -19,7 +19,7 @@ import numpy as np
 import torch
 
 from .. import _lib
-from ._workspace import on_device, stream_handle, stream_workspace
+from ._workspace import on_device, retire, stream_handle, stream_workspace
 from .int4_gemm import Int4Packed, int4_matmul
 
 _DTYPES = {torch.bfloat16: _lib.LOGITS_BF16, torch.float16: _lib.LOGITS_F16, torch.float32: _lib.LOGITS_F32}
@@ -243,6 +243,12 @@ def _workspace(dev):
     return stream_workspace(_WORKSPACES, dev, _BYTES[0], _lib.LOGITS_SAMPLE_STATE_BYTES)
 
 
+def reset_workspaces() -> None:
+    """The next call of every stream gets a new, zeroed workspace (wkv7.reset_workspaces calls this too)."""
+    with _LAUNCHES:
+        retire(_WORKSPACES)
+
+
 def sample_logits(logits, noise=None, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, counts=None, slots=None,
                   status=None):
     """(tokens int64, log-probabilities float32), each (B,) or (B, T): one token for each row of the logits.
@@ -296,7 +302,10 @@ def sample_logits(logits, noise=None, *, temperature=1.0, top_k=0, top_p=1.0, mi
             logits.data_ptr(), seq_stride, pos_stride, nz, nz_seq, nz_pos, t_p, k_p, p_p, m_p, token.data_ptr(),
             logprob.data_ptr(), ct, ct_stride, ct_rows, slots_p, _status(status, dev), ws.data_ptr(), ws.numel(), t, p, m,
             max(-1, min(int(k), 2 ** 31 - 1)), B, T, V, _DTYPES[logits.dtype], ct_type)  # in the order of the fields
-        _lib.check(_lib.load().logits_sample(args, stream_handle(dev)))
+        rc = _lib.load().logits_sample(args, stream_handle(dev))
+        if rc > 0:  # a launch failed, after others perhaps: what they left in the workspace serves no further call
+            retire(_WORKSPACES)
+        _lib.check(rc)
     return token, logprob
 
 

@@ -36,8 +36,10 @@ _WORKSPACES: dict = {}  # (device index, stream handle) -> [workspace, flags zer
 
 
 def reset_workspaces() -> None:
-    """Drop the cached per-stream workspaces (the next call creates a zeroed one)."""
+    """Drop the cached per-stream workspaces of the recurrence and of sample_logits (the next call creates a zeroed one)."""
+    from . import sampler
     _WORKSPACES.clear()
+    sampler.reset_workspaces()
 
 HEAD_SIZE = 64      # every RWKV-7 model's head size: the specialised kernels
 MAX_HEAD_SIZE = 256  # other head sizes run the generic token-serial kernel

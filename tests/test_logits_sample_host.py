@@ -28,7 +28,7 @@ class _Library:
     """Stands for the shared library: notes how many calls are inside logits_sample at once."""
 
     def __init__(self):
-        self.inside = self.most = self.calls = 0
+        self.inside = self.most = self.calls = self.code = 0
 
     def logits_sample(self, args, stream):
         self.inside += 1
@@ -36,7 +36,10 @@ class _Library:
         self.most = max(self.most, self.inside)
         time.sleep(0.02)  # as the real one: other threads go on meanwhile
         self.inside -= 1
-        return 0
+        return self.code
+
+    def wkv7_strerror(self, code):
+        return b"refused"
 
 
 @pytest.fixture
@@ -104,3 +107,22 @@ def test_one_workspace_serves_any_number_of_rows(monkeypatch):
     for rows in (1, 512, 10 ** 6):
         args = sampler._lib.SampleArgs(B=rows, T=3, V=100)
         assert real.logits_sample_workspace_size(ctypes.byref(args), ctypes.byref(size)) == 0 and size.value <= nbytes < 32 << 20
+
+
+def test_a_workspace_is_given_up_after_a_failed_launch_and_on_request(library, monkeypatch):
+    from rwkv_next_amd.kernels import _workspace, wkv7
+    ws = torch.zeros(8)
+    monkeypatch.setattr(sampler, "_workspace", lambda *_: ws)
+    monkeypatch.setattr(sampler, "_WORKSPACES", {(0, 0): [ws, True, None]})
+    monkeypatch.setattr(_workspace, "_RETIRED", [])
+    for code, left in ((0, 1), (sampler._lib.WKV7_ERR_SHAPE, 1), (1, 0)):  # done, refused before any launch, an error of a launch
+        library.code = code
+        if code:
+            with pytest.raises(sampler._lib.Wkv7Error):
+                sampler.sample_logits(_Logits(2, 8))
+        else:
+            sampler.sample_logits(_Logits(2, 8))
+        assert len(sampler._WORKSPACES) == left and len(_workspace._RETIRED) == 1 - left
+    sampler._WORKSPACES[0, 0] = [ws, True, None]
+    wkv7.reset_workspaces()
+    assert not sampler._WORKSPACES and len(_workspace._RETIRED) == 2  # captured graphs may still address them
