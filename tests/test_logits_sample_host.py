@@ -110,7 +110,8 @@ def test_one_workspace_serves_any_number_of_rows(monkeypatch):
 
 
 def test_a_workspace_is_given_up_after_a_failed_launch_and_on_request(library, monkeypatch):
-    from rwkv_next_amd.kernels import _workspace, wkv7
+    from rwkv_next_amd.kernels import _workspace
+    from rwkv_next_amd.kernels.wkv7 import reset_workspaces
     ws = torch.zeros(8)
     monkeypatch.setattr(sampler, "_workspace", lambda *_: ws)
     monkeypatch.setattr(sampler, "_WORKSPACES", {(0, 0): [ws, True, None]})
@@ -124,5 +125,5 @@ def test_a_workspace_is_given_up_after_a_failed_launch_and_on_request(library, m
             sampler.sample_logits(_Logits(2, 8))
         assert len(sampler._WORKSPACES) == left and len(_workspace._RETIRED) == 1 - left
     sampler._WORKSPACES[0, 0] = [ws, True, None]
-    wkv7.reset_workspaces()
+    reset_workspaces()
     assert not sampler._WORKSPACES and len(_workspace._RETIRED) == 2  # captured graphs may still address them
