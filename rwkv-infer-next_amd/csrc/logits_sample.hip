@@ -52,10 +52,13 @@ static_assert(LOGITS_SAMPLE_MAX_V == 1 << 21 && kCountAt > kWeightBits + 21 && k
 // A row's part of the workspace: all zero between calls.  The rows' lists, which need not be, follow the kRowsAtOnce of them.
 struct RowState {
     unsigned long long max_key;  // order_bits(max) << 32 | ~index
-    unsigned long long total;    // sum of the weights
+    unsigned long long total;    // sum of the weights, of whole()s
     unsigned long long won;      // the draw so far: w / noise as an integer << 32 | ~index
     uint32_t gathered;           // entries of the list
-    uint32_t unused[57];
+    uint32_t bin;                // a Part's bin, target and n, written by the gathering workgroup of the row's first segment
+    unsigned long long target;
+    uint32_t n;
+    uint32_t unused[53];
     unsigned long long bins[kBins];
 };
 static_assert(sizeof(RowState) * kRowsAtOnce == LOGITS_SAMPLE_STATE_BYTES, "include/logits.h");
@@ -342,16 +345,20 @@ __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_
 // Where a row's last kept token lies, from its histogram: in bin [from, to) of 32 d, where the prefix that ends with it has to
 // reach `target` tokens (top-k) or units of the bin (top-p) beside what lies before the bin.  The candidates' list begins at d_lo:
 // with top-k at 0, since top-p looks at them all again; with top-p alone at the bin, what lies before it being kept.
+// All gathering workgroups of a row make it of the same sums in the same order, and the choosing one takes it from the first of
+// them: sums in another order may be a last place apart, and so a bin.
 struct Part {
-    float d_lo, from, to;
+    uint32_t bin, n;  // n: candidates
     uint64_t target;
-    uint32_t n;    // candidates
-    double total;  // of the row's weights
+    __device__ float from() const { return bin > 0 ? end_of_bin(bin - 1) : 0.f; }
+    __device__ float to() const { return end_of_bin(bin); }
+    __device__ float d_lo(const Choice& c) const { return c.k > 0 ? 0.f : from(); }
 };
 
-template <int THREADS>
-__device__ __forceinline__ Part part_of(Scratch<THREADS>& s, const Choice& c, const RowState& state, bool wants_total) {
-    constexpr int kEach = kBins / THREADS;
+// `total`: of the row's weights, where the part needs it or wants_total.
+__device__ __forceinline__ Part part_of(Scratch<kSegThreads>& s, const Choice& c, const RowState& state, bool wants_total,
+                                        double& total) {
+    constexpr int kEach = kBins / kSegThreads;
     uint32_t counts[kEach], n;
     uint64_t numbers[kEach];
     double sums[kEach], all = 0;
@@ -364,8 +371,8 @@ __device__ __forceinline__ Part part_of(Scratch<THREADS>& s, const Choice& c, co
         all += sums[j];
     }
     Part part;
-    part.total = 0;
-    if (c.k <= 0 || wants_total) part.total = block_reduce(s, all, plus<double>);
+    total = 0;
+    if (c.k <= 0 || wants_total) total = block_reduce(s, all, plus<double>);
     if (c.k > 0) {
         uint64_t base;
         const uint32_t b = reaching_bin(s, numbers, counts, (uint64_t)c.k, base, n);
@@ -375,14 +382,14 @@ __device__ __forceinline__ Part part_of(Scratch<THREADS>& s, const Choice& c, co
             for (int j = 0; j < kEach; ++j) mine += numbers[j];
             base = block_reduce(s, mine, plus<uint64_t>);
         }
-        part.from = b > 0 ? end_of_bin(b - 1) : 0.f, part.to = end_of_bin(b), part.d_lo = 0.f;
+        part.bin = b;
         part.target = (uint64_t)c.k - (b == kBins ? 0 : base);
         part.n = (uint32_t)base + n;
     } else {
         double base;
-        const uint32_t b = reaching_bin(s, sums, counts, fmax((double)c.top_p * part.total, 1e-300), base, n);
-        part.from = b > 0 ? end_of_bin(b - 1) : 0.f, part.to = end_of_bin(b), part.d_lo = part.from;
-        const double rest = ceil(((double)c.top_p * part.total - base) / unit_of_bin(b));
+        const uint32_t b = reaching_bin(s, sums, counts, fmax((double)c.top_p * total, 1e-300), base, n);
+        part.bin = b;
+        const double rest = ceil(((double)c.top_p * total - base) / unit_of_bin(b));
         part.target = rest >= 1.0 ? (uint64_t)rest : 1;
         part.n = b == kBins ? kList + 1 : n;  // past all bins only if someone writes the logits meanwhile
     }
@@ -405,8 +412,14 @@ __global__ __launch_bounds__(kSegThreads) void gather_kernel(const logits_sample
     const uint32_t top = ~(uint32_t)max_key;
     c.row.max = from_order((uint32_t)(max_key >> 32));
     if (c.row.max == -__builtin_inff()) return;
-    const Part part = part_of(s, c, state, false);
+    double total;
+    const Part part = part_of(s, c, state, first == 0, total);
+    if (first == 0 && tid == 0) {
+        state.bin = part.bin, state.n = part.n, state.target = part.target;
+        state.total = (unsigned long long)(total * (double)kOne);
+    }
     if (part.n > kList) return;  // the choosing workgroup's work
+    const float d_lo = part.d_lo(c);
 
     float nearest[PIECES];  // x becomes 32 d, nearest a piece's smallest
 #pragma unroll
@@ -419,27 +432,27 @@ __global__ __launch_bounds__(kSegThreads) void gather_kernel(const logits_sample
     }
     float best = 0.f;
     uint32_t where = 0;
-    if (part.d_lo > 0.f) {  // kept for sure
+    if (d_lo > 0.f) {  // kept for sure
         float e[PIECES][8];
 #pragma unroll
         for (int a = 0; a < PIECES; ++a) {
             const int64_t i = first + (a * kSegThreads + tid) * 8;
-            load8<LOGITS_F32>(c.noise, i, nearest[a] < part.d_lo ? piece(i, p.V) : 0, 1.f, e[a]);
+            load8<LOGITS_F32>(c.noise, i, nearest[a] < d_lo ? piece(i, p.V) : 0, 1.f, e[a]);
         }
 #pragma unroll
         for (int a = 0; a < PIECES; ++a)
-            if (nearest[a] < part.d_lo)
+            if (nearest[a] < d_lo)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const uint32_t i = (uint32_t)(first + (a * kSegThreads + tid) * 8 + j);
                     const float w = weight(x[a][j]);
-                    if (x[a][j] < part.d_lo && w > 0.f && (w >= c.min_p || i == top)) draw(w, e[a][j], i, best, where);
+                    if (x[a][j] < d_lo && w > 0.f && (w >= c.min_p || i == top)) draw(w, e[a][j], i, best, where);
                 }
         const uint64_t key = wave_reduce(draw_key(best, where), larger);
         if ((tid & 63) == 0 && key) atomicMax(&state.won, (unsigned long long)key);
     }
     // bits of non-negative floats order as they do
-    const uint32_t from = __float_as_uint(part.d_lo), span = __float_as_uint(part.to) - from;
+    const uint32_t from = __float_as_uint(d_lo), span = __float_as_uint(part.to()) - from;
     uint32_t hits = 0;  // a bit for each of the 8 PIECES elements, the first the highest
 #pragma unroll
     for (int a = 0; a < PIECES; ++a)
@@ -554,18 +567,15 @@ __device__ uint64_t last_kept(Shared& s, All&& all, uint64_t lo, uint64_t hi, ui
 
 constexpr uint64_t kEveryKey = (uint64_t)kInfBits << 32;  // past every token that can be drawn
 
-// The choice in a row with top-k or top-p, as draw_key; `won`: the draw among the tokens that the gathering workgroups kept;
-// `total` becomes the sum of the row's weights.
+// The choice in a row with top-k or top-p, as draw_key; `won`: the draw among the tokens that the gathering workgroups kept.
 template <int DT>
-__device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const uint64_t* list, uint32_t top, uint64_t won,
-                           double& total) {
+__device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const uint64_t* list, uint32_t top, uint64_t won) {
     const int tid = threadIdx.x;
     uint64_t mine[kOwn];  // asked for before it is known how many of them are there
 #pragma unroll
     for (int j = 0; j < kOwn; ++j) mine[j] = list[tid + j * kThreads];
     const uint32_t n = min(state.gathered, (uint32_t)kList);
-    const Part part = part_of(s.scratch, c, state, true);
-    total = part.total;
+    const Part part = {state.bin, state.n, state.target};
     for (int b = tid; b < kBins; b += kThreads) state.bins[b] = 0;
     float best = 0.f;
     uint32_t where = 0;
@@ -607,7 +617,7 @@ __device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const ui
         for (int j = 0; j < kOwn; ++j)
             if (key[j] <= limit) f(key[j]);
     };
-    const uint64_t lo = key_of(part.from, 0), hi = key_of(part.to, 0);
+    const uint64_t lo = key_of(part.from(), 0), hi = key_of(part.to(), 0);
     if (c.k > 0) {
         if (n > (uint32_t)c.k) limit = last_kept<kNumber, false>(s, all, lo, hi, part.target, limit);
         if (c.top_p < 1.f) {
@@ -640,18 +650,18 @@ __global__ __launch_bounds__(kThreads, 4) void choose_kernel(const logits_sample
     Choice c = choice_of<DT>(p, row);
     const uint64_t max_key = state.max_key;
     uint64_t won = state.won;
-    double total = (double)state.total * (1.0 / kOne);
+    const double total = (double)state.total * (1.0 / kOne);
     uint32_t token = ~(uint32_t)max_key;
     c.row.max = from_order((uint32_t)(max_key >> 32));
     const bool none = c.row.max == -__builtin_inff();  // nothing is allowed
-    if (c.searches && !none) won = choose<DT>(s, c, state, lists + (int64_t)blockIdx.x * kList, token, won, total);
+    if (c.searches && !none) won = choose<DT>(s, c, state, lists + (int64_t)blockIdx.x * kList, token, won);
     if (won) token = ~(uint32_t)won;  // else greedy, or no noise was a number: the most likely token
     // A token past the row comes only out of a workspace that calls used at the same time: no memory is touched for it.
     const bool chosen = !none && token < (uint32_t)p.V;
     __syncthreads();
     if (threadIdx.x == 0) {
-        state.max_key = state.total = state.won = 0;
-        state.gathered = 0;
+        state.max_key = state.total = state.won = state.target = 0;
+        state.gathered = state.bin = state.n = 0;
         p.token[row] = chosen ? (int64_t)token : -1;
         if (p.logprob) {
             float x[8];
