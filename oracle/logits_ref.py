@@ -51,7 +51,7 @@ def choices_ref(x, noise, temperature, top_k, top_p, min_p, slack):
         return set(), np.full(V, -np.inf)
     x = np.minimum(x, np.finfo(np.float32).max)
     greedy = noise is None or not temperature > 0
-    d = (x.max() - x) / (temperature if temperature > 0 else 1.0)
+    d = (x.max() - x) / (1.0 if greedy else temperature)
     w = np.exp(-d)
     logprob = -d - np.log(w.sum())
     if greedy:

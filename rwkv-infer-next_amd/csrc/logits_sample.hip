@@ -222,7 +222,7 @@ __device__ __forceinline__ Choice choice_of(const logits_sample_args& p, int64_t
     c.row.x = static_cast<const char*>(p.logits) + (c.b * p.seq_stride + c.t * p.pos_stride) * element_bytes(DT);
     c.row.V = p.V;
     c.row.max = 0.f;
-    c.row.inv = kPerUnit * (temperature > 0.f ? fminf(fmaxf(1.f / temperature, 1e-25f), 1e30f) : 1.f);
+    c.row.inv = kPerUnit * (c.greedy ? 1.f : fminf(fmaxf(1.f / temperature, 1e-25f), 1e30f));
     c.noise = p.noise + c.b * p.noise_seq_stride + c.t * p.noise_pos_stride;
     c.k = p.top_k ? p.top_k[c.b] : p.top_k_all;
     if (c.k < 0 || c.k >= p.V) c.k = 0;

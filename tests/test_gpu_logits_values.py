@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+import oracle
 from gpu_util import say
 
 torch = pytest.importorskip("torch")
@@ -12,6 +13,22 @@ DEV = "cuda:0"
 
 def _dev(x):
     return torch.from_numpy(np.ascontiguousarray(x)).to(DEV)
+
+
+def test_greedy_rows_have_a_temperature_of_one():
+    """Rows without noise are greedy: whatever their temperature, the log-probability is that of the plain softmax."""
+    from rwkv_next_amd import kernels
+    say("sample greedy log-probabilities")
+    rng = np.random.default_rng(1)
+    x = (rng.standard_normal((5, 1, 3001)) * 3).astype(np.float32)
+    logits = _dev(x[:, 0])
+    want, want_lp = kernels.sample_logits(logits)
+    for t in (0.6, 2.5, torch.tensor([0.3, 0.0, 1.0, 7.0, -1.0], device=DEV)):
+        token, logprob = kernels.sample_logits(logits, temperature=t, top_k=4, top_p=0.7)
+        assert torch.equal(token, want) and torch.equal(logprob, want_lp)
+    for b in range(5):
+        ok, lp = oracle.logits_ref.choices_ref(x[b, 0], None, 0.6, 0, 1.0, 0.0, 1e-6)
+        assert ok == {int(want[b])} and abs(float(want_lp[b]) - lp[int(want[b])]) <= 1e-5 * (1 + abs(lp[int(want[b])]))
 
 
 def test_top_p_at_a_bins_end():
