@@ -315,7 +315,10 @@ __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_
             if (bins[b]) atomicAdd(&state.bins[b], (unsigned long long)bins[b]);
     } else {
         const bool draws = !c.greedy;
-        float total = 0.f, best = 0.f;
+        // Eight neighbours' weights are added in order and then taken as a whole number: the same sum whatever the segments' length,
+        // which follows from the number of rows.
+        uint64_t total = 0;
+        float best = 0.f;
         uint32_t where = 0;
         float e[PIECES][8];
         if (draws)
@@ -325,19 +328,22 @@ __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_
                 load8<LOGITS_F32>(c.noise, i, piece(i, p.V), 1.f, e[a]);
             }
 #pragma unroll
-        for (int a = 0; a < PIECES; ++a)
+        for (int a = 0; a < PIECES; ++a) {
+            float eight = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float w = weight(distance(c.row, x[a][j]));
-                total += w;
+                eight += w;
                 if (draws && w >= c.min_p && w > 0.f)
                     draw(w, e[a][j], (uint32_t)(first + (a * kSegThreads + tid) * 8 + j), best, where);
             }
+            total += whole(eight);
+        }
         if (draws) {
             const uint64_t key = wave_reduce(draw_key(best, where), larger);
             if ((tid & 63) == 0 && key) atomicMax(&state.won, (unsigned long long)key);
         }
-        const uint64_t sum = wave_reduce(whole(total), plus<uint64_t>);
+        const uint64_t sum = wave_reduce(total, plus<uint64_t>);
         if ((tid & 63) == 0) atomicAdd(&state.total, (unsigned long long)sum);
     }
 }

@@ -31,6 +31,26 @@ def test_greedy_rows_have_a_temperature_of_one():
         assert ok == {int(want[b])} and abs(float(want_lp[b]) - lp[int(want[b])]) <= 1e-5 * (1 + abs(lp[int(want[b])]))
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(min_p=0.01), dict(top_p=0.9), dict(top_k=40)])
+def test_a_row_has_the_same_bits_beside_others(kw):
+    """80 rows of 66000 go by segments of 8192 elements, one row by segments of 2048.  In every other row only such tokens are allowed
+    as one thread of a long segment has, four of a short one's."""
+    from rwkv_next_amd import kernels
+    say("sample rows by themselves", kw)
+    rng = np.random.default_rng(2)
+    x = (rng.standard_normal((80, 66000)) * 2).astype(np.float32)
+    near = np.arange(66000) % 2048 < 8
+    near[8192:] = False
+    x[::2, ~near] = -np.inf
+    x, noise = _dev(x), _dev(rng.exponential(size=(80, 66000)).astype(np.float32))
+    temperature = _dev(rng.uniform(0.5, 1.8, 80).astype(np.float32))
+    temperature[7] = 0
+    token, logprob = kernels.sample_logits(x, noise, temperature=temperature, **kw)
+    for b in range(80):
+        one, one_lp = kernels.sample_logits(x[b:b + 1], noise[b:b + 1], temperature=temperature[b:b + 1].clone(), **kw)
+        assert int(one) == int(token[b]) and float(one_lp) == float(logprob[b]), b
+
+
 def test_top_p_at_a_bins_end():
     """The first bin's weight is half of all, to the last bit of the sums: whether that reaches a top-p of a half or needs one token more,
     it never takes all of the next bin.  Logits are at the starts of bins, 32nds below the largest, so many tokens at each."""
