@@ -71,7 +71,7 @@ typedef struct logits_penalize_args {
  * largest logit's lowest index.  NaN counts as -infinity, and tokens of -infinity are never chosen: a row of nothing else gives
  * -1 and a log-probability of -infinity.
  * logprob = -d - log(sum of w over the row), before the filters, with a temperature of 1 in greedy rows.
- * What is added up by atomics are whole numbers (of 2^-20 of a bin's weights, of 2^-40): their order changes no result.
+ * What is added up by atomics are whole numbers (of 2^-20 or less of a bin's first weight, of 2^-40): their order changes no result.
  * V is at most LOGITS_SAMPLE_MAX_V. */
 #define LOGITS_SAMPLE_MAX_V 2097152
 typedef struct logits_sample_args {

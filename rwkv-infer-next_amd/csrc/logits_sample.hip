@@ -13,8 +13,8 @@
 // into finer parts.
 //
 // d is kept as 32 d (bins are its whole part), which the scaling by a power of two leaves as exact as d.  A bin's weights are
-// added up as whole numbers of 2^-20 of the weight at its start, beside its tokens' number in one 64-bit word: one atomic to a
-// token.
+// added up as whole numbers of 2^-24 of the weight at its start (the last place of an fp32 weight; 2^-23 .. 2^-20 where there are more
+// than 2^17 tokens), beside its tokens' number in one 64-bit word: one atomic to a token.
 //
 // Measured, V = 65536, us of max / weigh / gather / choose: one row fp32 with top-p 3.4 / 4.4 / 5.7 / 7.7 (19.3 together in a graph),
 // each bound by its chain of dependent reads; 64 rows with top-k and top-p 5.7 / 7.2 / 6.4 / 11.6; 320 rows bf16 with a wide nucleus
@@ -45,9 +45,15 @@ constexpr int kRowsAtOnce = 512;   // rows of one set of launches
 constexpr float kOne = 1099511627776.f;  // 2^40: a weight of 1
 constexpr uint32_t kInfBits = 0x7F800000u;
 constexpr float kExp2PerBin = -1.44269504088896341f / kPerUnit;  // w = 2^(32 d * this)
-// A bin's word: its tokens' number above their weights, each below 2^20 + 1 times the bin's first: 2^21 tokens at most.
-constexpr int kWeightBits = 20, kCountAt = 42;
-static_assert(LOGITS_SAMPLE_MAX_V == 1 << 21 && kCountAt > kWeightBits + 21 && kCountAt + 22 <= 64, "");
+// A bin's word: its tokens' number above their weights, each at most 2^weight_bits(V), V of them below 2^42.
+constexpr int kCountAt = 42;
+constexpr int weight_bits(int V) {
+    int bits = 24;
+    while ((int64_t)V << bits > (int64_t)1 << (kCountAt - 1)) --bits;
+    return bits;
+}
+static_assert(weight_bits(1 << 17) == 24 && weight_bits((1 << 17) + 1) == 23 && weight_bits(LOGITS_SAMPLE_MAX_V) == 20 &&
+              LOGITS_SAMPLE_MAX_V < 1 << (64 - kCountAt), "");
 
 // A row's part of the workspace: all zero between calls.  The rows' lists, which need not be, follow the kRowsAtOnce of them.
 struct RowState {
@@ -187,12 +193,13 @@ __device__ __forceinline__ float from_order(uint32_t u) { return __uint_as_float
 
 __device__ __forceinline__ float distance(const Row& r, float x) { return (r.max - x) * r.inv; }  // 32 d >= 0
 __device__ __forceinline__ float weight(float d32) { return __builtin_amdgcn_exp2f(d32 * kExp2PerBin); }
-__device__ __forceinline__ uint64_t whole(float w) { return (uint64_t)(w * kOne); }
-// A weight in its bin's units, and the unit.
-__device__ __forceinline__ uint32_t in_bin(float d32) {
-    return (uint32_t)__builtin_amdgcn_exp2f(fmaf(__builtin_amdgcn_fractf(d32), kExp2PerBin, (float)kWeightBits));
+// Whole numbers are the nearest ones: what is cut off would lean all sums to one side.
+__device__ __forceinline__ uint64_t whole(float w) { return (uint64_t)rintf(w * kOne); }
+// A weight in its bin's units, `units` = 2^weight_bits(V) of them to the bin's first weight, and the unit.
+__device__ __forceinline__ uint32_t in_bin(float d32, float units) {
+    return (uint32_t)rintf(__builtin_amdgcn_exp2f(__builtin_amdgcn_fractf(d32) * kExp2PerBin) * units);
 }
-__device__ __forceinline__ double unit_of_bin(uint32_t b) { return (double)weight((float)b) * (1.0 / (1 << kWeightBits)); }
+__device__ __forceinline__ double unit_of_bin(uint32_t b, float units) { return (double)weight((float)b) * (1.0 / units); }
 // The first 32 d past a bin; every finite one lies before the last bin's.
 __device__ __forceinline__ float end_of_bin(uint32_t b) { return b >= kBins - 1 ? __builtin_inff() : (float)(b + 1); }
 
@@ -206,6 +213,7 @@ struct Choice {
     const float* noise;
     int k;                  // 0: no top-k
     float top_p, min_p;
+    float units;            // of a bin's first weight
     bool greedy, searches;  // searches: top-k or top-p
     __device__ uint64_t want(uint64_t sum) const {  // the weight that a top-p prefix has to reach, of whole()s
         const double x = (double)top_p * (double)sum;
@@ -214,7 +222,7 @@ struct Choice {
 };
 
 template <int DT>
-__device__ __forceinline__ Choice choice_of(const logits_sample_args& p, int64_t row) {
+__device__ __forceinline__ Choice choice_of(const logits_sample_args& p, int64_t row, float units) {
     Choice c;
     c.b = row / p.T, c.t = row % p.T;
     const float temperature = p.temperature ? p.temperature[c.b] : p.temperature_all;
@@ -228,6 +236,7 @@ __device__ __forceinline__ Choice choice_of(const logits_sample_args& p, int64_t
     if (c.k < 0 || c.k >= p.V) c.k = 0;
     c.top_p = p.top_p ? p.top_p[c.b] : p.top_p_all;
     c.min_p = fminf(p.min_p ? p.min_p[c.b] : p.min_p_all, 1.f);
+    c.units = units;
     c.searches = !c.greedy && (c.k > 0 || c.top_p < 1.f);
     return c;
 }
@@ -249,11 +258,11 @@ __device__ __forceinline__ void load_segment(const Row& r, int64_t first, float 
 }
 
 template <int DT, int PIECES>
-__global__ __launch_bounds__(kSegThreads) void max_kernel(const logits_sample_args p, int64_t row0, uint32_t segments,
+__global__ __launch_bounds__(kSegThreads) void max_kernel(const logits_sample_args p, int64_t row0, float units, uint32_t segments,
                                                           RowState* states) {
     const uint32_t at = blockIdx.x / segments;
     const int64_t first = (int64_t)(blockIdx.x % segments) * (kSegThreads * PIECES * 8);
-    const Choice c = choice_of<DT>(p, row0 + at);
+    const Choice c = choice_of<DT>(p, row0 + at, units);
     float x[PIECES][8];
     load_segment<DT, PIECES>(c.row, first, x);
     float m = x[0][0];
@@ -282,14 +291,14 @@ __device__ __forceinline__ uint64_t draw_key(float best, uint32_t where) {  // 0
 }
 
 template <int DT, int PIECES>
-__global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_args p, int64_t row0, uint32_t segments,
+__global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_args p, int64_t row0, float units, uint32_t segments,
                                                             RowState* states) {
     __shared__ uint64_t bins[kBins];
     const int tid = threadIdx.x;
     const uint32_t at = blockIdx.x / segments;
     const int64_t first = (int64_t)(blockIdx.x % segments) * (kSegThreads * PIECES * 8);
     RowState& state = states[at];
-    Choice c = choice_of<DT>(p, row0 + at);
+    Choice c = choice_of<DT>(p, row0 + at, units);
     float x[PIECES][8];
     load_segment<DT, PIECES>(c.row, first, x);
     c.row.max = from_order((uint32_t)(state.max_key >> 32));
@@ -304,7 +313,7 @@ __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_
             for (int j = 0; j < 8; ++j) {
                 const float d = distance(c.row, x[a][j]);
                 if (d < (float)(kBins - 1))
-                    atomicAdd((unsigned long long*)&bins[(uint32_t)fmaxf(d, 0.f)], 1ull << kCountAt | in_bin(d));
+                    atomicAdd((unsigned long long*)&bins[(uint32_t)fmaxf(d, 0.f)], 1ull << kCountAt | in_bin(d, c.units));
                 else
                     far += d < __builtin_inff();
             }
@@ -373,7 +382,7 @@ __device__ __forceinline__ Part part_of(Scratch<kSegThreads>& s, const Choice& c
         const uint32_t b = threadIdx.x * kEach + j;
         const uint64_t word = state.bins[b];
         numbers[j] = counts[j] = (uint32_t)(word >> kCountAt);
-        sums[j] = (double)(word & ((1ull << kCountAt) - 1)) * unit_of_bin(b);
+        sums[j] = (double)(word & ((1ull << kCountAt) - 1)) * unit_of_bin(b, c.units);
         all += sums[j];
     }
     Part part;
@@ -395,7 +404,7 @@ __device__ __forceinline__ Part part_of(Scratch<kSegThreads>& s, const Choice& c
         double base;
         const uint32_t b = reaching_bin(s, sums, counts, fmax((double)c.top_p * total, 1e-300), base, n);
         part.bin = b;
-        const double rest = ceil(((double)c.top_p * total - base) / unit_of_bin(b));
+        const double rest = ceil(((double)c.top_p * total - base) / unit_of_bin(b, c.units));
         part.target = rest >= 1.0 ? (uint64_t)rest : 1;
         part.n = b == kBins ? kList + 1 : n;  // past all bins only if someone writes the logits meanwhile
     }
@@ -403,14 +412,14 @@ __device__ __forceinline__ Part part_of(Scratch<kSegThreads>& s, const Choice& c
 }
 
 template <int DT, int PIECES>
-__global__ __launch_bounds__(kSegThreads) void gather_kernel(const logits_sample_args p, int64_t row0, uint32_t segments,
+__global__ __launch_bounds__(kSegThreads) void gather_kernel(const logits_sample_args p, int64_t row0, float units, uint32_t segments,
                                                              RowState* states, uint64_t* lists) {
     __shared__ Scratch<kSegThreads> s;
     const int tid = threadIdx.x;
     const uint32_t at = blockIdx.x / segments;
     const int64_t first = (int64_t)(blockIdx.x % segments) * (kSegThreads * PIECES * 8);
     RowState& state = states[at];
-    Choice c = choice_of<DT>(p, row0 + at);
+    Choice c = choice_of<DT>(p, row0 + at, units);
     if (!c.searches) return;
     float x[PIECES][8];
     load_segment<DT, PIECES>(c.row, first, x);
@@ -518,7 +527,7 @@ enum Measure { kNumber, kUnits, kWhole };  // of a prefix: its tokens, their wei
 // `all(f)` (f(key) for each) with keys in [lo, hi); `none` where all do not reach it.  [lo, hi) is cut into 1024 parts, first
 // (BINS) by bins of d, until the part in which the target is reached has one token.
 template <Measure M, bool BINS, typename All>
-__device__ uint64_t last_kept(Shared& s, All&& all, uint64_t lo, uint64_t hi, uint64_t target, uint64_t none) {
+__device__ uint64_t last_kept(Shared& s, float units, All&& all, uint64_t lo, uint64_t hi, uint64_t target, uint64_t none) {
     constexpr int kEach = kBins / kThreads;
     const int tid = threadIdx.x;
     bool bins = BINS;
@@ -535,7 +544,7 @@ __device__ uint64_t last_kept(Shared& s, All&& all, uint64_t lo, uint64_t hi, ui
                 atomicAdd(&s.count[b], 1u);
                 if (M != kNumber)
                     atomicAdd((unsigned long long*)&s.weight[b],
-                              (unsigned long long)(M == kUnits ? in_bin(d) : whole(weight(d))));
+                              (unsigned long long)(M == kUnits ? in_bin(d, units) : whole(weight(d))));
             }
         });
         __syncthreads();
@@ -594,11 +603,11 @@ __device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const ui
                 if (key <= limit) f(key);
             });
         };
-        if (c.k > 0) limit = last_kept<kNumber, true>(s, all, 0, kEveryKey, (uint64_t)c.k, limit);
+        if (c.k > 0) limit = last_kept<kNumber, true>(s, c.units, all, 0, kEveryKey, (uint64_t)c.k, limit);
         if (c.top_p < 1.f) {
             uint64_t sum = 0;
             all([&](uint64_t key) { sum += whole(weight(d_of(key))); });
-            limit = last_kept<kWhole, true>(s, all, 0, kEveryKey, c.want(block_reduce(s.scratch, sum, plus<uint64_t>)), limit);
+            limit = last_kept<kWhole, true>(s, c.units, all, 0, kEveryKey, c.want(block_reduce(s.scratch, sum, plus<uint64_t>)), limit);
         }
         all([&](uint64_t key) {
             const float w = weight(d_of(key));
@@ -625,14 +634,14 @@ __device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const ui
     };
     const uint64_t lo = key_of(part.from(), 0), hi = key_of(part.to(), 0);
     if (c.k > 0) {
-        if (n > (uint32_t)c.k) limit = last_kept<kNumber, false>(s, all, lo, hi, part.target, limit);
+        if (n > (uint32_t)c.k) limit = last_kept<kNumber, false>(s, c.units, all, lo, hi, part.target, limit);
         if (c.top_p < 1.f) {
             uint64_t sum = 0;
             all([&](uint64_t k) { sum += whole(weight(d_of(k))); });
-            limit = last_kept<kWhole, true>(s, all, 0, hi, c.want(block_reduce(s.scratch, sum, plus<uint64_t>)), limit);
+            limit = last_kept<kWhole, true>(s, c.units, all, 0, hi, c.want(block_reduce(s.scratch, sum, plus<uint64_t>)), limit);
         }
     } else {
-        limit = last_kept<kUnits, false>(s, all, lo, hi, part.target, limit);
+        limit = last_kept<kUnits, false>(s, c.units, all, lo, hi, part.target, limit);
     }
 #pragma unroll
     for (int j = 0; j < kOwn; ++j)
@@ -648,12 +657,12 @@ __device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const ui
 }
 
 template <int DT>
-__global__ __launch_bounds__(kThreads, 4) void choose_kernel(const logits_sample_args p, int64_t row0, RowState* states,
+__global__ __launch_bounds__(kThreads, 4) void choose_kernel(const logits_sample_args p, int64_t row0, float units, RowState* states,
                                                           const uint64_t* lists) {
     __shared__ Shared s;
     const int64_t row = row0 + blockIdx.x;
     RowState& state = states[blockIdx.x];
-    Choice c = choice_of<DT>(p, row);
+    Choice c = choice_of<DT>(p, row, units);
     const uint64_t max_key = state.max_key;
     uint64_t won = state.won;
     const double total = (double)state.total * (1.0 / kOne);
@@ -696,15 +705,16 @@ hipError_t launch(const logits_sample_args& a, hipStream_t s) {
     uint64_t* const lists = reinterpret_cast<uint64_t*>(static_cast<char*>(a.workspace) + LOGITS_SAMPLE_STATE_BYTES);
     // rows' own parameters decide what the gathering kernel does; where one for all says that nothing is searched, it is left out
     const bool searches = a.noise && (a.top_k || a.top_p || (a.top_k_all > 0 && a.top_k_all < a.V) || a.top_p_all < 1.f);
+    const float units = (float)(1 << weight_bits(a.V));
     const int64_t at_once = std::min<int64_t>(kRowsAtOnce, 0xFFFFFF / segments);  // 256 threads each: below 2^32 work-items
     for (int64_t row0 = 0; row0 < rows; row0 += at_once) {
         const int64_t n = std::min(rows - row0, at_once);
         const dim3 grid((unsigned)(n * segments)), block(kSegThreads);
         const uint32_t seg = (uint32_t)segments;
-        hipLaunchKernelGGL((max_kernel<DT, PIECES>), grid, block, 0, s, a, row0, seg, states);
-        hipLaunchKernelGGL((weigh_kernel<DT, PIECES>), grid, block, 0, s, a, row0, seg, states);
-        if (searches) hipLaunchKernelGGL((gather_kernel<DT, PIECES>), grid, block, 0, s, a, row0, seg, states, lists);
-        hipLaunchKernelGGL((choose_kernel<DT>), dim3((unsigned)n), dim3(kThreads), 0, s, a, row0, states, lists);
+        hipLaunchKernelGGL((max_kernel<DT, PIECES>), grid, block, 0, s, a, row0, units, seg, states);
+        hipLaunchKernelGGL((weigh_kernel<DT, PIECES>), grid, block, 0, s, a, row0, units, seg, states);
+        if (searches) hipLaunchKernelGGL((gather_kernel<DT, PIECES>), grid, block, 0, s, a, row0, units, seg, states, lists);
+        hipLaunchKernelGGL((choose_kernel<DT>), dim3((unsigned)n), dim3(kThreads), 0, s, a, row0, units, states, lists);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

@@ -51,6 +51,38 @@ def test_a_row_has_the_same_bits_beside_others(kw):
         assert int(one) == int(token[b]) and float(one_lp) == float(logprob[b]), b
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=50), dict(top_p=0.9)])
+def test_sums_lean_to_no_side(kw):
+    """The mean error of 256 rows' log-probabilities at a temperature of 1, logits in whole 1024ths, so that every d is exact.  What may
+    lean to one side is the exponential instruction's last place, for a bin's first weight and for a weight in its bin, 2^-23 each;
+    roundings go both ways and leave less than 0.6e-7 in a mean over 256: 3e-7."""
+    from rwkv_next_amd import kernels
+    say("sample sums", kw)
+    rng = np.random.default_rng(3)
+    x = np.round(rng.standard_normal((256, 4096)) * 2048) / 1024
+    x[:, :40] += 4
+    noise = rng.exponential(size=x.shape)
+    token, logprob = kernels.sample_logits(_dev(x.astype(np.float32)), _dev(noise.astype(np.float32)), **kw)
+    d = x.max(axis=1, keepdims=True) - x
+    want = -d[np.arange(256), token.cpu().numpy()] - np.log(np.exp(-d).sum(axis=1))
+    error = (logprob.double().cpu().numpy() - want).mean()
+    assert abs(error) <= 3e-7, error
+
+
+@pytest.mark.parametrize("V", [131072, 131074, 600000, 2097152])
+def test_one_bin_of_a_whole_vocabulary(V):
+    """Equal logits: a bin's word holds V tokens at its first weight.  A top-p of a half keeps the first half, a top-k of k the first k;
+    the logarithm of V is off by its function's last place and a rounding: 2e-6."""
+    from rwkv_next_amd import kernels
+    say("sample one bin", V)
+    x, noise = torch.zeros(1, V, device=DEV), torch.ones(1, V, device=DEV)
+    for last, kw in ((V // 2 - 1, dict(top_p=0.5)), (V - 8, dict(top_k=V - 7)), (99, dict(top_k=100)), (V - 1, dict())):
+        noise[0, last:last + 2] = torch.tensor([1e-3, 1e-6], device=DEV)[:V - last]  # the token after the last one would win
+        token, logprob = kernels.sample_logits(x, noise, **kw)
+        assert int(token) == last and abs(float(logprob) + np.log(V)) <= 2e-6, kw
+        noise.fill_(1)
+
+
 def test_top_p_at_a_bins_end():
     """The first bin's weight is half of all, to the last bit of the sums: whether that reaches a top-p of a half or needs one token more,
     it never takes all of the next bin.  Logits are at the starts of bins, 32nds below the largest, so many tokens at each."""
