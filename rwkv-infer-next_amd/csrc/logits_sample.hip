@@ -192,7 +192,14 @@ __device__ __forceinline__ uint32_t order_bits(float x) {
 __device__ __forceinline__ float from_order(uint32_t u) { return __uint_as_float(u >> 31 ? u & 0x7FFFFFFFu : ~u); }
 
 __device__ __forceinline__ float distance(const Row& r, float x) { return (r.max - x) * r.inv; }  // 32 d >= 0
-__device__ __forceinline__ float weight(float d32) { return __builtin_amdgcn_exp2f(d32 * kExp2PerBin); }
+// 2^(32 d c): the product is rounded by up to 2^-19 for the rarest weights that matter, c itself by 2^-26 of it.  What both leave
+// out is `lo`, and 2^lo = 1 + lo ln 2.  (From 8192 on the weight is 0.)
+__device__ __forceinline__ float weight(float d32) {
+    constexpr float kRest = (float)(-1.44269504088896340736 / kPerUnit - (double)kExp2PerBin);
+    const float d = fminf(d32, 8192.f), hi = d * kExp2PerBin, lo = fmaf(d, kRest, fmaf(d, kExp2PerBin, -hi));
+    const float w = __builtin_amdgcn_exp2f(hi);
+    return fmaf(w, lo * 0.693147181f, w);
+}
 // Whole numbers are the nearest ones: what is cut off would lean all sums to one side.
 __device__ __forceinline__ uint64_t whole(float w) { return (uint64_t)rintf(w * kOne); }
 // A weight in its bin's units, `units` = 2^weight_bits(V) of them to the bin's first weight, and the unit.

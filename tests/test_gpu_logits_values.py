@@ -69,6 +69,30 @@ def test_sums_lean_to_no_side(kw):
     assert abs(error) <= 3e-7, error
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=2), dict(top_k=3, min_p=0.0)])
+def test_rare_tokens_have_their_weight(kw):
+    """Two tokens, d apart, their noise such that one's score is 5e-7 to 1.5e-6 above the other's.  A weight is off by the exponential
+    instruction's last place (2^-23) and two roundings, a score by one more: 3e-7 in all for a ratio of two."""
+    from rwkv_next_amd import kernels
+    say("sample rare tokens", kw)
+    rng = np.random.default_rng(4)
+    n = 3000
+    d = np.round(rng.uniform(1, 30, n) * 1024) / 1024
+    x = np.full((n, 16), -np.inf, np.float32)
+    x[:, 3], x[:, 9] = 0.0, -d
+    noise = np.ones((n, 16), np.float32)
+    noise[:, 3] = rng.uniform(0.5, 2, n)
+    noise[:, 9] = noise[:, 3] * np.exp(-d) * (1 + rng.choice([-1, 1], n) * rng.uniform(5.5e-7, 1.5e-6, n))
+    first, second = 1 / noise[:, 3].astype(np.float64), np.exp(-d) / noise[:, 9].astype(np.float64)
+    sure = np.abs(first / second - 1) >= 5e-7
+    assert sure.sum() > n * 0.9
+    token, _ = kernels.sample_logits(_dev(x), _dev(noise), **kw)
+    want = np.where(first > second, 3, 9)
+    got = token.cpu().numpy()
+    wrong = sure & (got != want)
+    assert not wrong.any(), (int(wrong.sum()), d[wrong][:8])
+
+
 @pytest.mark.parametrize("V", [131072, 131074, 600000, 2097152])
 def test_one_bin_of_a_whole_vocabulary(V):
     """Equal logits: a bin's word holds V tokens at its first weight.  A top-p of a half keeps the first half, a top-k of k the first k;
