@@ -193,10 +193,11 @@ __device__ __forceinline__ float from_order(uint32_t u) { return __uint_as_float
 
 __device__ __forceinline__ float distance(const Row& r, float x) { return (r.max - x) * r.inv; }  // 32 d >= 0
 // 2^(32 d c): the product is rounded by up to 2^-19 for the rarest weights that matter, c itself by 2^-26 of it.  What both leave
-// out is `lo`, and 2^lo = 1 + lo ln 2.  (From 8192 on the weight is 0.)
+// out is `lo`, and 2^lo = 1 + lo ln 2.  (NaN for infinity: no weight, or kFar in its place.)
+constexpr float kFar = 8192.f;  // of weight 0
 __device__ __forceinline__ float weight(float d32) {
     constexpr float kRest = (float)(-1.44269504088896340736 / kPerUnit - (double)kExp2PerBin);
-    const float d = fminf(d32, 8192.f), hi = d * kExp2PerBin, lo = fmaf(d, kRest, fmaf(d, kExp2PerBin, -hi));
+    const float hi = d32 * kExp2PerBin, lo = fmaf(d32, kRest, fmaf(d32, kExp2PerBin, -hi));
     const float w = __builtin_amdgcn_exp2f(hi);
     return fmaf(w, lo * 0.693147181f, w);
 }
@@ -287,15 +288,24 @@ __global__ __launch_bounds__(kSegThreads) void max_kernel(const logits_sample_ar
     if ((threadIdx.x & 63) == 0) atomicMax(&states[at].max_key, (unsigned long long)key);
 }
 
-// The better of a draw so far and of element i: the largest w / noise, NaN never; where indexes come upwards the first of equals
-// stays.  The reciprocal is the hardware's (1 ulp): both sides of a comparison have it.
-__device__ __forceinline__ void draw(float w, float noise, uint32_t i, float& best, uint32_t& where) {
-    const float score = w * __builtin_amdgcn_rcpf(noise);
-    if (score > best) best = score, where = i;
-}
-__device__ __forceinline__ uint64_t draw_key(float best, uint32_t where) {  // 0: nothing drawn
-    return best > 0.f ? (uint64_t)__float_as_uint(best) << 32 | (uint32_t)~where : 0;
-}
+// The best of a draw so far: the largest w / noise, of equals the first that was offered; nothing to begin with, and never an
+// element whose noise is negative or no number.  Quotients are compared as the products of one's weight and the other's noise: equal ones
+// are then equal, and an element costs no division (weights are at most 1, so no product is too large).
+struct Draw {
+    float w = 0.f, noise = 1.f;
+    uint32_t where = 0;
+    __device__ __forceinline__ void offer(float w1, float noise1, uint32_t i) {
+        if (w1 * noise > w * noise1 && noise1 >= 0.f) w = w1, noise = noise1, where = i;
+    }
+    __device__ __forceinline__ void offer_in_any_order(float w1, float noise1, uint32_t i) {
+        const float mine = w1 * noise, best = w * noise1;
+        if ((mine > best || (mine == best && i < where)) && noise1 >= 0.f) w = w1, noise = noise1, where = i;
+    }
+    __device__ __forceinline__ uint64_t key() const {  // 0: nothing drawn
+        const float score = w / noise;
+        return score > 0.f ? (uint64_t)__float_as_uint(score) << 32 | (uint32_t)~where : 0;
+    }
+};
 
 template <int DT, int PIECES>
 __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_args p, int64_t row0, float units, uint32_t segments,
@@ -334,8 +344,7 @@ __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_
         // Eight neighbours' weights are added in order and then taken as a whole number: the same sum whatever the segments' length,
         // which follows from the number of rows.
         uint64_t total = 0;
-        float best = 0.f;
-        uint32_t where = 0;
+        Draw best;
         float e[PIECES][8];
         if (draws)
 #pragma unroll
@@ -348,15 +357,15 @@ __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_
             float eight = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float w = weight(distance(c.row, x[a][j]));
+                const float w = weight(fminf(distance(c.row, x[a][j]), kFar));
                 eight += w;
                 if (draws && w >= c.min_p && w > 0.f)
-                    draw(w, e[a][j], (uint32_t)(first + (a * kSegThreads + tid) * 8 + j), best, where);
+                    best.offer(w, e[a][j], (uint32_t)(first + (a * kSegThreads + tid) * 8 + j));
             }
             total += whole(eight);
         }
         if (draws) {
-            const uint64_t key = wave_reduce(draw_key(best, where), larger);
+            const uint64_t key = wave_reduce(best.key(), larger);
             if ((tid & 63) == 0 && key) atomicMax(&state.won, (unsigned long long)key);
         }
         const uint64_t sum = wave_reduce(total, plus<uint64_t>);
@@ -452,9 +461,8 @@ __global__ __launch_bounds__(kSegThreads) void gather_kernel(const logits_sample
 #pragma unroll
         for (int j = 1; j < 8; ++j) nearest[a] = fminf(nearest[a], x[a][j]);
     }
-    float best = 0.f;
-    uint32_t where = 0;
     if (d_lo > 0.f) {  // kept for sure
+        Draw best;
         float e[PIECES][8];
 #pragma unroll
         for (int a = 0; a < PIECES; ++a) {
@@ -468,9 +476,9 @@ __global__ __launch_bounds__(kSegThreads) void gather_kernel(const logits_sample
                 for (int j = 0; j < 8; ++j) {
                     const uint32_t i = (uint32_t)(first + (a * kSegThreads + tid) * 8 + j);
                     const float w = weight(x[a][j]);
-                    if (x[a][j] < d_lo && w > 0.f && (w >= c.min_p || i == top)) draw(w, e[a][j], i, best, where);
+                    if (x[a][j] < d_lo && w > 0.f && (w >= c.min_p || i == top)) best.offer(w, e[a][j], i);
                 }
-        const uint64_t key = wave_reduce(draw_key(best, where), larger);
+        const uint64_t key = wave_reduce(best.key(), larger);
         if ((tid & 63) == 0 && key) atomicMax(&state.won, (unsigned long long)key);
     }
     // bits of non-negative floats order as they do
@@ -599,8 +607,7 @@ __device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const ui
     const uint32_t n = min(state.gathered, (uint32_t)kList);
     const Part part = {state.bin, state.n, state.target};
     for (int b = tid; b < kBins; b += kThreads) state.bins[b] = 0;
-    float best = 0.f;
-    uint32_t where = 0;
+    Draw best;
 
     if (part.n > kList) {  // the long way
         uint64_t limit = kEveryKey - 1;
@@ -619,9 +626,9 @@ __device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const ui
         all([&](uint64_t key) {
             const float w = weight(d_of(key));
             const uint32_t i = (uint32_t)key;
-            if (w > 0.f && (w >= c.min_p || i == top)) draw(w, c.noise[i], i, best, where);
+            if (w > 0.f && (w >= c.min_p || i == top)) best.offer(w, c.noise[i], i);
         });
-        return block_reduce(s.scratch, draw_key(best, where), larger);
+        return block_reduce(s.scratch, best.key(), larger);
     }
 
     uint64_t key[kOwn];
@@ -655,12 +662,9 @@ __device__ uint64_t choose(Shared& s, const Choice& c, RowState& state, const ui
         if (key[j] <= limit) {
             const float w = weight(d_of(key[j]));
             const uint32_t i = (uint32_t)key[j];
-            if (w > 0.f && (w >= c.min_p || i == top)) {
-                const float score = w * __builtin_amdgcn_rcpf(noise[j]);
-                if (score > best || (score == best && score > 0.f && i < where)) best = score, where = i;
-            }
+            if (w > 0.f && (w >= c.min_p || i == top)) best.offer_in_any_order(w, noise[j], i);
         }
-    return larger(won, block_reduce(s.scratch, draw_key(best, where), larger));
+    return larger(won, block_reduce(s.scratch, best.key(), larger));
 }
 
 template <int DT>

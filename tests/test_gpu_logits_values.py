@@ -93,6 +93,35 @@ def test_rare_tokens_have_their_weight(kw):
     assert not wrong.any(), (int(wrong.sum()), d[wrong][:8])
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=2), dict(top_p=0.9)])
+def test_scores_of_very_large_and_small_noise(kw):
+    """Scores below the normal numbers and noise whose reciprocal is none still have their order."""
+    from rwkv_next_amd import kernels
+    say("sample noise at its ends", kw)
+    x = torch.tensor([[0.0, -1.0], [-1.0, 0.0]], device=DEV)
+    big = torch.tensor([[3e38, 1e38], [1e38, 2.9e38]], device=DEV)    # 1 / 3e38 < e^-1 / 1e38, and so in the second row
+    assert kernels.sample_logits(x, big, **kw)[0].tolist() == [1, 0]
+    x = torch.tensor([[-1.0, 0.0]], device=DEV)
+    small = torch.tensor([[5e-39, 6e-39]], device=DEV)                # e^-1 / 5e-39 < 1 / 6e-39, both finite
+    assert kernels.sample_logits(x, small, **kw)[0].tolist() == [1]
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=4), dict(top_p=0.99)])
+def test_noise_of_nothing_and_below(kw):
+    """A noise of 0 wins, the lowest index of several; negative, infinite or no noise never does, and where nothing else is left the
+    largest logit is taken.  Equal quotients of different tokens: the lowest index."""
+    from rwkv_next_amd import kernels
+    say("sample noise at and below 0", kw)
+    inf, nan = float("inf"), float("nan")
+    x = torch.tensor([[0.0, -1.0, -0.5, -2.0]], device=DEV)
+    for noise, want in (([1.0, 0.0, 1e-30, 0.0], 1), ([1.0, -1e-3, 2.0, 0.2], 0), ([-1.0, nan, inf, -0.5], 0), ([inf, nan, -1.0, 5.0], 3)):
+        assert kernels.sample_logits(x, torch.tensor([noise], device=DEV), **kw)[0].tolist() == [want], noise
+    x = torch.zeros(1, 50, device=DEV)
+    noise = torch.full((1, 50), 3.0, device=DEV)
+    noise[0, 30:] = 0.1
+    assert kernels.sample_logits(x, noise, **dict(kw, **({"top_k": 45} if "top_k" in kw else {})))[0].tolist() == [30]
+
+
 @pytest.mark.parametrize("V", [131072, 131074, 600000, 2097152])
 def test_one_bin_of_a_whole_vocabulary(V):
     """Equal logits: a bin's word holds V tokens at its first weight.  A top-p of a half keeps the first half, a top-k of k the first k;
