@@ -115,8 +115,9 @@ def _counts(counts, slots, B, V, dev):
         return counts.data_ptr(), max(stride[0], V), shape[0], code, 0
     if not isinstance(slots, torch.Tensor):
         raise TypeError(f"slots must be an int64 tensor of {B} entries (got {type(slots).__name__})")
-    return (counts.data_ptr(), max(stride[0], V), shape[0], code,
-            _per_sequence(slots, torch.int64, B, dev, "slots")[0])
+    sl = _per_sequence(slots, torch.int64, B, dev, "slots")[0]
+    # a table without rows has no address, and NULL would be no table: every slot lies outside it, and its memory is not read
+    return counts.data_ptr() if shape[0] else sl, max(stride[0], V), shape[0], code, sl
 
 
 def _status(status, dev):
@@ -213,7 +214,7 @@ def penalize_logits(logits, *, counts=None, slots=None, repetition=1.0, presence
             m_rows = mask.size(0)
             m_stride = max(_rows(mask, torch.int32, (m_rows,), words, dev, "mask") if m_rows else 0, words)
             mr_p = mask_rows.data_ptr()
-        m_p = mask.data_ptr() if m_rows else 0
+        m_p = mask.data_ptr() if m_rows else mr_p  # as for counts: a table without rows is one that no index lies in
     elif mask_rows is not None:
         raise ValueError("mask_rows without a mask")
     args = _lib.pack_penalize(

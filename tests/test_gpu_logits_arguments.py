@@ -34,3 +34,26 @@ def test_out_beside_the_logits():
         with pytest.raises(ValueError, match="share memory"):
             kernels.penalize_logits(x, out=out)
     assert torch.equal(buf, before)
+
+
+def test_tables_without_rows():
+    """Every index into a table of no rows lies outside it: left out, and reported."""
+    from rwkv_next_amd import kernels
+    say("logits empty tables")
+    V = 70
+    x = torch.randn(2, V, device=DEV)
+    status = kernels.new_status(torch.device(DEV))
+    slots = torch.tensor([0, 3], device=DEV)
+    for dt in (torch.int32, torch.float32):
+        counts = torch.zeros(0, V, dtype=dt, device=DEV)
+        status.zero_()
+        y = kernels.penalize_logits(x, counts=counts, slots=slots, repetition=1.5, presence=1.0, status=status)
+        assert torch.equal(y, x) and int(status) == 256
+        status.zero_()
+        token, _ = kernels.sample_logits(x, counts=counts, slots=slots, status=status)
+        assert torch.equal(token, x.argmax(dim=1)) and int(status) == 256
+    mask = torch.zeros(0, 3, dtype=torch.int32, device=DEV)
+    for rows, bits in (([0, -1], 256), ([-1, -2], 0)):
+        status.zero_()
+        y = kernels.penalize_logits(x, mask=mask, mask_rows=torch.tensor(rows, device=DEV), status=status)
+        assert torch.equal(y, x) and int(status) == bits
