@@ -58,13 +58,17 @@ def _per_sequence(x, dtype, B, dev, name):
 
 
 def _rows(x, dtype, lead, least, dev, name):
-    """A tensor of rows of at least `least` contiguous elements whose leading sizes are `lead`: its row stride."""
+    """(tensor, its row stride) of a tensor of rows of at least `least` contiguous elements whose leading sizes are `lead`; a copy
+    where rows share memory, as one row broadcast to all sequences."""
     _on(x, dev, name)
     shape, stride = x.shape, x.stride()
     if x.dtype is not dtype or shape[:-1] != lead or shape[-1] < least or (stride[-1] != 1 and shape[-1] > 1):
         raise ValueError(f"{name} must be a {dtype} {(*lead, least)} tensor with contiguous rows "
                          f"(got {x.dtype} {tuple(shape)}, strides {stride})")
-    return stride[0] if lead[0] > 1 else max(stride[0], shape[-1])
+    if lead[0] > 1 and stride[0] < shape[-1]:
+        x = x.contiguous()
+        return x, x.stride(0)
+    return x, stride[0] if lead[0] > 1 else max(stride[0], shape[-1])
 
 
 def _overlaps(t):
@@ -181,15 +185,15 @@ def penalize_logits(logits, *, counts=None, slots=None, repetition=1.0, presence
         raise ValueError(f"repetition must be positive (got {rep})")
     dr_p = dr_stride = 0
     if drafts is not None and T > 1:
-        dr_stride = _rows(drafts, torch.int64, (B,), T - 1, dev, "drafts")
+        drafts, dr_stride = _rows(drafts, torch.int64, (B,), T - 1, dev, "drafts")
         dr_p = drafts.data_ptr()
     bi_p = bv_p = bias_stride = n_bias = 0
     if (bias_ids is None) != (bias_values is None):
         raise ValueError("bias_ids and bias_values go together")
     if bias_ids is not None:
         n_bias = bias_ids.size(-1)
-        bias_stride = _rows(bias_ids, torch.int64, (B,), 0, dev, "bias_ids")
-        value_stride = _rows(bias_values, torch.float32, (B,), 0, dev, "bias_values")
+        bias_ids, bias_stride = _rows(bias_ids, torch.int64, (B,), 0, dev, "bias_ids")
+        bias_values, value_stride = _rows(bias_values, torch.float32, (B,), 0, dev, "bias_values")
         if bias_values.size(-1) != n_bias:
             raise ValueError(f"bias_ids and bias_values must have one shape (got {n_bias} and {bias_values.size(-1)} places)")
         if value_stride != bias_stride:
@@ -199,7 +203,8 @@ def penalize_logits(logits, *, counts=None, slots=None, repetition=1.0, presence
     if mask is not None:
         words = (V + 31) // 32
         if mask_rows is None:
-            m_rows, m_stride = B * T, _rows(mask, torch.int32, lead, words, dev, "mask")
+            m_rows = B * T
+            mask, m_stride = _rows(mask, torch.int32, lead, words, dev, "mask")
             if len(lead) == 2:  # rows of (b, t) one after another
                 if not mask.is_contiguous():
                     mask = mask.contiguous()
@@ -212,7 +217,7 @@ def penalize_logits(logits, *, counts=None, slots=None, repetition=1.0, presence
             if mask.dim() != 2:
                 raise ValueError(f"mask must be a table (R, words) where mask_rows is given (got {tuple(mask.shape)})")
             m_rows = mask.size(0)
-            m_stride = max(_rows(mask, torch.int32, (m_rows,), words, dev, "mask") if m_rows else 0, words)
+            mask, m_stride = _rows(mask, torch.int32, (m_rows,), words, dev, "mask") if m_rows else (mask, words)
             mr_p = mask_rows.data_ptr()
         m_p = mask.data_ptr() if m_rows else mr_p  # as for counts: a table without rows is one that no index lies in
     elif mask_rows is not None:

@@ -57,3 +57,22 @@ def test_tables_without_rows():
         status.zero_()
         y = kernels.penalize_logits(x, mask=mask, mask_rows=torch.tensor(rows, device=DEV), status=status)
         assert torch.equal(y, x) and int(status) == bits
+
+
+def test_one_row_for_all_sequences():
+    """Broadcast rows (a stride of 0) of biases, drafts and masks: as their copies."""
+    from rwkv_next_amd import kernels
+    say("logits broadcast rows")
+    rng = np.random.default_rng(1)
+    B, T, V, P = 4, 3, 501, 5
+    x = torch.from_numpy(rng.standard_normal((B, T, V)).astype(np.float32)).to(DEV)
+    ids = torch.from_numpy(rng.integers(0, V, (1, P))).to(DEV).expand(B, P)
+    values = torch.from_numpy(rng.standard_normal((1, P)).astype(np.float32)).to(DEV).expand(B, P)
+    drafts = torch.from_numpy(rng.integers(0, V, (1, T - 1))).to(DEV).expand(B, T - 1)
+    bits = torch.from_numpy(rng.integers(0, 2 ** 32, (1, 16), dtype=np.uint32).view(np.int32)).to(DEV)
+    for logits, kw in [(x, dict(bias_ids=ids, bias_values=values)), (x, dict(bias_ids=ids.contiguous(), bias_values=values)),
+                       (x, dict(drafts=drafts, presence=0.5)), (x, dict(mask=bits.expand(B, T, 16))),
+                       (x[:, 0], dict(mask=bits.expand(B, 16))),
+                       (x[:, 0], dict(mask=bits.expand(3, 16), mask_rows=torch.tensor([0, 2, 1, -1], device=DEV)))]:
+        copies = {k: v.contiguous() if isinstance(v, torch.Tensor) else v for k, v in kw.items()}
+        assert torch.equal(kernels.penalize_logits(logits, **kw), kernels.penalize_logits(logits, **copies)), sorted(kw)
