@@ -16,12 +16,12 @@
 // added up as whole numbers of 2^-24 of the weight at its start (the last place of an fp32 weight; 2^-23 .. 2^-20 where there are more
 // than 2^17 tokens), beside its tokens' number in one 64-bit word: one atomic to a token.
 //
-// Measured, V = 65536, us of max / weigh / gather / choose: one row fp32 with top-p 3.4 / 4.4 / 5.7 / 7.7 (19.3 together in a graph),
-// each bound by its chain of dependent reads; 64 rows with top-k and top-p 5.7 / 7.2 / 6.4 / 11.6; 320 rows bf16 with a wide nucleus
-// 11.7 / 18.0 / 22.7 / 15.5: max by memory (42 MB, 3.6 TB/s), weigh and gather by vector instructions (43 and 41 % of the
-// time) and the histogram's reading by every workgroup.  A workgroup a row doing all took 78, 111 and 183 us.  Gather and choose in one
-// launch, the last workgroup of a row going on, took 20, 39 and 81 us together: its four wavefronts are too few for the
-// choosing rounds.
+// Measured, V = 65536, us of max / weigh / gather / choose: one row fp32 with top-p 3.5 / 4.3 / 5.7 / 6.8 (18.1 together in a graph),
+// each bound by its chain of dependent reads; 64 rows with top-k and top-p 5.6 / 8.5 / 6.6 / 10.4 (28.3); 320 rows bf16 with a wide
+// nucleus 12.0 / 19.0 / 24.0 / 14.7 (65.7): max by memory (42 MB, 3.5 TB/s), weigh and gather by vector instructions (46 and 45 % of
+// the time) and the histogram's reading by every gathering workgroup.  A workgroup a row doing all took 78, 111 and 183 us.  Gather
+// and choose in one launch, the last workgroup of a row going on, took 20, 39 and 81 us together: its four wavefronts are too few for
+// the choosing rounds.  The long way takes 0.75 ms for a row of 65536 equal logits, or for 64 of them at once.
 #include <hip/hip_runtime.h>
 #include <float.h>
 #include <stdint.h>
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_
     if (c.searches) {
         for (int b = tid; b < kBins; b += kSegThreads) bins[b] = 0;
         __syncthreads();
-        uint32_t far = 0;  // a long tail's tokens all fall into the last bin: counted in registers, their weights (e^-32) left out
+        uint32_t far = 0;  // a long tail's tokens all fall into the last bin: counted in registers, their weights left out: e^-32 each, 2^21 of them 2.7e-8
 #pragma unroll
         for (int a = 0; a < PIECES; ++a)
 #pragma unroll

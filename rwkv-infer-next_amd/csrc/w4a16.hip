@@ -87,11 +87,13 @@ __device__ __forceinline__ void store(void* out, int dtype, int64_t at, float x)
 
 // Strips, for up to 16 rows and for narrow products of more: a workgroup's wavefronts take the 128-row chunks of K in turn, each with
 // sums of its own; they are added in LDS in the wavefronts' order.  A wavefront reads A in operand order by itself, so 16 rows of A go
-// with up to 64 columns.  Measured (graph replays, weights cycled past the caches): 4096 x 65536, one row 28.6 us = 4.8 TB/s
-// where a large copy moves 4.9, bound by memory; 4096 x 4096, one row 4.2 us and 2560 x 10240, five rows 6.5 us, bound by the
-// trips to memory of a wavefront's two to four chunks, one after another.  Asked for a chunk ahead they took twice the
-// registers, and half the wavefronts were no faster (33 and 7.8 us for the first and last).  Workgroups of 32 and 64 rows, whose
-// wavefronts use a weight's operands two and four times, were slower than more workgroups: 64 rows, 4096 x 4096 19 us against 9.2.
+// with up to 64 columns.  Measured (graph replays; weights cycled past the 256 MB cache, in brackets three weights in turn):
+// 4096 x 65536, one row 30.6 us = 4.5 TB/s where a large copy moves 4.9, bound by memory; 4096 x 4096, one row 6.0 us (4.2) and
+// 2560 x 10240, five rows 7.4 us (6.5), bound by the trips to memory of a wavefront's two to four chunks, one after another.  Asked
+// for a chunk ahead, the first and the last of these took twice the registers and were slower (three weights 33 and 7.8 us, then by
+// 16 columns a workgroup for the last); for 4096 x 4096, whose 256 workgroups leave registers free, that was not tried.  Workgroups of 32
+// and 64 rows, whose wavefronts use a weight's operands two and four times, were slower than more workgroups: 64 rows, 4096 x 4096
+// 19 us against 9.2.
 template <int AT, int NT, int SPC>
 __global__ __launch_bounds__(512) void w4a16_strip_kernel(const Params p) {
     extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][16][16 * NT]
@@ -173,7 +175,7 @@ constexpr int kPanelBytes = 16 * MT * kPanelStride<MT, WK>;
 // Blocks, from 17 rows on: a workgroup's WN WK wavefronts are WN groups of columns by WK groups of chunks.  They share A, a panel of
 // WK chunks at a time, through LDS, which loads of whole lines fill (in operand order a load of A takes four times as long, and
 // every wavefront would read all of it); weights come two panels ahead into registers.  Measured: 64 rows, 4096 x 65536 57.7 us (93 by
-// strips), 203 rows, 2560 x 8191, groups of 32 24 us (33).  In the first the matrix cores work 37 % of the time, the vector units
+// strips; 61.3 with weights cycled past the caches), 203 rows, 2560 x 8191, groups of 32 25 us (33).  In the first the matrix cores work 37 % of the time, the vector units
 // 31 % and LDS 28 %, hardly at once: two wavefronts a SIMD is what registers and 256 workgroups leave.  A two panels ahead as well,
 // and four strips a wavefront at one wavefront a SIMD, were not faster (62 to 82 us).
 template <int AT, int MT, int NT, int SPC, int WN, int WK>

@@ -37,7 +37,8 @@ inline int64_t groups(int32_t N, int columns) { return ((int64_t)N + columns - 1
 // that, strips of 16 rows: more workgroups, and as many columns to each as leave three CUs in five one.  us, K = 4096, strips /
 // blocks: 64 rows N = 65536 97 / 62, 16384 26.6 / 24.3, 4096 9.0 / 21.5; 256 rows N = 4096 24.1 / 22.6; 203 rows, K = 2560, N = 8191
 // 30.8 / 25.2; but N = 10240 64 rows, 160 blocks, 14.3 / 16.5.  Strips of 64 / 32 / 16 columns: 64 rows, K = N = 2560 (160, 320, 640
-// workgroups) 7.1 / 8.9 / 10.8; 24 rows, N = 4096 (128, 256, 512) 8.7 / 7.7 / 10.7; one row, N = 4096 (64, 128, 256) 8.0 / 6.2 / 5.4.
+// workgroups) 7.1 / 8.9 / 10.8; 24 rows, N = 4096 (128, 256, 512) 8.7 / 7.7 / 10.7; one row, N = 4096 (64, 128, 256) 8.0 / 6.2 / 5.4:
+// the bound lies between 128 and 160 workgroups, where nothing else was measured.
 inline Plan plan(int32_t M, int32_t N, int32_t K, int cus) {
     Plan p;
     const int rows = M <= 32 ? 32 : 64;
