@@ -323,7 +323,8 @@ __global__ __launch_bounds__(kSegThreads) void weigh_kernel(const logits_sample_
     if (c.searches) {
         for (int b = tid; b < kBins; b += kSegThreads) bins[b] = 0;
         __syncthreads();
-        uint32_t far = 0;  // a long tail's tokens all fall into the last bin: counted in registers, their weights left out: e^-32 each, 2^21 of them 2.7e-8
+        // A long tail's tokens all fall into the last bin: counted in registers, their weights left out (e^-32 each, 2^21 of them 2.7e-8).
+        uint32_t far = 0;
 #pragma unroll
         for (int a = 0; a < PIECES; ++a)
 #pragma unroll

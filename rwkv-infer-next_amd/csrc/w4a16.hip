@@ -175,9 +175,9 @@ constexpr int kPanelBytes = 16 * MT * kPanelStride<MT, WK>;
 // Blocks, from 17 rows on: a workgroup's WN WK wavefronts are WN groups of columns by WK groups of chunks.  They share A, a panel of
 // WK chunks at a time, through LDS, which loads of whole lines fill (in operand order a load of A takes four times as long, and
 // every wavefront would read all of it); weights come two panels ahead into registers.  Measured: 64 rows, 4096 x 65536 57.7 us (93 by
-// strips; 61.3 with weights cycled past the caches), 203 rows, 2560 x 8191, groups of 32 25 us (33).  In the first the matrix cores work 37 % of the time, the vector units
-// 31 % and LDS 28 %, hardly at once: two wavefronts a SIMD is what registers and 256 workgroups leave.  A two panels ahead as well,
-// and four strips a wavefront at one wavefront a SIMD, were not faster (62 to 82 us).
+// strips; 61.3 with weights cycled past the caches), 203 rows, 2560 x 8191, groups of 32 25 us (33).  In the first the matrix cores
+// work 37 % of the time, the vector units 31 % and LDS 28 %, hardly at once: two wavefronts a SIMD is what registers and 256
+// workgroups leave.  A two panels ahead as well, and four strips a wavefront at one wavefront a SIMD, were not faster (62 to 82 us).
 template <int AT, int MT, int NT, int SPC, int WN, int WK>
 __global__ __launch_bounds__(64 * WN * WK, 2) void w4a16_block_kernel(const Params p) {
     constexpr int kThreads = 64 * WN * WK;
