@@ -1,5 +1,5 @@
-"""Build librwkv7_hip.so: the HIP kernels and the C ABI of include/wkv7.h, w6a16.h, w4a16.h and logits.h, compiled for gfx950 with hipcc;
-and librwkv7_noalloc.so (include/wkv7_noalloc.h), the allocation-free entry with its static device scratch array,
+"""Build librwkv7_hip.so: the HIP kernels and the C ABI of include/wkv7.h, w6a16.h, w4a16.h, logits.h, dense.h, delta.h and slots.h,
+compiled for gfx950 with hipcc; and librwkv7_noalloc.so (include/wkv7_noalloc.h), the allocation-free entry with its static device scratch array,
 linked against librwkv7_hip.so so that only processes that load it hold that array.
 
 The libraries are plain shared objects (no torch symbols); the Python layer loads them with ctypes after torch, so
@@ -25,10 +25,11 @@ BUILD_DIR = os.path.join(PROJECT_DIR, "_build")
 
 SOURCES = ("wkv7_recurrent.hip", "wkv7_chunked.hip", "wkv7_seg.hip", "wkv7_generic.hip", "wkv7_pool.hip",
            "wkv7_timemix.hip", "w6a16.hip", "w4a16.hip", "logits_penalize.hip", "logits_sample.hip",
-           "wkv7_capi.hip")
+           "dense.hip", "delta_token.hip", "delta_capi.hip", "slots.hip", "wkv7_capi.hip")
 NOALLOC_SOURCE = "wkv7_noalloc.hip"
 NOALLOC_LIB_PATH = os.path.join(PKG_DIR, "librwkv7_noalloc.so")
-HEADERS = ("logits_device.h", "w4a16_plan.h", "w6a16_grid.h", "w6a16_plan.h", "wkv7_device.h", "wkv7_launch.h", "wkv7_token.h")
+HEADERS = ("delta_device.h", "dense_plan.h", "logits_device.h", "w4a16_plan.h", "w6a16_grid.h", "w6a16_plan.h", "wkv7_device.h", "wkv7_launch.h",
+           "wkv7_token.h")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
@@ -83,7 +84,8 @@ def sources_newer_than_library() -> bool:
         return True
     t = os.path.getmtime(LIB_PATH)
     files = [os.path.join(CSRC, f) for f in SOURCES + HEADERS + (NOALLOC_SOURCE,)] + \
-        [os.path.join(INCLUDE, h) for h in ("wkv7.h", "w6a16.h", "w4a16.h", "logits.h", "wkv7_noalloc.h")]
+        [os.path.join(INCLUDE, h) for h in ("wkv7.h", "w6a16.h", "w4a16.h", "logits.h", "dense.h", "delta.h", "slots.h",
+                                             "wkv7_noalloc.h")]
     return any(os.path.getmtime(f) > t for f in files)
 
 

@@ -1,5 +1,5 @@
-"""ctypes binding of librwkv7_hip.so (the C ABI declared in include/wkv7.h, w6a16.h, w4a16.h and logits.h) and of
-librwkv7_noalloc.so (include/wkv7_noalloc.h, loaded only on request by load_noalloc).
+"""ctypes binding of librwkv7_hip.so (the C ABI declared in include/wkv7.h, w6a16.h, w4a16.h, logits.h, dense.h, delta.h and
+slots.h) and of librwkv7_noalloc.so (include/wkv7_noalloc.h, loaded only on request by load_noalloc).
 
 The library must have been built (rwkv_next_amd._build / __graft_entry__.build()).  There is no fallback: if the
 shared object is missing or does not match this binding, importing the kernels raises.
@@ -69,6 +69,29 @@ LOGITS_COUNTS_F32 = 1
 LOGITS_SAMPLE_STATE_BYTES = 4325376  # leading workspace region that is zero between calls
 LOGITS_STATUS_ROW = 256
 LOGITS_STATUS_TOKEN = 512
+DENSE_EXPORTED = ("dense_args_size", "dense_packed_size", "dense_pack", "dense_matmul")
+DENSE_BF16 = 0
+DENSE_F16 = 1
+DENSE_F32 = 2
+DENSE_NONE = 0
+DENSE_RELU = 1
+DENSE_RELU2 = 2
+DENSE_TANH = 3
+DENSE_SIGMOID = 4
+DENSE_SILU = 5
+DENSE_GELU = 6
+DENSE_MAX_ROW_STRIDE = 1 << 24
+DELTA_EXPORTED = ("delta_args_size", "delta_workspace_size", "delta_run")
+DELTA_STATUS_SLOT = 2048
+DELTA_STATUS_SEQLENS = 4096
+DELTA_STATUS_NKEEP = 8192
+DELTA_STATUS_CLASH = 16384
+DELTA_MAX_STRIDE = 1 << 24
+SLOTS_EXPORTED = ("slots_cache_size", "slots_copy", "slots_free", "slots_compact")
+SLOTS_MAX_CACHES = 16
+SLOTS_MAX_PAIRS = 1024
+SLOTS_MAX_COMPACT = 8192
+SLOTS_STATUS_SLOT = 1024
 MAX_MOVES = 1024
 
 _vp = ctypes.c_void_p
@@ -176,6 +199,41 @@ class SampleArgs(ctypes.Structure):
     ]
 
 
+class DenseArgs(ctypes.Structure):
+    """Mirror of `dense_args` (include/dense.h)."""
+    _fields_ = [
+        ("a", _vp), ("a_row_stride", ctypes.c_int64), ("weight", _vp), ("bias", _vp), ("residual", _vp),
+        ("residual_row_stride", ctypes.c_int64), ("out", _vp), ("out_row_stride", ctypes.c_int64),
+        ("M", ctypes.c_int32), ("N", ctypes.c_int32), ("K", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32), ("residual_dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+    ]
+
+
+class DeltaArgs(ctypes.Structure):
+    """Mirror of `delta_args` (include/delta.h)."""
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64),
+        ("v_stride", ctypes.c_int64), ("g", _vp), ("beta", _vp), ("g_stride", ctypes.c_int64),
+        ("beta_stride", ctypes.c_int64), ("o", _vp), ("o_stride", ctypes.c_int64),
+        ("h0", _vp), ("h0_idx", _vp), ("h0_rows", ctypes.c_int64), ("ht", _vp), ("ht_idx", _vp),
+        ("ht_rows", ctypes.c_int64), ("fresh", _vp), ("cu_seqlens", _vp), ("n_keep", _vp), ("snapshots", _vp),
+        ("status", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t), ("total_tokens", ctypes.c_int64),
+        ("num_seqs", ctypes.c_int32), ("T", ctypes.c_int32), ("Hk", ctypes.c_int32), ("Hv", ctypes.c_int32),
+        ("K", ctypes.c_int32), ("V", ctypes.c_int32), ("scale", ctypes.c_float), ("qk_norm", ctypes.c_int32),
+        ("token_len", ctypes.c_int32),
+    ]
+
+
+class SlotsCache(ctypes.Structure):
+    """Mirror of `slots_cache` (include/slots.h)."""
+    _fields_ = [
+        ("from_", _vp), ("to", _vp), ("from_layer_stride", ctypes.c_int64), ("from_slot_stride", ctypes.c_int64),
+        ("to_layer_stride", ctypes.c_int64), ("to_slot_stride", ctypes.c_int64), ("row_bytes", ctypes.c_int64),
+        ("layers", ctypes.c_int64),
+    ]
+
+
 _PACK = {_vp: "Q", ctypes.c_int64: "q", ctypes.c_size_t: "Q", ctypes.c_int32: "i", ctypes.c_float: "f"}
 
 
@@ -188,6 +246,7 @@ def _packer(mirror):
 
 
 pack_w4a16, pack_penalize, pack_sample = _packer(W4a16Args), _packer(PenalizeArgs), _packer(SampleArgs)
+pack_dense, pack_delta = _packer(DenseArgs), _packer(DeltaArgs)
 
 
 class Wkv7Error(RuntimeError):
@@ -270,6 +329,26 @@ def load(path: str = LIB_PATH):
     lib.logits_sample_workspace_size.argtypes = [ctypes.POINTER(SampleArgs), psz]
     lib.logits_sample.restype = ctypes.c_int
     lib.logits_sample.argtypes = [_vp, _vp]
+    lib.dense_args_size.restype = ctypes.c_size_t
+    lib.dense_packed_size.restype = ctypes.c_int
+    lib.dense_packed_size.argtypes = [i32, i32, psz]
+    lib.dense_pack.restype = ctypes.c_int
+    lib.dense_pack.argtypes = [_vp, i64, i64, i32, i32, _vp, _vp]
+    lib.dense_matmul.restype = ctypes.c_int
+    lib.dense_matmul.argtypes = [_vp, _vp]  # a DenseArgs by reference, or pack_dense's bytes
+    lib.delta_args_size.restype = ctypes.c_size_t
+    lib.delta_workspace_size.restype = ctypes.c_int
+    lib.delta_workspace_size.argtypes = [_vp, psz]
+    lib.delta_run.restype = ctypes.c_int
+    lib.delta_run.argtypes = [_vp, _vp]  # a DeltaArgs by reference, or pack_delta's bytes
+    lib.slots_cache_size.restype = ctypes.c_size_t
+    pcache = ctypes.POINTER(SlotsCache)
+    lib.slots_copy.restype = ctypes.c_int
+    lib.slots_copy.argtypes = [pcache, i32, _vp, _vp, i32, i64, i64, _vp, _vp]
+    lib.slots_free.restype = ctypes.c_int
+    lib.slots_free.argtypes = [pcache, i32, _vp, i32, i64, _vp, _vp]
+    lib.slots_compact.restype = ctypes.c_int
+    lib.slots_compact.argtypes = [pcache, i32, _vp, i64, _vp, _vp, _vp]
     if lib.wkv7_abi_version() != WKV7_ABI_VERSION:
         raise ImportError(f"{path}: ABI version {lib.wkv7_abi_version()} != {WKV7_ABI_VERSION}")
     if lib.wkv7_args_size() != ctypes.sizeof(Wkv7Args):
@@ -279,7 +358,8 @@ def load(path: str = LIB_PATH):
     if lib.w6a16_args_size() != ctypes.sizeof(W6a16Args):
         raise ImportError(f"{path}: sizeof(w6a16_args) {lib.w6a16_args_size()} != binding {ctypes.sizeof(W6a16Args)}")
     for size, mirror in ((lib.w4a16_args_size(), W4a16Args), (lib.logits_penalize_args_size(), PenalizeArgs),
-                         (lib.logits_sample_args_size(), SampleArgs)):
+                         (lib.logits_sample_args_size(), SampleArgs), (lib.dense_args_size(), DenseArgs),
+                         (lib.delta_args_size(), DeltaArgs), (lib.slots_cache_size(), SlotsCache)):
         if size != ctypes.sizeof(mirror):
             raise ImportError(f"{path}: {mirror.__name__} has {size} bytes, binding {ctypes.sizeof(mirror)}")
     _lib = lib

@@ -1,0 +1,196 @@
+"""The gated delta rule on MI355X over the HIP library (include/delta.h): a recurrence beside wkv7, on the same kind of slot pools.
+
+Per value head h, with query/key head h // (Hv // Hk) and the state S (K x V, fp32):
+
+    S_t = a_t S_{t-1} + k_t d_t^T,   d_t = beta_t (v_t - a_t S_{t-1}^T k_t),   a_t = exp(g_t)
+    o_t = scale S_t^T q_t
+
+    gated_delta(q, k, v, g, beta, state=None, ...)      -> (o, final state | None)
+    gated_delta_pool_(q, k, v, g, beta, pool, slots, ...) -> o, states in a pool of slots, updated in place
+                                                        (op rwkv_next_amd::gated_delta_pool_)
+
+Layouts: q, k (B, T, Hk, K) and v (B, T, Hv, V) bfloat16, parts of one projection's result or tensors of their own (the strides
+between tokens are free); g (B, T, Hv) log decays <= 0 and beta (B, T, Hv), float32; states (N, Hv, K, V) float32; o like v.
+K is 64 or 128, V a multiple of 16 up to 256, Hv a multiple of Hk.  Inference only: there is no backward pass.  Every call runs on
+the current stream, no host sync, and can be recorded into a HIP graph.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from .. import _lib
+from ._workspace import on_device, stream_handle
+from .wkv7 import _index_tensor, _require
+
+
+def _tokens(t, dtype, shape, align, name):
+    """`t` (B, T, ...) as it is where its tokens follow each other at one stride and each is contiguous, else a contiguous copy;
+    with that stride in elements."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype} (got {t.dtype})")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)} (got {tuple(t.shape)})")
+    B, T = shape[:2]
+    inner = 1
+    for n in shape[2:]:
+        inner *= n
+    st = t.stride()
+    token = st[1] if T > 1 else st[0] if B > 1 else inner
+    ok = (B == 1 or T == 1 or st[0] == T * st[1]) and inner <= token <= _lib.DELTA_MAX_STRIDE
+    want = 1
+    for n, s in zip(reversed(shape[2:]), reversed(st[2:])):
+        ok = ok and (n == 1 or s == want)
+        want *= n
+    if not ok or token % align or t.data_ptr() % (16 if align > 1 else 4):
+        # (a copy has its own memory, aligned)
+        return t.clone(memory_format=torch.contiguous_format), inner
+    return t, token
+
+
+def _launch(q, k, v, g, beta, *, o, h0=None, h0_idx=None, ht=None, ht_idx=None, fresh=None, cu=None, n_keep=None,
+            snapshots=None, status=None, scale, qk_norm, token_len):
+    if q.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"q, k must be (B, T, Hk, K) and v (B, T, Hv, V) (got {tuple(q.shape)}, {tuple(v.shape)})")
+    B, T, Hk, K = q.shape
+    Hv, V = v.shape[2:]
+    if K not in (64, 128) or V % 16 or not 16 <= V <= 256:
+        raise ValueError(f"head sizes must be K in (64, 128) and V a multiple of 16 up to 256 (got K={K}, V={V})")
+    if Hk < 1 or Hv < Hk or Hv % Hk:
+        raise ValueError(f"value heads must be a multiple of the query/key heads (got Hk={Hk}, Hv={Hv})")
+    dev = q.device
+    if dev.type != "cuda":
+        raise ValueError(f"operands must be on a GPU (got {dev})")
+    for t, name in ((k, "k"), (v, "v"), (g, "g"), (beta, "beta"), (h0, "state"), (h0_idx, "slots"), (fresh, "fresh"),
+                    (cu, "cu_seqlens"), (n_keep, "n_keep"), (snapshots, "snapshots"), (status, "status")):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} must be on {dev} (got {t.device})")
+    q, q_s = _tokens(q, torch.bfloat16, (B, T, Hk, K), 8, "q")
+    k, k_s = _tokens(k, torch.bfloat16, (B, T, Hk, K), 8, "k")
+    v, v_s = _tokens(v, torch.bfloat16, (B, T, Hv, V), 8, "v")
+    g, g_s = _tokens(g, torch.float32, (B, T, Hv), 1, "g")
+    beta, b_s = _tokens(beta, torch.float32, (B, T, Hv), 1, "beta")
+    N = B if cu is None else cu.numel() - 1
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    rows = lambda t: 0 if t is None else t.shape[0]  # noqa: E731
+    fields = [q.data_ptr(), k.data_ptr(), v.data_ptr(), q_s, k_s, v_s, g.data_ptr(), beta.data_ptr(), g_s, b_s,
+              ptr(o), Hv * V, ptr(h0), ptr(h0_idx), rows(h0), ptr(ht), ptr(ht_idx), rows(ht), ptr(fresh), ptr(cu),
+              ptr(n_keep), ptr(snapshots), ptr(status), 0, 0, B * T, N, 0 if cu is not None else T, Hk, Hv, K, V,
+              K ** -0.5 if scale is None else float(scale), int(qk_norm), token_len]  # in the order of the fields
+    lib, size = _lib.load(), ctypes.c_size_t(0)
+    args = _lib.pack_delta(*fields)
+    _lib.check(lib.delta_workspace_size(args, ctypes.byref(size)))
+    if size.value:  # what it holds does not matter: from the caching allocator, in the stream's order
+        workspace = torch.empty(size.value, dtype=torch.uint8, device=dev)
+        fields[23:25] = workspace.data_ptr(), size.value
+        args = _lib.pack_delta(*fields)
+    with on_device(dev):
+        _lib.check(lib.delta_run(args, stream_handle(dev)))
+
+
+def _state(t, N, Hv, K, V, name):
+    if t is None:
+        return None
+    if t.dtype is not torch.float32 or t.shape[1:] != (Hv, K, V) or t.dim() != 4 or (N is not None and t.shape[0] != N):
+        raise ValueError(f"{name} must be a float32 ({'S' if N is None else N}, {Hv}, {K}, {V}) tensor "
+                         f"(got {t.dtype} {tuple(t.shape)})")
+    return t
+
+
+def _rows(q, cu_seqlens):
+    """(cu_seqlens as int32 on the device or None, number of sequences)"""
+    if q.dim() != 4:
+        raise ValueError(f"q, k must be (B, T, Hk, K) (got {tuple(q.shape)})")
+    if cu_seqlens is None:
+        return None, q.shape[0]
+    if q.shape[0] != 1:
+        raise ValueError("cu_seqlens requires B == 1 (packed varlen)")
+    cu = _index_tensor(cu_seqlens, q.device, torch.int32, "cu_seqlens")
+    if cu.dim() != 1 or cu.numel() < 1:
+        raise ValueError(f"cu_seqlens must hold N + 1 offsets (got {tuple(cu.shape)})")
+    return cu, cu.numel() - 1
+
+
+@torch.no_grad()
+def gated_delta(q, k, v, g, beta, state=None, *, cu_seqlens=None, scale=None, qk_norm: bool = False, final: bool = True,
+                token_len: int = -1):
+    """(o, final state (N, Hv, K, V) or None) from `state` (N, Hv, K, V) float32 or None (zeros); N = B rows of T tokens, or
+    the rows of cu_seqlens (N + 1,) in a packed (1, sumT, ..) batch.
+
+    scale: K ** -0.5 where None.  qk_norm: q and k are divided by sqrt(sum of squares + 1e-6) first.  token_len: rows of at most
+    so many tokens run token by token instead of by chunks (-1: the library's choice)."""
+    cu, N = _rows(q, cu_seqlens)
+    K, (Hv, V) = q.shape[3], v.shape[2:]
+    h0 = _state(state, N, Hv, K, V, "state")
+    h0 = None if h0 is None else h0.contiguous()
+    o = torch.empty(v.shape, dtype=torch.bfloat16, device=v.device)
+    ht = torch.empty(N, Hv, K, V, dtype=torch.float32, device=v.device) if final else None
+    _launch(q, k, v, g, beta, o=o, h0=h0, ht=ht, cu=cu, scale=scale, qk_norm=qk_norm, token_len=token_len)
+    return o, ht
+
+
+@torch.library.custom_op("rwkv_next_amd::gated_delta_pool_", mutates_args=("pool", "snapshots", "status"))
+def gated_delta_pool_op(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, pool: Tensor, slots: Tensor,
+                        cu_seqlens: Optional[Tensor], n_keep: Optional[Tensor], fresh: Optional[Tensor],
+                        scale: Optional[float], qk_norm: bool, final: bool, store_o: bool, snapshots: Optional[Tensor],
+                        status: Optional[Tensor], token_len: int) -> Tensor:
+    """The slot-pool recurrence as a registered op (indices int64, cu_seqlens int32, fresh uint8).  Returns o, or an empty tensor
+    when store_o is False."""
+    N = q.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1
+    K, (Hv, V) = q.shape[3], v.shape[2:]
+    _require(pool, "pool", torch.float32, (None, Hv, K, V))
+    _require(slots, "slots", torch.int64, (N,))
+    if cu_seqlens is not None:
+        _require(cu_seqlens, "cu_seqlens", torch.int32, (None,))
+    if n_keep is not None:
+        _require(n_keep, "n_keep", torch.int64, (N,))
+    if fresh is not None:
+        _require(fresh, "fresh", torch.uint8, (N,))
+    if snapshots is not None:
+        if cu_seqlens is not None:
+            raise ValueError("snapshots are kept for dense (N, T) rows")
+        _require(snapshots, "snapshots", torch.float32, (N, q.shape[1], Hv, K, V))
+    if status is not None:
+        _require(status, "status", torch.int32, (None,))
+        if status.numel() < 1:
+            raise ValueError("status must hold at least one int32")
+    o = torch.empty(v.shape if store_o else (0,), dtype=torch.bfloat16, device=v.device)
+    _launch(q, k, v, g, beta, o=o if store_o else None, h0=pool, h0_idx=slots, ht=pool if final else None,
+            ht_idx=slots if final else None, fresh=fresh, cu=cu_seqlens, n_keep=n_keep, snapshots=snapshots, status=status,
+            scale=scale, qk_norm=qk_norm, token_len=token_len)
+    return o
+
+
+@gated_delta_pool_op.register_fake
+def _(q, k, v, g, beta, pool, slots, cu_seqlens, n_keep, fresh, scale, qk_norm, final, store_o, snapshots, status, token_len):
+    return v.new_empty(v.shape if store_o else (0,))
+
+
+def gated_delta_pool_(q, k, v, g, beta, pool, slots, *, cu_seqlens=None, n_keep=None, fresh=None, scale=None,
+                      qk_norm: bool = False, final: bool = True, store_o: bool = True, snapshots=None, status=None,
+                      token_len: int = -1):
+    """The recurrence for N sequences whose states live in `pool` (S, Hv, K, V) float32, updated in place.
+
+    slots (N,) int64: each sequence's row of the pool, distinct within a call.  Rows, cu_seqlens, scale, qk_norm and token_len as in
+    gated_delta; fresh, n_keep, final, store_o and status as in wkv7_pool_.
+    snapshots: optional (N, T, Hv, K, V) float32, the state after each token of dense rows; they run token by token.  Rolling back
+    to the first n tokens is SlotCaches((snapshots.flatten(0, 1), 0)).copy_slots(row * T + n - 1, slots,
+    into=SlotCaches((pool, 0))), or, on the pool as it was before, a call with n_keep=n, store_o=False on the same operands: where
+    token by token, the same bits.
+    Returns o like v (None when store_o is False).  Runs as the registered op rwkv_next_amd::gated_delta_pool_."""
+    cu, N = _rows(q, cu_seqlens)
+    dev = q.device
+    sl = _index_tensor(slots, dev, torch.int64, "slots")
+    nk = _index_tensor(n_keep, dev, torch.int64, "n_keep")
+    fr = None
+    if fresh is not None:
+        fr = fresh if isinstance(fresh, Tensor) and fresh.device == dev else torch.as_tensor(fresh, device=dev)
+        if fr.dtype == torch.bool:
+            fr = fr.view(torch.uint8)
+        fr = (fr if fr.dtype == torch.uint8 else fr.to(torch.uint8)).contiguous()
+    o = gated_delta_pool_op(q, k, v, g, beta, pool, sl, cu, nk, fr, scale, bool(qk_norm), final, store_o, snapshots, status,
+                            int(token_len))
+    return o if store_o else None

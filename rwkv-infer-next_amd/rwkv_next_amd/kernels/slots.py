@@ -1,0 +1,124 @@
+"""The slots of a served model's caches (include/slots.h): copies and forks, compaction, freeing, over all tensors at once, beside
+StatePool's reset_slots and move_slots (rwkv_next/model.py:310-316), which know one tensor of fp32 states.
+
+    caches = SlotCaches(pool.wkv, (shifts, 1), (counts, 0))   # (layers, slots, ..) tensors, or (tensor, dimension of its slots)
+    caches.copy_slots(src, dst)                # one source may go to many: a shared prompt forked
+    caches.copy_slots(src, dst, into=other)    # to caches of as many slots as they like: a store of prompts, and back
+    caches.free_slots(idx)                     # zeroed
+    where, count = caches.compact_slots(live)  # live slots to the front; where each went
+
+Indices are int64 on the device; one launch a call, on the current stream, no host sync, can be recorded into a HIP graph.
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+from ._workspace import on_device, stream_handle
+
+
+class SlotCaches:
+    """A model's cache tensors that share their slots.  Each argument is a tensor (layers, slots, ..) or (tensor, dim) with dim 0 for
+    (slots, ..) and 1 for (layers, slots, ..); a slot's part of a layer is contiguous.  At most 16 tensors, of any types."""
+
+    def __init__(self, *caches):
+        if not 1 <= len(caches) <= _lib.SLOTS_MAX_CACHES:
+            raise ValueError(f"SlotCaches takes 1 to {_lib.SLOTS_MAX_CACHES} tensors (got {len(caches)})")
+        self._rows, self.slots, self.device = [], None, None
+        for x in caches:
+            t, dim = x if isinstance(x, tuple) else (x, 1)
+            if dim not in (0, 1) or t.dim() <= dim:
+                raise ValueError(f"the slots are dimension 0 or 1 of a cache (got dimension {dim} of {tuple(t.shape)})")
+            if not t.is_cuda:
+                raise ValueError(f"caches must be on a GPU (got {t.device})")
+            if self.device is None:
+                self.device, self.slots = t.device, t.shape[dim]
+            if t.device != self.device or t.shape[dim] != self.slots:
+                raise ValueError(f"caches must have {self.slots} slots on {self.device} (got {t.shape[dim]} on {t.device})")
+            layers, shape, strides, size = t.shape[0] if dim else 1, t.shape[dim + 1:], t.stride(), t.element_size()
+            row = 1
+            for n, s in zip(reversed(shape), reversed(strides[dim + 1:])):
+                if n > 1 and s != row:
+                    raise ValueError(f"a slot's part of a cache must be contiguous (got {tuple(t.shape)}, strides {strides})")
+                row *= n
+            row *= size
+            slot = strides[dim] * size if self.slots > 1 else row
+            layer = strides[0] * size if dim and layers > 1 else 0
+            if row and (slot < row or (layers > 1 and layer < row)):
+                raise ValueError(f"slots of a cache must not share memory (got {tuple(t.shape)}, strides {strides})")
+            # layers outside slots or within them, but not interlocked
+            if row and layers > 1 and self.slots > 1 and layer < self.slots * slot and slot < layers * layer:
+                raise ValueError(f"slots of a cache must not share memory (got {tuple(t.shape)}, strides {strides})")
+            self._rows.append((t, layer, slot, row, layers))
+        self._own = self._pairs(self)
+
+    def _pairs(self, other):
+        a = (_lib.SlotsCache * len(self._rows))()
+        for x, (t, layer, slot, row, layers), (u, to_layer, to_slot, to_row, to_layers) in zip(a, self._rows, other._rows):
+            if (row, layers) != (to_row, to_layers) or t.dtype != u.dtype:
+                raise ValueError(f"caches of one shape but for their slots are needed (got {tuple(t.shape)}, {tuple(u.shape)})")
+            x.from_, x.to, x.from_layer_stride, x.from_slot_stride = t.data_ptr(), u.data_ptr(), layer, slot
+            x.to_layer_stride, x.to_slot_stride, x.row_bytes, x.layers = to_layer, to_slot, row, layers
+        return a
+
+    def _index(self, x, name):
+        if not isinstance(x, torch.Tensor):
+            x = torch.as_tensor(x, dtype=torch.int64, device=self.device)
+        if x.device != self.device:
+            raise ValueError(f"{name} must be on {self.device} (got {x.device})")
+        if x.dtype is not torch.int64 or x.dim() != 1:
+            raise ValueError(f"{name} must be an int64 tensor of one dimension (got {x.dtype} {tuple(x.shape)})")
+        return x.contiguous()
+
+    def _status(self, status):
+        if status is None:
+            return None
+        if status.device != self.device or status.dtype != torch.int32 or status.numel() < 1:
+            raise ValueError(f"status must be an int32 tensor on {self.device} (new_status)")
+        return status.data_ptr()
+
+    def copy_slots(self, src, dst, *, into: "SlotCaches | None" = None, status=None) -> None:
+        """into's slot dst[i] = this one's slot src[i] (into: these caches themselves where None), as if all sources were read
+        before any destination is written: swaps and chains are exact.  A source may be named any number of times; of equal
+        destinations the last one counts.  A negative index leaves its entry out, one past the slots does too and sets
+        SLOTS_STATUS_SLOT in `status`.  At most 1024 entries."""
+        src, dst = self._index(src, "src"), self._index(dst, "dst")
+        n = src.numel()
+        if n != dst.numel():
+            raise ValueError(f"src and dst must have the same length (got {n} and {dst.numel()})")
+        if n > _lib.SLOTS_MAX_PAIRS:
+            raise ValueError(f"at most {_lib.SLOTS_MAX_PAIRS} copies per call (got {n})")
+        a, to = self._own, self.slots
+        if into is not None and into is not self:
+            if into.device != self.device or len(into._rows) != len(self._rows):
+                raise ValueError(f"into must be {len(self._rows)} caches on {self.device}")
+            a, to = self._pairs(into), into.slots
+        with on_device(self.device):
+            _lib.check(_lib.load().slots_copy(a, len(a), src.data_ptr(), dst.data_ptr(), n, self.slots, to,
+                                              self._status(status), stream_handle(self.device)))
+
+    def free_slots(self, idx, *, status=None) -> None:
+        """Slot idx[i] = 0 in every cache, indices as in copy_slots.  At most 65535."""
+        idx = self._index(idx, "idx")
+        if idx.numel() > 65535:
+            raise ValueError(f"at most 65535 slots per call (got {idx.numel()})")
+        with on_device(self.device):
+            _lib.check(_lib.load().slots_free(self._own, len(self._own), idx.data_ptr(), idx.numel(), self.slots,
+                                              self._status(status), stream_handle(self.device)))
+
+    def compact_slots(self, live):
+        """Moves the live slots to the front: with k the number of live ones (live (S,) bool), those at k and behind go, in their
+        order, to the free ones before k, in theirs.  Returns (where, count): where (S,) int64 a slot's place after, -1 for a free
+        one, count (1,) int32 k, both on the device.  Slots that nothing moves to keep what they hold (free_slots zeroes)."""
+        if not isinstance(live, torch.Tensor) or live.device != self.device or live.dtype not in (torch.bool, torch.uint8) or \
+                live.shape != (self.slots,):
+            raise ValueError(f"live must be a bool ({self.slots},) tensor on {self.device}")
+        if self.slots > _lib.SLOTS_MAX_COMPACT:
+            raise ValueError(f"at most {_lib.SLOTS_MAX_COMPACT} slots are compacted (got {self.slots})")
+        live = live.contiguous()
+        where = torch.empty(self.slots, dtype=torch.int64, device=self.device)
+        count = torch.empty(1, dtype=torch.int32, device=self.device)
+        with on_device(self.device):
+            _lib.check(_lib.load().slots_compact(self._own, len(self._own), live.data_ptr(), self.slots, where.data_ptr(),
+                                                 count.data_ptr(), stream_handle(self.device)))
+        return where, count

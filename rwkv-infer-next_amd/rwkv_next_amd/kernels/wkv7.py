@@ -361,17 +361,23 @@ STATUS_REASONS = {_lib.WKV7_STATUS_H0_SLOT: "initial-state slot index outside th
 # the logit operators' bits of the same word (include/logits.h)
 LOGITS_STATUS_REASONS = {_lib.LOGITS_STATUS_ROW: "a slot outside the count table, or a mask row past the masks",
                          _lib.LOGITS_STATUS_TOKEN: "a draft or bias token outside the vocabulary"}
+# those of the slot operators (include/slots.h) and of the gated delta rule (include/delta.h)
+SLOTS_STATUS_REASONS = {_lib.SLOTS_STATUS_SLOT: "a slot past the caches' slots"}
+DELTA_STATUS_REASONS = {_lib.DELTA_STATUS_SLOT: "a slot outside the pool",
+                        _lib.DELTA_STATUS_SEQLENS: "cu_seqlens not non-decreasing within [0, total tokens]",
+                        _lib.DELTA_STATUS_NKEEP: "negative n_keep",
+                        _lib.DELTA_STATUS_CLASH: "two sequences share a state slot: the result depends on timing"}
 
 
 def check_status(status: torch.Tensor) -> None:
-    """Raise ValueError naming every WKV7_STATUS_* or LOGITS_STATUS_* bit set in `status` (synchronises the host: call it outside
-    graph capture and the hot loop)."""
+    """Raise ValueError naming every WKV7_STATUS_*, LOGITS_STATUS_*, SLOTS_STATUS_* or DELTA_STATUS_* bit set in `status`
+    (synchronises the host: call it outside graph capture and the hot loop)."""
     bits = int(status.reshape(-1)[0].item())
     if bits:
-        wkv7 = [m for bit, m in STATUS_REASONS.items() if bits & bit]
-        logits = [m for bit, m in LOGITS_STATUS_REASONS.items() if bits & bit]
-        raise ValueError("; ".join(f"{name}: " + "; ".join(found) for name, found in (("wkv7", wkv7), ("logits", logits))
-                                   if found))
+        of = {"wkv7": STATUS_REASONS, "logits": LOGITS_STATUS_REASONS, "slots": SLOTS_STATUS_REASONS,
+              "gated_delta": DELTA_STATUS_REASONS}
+        found = {name: [m for bit, m in reasons.items() if bits & bit] for name, reasons in of.items()}
+        raise ValueError("; ".join(f"{name}: " + "; ".join(why) for name, why in found.items() if why))
 
 
 def check_distinct_slots(slots: torch.Tensor, num_slots: int) -> None:
