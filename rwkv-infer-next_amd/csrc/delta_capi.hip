@@ -1,11 +1,33 @@
 // delta_capi.hip -- the C entry points of include/delta.h: checks of arguments, the choice between the kernels, the launches.
 // Everything is decided from sizes and flags that the host knows.
 #include "delta_device.h"
+#include "wkv7_launch.h"
 
 namespace delta {
 namespace {
 
 constexpr int kClashRows = 1024;
+// Rows of at most so many tokens run token by token.
+constexpr int kTokenLen = 16;
+
+struct Plan {
+    bool tokens, chunks;
+    int32_t token_len;
+    int64_t slots;
+    size_t bytes;
+};
+Plan make_plan(const delta_args* a) {
+    Plan pl{};
+    pl.token_len = a->token_len >= 0 ? a->token_len : kTokenLen;
+    const int64_t longest = a->cu_seqlens ? a->total_tokens : a->T;
+    pl.chunks = !a->snapshots && longest > pl.token_len;
+    pl.tokens = !pl.chunks || a->cu_seqlens;
+    if (pl.chunks) {
+        pl.slots = delta::chunk_slots(a->num_seqs, a->T, a->total_tokens, a->cu_seqlens != nullptr);
+        pl.bytes = delta::chunk_workspace(pl.slots, a->Hk, a->Hv, a->K);
+    }
+    return pl;
+}
 
 // What the kernels will leave out, into the status word.
 __global__ __launch_bounds__(256) void delta_status_kernel(const Params p) {
@@ -71,7 +93,9 @@ size_t delta_args_size(void) { return sizeof(delta_args); }
 int delta_workspace_size(const delta_args* a, size_t* bytes) {
     if (!a || !bytes) return WKV7_ERR_NULL;
     *bytes = 0;
-    return delta::check_sizes(a);
+    const int rc = delta::check_sizes(a);
+    if (rc == WKV7_OK && a->num_seqs > 0) *bytes = delta::make_plan(a).bytes;
+    return rc;
 }
 
 int delta_run(const delta_args* a, void* stream) {
@@ -79,6 +103,11 @@ int delta_run(const delta_args* a, void* stream) {
     const int rc = delta::check(a);
     if (rc != WKV7_OK) return rc;
     if (a->num_seqs == 0) return WKV7_OK;
+    const delta::Plan pl = delta::make_plan(a);
+    if (pl.bytes && (!a->workspace || a->workspace_bytes < pl.bytes)) return WKV7_ERR_WORKSPACE;
+    if (pl.bytes && !delta::aligned(a->workspace, 256)) return WKV7_ERR_ALIGN;
+    if (pl.chunks && (pl.slots * a->Hk > 0xFFFFFF || delta::chunk_groups(a->num_seqs, a->Hv, a->V) > 0xFFFFFF))
+        return WKV7_ERR_SHAPE;  // work-items of a launch below 2^32
     delta::Params p;
     p.q = a->q, p.k = a->k, p.v = a->v, p.q_stride = a->q_stride, p.k_stride = a->k_stride, p.v_stride = a->v_stride;
     p.g = a->g, p.beta = a->beta, p.g_stride = a->g_stride, p.beta_stride = a->beta_stride;
@@ -87,7 +116,7 @@ int delta_run(const delta_args* a, void* stream) {
     p.fresh = a->fresh, p.cu = a->cu_seqlens, p.n_keep = a->n_keep, p.snapshots = a->snapshots, p.status = a->status;
     p.workspace = static_cast<char*>(a->workspace), p.total_tokens = a->total_tokens;
     p.num_seqs = a->num_seqs, p.T = a->T, p.Hk = a->Hk, p.Hv = a->Hv, p.K = a->K, p.V = a->V, p.share = a->Hv / a->Hk;
-    p.scale = a->scale, p.qk_norm = a->qk_norm, p.token_len = 0x7FFFFFFF;
+    p.scale = a->scale, p.qk_norm = a->qk_norm, p.token_len = pl.token_len;
     const auto s = static_cast<hipStream_t>(stream);
     if (p.status) {
         hipLaunchKernelGGL(delta::delta_status_kernel, dim3((unsigned)((p.num_seqs + 255) / 256 < 64 ? (p.num_seqs + 255) / 256 : 64)),
@@ -95,7 +124,11 @@ int delta_run(const delta_args* a, void* stream) {
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return static_cast<int>(e);
     }
-    return static_cast<int>(delta::launch_tokens(p, s));
+    if (pl.chunks) {
+        const hipError_t e = delta::launch_chunks(p, wkv7::device_cu_count(), s);
+        if (e != hipSuccess) return static_cast<int>(e);
+    }
+    return pl.tokens ? static_cast<int>(delta::launch_tokens(p, s)) : WKV7_OK;
 }
 
 }  // extern "C"

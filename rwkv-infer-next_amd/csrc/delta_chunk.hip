@@ -1,0 +1,561 @@
+// delta_chunk.hip -- the gated delta rule by chunks of 64 tokens, on the matrix cores (include/delta.h).
+//
+// With c_i the sum of g up to token i of a chunk, k and q normalised and q scaled, S the state before the chunk:
+//     A_ij = beta_i (k_i . k_j) e^(c_i - c_j), i > j           T = (1 + A)^-1, lower triangular
+//     R_i = beta_i (v_i - e^c_i S^T k_i)                       D = T R           (what each token writes)
+//     B_ij = (q_i . k_j) e^(c_i - c_j), i >= j                 o_i = e^c_i S^T q_i + sum_j B_ij D_j
+//     S <- e^c_63 S + sum_j e^(c_63 - c_j) k_j D_j^T
+// Two launches: one makes T, B and the tokens' factors of every chunk, all chunks at once; the other goes through a row's chunks in
+// order.  Norms, decays and beta are factors of rows, kept apart from the products, whose one operand is so the caller's bf16, exact.
+// The other, fp32, is split into three bf16 parts, 24 bits, wherever it leads to the state; the outputs, bf16, take two parts.
+#include "delta_device.h"
+
+namespace delta {
+namespace {
+
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// Waits for this wavefront's LDS traffic and then for the workgroup; global loads stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+constexpr int kRow = 68;           // floats between rows of a matrix in LDS: 16-byte reads of 16 rows meet no bank twice
+constexpr float kLeast = -1e4f;    // decays below e^-10000 are 0 all the same, and differences of their sums stay finite
+
+// Of a 64 x 64 lower triangle in blocks of 16 x 32: tile t = 0, 1 has one, tile 2, 3 have two.
+__device__ __forceinline__ constexpr int block_of(int tile, int half) { return tile < 2 ? tile : 2 * tile - 2 + half; }
+// Token of row `row` of tile t.  Rows are dealt out so that the four rows which a lane holds of tile 2b and the four of tile 2b + 1
+// are eight tokens in a row: a result is the next product's operand without an exchange between lanes.  Rows of the state too.
+__device__ __forceinline__ int token_of(int tile, int row) { return 32 * (tile >> 1) + 8 * (row >> 2) + 4 * (tile & 1) + (row & 3); }
+
+// Which row and chunk a slot of the workspace holds; false for a slot that holds none.  Ragged rows begin at slot
+// cu[n] / 64 + n, which leaves each one room enough.
+__device__ __forceinline__ int64_t first_slot(const Params& p, int n, int64_t first) {
+    return p.cu ? first / kChunk + n : (int64_t)n * ((p.T + kChunk - 1) / kChunk);
+}
+__device__ __forceinline__ bool locate(const Params& p, int64_t slot, int& n, int64_t& first, int& len, int& chunk) {
+    if (p.cu) {
+        int lo = 0, hi = p.num_seqs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            int64_t s = p.cu[mid];
+            s = s < 0 ? 0 : s > p.total_tokens ? p.total_tokens : s;
+            if (s / kChunk + mid <= slot) lo = mid; else hi = mid;
+        }
+        n = lo;
+    } else {
+        n = (int)(slot / ((p.T + kChunk - 1) / kChunk));
+    }
+    extent(p, n, first, len);
+    const int64_t c = slot - first_slot(p, n, first);
+    chunk = (int)c;
+    return c >= 0 && c * kChunk < len && !(p.cu && len <= p.token_len);
+}
+
+// One workgroup: a chunk of a query/key head, then each of the value heads that share it.
+template <int K>
+__global__ __launch_bounds__(256) void delta_prep_kernel(const Params p, const Work w) {
+    constexpr int kSteps = K / 32, kPitch = K + 8;
+    __shared__ __attribute__((aligned(16))) float am[64 * kRow];   // A, then T
+    __shared__ __attribute__((aligned(16))) float bm[64 * kRow];   // K's tile, then B
+    __shared__ __attribute__((aligned(16))) float mm[32 * kRow];
+    __shared__ double cs[64];
+    __shared__ float rk[64], rq[64], be[64];
+    static_assert(64 * kPitch * 2 <= (int)sizeof(bm), "");
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int row = lane & 15, quad = lane >> 4;
+    const int64_t slot = blockIdx.x / (uint32_t)p.Hk;
+    const int hk = (int)(blockIdx.x % (uint32_t)p.Hk);
+    int n, len, chunk;
+    int64_t first;
+    if (!locate(p, slot, n, first, len, chunk)) return;
+    first += (int64_t)chunk * kChunk;
+    len = min(len - chunk * kChunk, kChunk);  // tokens of this chunk
+
+    const auto rows = [&](const uint16_t* x, int64_t stride, int block, u4* f) {
+        const int t = 16 * block + row;
+        const uint16_t* const at = x + (first + min(t, len - 1)) * stride + hk * K + quad * 8;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            f[s] = *reinterpret_cast<const u4*>(at + 32 * s);
+            if (t >= len) f[s] = u4{0, 0, 0, 0};
+        }
+    };
+    u4 kf[kSteps], qf[kSteps];
+    rows(p.k, p.k_stride, wave, kf);
+    rows(p.q, p.q_stride, wave, qf);
+    f4 kk[4], qk[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        kk[j] = qk[j] = f4{0.f, 0.f, 0.f, 0.f};
+        if (j <= wave) {
+            u4 of[kSteps];
+            rows(p.k, p.k_stride, j, of);
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                kk[j] = mfma(kf[s], of[s], kk[j]);
+                qk[j] = mfma(qf[s], of[s], qk[j]);
+            }
+        }
+    }
+    float nk = 0.f, nq = 0.f;
+    uint16_t* const tile = reinterpret_cast<uint16_t*>(bm);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x = bf16_at(kf[s], i), y = bf16_at(qf[s], i);
+            nk = fmaf(x, x, nk);
+            nq = fmaf(y, y, nq);
+        }
+        *reinterpret_cast<u4*>(tile + (16 * wave + row) * kPitch + 32 * s + 8 * quad) = kf[s];
+    }
+    nk += __shfl_xor(nk, 16), nq += __shfl_xor(nq, 16);
+    nk += __shfl_xor(nk, 32), nq += __shfl_xor(nq, 32);
+    if (quad == 0) {
+        rk[16 * wave + row] = p.qk_norm ? 1.f / sqrtf(nk + kNormEps) : 1.f;
+        rq[16 * wave + row] = p.qk_norm ? p.scale / sqrtf(nq + kNormEps) : p.scale;
+    }
+    __syncthreads();
+    // K^T in operand order: tile of 16 rows of the state, half of the tokens, lane
+    u4* const kt = reinterpret_cast<u4*>(w.kt + (slot * p.Hk + hk) * (K * kChunk * 2));
+    for (int e = tid; e < K / 16 * 2 * 64; e += 256) {
+        const int l = e & 63, half = (e >> 6) & 1, t = e >> 7, d = token_of(t, l & 15);
+        u4 x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint16_t* const at = tile + (32 * half + 8 * (l >> 4) + 2 * j) * kPitch + d;
+            x[j] = (uint32_t)at[0] | (uint32_t)at[kPitch] << 16;
+        }
+        kt[e] = x;
+    }
+
+    for (int h = hk * p.share; h < (hk + 1) * p.share; ++h) {
+        char* const rec = w.rec + (slot * p.Hv + h) * kRecord;
+        // the sums of g, in 64 bits: differences of far tokens' sums lose nothing
+        const int64_t token = first + min(lane, len - 1);
+        const float g = p.g[token * p.g_stride + h], b = p.beta[token * p.beta_stride + h];
+        double c = lane < len ? (double)(g < kLeast ? kLeast : g) : 0.0;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const double other = __shfl_up(c, d);
+            c += lane >= d ? other : 0.0;
+        }
+        const double last = __shfl(c, 63);
+        const float beta = lane < len ? b : 0.f;
+        __syncthreads();  // K's tile is read; the head before is written
+        if (wave == 0) {
+            cs[lane] = c;
+            be[lane] = beta;
+            float* const f = reinterpret_cast<float*>(rec + kRecordFactors);
+            const float gamma = expf((float)c);
+            f[lane] = beta;
+            f[64 + lane] = beta * gamma * rk[lane];
+            f[128 + lane] = expf((float)(last - c)) * rk[lane];
+            f[192 + lane] = gamma * rq[lane];
+            if (lane == 0) f[256] = expf((float)last);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j <= wave) {
+                const int col = 16 * j + row;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = 16 * wave + 4 * quad + r;
+                    const float decay = i >= col ? expf((float)(cs[i] - cs[col])) * rk[col] : 0.f;
+                    am[i * kRow + col] = i > col ? kk[j][r] * (be[i] * rk[i]) * decay : 0.f;
+                    bm[i * kRow + col] = qk[j][r] * rq[i] * decay;
+                }
+            }
+        wkv7::wave_lds_sync();
+        // the inverse of this wavefront's 16 x 16 block, a column a lane, by forward substitution
+        {
+            const float* const a = am + 16 * wave * (kRow + 1);
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float s0 = i == row ? 1.f : 0.f, s1 = 0.f;
+#pragma unroll
+                for (int m = 0; m < (i + 3) / 4; ++m) {
+                    const f4 y = *reinterpret_cast<const f4*>(a + i * kRow + 4 * m);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (4 * m + r < i) (r & 1 ? s1 : s0) = fmaf(-y[r], x[4 * m + r], r & 1 ? s1 : s0);
+                }
+                x[i] = s0 + s1;
+            }
+            wkv7::wave_lds_sync();
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (i >> 2 == quad) am[(16 * wave + i) * kRow + 16 * wave + row] = x[i];
+        }
+        __syncthreads();
+        // Products of 16 x 16 blocks in fp32: of the second operand lane `quad` holds rows 4 quad .., which are then the ones that
+        // step s of the sum takes (4 quad + s), as they lie in a result.
+        const auto left = [&](const float* m, int i, int k) {
+            return *reinterpret_cast<const f4*>(m + (16 * i + row) * kRow + 16 * k + 4 * quad);
+        };
+        const auto right = [&](const float* m, int k, int j) {
+            f4 x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = m[(16 * k + 4 * quad + r) * kRow + 16 * j + row];
+            return x;
+        };
+        const auto times = [&](f4 a, f4 b, f4 c) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) c = mfma4(a[s], b[s], c);
+            return c;
+        };
+        const auto put = [&](float* m, int i, int j, f4 x) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) m[(16 * i + 4 * quad + r) * kRow + 16 * j + row] = x[r];
+        };
+        const f4 zero = {0.f, 0.f, 0.f, 0.f};
+        // [[P, 0], [X, Q]]^-1 = [[P^-1, 0], [-Q^-1 X P^-1, Q^-1]], for blocks of 16, then of 32
+        if (wave < 2) {
+            const f4 m = times(left(am, 2 * wave + 1, 2 * wave), right(am, 2 * wave, 2 * wave), zero);
+            const f4 x = times(left(am, 2 * wave + 1, 2 * wave + 1), m, zero);
+            put(am, 2 * wave + 1, 2 * wave, -x);
+        }
+        __syncthreads();
+        const int i = wave >> 1, j = wave & 1;
+        {
+            f4 m = zero;
+            for (int k = j; k < 2; ++k) m = times(left(am, 2 + i, k), right(am, k, j), m);
+            put(mm, i, j, m);
+        }
+        __syncthreads();
+        {
+            f4 x = zero;
+            for (int k = 0; k <= i; ++k) x = times(left(am, 2 + i, 2 + k), right(mm, k, j), x);
+            put(am, 2 + i, j, -x);
+        }
+        __syncthreads();
+        // T in fp32 and B in two bf16 parts, in operand order
+        for (int e = tid; e < 6 * 64; e += 256) {
+            const int block = e >> 6, l = e & 63;
+            const int t = block < 2 ? block : (block + 2) >> 1, half = block < 2 ? 0 : block & 1;
+            const int i = token_of(t, l & 15), at = 32 * half + 8 * (l >> 4);
+            f4 x[2], y[2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                x[m] = *reinterpret_cast<const f4*>(am + i * kRow + at + 4 * m);
+                y[m] = *reinterpret_cast<const f4*>(bm + i * kRow + at + 4 * m);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)  // above the diagonal nothing was computed
+                    if (at + 4 * m + r > i) x[m][r] = y[m][r] = 0.f;
+                *reinterpret_cast<f4*>(rec + kRecordT + ((block * 2 + m) * 64 + l) * 16) = x[m];
+            }
+            u4 hi, lo;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                uint32_t a, b;
+                wkv7::split_pair(y[m >> 1][2 * (m & 1)], y[m >> 1][2 * (m & 1) + 1], a, b);
+                hi[m] = a, lo[m] = b;
+            }
+            *reinterpret_cast<u4*>(rec + kRecordB + ((block * 2) * 64 + l) * 16) = hi;
+            *reinterpret_cast<u4*>(rec + kRecordB + ((block * 2 + 1) * 64 + l) * 16) = lo;
+        }
+    }
+}
+
+// x as three bf16 parts (24 bits), for two values at a time
+__device__ __forceinline__ void split3(float x0, float x1, uint32_t& a, uint32_t& b, uint32_t& c) {
+    typedef wkv7::f2_t f2;
+    const f2 x = {x0, x1};
+    const wkv7::bf16x2_t h = __builtin_convertvector(x, wkv7::bf16x2_t);
+    const wkv7::bf16x2_t m0 = wkv7::bf16_pair_in_register(0x0000BF80u), m1 = wkv7::bf16_pair_in_register(0xBF800000u);
+    const f2 y = {__builtin_amdgcn_fdot2_f32_bf16(h, m0, x0, false), __builtin_amdgcn_fdot2_f32_bf16(h, m1, x1, false)};
+    a = __builtin_bit_cast(uint32_t, h);
+    wkv7::split_pair(y[0], y[1], b, c);
+}
+
+// What a wavefront reads of a chunk.
+template <int K, int NT>
+struct Operands {
+    u4 k[K / 32], q[K / 32];     // its 16 tokens
+    u4 kt[K / 64][2];            // its rows of the state
+    f4 t[2][2];                  // its rows of T
+    u4 b[2][2];                  // its rows of B
+    f4 beta, seen, left, gamma;  // the factors of its tokens' four rows of a lane
+    float keep;
+    uint16_t v[NT][4];
+};
+
+// One workgroup: 16 NT columns of a head's state, through a row's chunks.  Its four wavefronts have a quarter of the chunk's tokens
+// and of the state's rows each, and hand each other operands through LDS: the state, R, D.
+template <int K, int NT>
+__global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void delta_scan_kernel(const Params p, const Work w) {
+    constexpr int kSteps = K / 32, kTiles = K / 64;  // of the state's rows: MFMA steps, tiles of a wavefront
+    __shared__ u4 sf[kSteps][3][NT][64];             // the state, three parts
+    __shared__ u4 rf[2][3][NT][64];                  // R
+    __shared__ u4 df[2][2][NT][64];                  // D, two parts
+    __shared__ u4 ef[2][3][NT][64];                  // D with the decay to the chunk's end
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, quad = lane >> 4;
+    // the columns of `together` heads follow each other on one XCD, whose L2 they share
+    const uint32_t slices = (uint32_t)(p.V / (16 * NT)), each = slices * (uint32_t)w.together;
+    const uint32_t group = blockIdx.x / 8 / each * 8 + blockIdx.x % 8, in = blockIdx.x / 8 % each;
+    const int64_t unit = (int64_t)group * w.together + in / slices;
+    if (unit >= (int64_t)p.num_seqs * p.Hv) return;
+    const int n = (int)(unit / p.Hv), h = (int)(unit % p.Hv), hk = h / p.share, col0 = (int)(in % slices) * 16 * NT;
+    int64_t first;
+    int len;
+    extent(p, n, first, len);
+    if (p.cu && len <= p.token_len) return;
+    const int chunks = (len + kChunk - 1) / kChunk;
+    const int64_t slot = first_slot(p, n, first);
+
+    // rows of the state in tile 2b + j, row r of a lane: 32 b + 8 quad + 4 j + r
+    const float* const from = initial(p, n, h);
+    float* const to = final_state(p, n, h);
+    const auto state_at = [&](int tile, int r) {
+        const int t = wave * kTiles + tile;
+        return (int64_t)(32 * (t >> 1) + 8 * quad + 4 * (t & 1) + r) * p.V + col0 + col;
+    };
+    f4 S[kTiles][NT];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) S[t][x][r] = from ? from[state_at(t, r) + 16 * x] : 0.f;
+
+    const auto fetch = [&](int chunk, Operands<K, NT>& o) {
+        const int64_t t0 = first + (int64_t)chunk * kChunk;
+        const int most = min(len - chunk * kChunk, kChunk) - 1;
+        const char* const rec = w.rec + ((slot + chunk) * p.Hv + h) * kRecord;
+        const u4* const kt = reinterpret_cast<const u4*>(w.kt + ((slot + chunk) * p.Hk + hk) * (K * kChunk * 2));
+        const uint32_t token = (uint32_t)min(token_of(wave, col), most);  // past the last token: it again, with a factor of 0
+        const uint16_t* const kp = wkv7::uniform_ptr(p.k + t0 * p.k_stride + hk * K);
+        const uint16_t* const qp = wkv7::uniform_ptr(p.q + t0 * p.q_stride + hk * K);
+        const uint16_t* const vp = wkv7::uniform_ptr(p.v + t0 * p.v_stride + (int64_t)h * p.V + col0);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            o.k[s] = *reinterpret_cast<const u4*>(kp + token * (uint32_t)p.k_stride + quad * 8 + 32 * s);
+            o.q[s] = *reinterpret_cast<const u4*>(qp + token * (uint32_t)p.q_stride + quad * 8 + 32 * s);
+        }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) o.kt[t][half] = kt[((wave * kTiles + t) * 2 + half) * 64 + lane];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int block = block_of(wave, wave < 2 ? 0 : half);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                o.t[half][m] = *reinterpret_cast<const f4*>(rec + kRecordT + ((block * 2 + m) * 64 + lane) * 16);
+                o.b[half][m] = *reinterpret_cast<const u4*>(rec + kRecordB + ((block * 2 + m) * 64 + lane) * 16);
+            }
+        }
+        const float* const f = reinterpret_cast<const float*>(rec + kRecordFactors) + token_of(wave, 4 * quad);
+        o.beta = *reinterpret_cast<const f4*>(f);
+        o.seen = *reinterpret_cast<const f4*>(f + 64);
+        o.left = *reinterpret_cast<const f4*>(f + 128);
+        o.gamma = *reinterpret_cast<const f4*>(f + 192);
+        o.keep = *reinterpret_cast<const float*>(rec + kRecordFactors + 1024);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t at = (uint32_t)min(token_of(wave, 4 * quad + r), most) * (uint32_t)p.v_stride + col;
+#pragma unroll
+            for (int x = 0; x < NT; ++x) o.v[x][r] = vp[at + 16 * x];
+        }
+    };
+    const auto share_state = [&] {
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+                const int tile = wave * kTiles + t;
+                u2 a, b, c;
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    uint32_t i, j, k;
+                    split3(S[t][x][2 * m], S[t][x][2 * m + 1], i, j, k);
+                    a[m] = i, b[m] = j, c[m] = k;
+                }
+                reinterpret_cast<u2*>(&sf[tile >> 1][0][x][lane])[tile & 1] = a;
+                reinterpret_cast<u2*>(&sf[tile >> 1][1][x][lane])[tile & 1] = b;
+                reinterpret_cast<u2*>(&sf[tile >> 1][2][x][lane])[tile & 1] = c;
+            }
+    };
+    const f4 zero = {0.f, 0.f, 0.f, 0.f};
+    const auto step = [&](int chunk, const Operands<K, NT>& o) {
+        f4 P[NT], O[NT];
+#pragma unroll
+        for (int x = 0; x < NT; ++x) P[x] = O[x] = zero;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+                const u4 a = sf[s][0][x][lane], b = sf[s][1][x][lane], c = sf[s][2][x][lane];
+                P[x] = mfma(o.k[s], c, P[x]);
+                O[x] = mfma(o.q[s], b, O[x]);
+                P[x] = mfma(o.k[s], b, P[x]);
+                O[x] = mfma(o.q[s], a, O[x]);
+                P[x] = mfma(o.k[s], a, P[x]);
+            }
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+            f4 R;
+            u2 a, b, c;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                R[r] = fmaf(-o.seen[r], P[x][r], o.beta[r] * wkv7::bf16_to_f32(o.v[x][r]));
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                uint32_t i, j, k;
+                split3(R[2 * m], R[2 * m + 1], i, j, k);
+                a[m] = i, b[m] = j, c[m] = k;
+            }
+            reinterpret_cast<u2*>(&rf[wave >> 1][0][x][lane])[wave & 1] = a;
+            reinterpret_cast<u2*>(&rf[wave >> 1][1][x][lane])[wave & 1] = b;
+            reinterpret_cast<u2*>(&rf[wave >> 1][2][x][lane])[wave & 1] = c;
+        }
+        u4 th[2], tm[2], tl[2];  // T in three parts
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                uint32_t i, j, k;
+                split3(o.t[half][m >> 1][2 * (m & 1)], o.t[half][m >> 1][2 * (m & 1) + 1], i, j, k);
+                th[half][m] = i, tm[half][m] = j, tl[half][m] = k;
+            }
+        lds_barrier();
+        f4 D[NT];
+#pragma unroll
+        for (int x = 0; x < NT; ++x) D[x] = zero;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+            if (half == 0 || wave >= 2)
+#pragma unroll
+                for (int x = 0; x < NT; ++x) {
+                    const u4 a = rf[half][0][x][lane], b = rf[half][1][x][lane], c = rf[half][2][x][lane];
+                    D[x] = mfma(tl[half], a, D[x]);
+                    D[x] = mfma(th[half], c, D[x]);
+                    D[x] = mfma(tm[half], b, D[x]);
+                    D[x] = mfma(tm[half], a, D[x]);
+                    D[x] = mfma(th[half], b, D[x]);
+                    D[x] = mfma(th[half], a, D[x]);
+                }
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+            u2 a, b, c, d, e;
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                uint32_t i, j, k;
+                wkv7::split_pair(D[x][2 * m], D[x][2 * m + 1], i, j);
+                a[m] = i, b[m] = j;
+                split3(D[x][2 * m] * o.left[2 * m], D[x][2 * m + 1] * o.left[2 * m + 1], i, j, k);
+                c[m] = i, d[m] = j, e[m] = k;
+            }
+            reinterpret_cast<u2*>(&df[wave >> 1][0][x][lane])[wave & 1] = a;
+            reinterpret_cast<u2*>(&df[wave >> 1][1][x][lane])[wave & 1] = b;
+            reinterpret_cast<u2*>(&ef[wave >> 1][0][x][lane])[wave & 1] = c;
+            reinterpret_cast<u2*>(&ef[wave >> 1][1][x][lane])[wave & 1] = d;
+            reinterpret_cast<u2*>(&ef[wave >> 1][2][x][lane])[wave & 1] = e;
+        }
+        lds_barrier();
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int x = 0; x < NT; ++x) S[t][x] *= o.keep;
+#pragma unroll
+        for (int part = 2; part >= 0; --part)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int x = 0; x < NT; ++x) {
+                    const u4 e = ef[half][part][x][lane];
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) S[t][x] = mfma(o.kt[t][half], e, S[t][x]);
+                }
+        share_state();
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) O[x][r] *= o.gamma[r];
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                if (half == 0 || wave >= 2) {
+                    const u4 a = df[half][0][x][lane], b = df[half][1][x][lane];
+                    O[x] = mfma(o.b[half][1], a, O[x]);
+                    O[x] = mfma(o.b[half][0], b, O[x]);
+                    O[x] = mfma(o.b[half][0], a, O[x]);
+                }
+        }
+        if (p.o)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int t = chunk * kChunk + token_of(wave, 4 * quad + r);
+                if (t < len)
+#pragma unroll
+                    for (int x = 0; x < NT; ++x)
+                        p.o[(first + t) * p.o_stride + (int64_t)h * p.V + col0 + 16 * x + col] = wkv7::f32_to_bf16(O[x][r]);
+            }
+        lds_barrier();
+    };
+    share_state();
+    lds_barrier();
+    Operands<K, NT> even, odd;
+    if (chunks > 0) fetch(0, even);
+    for (int c = 0; c < chunks; c += 2) {
+        fetch(min(c + 1, chunks - 1), odd);
+        step(c, even);
+        if (c + 1 < chunks) {
+            fetch(min(c + 2, chunks - 1), even);
+            step(c + 1, odd);
+        }
+    }
+    if (to)
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int x = 0; x < NT; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) to[state_at(t, r) + 16 * x] = S[t][x][r];
+}
+
+template <int K>
+hipError_t launch(const Params& p, const Work& w, int64_t slots, bool wide, hipStream_t stream) {
+    hipLaunchKernelGGL(delta_prep_kernel<K>, dim3((unsigned)(slots * p.Hk)), dim3(256), 0, stream, p, w);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const int64_t groups = ((int64_t)p.num_seqs * p.Hv / w.together + 7) / 8 * 8;
+    if (wide)
+        hipLaunchKernelGGL((delta_scan_kernel<K, 2>), dim3((unsigned)(groups * w.together * (p.V / 32))), dim3(256), 0, stream, p, w);
+    else
+        hipLaunchKernelGGL((delta_scan_kernel<K, 1>), dim3((unsigned)(groups * w.together * (p.V / 16))), dim3(256), 0, stream, p, w);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t chunk_slots(int32_t num_seqs, int32_t T, int64_t total_tokens, bool ragged) {
+    return ragged ? total_tokens / kChunk + num_seqs : (int64_t)num_seqs * ((T + kChunk - 1) / kChunk);
+}
+int64_t chunk_groups(int32_t num_seqs, int32_t Hv, int32_t V) { return ((int64_t)num_seqs + 7) / 8 * 8 * Hv * (V / 16); }
+size_t chunk_workspace(int64_t slots, int32_t Hk, int32_t Hv, int32_t K) {
+    return (size_t)slots * (Hk * (size_t)(K * kChunk * 2) + Hv * (size_t)kRecord);
+}
+
+hipError_t launch_chunks(const Params& p, int cus, hipStream_t stream) {
+    const int64_t slots = chunk_slots(p.num_seqs, p.T, p.total_tokens, p.cu != nullptr);
+    Work w;
+    w.kt = p.workspace;
+    w.rec = p.workspace + slots * p.Hk * (int64_t)(p.K * kChunk * 2);
+    w.together = (int64_t)p.num_seqs * p.Hk >= 8 ? p.share : 1;
+    const bool wide = p.V % 32 == 0 && (int64_t)p.num_seqs * p.Hv * (p.V / 32) >= 2 * cus;
+    return p.K == 64 ? launch<64>(p, w, slots, wide, stream) : launch<128>(p, w, slots, wide, stream);
+}
+
+}  // namespace delta

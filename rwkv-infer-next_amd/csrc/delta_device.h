@@ -75,6 +75,20 @@ __device__ __forceinline__ float bf16_at(u4 x, int i) {  // element i of eight
     return __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16);
 }
 
+// The workspace of the chunks' kernels.  For each slot (a chunk's place) and query/key head K^T in operand order, and for each slot and
+// value head a record: T (fp32) and B (two bf16 parts) of the lower triangle's blocks, six each, and the tokens' factors.
+constexpr int kChunk = 64;
+constexpr int64_t kRecordT = 0, kRecordB = 6 * 2048, kRecordFactors = 12 * 2048, kRecord = 12 * 2048 + 1280;
+struct Work {
+    char *kt, *rec;
+    int32_t together;  // heads whose workgroups follow each other on one XCD
+};
+int64_t chunk_slots(int32_t num_seqs, int32_t T, int64_t total_tokens, bool ragged);
+int64_t chunk_groups(int32_t num_seqs, int32_t Hv, int32_t V);  // most workgroups of the chunks' scan
+size_t chunk_workspace(int64_t slots, int32_t Hk, int32_t Hv, int32_t K);
+
+// All rows (ragged: those longer than token_len) by chunks; by tokens (ragged: those up to token_len).
+hipError_t launch_chunks(const Params& p, int cus, hipStream_t stream);
 hipError_t launch_tokens(const Params& p, hipStream_t stream);
 
 }  // namespace delta
