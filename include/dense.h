@@ -48,6 +48,8 @@ typedef struct dense_args {
     int32_t M, N, K;               /* K % 32 == 0 */
     int32_t dtype, out_dtype, bias_dtype, residual_dtype;
     int32_t activation;
+    void *workspace;               /* dense_workspace_size bytes, 16-byte aligned; what it holds does not matter */
+    size_t workspace_bytes;
 } dense_args;
 
 /* sizeof(dense_args) as compiled into the library (bindings check their struct layout against it). */
@@ -59,6 +61,9 @@ int dense_packed_size(int32_t K, int32_t N, size_t *bytes);
 /* Lays a weight of 16-bit elements [K][N] out for dense_matmul, on `stream`: element (k, n) at w + k k_stride + n n_stride (elements),
  * so either order of a matrix is taken.  packed is 16-byte aligned. */
 int dense_pack(const uint16_t *w, int64_t k_stride, int64_t n_stride, int32_t K, int32_t N, void *packed, void *stream);
+
+/* Bytes of workspace that a product of M rows needs on the current device: 0, or the sums of K's parts where it is split. */
+int dense_workspace_size(int32_t M, int32_t N, int32_t K, size_t *bytes);
 
 /* The product, on `stream`.  The order of the sums follows from M, N, K and the device's CU count: equal calls give equal bits. */
 int dense_matmul(const dense_args *args, void *stream);

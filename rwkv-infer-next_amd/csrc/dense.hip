@@ -1,75 +1,10 @@
 // dense.hip -- products of bf16 / fp16 activations with 16-bit weights, bias, activation and residual in the epilogue
 // (include/dense.h), on the matrix cores (16x16x32, fp32 accumulation).
-#include <hip/hip_runtime.h>
-#include <stdint.h>
-
-#include "dense.h"
-#include "dense_plan.h"
-#include "wkv7_device.h"
+#include "dense_device.h"
 #include "wkv7_launch.h"
 
 namespace dense {
 namespace {
-
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-
-struct Params {
-    const uint16_t* a;
-    int64_t a_row_stride;
-    const uint8_t* weight;
-    const void *bias, *residual;
-    int64_t residual_row_stride;
-    void* out;
-    int64_t out_row_stride;
-    int32_t M, N, K, steps, row_groups, strip_groups, strips;
-    int32_t out_dtype, bias_dtype, residual_dtype, activation;
-};
-
-template <int AT>
-__device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
-    if constexpr (AT == DENSE_BF16)
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
-}
-
-__device__ __forceinline__ float load(const void* x, int dtype, int64_t at) {
-    if (dtype == DENSE_F32) return static_cast<const float*>(x)[at];
-    if (dtype == DENSE_BF16) return wkv7::bf16_to_f32(static_cast<const uint16_t*>(x)[at]);
-    return (float)static_cast<const _Float16*>(x)[at];
-}
-
-__device__ __forceinline__ void store(void* out, int dtype, int64_t at, float x) {
-    if (dtype == DENSE_F32)
-        static_cast<float*>(out)[at] = x;
-    else if (dtype == DENSE_BF16)
-        static_cast<uint16_t*>(out)[at] = wkv7::f32_to_bf16(x);
-    else
-        static_cast<_Float16*>(out)[at] = (_Float16)x;
-}
-
-__device__ __forceinline__ float activate(float x, int activation) {
-    switch (activation) {
-        case DENSE_RELU: return x > 0.f ? x : x == x ? 0.f : x;  // NaN stays NaN
-        case DENSE_RELU2: return x > 0.f ? x * x : x == x ? 0.f : x;
-        case DENSE_TANH: return tanhf(x);
-        case DENSE_SIGMOID: return 1.f / (1.f + expf(-x));
-        case DENSE_SILU: return x / (1.f + expf(-x));
-        case DENSE_GELU: return 0.5f * x * erfcf(x * -0.70710678118654752f);
-        default: return x;
-    }
-}
-
-// The sum x of (row, column n) through the epilogue.
-__device__ __forceinline__ void finish(const Params& p, int64_t row, int64_t n, float x) {
-    if (p.bias) x += load(p.bias, p.bias_dtype, n);
-    x = activate(x, p.activation);
-    if (p.residual) x += load(p.residual, p.residual_dtype, row * p.residual_row_stride + n);
-    store(p.out, p.out_dtype, row * p.out_row_stride + n, x);
-}
 
 // Strips: a workgroup's wavefronts take the 128-row chunks of K in turn, each with sums of its own for 16 rows by 16 NT columns; they
 // are added in LDS in the wavefronts' order.
@@ -179,6 +114,13 @@ int dense_pack(const uint16_t* w, int64_t k_stride, int64_t n_stride, int32_t K,
     return static_cast<int>(hipGetLastError());
 }
 
+int dense_workspace_size(int32_t M, int32_t N, int32_t K, size_t* bytes) {
+    if (!bytes) return WKV7_ERR_NULL;
+    if (!dense::good_weight(K, N) || M < 0) return WKV7_ERR_SHAPE;
+    *bytes = M == 0 ? 0 : dense::plan(M, N, K, wkv7::device_cu_count()).workspace;
+    return WKV7_OK;
+}
+
 int dense_matmul(const dense_args* x, void* stream) {
     if (!x) return WKV7_ERR_NULL;
     if (!dense::good_weight(x->K, x->N) || x->M < 0) return WKV7_ERR_SHAPE;
@@ -197,15 +139,24 @@ int dense_matmul(const dense_args* x, void* stream) {
         return WKV7_ERR_SHAPE;
     const dense::Plan pl = dense::plan(x->M, x->N, x->K, wkv7::device_cu_count());
     if (pl.grid > dense::kMaxGrid) return WKV7_ERR_SHAPE;
+    if (pl.workspace && (!x->workspace || x->workspace_bytes < pl.workspace)) return WKV7_ERR_WORKSPACE;
+    if (pl.workspace && !dense::aligned(x->workspace, 16)) return WKV7_ERR_ALIGN;
     dense::Params p;
     p.a = x->a, p.a_row_stride = x->M > 1 ? x->a_row_stride : x->K, p.weight = static_cast<const uint8_t*>(x->weight);
     p.bias = x->bias, p.residual = x->residual, p.residual_row_stride = x->residual_row_stride;
     p.out = x->out, p.out_row_stride = x->out_row_stride;
+    p.sums = static_cast<float*>(x->workspace), p.parts = pl.parts;
+    // four columns at once: bias, residual and result in steps of four elements, aligned to them
+    p.fours = x->N % 4 == 0 && dense::aligned(x->out, 4 * dense::size_of(x->out_dtype)) && (x->M == 1 || x->out_row_stride % 4 == 0) &&
+              (!x->bias || dense::aligned(x->bias, 4 * dense::size_of(x->bias_dtype))) &&
+              (!x->residual || (dense::aligned(x->residual, 4 * dense::size_of(x->residual_dtype)) &&
+                                (x->M == 1 || x->residual_row_stride % 4 == 0)));
     p.M = x->M, p.N = x->N, p.K = x->K;
     p.steps = (int32_t)dense::steps(x->K), p.strips = (int32_t)dense::strips(x->N);
     p.row_groups = (int32_t)pl.row_groups, p.strip_groups = (int32_t)pl.strip_groups;
     p.out_dtype = x->out_dtype, p.bias_dtype = x->bias_dtype, p.residual_dtype = x->residual_dtype, p.activation = x->activation;
     const auto s = static_cast<hipStream_t>(stream);
+    if (pl.shape != dense::kStrips) return static_cast<int>(dense::launch_tiles(p, pl, x->dtype, s));
     if (x->dtype == DENSE_BF16)
         dense::launch<DENSE_BF16>(p, pl, s);
     else

@@ -69,7 +69,7 @@ LOGITS_COUNTS_F32 = 1
 LOGITS_SAMPLE_STATE_BYTES = 4325376  # leading workspace region that is zero between calls
 LOGITS_STATUS_ROW = 256
 LOGITS_STATUS_TOKEN = 512
-DENSE_EXPORTED = ("dense_args_size", "dense_packed_size", "dense_pack", "dense_matmul")
+DENSE_EXPORTED = ("dense_args_size", "dense_packed_size", "dense_pack", "dense_workspace_size", "dense_matmul")
 DENSE_BF16 = 0
 DENSE_F16 = 1
 DENSE_F32 = 2
@@ -206,7 +206,7 @@ class DenseArgs(ctypes.Structure):
         ("residual_row_stride", ctypes.c_int64), ("out", _vp), ("out_row_stride", ctypes.c_int64),
         ("M", ctypes.c_int32), ("N", ctypes.c_int32), ("K", ctypes.c_int32), ("dtype", ctypes.c_int32),
         ("out_dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32), ("residual_dtype", ctypes.c_int32),
-        ("activation", ctypes.c_int32),
+        ("activation", ctypes.c_int32), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -334,6 +334,8 @@ def load(path: str = LIB_PATH):
     lib.dense_packed_size.argtypes = [i32, i32, psz]
     lib.dense_pack.restype = ctypes.c_int
     lib.dense_pack.argtypes = [_vp, i64, i64, i32, i32, _vp, _vp]
+    lib.dense_workspace_size.restype = ctypes.c_int
+    lib.dense_workspace_size.argtypes = [i32, i32, i32, psz]
     lib.dense_matmul.restype = ctypes.c_int
     lib.dense_matmul.argtypes = [_vp, _vp]  # a DenseArgs by reference, or pack_dense's bytes
     lib.delta_args_size.restype = ctypes.c_size_t

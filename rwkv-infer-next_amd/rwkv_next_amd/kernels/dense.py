@@ -111,10 +111,18 @@ def dense_matmul(a, packed: DensePacked, *, bias=None, activation: Optional[str]
     if x.stride(1) != 1 or row % 8 or row < K or row > _lib.DENSE_MAX_ROW_STRIDE or ptr % 16:
         x = x.clone(memory_format=torch.contiguous_format)
         row, ptr = K, x.data_ptr()
-    args = _lib.pack_dense(ptr, row, weight.data_ptr(), b_p, r_p, r_row, out.data_ptr(), N, M, N, K, _CODES[adt], _CODES[odt],
-                           b_t, r_t, ACTIVATIONS[activation])  # in the order of the fields
+    lib, sums, sums_p, size = _lib.load(), None, 0, 0
     with on_device(dev):
-        _lib.check(_lib.load().dense_matmul(args, stream_handle(dev)))
+        if M > 16:  # fewer rows are not split
+            need = ctypes.c_size_t(0)
+            _lib.check(lib.dense_workspace_size(M, N, K, ctypes.byref(need)))
+            size = need.value
+            if size:  # what it holds does not matter: from the caching allocator, in the stream's order
+                sums = torch.empty(size, dtype=torch.uint8, device=dev)
+                sums_p = sums.data_ptr()
+        args = _lib.pack_dense(ptr, row, weight.data_ptr(), b_p, r_p, r_row, out.data_ptr(), N, M, N, K, _CODES[adt], _CODES[odt],
+                               b_t, r_t, ACTIVATIONS[activation], sums_p, size)  # in the order of the fields
+        _lib.check(lib.dense_matmul(args, stream_handle(dev)))
     return out
 
 
