@@ -6,56 +6,6 @@
 namespace dense {
 namespace {
 
-// Strips: a workgroup's wavefronts take the 128-row chunks of K in turn, each with sums of its own for 16 rows by 16 NT columns; they
-// are added in LDS in the wavefronts' order.
-template <int AT, int NT>
-__global__ __launch_bounds__(512) void dense_strip_kernel(const Params p) {
-    extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][16][16 * NT]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const uint32_t on_xcd = blockIdx.x >> 3;
-    const uint32_t group = on_xcd / (uint32_t)p.row_groups * 8 + (blockIdx.x & 7);
-    const int row0 = (int)(on_xcd % (uint32_t)p.row_groups) * 16;
-    if (group >= (uint32_t)p.strip_groups) return;
-    const int strip0 = (int)group * NT, col = lane & 15, quad = lane >> 4;
-
-    const uint8_t* wp[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)  // past the last strip: that strip again, not stored
-        wp[t] = p.weight + (int64_t)min(strip0 + t, p.strips - 1) * p.steps * kBlockBytes + lane * 16;
-    const uint16_t* const ap = p.a + (int64_t)min(row0 + col, p.M - 1) * p.a_row_stride + quad * 8;  // past the last row: it again
-
-    f4 acc[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) acc[t] = f4{0.f, 0.f, 0.f, 0.f};
-    for (int s0 = wave * 4; s0 < p.steps; s0 += waves * 4) {
-        u4 w[4][NT], a[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int s = min(s0 + k, p.steps - 1);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) w[k][t] = *reinterpret_cast<const u4*>(wp[t] + (int64_t)s * kBlockBytes);
-            a[k] = *reinterpret_cast<const u4*>(ap + s * kStep);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (s0 + k < p.steps)
-#pragma unroll
-                for (int t = 0; t < NT; ++t) acc[t] = mfma<AT>(a[k], w[k][t], acc[t]);
-    }
-    float* const mine = part + wave * (NT * 256);
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) mine[(quad * 4 + r) * (16 * NT) + 16 * t + col] = acc[t][r];
-    __syncthreads();
-    for (int e = threadIdx.x; e < NT * 256; e += blockDim.x) {
-        float x = 0.f;
-        for (int v = 0; v < waves; ++v) x += part[v * (NT * 256) + e];
-        const int64_t row = row0 + e / (16 * NT), n = (int64_t)strip0 * kStrip + e % (16 * NT);
-        if (row < p.M && n < p.N) finish(p, row, n, x);
-    }
-}
-
 // One 16-byte piece of the packed weight a thread: lane l of (strip, step) holds column l % 16, rows 8 (l / 16) + 0..7 of the step;
 // zeros past the last column.
 __global__ __launch_bounds__(256) void dense_pack_kernel(const uint16_t* w, int64_t k_stride, int64_t n_stride, uint8_t* packed,
@@ -76,18 +26,6 @@ bool good_weight(int32_t K, int32_t N) { return K >= kStep && N >= 1 && K % kSte
 uintptr_t size_of(int32_t dtype) { return dtype == DENSE_F32 ? 4 : 2; }
 bool good_type(int32_t dtype) { return dtype >= DENSE_BF16 && dtype <= DENSE_F32; }
 constexpr int64_t kMaxGrid = 0x7FFFFF;  // workgroups of one launch: with 512 threads below 2^32 work-items
-
-template <int AT>
-void launch(const Params& p, const Plan& pl, hipStream_t s) {
-    const dim3 grid((unsigned)pl.grid), block(64 * pl.waves);
-    const size_t lds = (size_t)pl.waves * pl.nt * 256 * sizeof(float);
-    if (pl.nt == 1)
-        hipLaunchKernelGGL((dense_strip_kernel<AT, 1>), grid, block, lds, s, p);
-    else if (pl.nt == 2)
-        hipLaunchKernelGGL((dense_strip_kernel<AT, 2>), grid, block, lds, s, p);
-    else
-        hipLaunchKernelGGL((dense_strip_kernel<AT, 4>), grid, block, lds, s, p);
-}
 
 }  // namespace
 }  // namespace dense
@@ -155,13 +93,7 @@ int dense_matmul(const dense_args* x, void* stream) {
     p.steps = (int32_t)dense::steps(x->K), p.strips = (int32_t)dense::strips(x->N);
     p.row_groups = (int32_t)pl.row_groups, p.strip_groups = (int32_t)pl.strip_groups;
     p.out_dtype = x->out_dtype, p.bias_dtype = x->bias_dtype, p.residual_dtype = x->residual_dtype, p.activation = x->activation;
-    const auto s = static_cast<hipStream_t>(stream);
-    if (pl.shape != dense::kStrips) return static_cast<int>(dense::launch_tiles(p, pl, x->dtype, s));
-    if (x->dtype == DENSE_BF16)
-        dense::launch<DENSE_BF16>(p, pl, s);
-    else
-        dense::launch<DENSE_F16>(p, pl, s);
-    return static_cast<int>(hipGetLastError());
+    return static_cast<int>(dense::launch_tiles(p, pl, x->dtype, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"
