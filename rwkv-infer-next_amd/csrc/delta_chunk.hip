@@ -60,6 +60,17 @@ __device__ __forceinline__ bool locate(const Params& p, int64_t slot, int& n, in
     return c >= 0 && c * kChunk < len && !(p.cu && len <= p.token_len);
 }
 
+// x as three bf16 parts (24 bits), for two values at a time
+__device__ __forceinline__ void split3(float x0, float x1, uint32_t& a, uint32_t& b, uint32_t& c) {
+    typedef wkv7::f2_t f2;
+    const f2 x = {x0, x1};
+    const wkv7::bf16x2_t h = __builtin_convertvector(x, wkv7::bf16x2_t);
+    const wkv7::bf16x2_t m0 = wkv7::bf16_pair_in_register(0x0000BF80u), m1 = wkv7::bf16_pair_in_register(0xBF800000u);
+    const f2 y = {__builtin_amdgcn_fdot2_f32_bf16(h, m0, x0, false), __builtin_amdgcn_fdot2_f32_bf16(h, m1, x1, false)};
+    a = __builtin_bit_cast(uint32_t, h);
+    wkv7::split_pair(y[0], y[1], b, c);
+}
+
 // One workgroup: a chunk of a query/key head, then each of the value heads that share it.
 template <int K>
 __global__ __launch_bounds__(256) void delta_prep_kernel(const Params p, const Work w) {
@@ -240,7 +251,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const Params p, const W
             put(am, 2 + i, j, -x);
         }
         __syncthreads();
-        // T in fp32 and B in two bf16 parts, in operand order
+        // T in three bf16 parts and B in two, in operand order
         for (int e = tid; e < 6 * 64; e += 256) {
             const int block = e >> 6, l = e & 63;
             const int t = block < 2 ? block : (block + 2) >> 1, half = block < 2 ? 0 : block & 1;
@@ -253,54 +264,54 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const Params p, const W
 #pragma unroll
                 for (int r = 0; r < 4; ++r)  // above the diagonal nothing was computed
                     if (at + 4 * m + r > i) x[m][r] = y[m][r] = 0.f;
-                *reinterpret_cast<f4*>(rec + kRecordT + ((block * 2 + m) * 64 + l) * 16) = x[m];
             }
-            u4 hi, lo;
+            u4 hi, lo, part[3];
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-                uint32_t a, b;
+                uint32_t a, b, c;
                 wkv7::split_pair(y[m >> 1][2 * (m & 1)], y[m >> 1][2 * (m & 1) + 1], a, b);
                 hi[m] = a, lo[m] = b;
+                split3(x[m >> 1][2 * (m & 1)], x[m >> 1][2 * (m & 1) + 1], a, b, c);
+                part[0][m] = a, part[1][m] = b, part[2][m] = c;
             }
+#pragma unroll
+            for (int m = 0; m < 3; ++m) *reinterpret_cast<u4*>(rec + kRecordT + ((block * 3 + m) * 64 + l) * 16) = part[m];
             *reinterpret_cast<u4*>(rec + kRecordB + ((block * 2) * 64 + l) * 16) = hi;
             *reinterpret_cast<u4*>(rec + kRecordB + ((block * 2 + 1) * 64 + l) * 16) = lo;
         }
     }
 }
 
-// x as three bf16 parts (24 bits), for two values at a time
-__device__ __forceinline__ void split3(float x0, float x1, uint32_t& a, uint32_t& b, uint32_t& c) {
-    typedef wkv7::f2_t f2;
-    const f2 x = {x0, x1};
-    const wkv7::bf16x2_t h = __builtin_convertvector(x, wkv7::bf16x2_t);
-    const wkv7::bf16x2_t m0 = wkv7::bf16_pair_in_register(0x0000BF80u), m1 = wkv7::bf16_pair_in_register(0xBF800000u);
-    const f2 y = {__builtin_amdgcn_fdot2_f32_bf16(h, m0, x0, false), __builtin_amdgcn_fdot2_f32_bf16(h, m1, x1, false)};
-    a = __builtin_bit_cast(uint32_t, h);
-    wkv7::split_pair(y[0], y[1], b, c);
-}
-
-// What a wavefront reads of a chunk.
+// What a wavefront reads of a chunk: one of those that carry the state ..
 template <int K, int NT>
-struct Operands {
-    u4 k[K / 32], q[K / 32];     // its 16 tokens
-    u4 kt[K / 64][2];            // its rows of the state
-    f4 t[2][2];                  // its rows of T
-    u4 b[2][2];                  // its rows of B
-    f4 beta, seen, left, gamma;  // the factors of its tokens' four rows of a lane
+struct StateOperands {
+    u4 k[K / 32];            // its 16 tokens
+    u4 kt[K / 64][2];        // its rows of the state
+    u4 t[2][3];              // its rows of T, in halves, three parts
+    f4 beta, seen, left;     // the factors of its tokens' four rows of a lane
     float keep;
     uint16_t v[NT][4];
 };
+// .. and one of those that make the outputs.
+template <int K>
+struct OutputOperands {
+    u4 q[K / 32];
+    u4 b[2][2];
+    f4 gamma;
+};
 
-// One workgroup: 16 NT columns of a head's state, through a row's chunks.  Its four wavefronts have a quarter of the chunk's tokens
-// and of the state's rows each, and hand each other operands through LDS: the state, R, D.
+// One workgroup: 16 NT columns of a head's state, through a row's chunks.  Wavefronts 0 to 3 carry the state, a quarter of the chunk's
+// tokens and of the state's rows each, and hand each other operands through LDS: the state, R, D; the chain from one state to the
+// next is what a long row waits for, so that nothing else is on it.  Wavefronts 4 to 7 have a quarter of the tokens each and make the outputs beside it.
 template <int K, int NT>
-__global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void delta_scan_kernel(const Params p, const Work w) {
+__global__ __launch_bounds__(512, 2) void delta_scan_kernel(const Params p, const Work w) {
     constexpr int kSteps = K / 32, kTiles = K / 64;  // of the state's rows: MFMA steps, tiles of a wavefront
     __shared__ u4 sf[kSteps][3][NT][64];             // the state, three parts
     __shared__ u4 rf[2][3][NT][64];                  // R
     __shared__ u4 df[2][2][NT][64];                  // D, two parts
     __shared__ u4 ef[2][3][NT][64];                  // D with the decay to the chunk's end
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, role = __builtin_amdgcn_readfirstlane(tid >> 8),
+              wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
     const int col = lane & 15, quad = lane >> 4;
     // the columns of `together` heads follow each other on one XCD, whose L2 they share
     const uint32_t slices = (uint32_t)(p.V / (16 * NT)), each = slices * (uint32_t)w.together;
@@ -314,6 +325,74 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void delta_scan_kernel(const 
     if (p.cu && len <= p.token_len) return;
     const int chunks = (len + kChunk - 1) / kChunk;
     const int64_t slot = first_slot(p, n, first);
+    const f4 zero = {0.f, 0.f, 0.f, 0.f};
+    const auto record = [&](int chunk) { return wkv7::uniform_ptr(w.rec + ((slot + chunk) * p.Hv + h) * kRecord); };
+    const bool two = wave >= 2;  // these rows of the lower triangles have a second half
+
+    if (role == 1) {
+        const auto fetch = [&](int chunk, OutputOperands<K>& o) {
+            const int most = min(len - chunk * kChunk, kChunk) - 1;
+            const char* const rec = record(chunk);
+            const uint32_t token = (uint32_t)min(token_of(wave, col), most);  // past the last token: it again, not stored
+            const uint16_t* const qp = wkv7::uniform_ptr(p.q + (first + (int64_t)chunk * kChunk) * p.q_stride + hk * K);
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+                o.q[s] = *reinterpret_cast<const u4*>(qp + (token * (uint32_t)p.q_stride + quad * 8) + 32 * s);
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+                    o.b[half][m] = *reinterpret_cast<const u4*>(rec + kRecordB + (block_of(wave, two ? half : 0) * 2 + m) * 1024 + lane * 16u);
+            o.gamma = *reinterpret_cast<const f4*>(rec + kRecordFactors + 768 + token_of(wave, 4 * quad) * 4u);
+        };
+        const auto step = [&](int chunk, const OutputOperands<K>& o) {
+            f4 O[NT][2];
+#pragma unroll
+            for (int x = 0; x < NT; ++x) O[x][0] = O[x][1] = zero;
+            if (p.o)
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) {
+                        O[x][0] = mfma(o.q[s], sf[s][0][x][lane], O[x][0]);
+                        O[x][1] = mfma(o.q[s], sf[s][1][x][lane], O[x][1]);
+                    }
+            lds_barrier();
+            lds_barrier();
+            if (p.o) {
+#pragma unroll
+                for (int x = 0; x < NT; ++x) {
+                    f4 y = (O[x][0] + O[x][1]) * o.gamma;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+                        if (half == 0 || two) {
+                            const u4 a = df[half][0][x][lane], b = df[half][1][x][lane];
+                            y = mfma(o.b[half][1], a, y);
+                            y = mfma(o.b[half][0], b, y);
+                            y = mfma(o.b[half][0], a, y);
+                        }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int t = chunk * kChunk + token_of(wave, 4 * quad + r);
+                        if (t < len) p.o[(first + t) * p.o_stride + (int64_t)h * p.V + col0 + 16 * x + col] = wkv7::f32_to_bf16(y[r]);
+                    }
+                }
+            }
+            lds_barrier();
+        };
+        lds_barrier();
+        OutputOperands<K> even, odd;
+        if (chunks > 0) fetch(0, even);
+        for (int c = 0; c < chunks; c += 2) {
+            fetch(min(c + 1, chunks - 1), odd);
+            step(c, even);
+            if (c + 1 < chunks) {
+                fetch(min(c + 2, chunks - 1), even);
+                step(c + 1, odd);
+            }
+        }
+        return;
+    }
 
     // rows of the state in tile 2b + j, row r of a lane: 32 b + 8 quad + 4 j + r
     const float* const from = initial(p, n, h);
@@ -330,45 +409,38 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void delta_scan_kernel(const 
 #pragma unroll
             for (int r = 0; r < 4; ++r) S[t][x][r] = from ? from[state_at(t, r) + 16 * x] : 0.f;
 
-    const auto fetch = [&](int chunk, Operands<K, NT>& o) {
+    const auto fetch = [&](int chunk, StateOperands<K, NT>& o) {
         const int64_t t0 = first + (int64_t)chunk * kChunk;
         const int most = min(len - chunk * kChunk, kChunk) - 1;
-        const char* const rec = w.rec + ((slot + chunk) * p.Hv + h) * kRecord;
-        const u4* const kt = reinterpret_cast<const u4*>(w.kt + ((slot + chunk) * p.Hk + hk) * (K * kChunk * 2));
+        const char* const rec = record(chunk);
+        const char* const kt = wkv7::uniform_ptr(w.kt + ((slot + chunk) * p.Hk + hk) * (K * kChunk * 2) + wave * (kTiles * 2048));
         const uint32_t token = (uint32_t)min(token_of(wave, col), most);  // past the last token: it again, with a factor of 0
         const uint16_t* const kp = wkv7::uniform_ptr(p.k + t0 * p.k_stride + hk * K);
-        const uint16_t* const qp = wkv7::uniform_ptr(p.q + t0 * p.q_stride + hk * K);
         const uint16_t* const vp = wkv7::uniform_ptr(p.v + t0 * p.v_stride + (int64_t)h * p.V + col0);
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            o.k[s] = *reinterpret_cast<const u4*>(kp + token * (uint32_t)p.k_stride + quad * 8 + 32 * s);
-            o.q[s] = *reinterpret_cast<const u4*>(qp + token * (uint32_t)p.q_stride + quad * 8 + 32 * s);
+        for (int s = 0; s < kSteps; ++s)
+            o.k[s] = *reinterpret_cast<const u4*>(kp + (token * (uint32_t)p.k_stride + quad * 8) + 32 * s);
+        const char* const f = rec + kRecordFactors;
+        const uint32_t at = token_of(wave, 4 * quad) * 4u;
+        o.beta = *reinterpret_cast<const f4*>(f + at);
+        o.seen = *reinterpret_cast<const f4*>(f + 256 + at);
+        o.left = *reinterpret_cast<const f4*>(f + 512 + at);
+        o.keep = *reinterpret_cast<const float*>(f + 1024);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t v_at = (uint32_t)min(token_of(wave, 4 * quad + r), most) * (uint32_t)p.v_stride + col;
+#pragma unroll
+            for (int x = 0; x < NT; ++x) o.v[x][r] = vp[v_at + 16 * x];
         }
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int m = 0; m < 3; ++m)
+                o.t[half][m] = *reinterpret_cast<const u4*>(rec + kRecordT + (block_of(wave, two ? half : 0) * 3 + m) * 1024 + lane * 16u);
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) o.kt[t][half] = kt[((wave * kTiles + t) * 2 + half) * 64 + lane];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int block = block_of(wave, wave < 2 ? 0 : half);
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                o.t[half][m] = *reinterpret_cast<const f4*>(rec + kRecordT + ((block * 2 + m) * 64 + lane) * 16);
-                o.b[half][m] = *reinterpret_cast<const u4*>(rec + kRecordB + ((block * 2 + m) * 64 + lane) * 16);
-            }
-        }
-        const float* const f = reinterpret_cast<const float*>(rec + kRecordFactors) + token_of(wave, 4 * quad);
-        o.beta = *reinterpret_cast<const f4*>(f);
-        o.seen = *reinterpret_cast<const f4*>(f + 64);
-        o.left = *reinterpret_cast<const f4*>(f + 128);
-        o.gamma = *reinterpret_cast<const f4*>(f + 192);
-        o.keep = *reinterpret_cast<const float*>(rec + kRecordFactors + 1024);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t at = (uint32_t)min(token_of(wave, 4 * quad + r), most) * (uint32_t)p.v_stride + col;
-#pragma unroll
-            for (int x = 0; x < NT; ++x) o.v[x][r] = vp[at + 16 * x];
-        }
+            for (int half = 0; half < 2; ++half) o.kt[t][half] = *reinterpret_cast<const u4*>(kt + (t * 2 + half) * 1024 + lane * 16u);
     };
     const auto share_state = [&] {
 #pragma unroll
@@ -388,29 +460,23 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void delta_scan_kernel(const 
                 reinterpret_cast<u2*>(&sf[tile >> 1][2][x][lane])[tile & 1] = c;
             }
     };
-    const f4 zero = {0.f, 0.f, 0.f, 0.f};
-    const auto step = [&](int chunk, const Operands<K, NT>& o) {
-        f4 P[NT], O[NT];
+    const auto step = [&](const StateOperands<K, NT>& o) {
+        f4 P[NT][3];
 #pragma unroll
-        for (int x = 0; x < NT; ++x) P[x] = O[x] = zero;
+        for (int x = 0; x < NT; ++x) P[x][0] = P[x][1] = P[x][2] = zero;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-            for (int x = 0; x < NT; ++x) {
-                const u4 a = sf[s][0][x][lane], b = sf[s][1][x][lane], c = sf[s][2][x][lane];
-                P[x] = mfma(o.k[s], c, P[x]);
-                O[x] = mfma(o.q[s], b, O[x]);
-                P[x] = mfma(o.k[s], b, P[x]);
-                O[x] = mfma(o.q[s], a, O[x]);
-                P[x] = mfma(o.k[s], a, P[x]);
-            }
+            for (int x = 0; x < NT; ++x)
+#pragma unroll
+                for (int m = 0; m < 3; ++m) P[x][m] = mfma(o.k[s], sf[s][m][x][lane], P[x][m]);
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
             f4 R;
             u2 a, b, c;
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                R[r] = fmaf(-o.seen[r], P[x][r], o.beta[r] * wkv7::bf16_to_f32(o.v[x][r]));
+                R[r] = fmaf(-o.seen[r], P[x][0][r] + (P[x][1][r] + P[x][2][r]), o.beta[r] * wkv7::bf16_to_f32(o.v[x][r]));
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 uint32_t i, j, k;
@@ -421,48 +487,40 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void delta_scan_kernel(const 
             reinterpret_cast<u2*>(&rf[wave >> 1][1][x][lane])[wave & 1] = b;
             reinterpret_cast<u2*>(&rf[wave >> 1][2][x][lane])[wave & 1] = c;
         }
-        u4 th[2], tm[2], tl[2];  // T in three parts
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                uint32_t i, j, k;
-                split3(o.t[half][m >> 1][2 * (m & 1)], o.t[half][m >> 1][2 * (m & 1) + 1], i, j, k);
-                th[half][m] = i, tm[half][m] = j, tl[half][m] = k;
-            }
         lds_barrier();
-        f4 D[NT];
+        f4 D[NT][3];
 #pragma unroll
-        for (int x = 0; x < NT; ++x) D[x] = zero;
+        for (int x = 0; x < NT; ++x) D[x][0] = D[x][1] = D[x][2] = zero;
 #pragma unroll
         for (int half = 0; half < 2; ++half)
-            if (half == 0 || wave >= 2)
+            if (half == 0 || two)
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
                     const u4 a = rf[half][0][x][lane], b = rf[half][1][x][lane], c = rf[half][2][x][lane];
-                    D[x] = mfma(tl[half], a, D[x]);
-                    D[x] = mfma(th[half], c, D[x]);
-                    D[x] = mfma(tm[half], b, D[x]);
-                    D[x] = mfma(tm[half], a, D[x]);
-                    D[x] = mfma(th[half], b, D[x]);
-                    D[x] = mfma(th[half], a, D[x]);
+                    D[x][2] = mfma(o.t[half][2], a, D[x][2]);
+                    D[x][1] = mfma(o.t[half][1], a, D[x][1]);
+                    D[x][0] = mfma(o.t[half][0], a, D[x][0]);
+                    D[x][2] = mfma(o.t[half][0], c, D[x][2]);
+                    D[x][1] = mfma(o.t[half][0], b, D[x][1]);
+                    D[x][2] = mfma(o.t[half][1], b, D[x][2]);
                 }
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
-            u2 a, b, c, d, e;
+            const f4 d = D[x][0] + (D[x][1] + D[x][2]);
+            u2 a, b, c, g, e;
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 uint32_t i, j, k;
-                wkv7::split_pair(D[x][2 * m], D[x][2 * m + 1], i, j);
+                split3(d[2 * m] * o.left[2 * m], d[2 * m + 1] * o.left[2 * m + 1], i, j, k);
+                c[m] = i, g[m] = j, e[m] = k;
+                wkv7::split_pair(d[2 * m], d[2 * m + 1], i, j);
                 a[m] = i, b[m] = j;
-                split3(D[x][2 * m] * o.left[2 * m], D[x][2 * m + 1] * o.left[2 * m + 1], i, j, k);
-                c[m] = i, d[m] = j, e[m] = k;
             }
+            reinterpret_cast<u2*>(&ef[wave >> 1][0][x][lane])[wave & 1] = c;
+            reinterpret_cast<u2*>(&ef[wave >> 1][1][x][lane])[wave & 1] = g;
+            reinterpret_cast<u2*>(&ef[wave >> 1][2][x][lane])[wave & 1] = e;
             reinterpret_cast<u2*>(&df[wave >> 1][0][x][lane])[wave & 1] = a;
             reinterpret_cast<u2*>(&df[wave >> 1][1][x][lane])[wave & 1] = b;
-            reinterpret_cast<u2*>(&ef[wave >> 1][0][x][lane])[wave & 1] = c;
-            reinterpret_cast<u2*>(&ef[wave >> 1][1][x][lane])[wave & 1] = d;
-            reinterpret_cast<u2*>(&ef[wave >> 1][2][x][lane])[wave & 1] = e;
         }
         lds_barrier();
 #pragma unroll
@@ -480,40 +538,18 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void delta_scan_kernel(const 
                     for (int t = 0; t < kTiles; ++t) S[t][x] = mfma(o.kt[t][half], e, S[t][x]);
                 }
         share_state();
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) O[x][r] *= o.gamma[r];
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-                if (half == 0 || wave >= 2) {
-                    const u4 a = df[half][0][x][lane], b = df[half][1][x][lane];
-                    O[x] = mfma(o.b[half][1], a, O[x]);
-                    O[x] = mfma(o.b[half][0], b, O[x]);
-                    O[x] = mfma(o.b[half][0], a, O[x]);
-                }
-        }
-        if (p.o)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = chunk * kChunk + token_of(wave, 4 * quad + r);
-                if (t < len)
-#pragma unroll
-                    for (int x = 0; x < NT; ++x)
-                        p.o[(first + t) * p.o_stride + (int64_t)h * p.V + col0 + 16 * x + col] = wkv7::f32_to_bf16(O[x][r]);
-            }
         lds_barrier();
     };
     share_state();
-    lds_barrier();
-    Operands<K, NT> even, odd;
+    StateOperands<K, NT> even, odd;
     if (chunks > 0) fetch(0, even);
+    lds_barrier();
     for (int c = 0; c < chunks; c += 2) {
         fetch(min(c + 1, chunks - 1), odd);
-        step(c, even);
+        step(even);
         if (c + 1 < chunks) {
             fetch(min(c + 2, chunks - 1), even);
-            step(c + 1, odd);
+            step(odd);
         }
     }
     if (to)
@@ -532,9 +568,9 @@ hipError_t launch(const Params& p, const Work& w, int64_t slots, bool wide, hipS
     if (e != hipSuccess) return e;
     const int64_t groups = ((int64_t)p.num_seqs * p.Hv / w.together + 7) / 8 * 8;
     if (wide)
-        hipLaunchKernelGGL((delta_scan_kernel<K, 2>), dim3((unsigned)(groups * w.together * (p.V / 32))), dim3(256), 0, stream, p, w);
+        hipLaunchKernelGGL((delta_scan_kernel<K, 2>), dim3((unsigned)(groups * w.together * (p.V / 32))), dim3(512), 0, stream, p, w);
     else
-        hipLaunchKernelGGL((delta_scan_kernel<K, 1>), dim3((unsigned)(groups * w.together * (p.V / 16))), dim3(256), 0, stream, p, w);
+        hipLaunchKernelGGL((delta_scan_kernel<K, 1>), dim3((unsigned)(groups * w.together * (p.V / 16))), dim3(512), 0, stream, p, w);
     return hipGetLastError();
 }
 

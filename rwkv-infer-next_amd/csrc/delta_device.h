@@ -76,9 +76,9 @@ __device__ __forceinline__ float bf16_at(u4 x, int i) {  // element i of eight
 }
 
 // The workspace of the chunks' kernels.  For each slot (a chunk's place) and query/key head K^T in operand order, and for each slot and
-// value head a record: T (fp32) and B (two bf16 parts) of the lower triangle's blocks, six each, and the tokens' factors.
+// value head a record: T (three bf16 parts) and B (two) of the lower triangle's blocks, six each, and the tokens' factors.
 constexpr int kChunk = 64;
-constexpr int64_t kRecordT = 0, kRecordB = 6 * 2048, kRecordFactors = 12 * 2048, kRecord = 12 * 2048 + 1280;
+constexpr int64_t kRecordT = 0, kRecordB = 18 * 1024, kRecordFactors = 30 * 1024, kRecord = 30 * 1024 + 1280;
 struct Work {
     char *kt, *rec;
     int32_t together;  // heads whose workgroups follow each other on one XCD
