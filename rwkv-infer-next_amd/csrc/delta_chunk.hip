@@ -73,16 +73,16 @@ __device__ __forceinline__ void split3(float x0, float x1, uint32_t& a, uint32_t
 
 // One workgroup: a chunk of a query/key head, then each of the value heads that share it.
 template <int K>
-__global__ __launch_bounds__(256) void delta_prep_kernel(const Params p, const Work w) {
+__global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, const Work w) {
     constexpr int kSteps = K / 32, kPitch = K + 8;
-    __shared__ __attribute__((aligned(16))) float am[64 * kRow];   // A, then T
-    __shared__ __attribute__((aligned(16))) float bm[64 * kRow];   // K's tile, then B
+    __shared__ __attribute__((aligned(16))) float am[64 * kRow];   // K's tile, then A, then T
+    __shared__ __attribute__((aligned(16))) float bm[64 * kRow];   // Q's tile, then B
     __shared__ __attribute__((aligned(16))) float mm[32 * kRow];
     __shared__ double cs[64];
     __shared__ float rk[64], rq[64], be[64];
     static_assert(64 * kPitch * 2 <= (int)sizeof(bm), "");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int row = lane & 15, quad = lane >> 4;
+    int row = lane & 15, quad = lane >> 4;
     const int64_t slot = blockIdx.x / (uint32_t)p.Hk;
     const int hk = (int)(blockIdx.x % (uint32_t)p.Hk);
     int n, len, chunk;
@@ -91,70 +91,96 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const Params p, const W
     first += (int64_t)chunk * kChunk;
     len = min(len - chunk * kChunk, kChunk);  // tokens of this chunk
 
-    const auto rows = [&](const uint16_t* x, int64_t stride, int block, u4* f) {
-        const int t = 16 * block + row;
-        const uint16_t* const at = x + (first + min(t, len - 1)) * stride + hk * K + quad * 8;
+    // K and Q by whole rows into LDS, zeros past the last token, and from there in operand order
+    constexpr int kRowPieces = K / 8, kPieces = 64 * kRowPieces / 256;
+    uint16_t* const k_tile = reinterpret_cast<uint16_t*>(am);
+    uint16_t* const q_tile = reinterpret_cast<uint16_t*>(bm);
+    {
+        u4 x[kPieces], y[kPieces];
+        const int at = tid / kRowPieces, piece = tid % kRowPieces * 8;
+        const uint16_t* const kp = p.k + first * p.k_stride + hk * K + piece;
+        const uint16_t* const qp = p.q + first * p.q_stride + hk * K + piece;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            f[s] = *reinterpret_cast<const u4*>(at + 32 * s);
-            if (t >= len) f[s] = u4{0, 0, 0, 0};
+        for (int i = 0; i < kPieces; ++i) {
+            const int t = at + i * (256 / kRowPieces), from = min(t, len - 1);
+            x[i] = *reinterpret_cast<const u4*>(kp + from * p.k_stride);
+            y[i] = *reinterpret_cast<const u4*>(qp + from * p.q_stride);
+            if (t >= len) x[i] = y[i] = u4{0, 0, 0, 0};
         }
-    };
-    u4 kf[kSteps], qf[kSteps];
-    rows(p.k, p.k_stride, wave, kf);
-    rows(p.q, p.q_stride, wave, qf);
-    f4 kk[4], qk[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        kk[j] = qk[j] = f4{0.f, 0.f, 0.f, 0.f};
-        if (j <= wave) {
-            u4 of[kSteps];
-            rows(p.k, p.k_stride, j, of);
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                kk[j] = mfma(kf[s], of[s], kk[j]);
-                qk[j] = mfma(qf[s], of[s], qk[j]);
-            }
+        for (int i = 0; i < kPieces; ++i) {
+            const int t = at + i * (256 / kRowPieces);
+            *reinterpret_cast<u4*>(k_tile + t * kPitch + piece) = x[i];
+            *reinterpret_cast<u4*>(q_tile + t * kPitch + piece) = y[i];
         }
-    }
-    float nk = 0.f, nq = 0.f;
-    uint16_t* const tile = reinterpret_cast<uint16_t*>(bm);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float x = bf16_at(kf[s], i), y = bf16_at(qf[s], i);
-            nk = fmaf(x, x, nk);
-            nq = fmaf(y, y, nq);
-        }
-        *reinterpret_cast<u4*>(tile + (16 * wave + row) * kPitch + 32 * s + 8 * quad) = kf[s];
-    }
-    nk += __shfl_xor(nk, 16), nq += __shfl_xor(nq, 16);
-    nk += __shfl_xor(nk, 32), nq += __shfl_xor(nq, 32);
-    if (quad == 0) {
-        rk[16 * wave + row] = p.qk_norm ? 1.f / sqrtf(nk + kNormEps) : 1.f;
-        rq[16 * wave + row] = p.qk_norm ? p.scale / sqrtf(nq + kNormEps) : p.scale;
     }
     __syncthreads();
+    const auto rows = [&](const uint16_t* x, int block, u4* f) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) f[s] = *reinterpret_cast<const u4*>(x + (16 * block + row) * kPitch + 32 * s + 8 * quad);
+    };
+    f4 kk[4], qk[4];
+    char* const operands = w.kq + (slot * p.Hk + hk) * (3 * K * kChunk * 2);
+    {
+        u4 kf[kSteps], qf[kSteps];
+        rows(k_tile, wave, kf);
+        rows(q_tile, wave, qf);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            kk[j] = qk[j] = f4{0.f, 0.f, 0.f, 0.f};
+            if (j <= wave) {
+                u4 of[kSteps];
+                rows(k_tile, j, of);
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) {
+                    kk[j] = mfma(kf[s], of[s], kk[j]);
+                    qk[j] = mfma(qf[s], of[s], qk[j]);
+                }
+            }
+        }
+        float nk = 0.f, nq = 0.f;
+        const int t = 16 * wave + row, tile = 2 * (t >> 5) + (t >> 2 & 1), to = 16 * quad + 4 * (t >> 3 & 3) + (t & 3);  // token_of(tile, to) = t
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = bf16_at(kf[s], i), y = bf16_at(qf[s], i);
+                nk = fmaf(x, x, nk);
+                nq = fmaf(y, y, nq);
+            }
+            *reinterpret_cast<u4*>(operands + ((tile * kSteps + s) * 64 + to) * 16) = kf[s];
+            *reinterpret_cast<u4*>(operands + K * kChunk * 2 + ((tile * kSteps + s) * 64 + to) * 16) = qf[s];
+        }
+        nk += __shfl_xor(nk, 16), nq += __shfl_xor(nq, 16);
+        nk += __shfl_xor(nk, 32), nq += __shfl_xor(nq, 32);
+        if (quad == 0) {
+            rk[16 * wave + row] = p.qk_norm ? 1.f / sqrtf(nk + kNormEps) : 1.f;
+            rq[16 * wave + row] = p.qk_norm ? p.scale / sqrtf(nq + kNormEps) : p.scale;
+        }
+    }
     // K^T in operand order: tile of 16 rows of the state, half of the tokens, lane
-    u4* const kt = reinterpret_cast<u4*>(w.kt + (slot * p.Hk + hk) * (K * kChunk * 2));
+    u4* const kt = reinterpret_cast<u4*>(operands + 2 * K * kChunk * 2);
     for (int e = tid; e < K / 16 * 2 * 64; e += 256) {
         const int l = e & 63, half = (e >> 6) & 1, t = e >> 7, d = token_of(t, l & 15);
         u4 x;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint16_t* const at = tile + (32 * half + 8 * (l >> 4) + 2 * j) * kPitch + d;
+            const uint16_t* const at = k_tile + (32 * half + 8 * (l >> 4) + 2 * j) * kPitch + d;
             x[j] = (uint32_t)at[0] | (uint32_t)at[kPitch] << 16;
         }
         kt[e] = x;
     }
 
+#pragma unroll 1
     for (int h = hk * p.share; h < (hk + 1) * p.share; ++h) {
+        // (without this the addresses of a head's work are kept from head to head, in more registers than there are)
+        asm("" : "+v"(row), "+v"(quad));
         char* const rec = w.rec + (slot * p.Hv + h) * kRecord;
-        // the sums of g, in 64 bits: differences of far tokens' sums lose nothing
+        // The sums of g log2(e), in 64 bits: differences of far tokens' sums lose nothing, and the hardware's exp2, good to one unit in
+        // the last place, takes them as they are.
         const int64_t token = first + min(lane, len - 1);
         const float g = p.g[token * p.g_stride + h], b = p.beta[token * p.beta_stride + h];
-        double c = lane < len ? (double)(g < kLeast ? kLeast : g) : 0.0;
+        double c = lane < len ? (double)(g < kLeast ? kLeast : g) * 1.4426950408889634 : 0.0;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
             const double other = __shfl_up(c, d);
@@ -162,17 +188,17 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const Params p, const W
         }
         const double last = __shfl(c, 63);
         const float beta = lane < len ? b : 0.f;
-        __syncthreads();  // K's tile is read; the head before is written
+        __syncthreads();  // the tiles are read; the head before is written
         if (wave == 0) {
             cs[lane] = c;
             be[lane] = beta;
             float* const f = reinterpret_cast<float*>(rec + kRecordFactors);
-            const float gamma = expf((float)c);
+            const float gamma = __builtin_amdgcn_exp2f((float)c);
             f[lane] = beta;
             f[64 + lane] = beta * gamma * rk[lane];
-            f[128 + lane] = expf((float)(last - c)) * rk[lane];
+            f[128 + lane] = __builtin_amdgcn_exp2f((float)(last - c)) * rk[lane];
             f[192 + lane] = gamma * rq[lane];
-            if (lane == 0) f[256] = expf((float)last);
+            if (lane == 0) f[256] = __builtin_amdgcn_exp2f((float)last);
         }
         __syncthreads();
 #pragma unroll
@@ -182,7 +208,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const Params p, const W
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int i = 16 * wave + 4 * quad + r;
-                    const float decay = i >= col ? expf((float)(cs[i] - cs[col])) * rk[col] : 0.f;
+                    const float decay = i >= col ? __builtin_amdgcn_exp2f((float)(cs[i] - cs[col])) * rk[col] : 0.f;
                     am[i * kRow + col] = i > col ? kk[j][r] * (be[i] * rk[i]) * decay : 0.f;
                     bm[i * kRow + col] = qk[j][r] * rq[i] * decay;
                 }
@@ -203,6 +229,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const Params p, const W
                         if (4 * m + r < i) (r & 1 ? s1 : s0) = fmaf(-y[r], x[4 * m + r], r & 1 ? s1 : s0);
                 }
                 x[i] = s0 + s1;
+                if (i == 7 || i == 11) __builtin_amdgcn_sched_barrier(0);  // a few rows of A at a time: all of them are 144 registers
             }
             wkv7::wave_lds_sync();
 #pragma unroll
@@ -327,17 +354,16 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(const Params p, cons
     const int64_t slot = first_slot(p, n, first);
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
     const auto record = [&](int chunk) { return wkv7::uniform_ptr(w.rec + ((slot + chunk) * p.Hv + h) * kRecord); };
+    const auto heads = [&](int chunk) { return wkv7::uniform_ptr(w.kq + ((slot + chunk) * p.Hk + hk) * (3 * K * kChunk * 2)); };
     const bool two = wave >= 2;  // these rows of the lower triangles have a second half
 
     if (role == 1) {
         const auto fetch = [&](int chunk, OutputOperands<K>& o) {
-            const int most = min(len - chunk * kChunk, kChunk) - 1;
             const char* const rec = record(chunk);
-            const uint32_t token = (uint32_t)min(token_of(wave, col), most);  // past the last token: it again, not stored
-            const uint16_t* const qp = wkv7::uniform_ptr(p.q + (first + (int64_t)chunk * kChunk) * p.q_stride + hk * K);
+            const char* const q = heads(chunk) + (4 + wave) * (kSteps * 1024);
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)
-                o.q[s] = *reinterpret_cast<const u4*>(qp + (token * (uint32_t)p.q_stride + quad * 8) + 32 * s);
+                o.q[s] = *reinterpret_cast<const u4*>(q + s * 1024 + lane * 16u);
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -413,13 +439,11 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(const Params p, cons
         const int64_t t0 = first + (int64_t)chunk * kChunk;
         const int most = min(len - chunk * kChunk, kChunk) - 1;
         const char* const rec = record(chunk);
-        const char* const kt = wkv7::uniform_ptr(w.kt + ((slot + chunk) * p.Hk + hk) * (K * kChunk * 2) + wave * (kTiles * 2048));
-        const uint32_t token = (uint32_t)min(token_of(wave, col), most);  // past the last token: it again, with a factor of 0
-        const uint16_t* const kp = wkv7::uniform_ptr(p.k + t0 * p.k_stride + hk * K);
+        const char *const k = heads(chunk) + wave * (kSteps * 1024), *const kt = heads(chunk) + (8 * kSteps + 2 * kTiles * wave) * 1024;
         const uint16_t* const vp = wkv7::uniform_ptr(p.v + t0 * p.v_stride + (int64_t)h * p.V + col0);
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
-            o.k[s] = *reinterpret_cast<const u4*>(kp + (token * (uint32_t)p.k_stride + quad * 8) + 32 * s);
+            o.k[s] = *reinterpret_cast<const u4*>(k + s * 1024 + lane * 16u);
         const char* const f = rec + kRecordFactors;
         const uint32_t at = token_of(wave, 4 * quad) * 4u;
         o.beta = *reinterpret_cast<const f4*>(f + at);
@@ -581,14 +605,14 @@ int64_t chunk_slots(int32_t num_seqs, int32_t T, int64_t total_tokens, bool ragg
 }
 int64_t chunk_groups(int32_t num_seqs, int32_t Hv, int32_t V) { return ((int64_t)num_seqs + 7) / 8 * 8 * Hv * (V / 16); }
 size_t chunk_workspace(int64_t slots, int32_t Hk, int32_t Hv, int32_t K) {
-    return (size_t)slots * (Hk * (size_t)(K * kChunk * 2) + Hv * (size_t)kRecord);
+    return (size_t)slots * (Hk * (size_t)(3 * K * kChunk * 2) + Hv * (size_t)kRecord);
 }
 
 hipError_t launch_chunks(const Params& p, int cus, hipStream_t stream) {
     const int64_t slots = chunk_slots(p.num_seqs, p.T, p.total_tokens, p.cu != nullptr);
     Work w;
-    w.kt = p.workspace;
-    w.rec = p.workspace + slots * p.Hk * (int64_t)(p.K * kChunk * 2);
+    w.kq = p.workspace;
+    w.rec = p.workspace + slots * p.Hk * (int64_t)(3 * p.K * kChunk * 2);
     w.together = (int64_t)p.num_seqs * p.Hk >= 8 ? p.share : 1;
     const bool wide = p.V % 32 == 0 && (int64_t)p.num_seqs * p.Hv * (p.V / 32) >= 2 * cus;
     return p.K == 64 ? launch<64>(p, w, slots, wide, stream) : launch<128>(p, w, slots, wide, stream);

@@ -75,12 +75,12 @@ __device__ __forceinline__ float bf16_at(u4 x, int i) {  // element i of eight
     return __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16);
 }
 
-// The workspace of the chunks' kernels.  For each slot (a chunk's place) and query/key head K^T in operand order, and for each slot and
+// The workspace of the chunks' kernels.  For each slot (a chunk's place) and query/key head K, Q and K^T in operand order, and for each slot and
 // value head a record: T (three bf16 parts) and B (two) of the lower triangle's blocks, six each, and the tokens' factors.
 constexpr int kChunk = 64;
 constexpr int64_t kRecordT = 0, kRecordB = 18 * 1024, kRecordFactors = 30 * 1024, kRecord = 30 * 1024 + 1280;
 struct Work {
-    char *kt, *rec;
+    char *kq, *rec;
     int32_t together;  // heads whose workgroups follow each other on one XCD
 };
 int64_t chunk_slots(int32_t num_seqs, int32_t T, int64_t total_tokens, bool ragged);
