@@ -309,31 +309,17 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, cons
     }
 }
 
-// What a wavefront reads of a chunk: one of those that carry the state ..
-template <int K, int NT>
-struct StateOperands {
-    u4 k[K / 32];            // its 16 tokens
-    u4 kt[K / 64][2];        // its rows of the state
-    u4 t[2][3];              // its rows of T, in halves, three parts
-    f4 beta, seen, left;     // the factors of its tokens' four rows of a lane
-    float keep;
-    uint16_t v[NT][4];
-};
-// .. and one of those that make the outputs.
-template <int K>
-struct OutputOperands {
-    u4 q[K / 32];
-    u4 b[2][2];
-    f4 gamma;
-};
-
-// One workgroup: 16 NT columns of a head's state, through a row's chunks.  Wavefronts 0 to 3 carry the state, a quarter of the chunk's
-// tokens and of the state's rows each, and hand each other operands through LDS: the state, R, D; the chain from one state to the
-// next is what a long row waits for, so that nothing else is on it.  Wavefronts 4 to 7 have a quarter of the tokens each and make the outputs beside it.
+// One workgroup: 16 NT columns of a head's state, through a row's chunks.  Wavefronts 0 to 3 carry the state, a quarter of its rows
+// each; the chain from one state to the next is what a long row waits for, so that nothing else is on it:
+//     its rows' share of S^T k for all tokens, from registers | summed over the wavefronts, R, for its tokens | D for them | S
+// with barriers between.  Wavefronts 4 to 7 have a quarter of the tokens each and make the outputs beside it.  Operands of the next
+// chunk are asked for as soon as those of this one are used, so the loads, 78 KiB a chunk, are spread over it: asked for together, at
+// its begin, they held the chain up for a third of its time.
 template <int K, int NT>
 __global__ __launch_bounds__(512, 2) void delta_scan_kernel(const Params p, const Work w) {
     constexpr int kSteps = K / 32, kTiles = K / 64;  // of the state's rows: MFMA steps, tiles of a wavefront
-    __shared__ u4 sf[kSteps][3][NT][64];             // the state, three parts
+    __shared__ f4 pf[4][4][NT][64];                  // S^T k: [wavefront][tile of tokens]
+    __shared__ u4 sf[kSteps][2][NT][64];             // the state, two parts
     __shared__ u4 rf[2][3][NT][64];                  // R
     __shared__ u4 df[2][2][NT][64];                  // D, two parts
     __shared__ u4 ef[2][3][NT][64];                  // D with the decay to the chunk's end
@@ -353,73 +339,81 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(const Params p, cons
     const int chunks = (len + kChunk - 1) / kChunk;
     const int64_t slot = first_slot(p, n, first);
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
-    const auto record = [&](int chunk) { return wkv7::uniform_ptr(w.rec + ((slot + chunk) * p.Hv + h) * kRecord); };
-    const auto heads = [&](int chunk) { return wkv7::uniform_ptr(w.kq + ((slot + chunk) * p.Hk + hk) * (3 * K * kChunk * 2)); };
+    const char* const records = wkv7::uniform_ptr(w.rec + (slot * p.Hv + h) * kRecord);
+    const char* const operands = wkv7::uniform_ptr(w.kq + (slot * p.Hk + hk) * (3 * K * kChunk * 2));
+    const int64_t record_size = p.Hv * kRecord, operand_size = (int64_t)p.Hk * (3 * K * kChunk * 2);
     const bool two = wave >= 2;  // these rows of the lower triangles have a second half
+    const uint32_t at = lane * 16u, tokens_at = token_of(wave, 4 * quad) * 4u;
 
     if (role == 1) {
-        const auto fetch = [&](int chunk, OutputOperands<K>& o) {
-            const char* const rec = record(chunk);
-            const char* const q = heads(chunk) + (4 + wave) * (kSteps * 1024);
+        u4 q[kSteps], b[2][2];
+        f4 gamma;
+        const char *x = operands + (4 + wave) * (kSteps * 1024), *rec = records;
+        const auto fetch_q = [&] {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s)
-                o.q[s] = *reinterpret_cast<const u4*>(q + s * 1024 + lane * 16u);
+            for (int s = 0; s < kSteps; ++s) q[s] = *reinterpret_cast<const u4*>(x + s * 1024 + at);
+        };
+        const auto fetch_b = [&] {
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
-                    o.b[half][m] = *reinterpret_cast<const u4*>(rec + kRecordB + (block_of(wave, two ? half : 0) * 2 + m) * 1024 + lane * 16u);
-            o.gamma = *reinterpret_cast<const f4*>(rec + kRecordFactors + 768 + token_of(wave, 4 * quad) * 4u);
+                    b[half][m] = *reinterpret_cast<const u4*>(rec + kRecordB + (block_of(wave, two ? half : 0) * 2 + m) * 1024 + at);
+            gamma = *reinterpret_cast<const f4*>(rec + kRecordFactors + 768 + tokens_at);
         };
-        const auto step = [&](int chunk, const OutputOperands<K>& o) {
+        if (chunks > 0 && p.o) {
+            fetch_q();
+            fetch_b();
+        }
+        for (int c = 0; c < chunks; ++c) {
+            x += c + 1 < chunks ? operand_size : 0;  // behind the last chunk: it again
+            rec += c + 1 < chunks ? record_size : 0;
+            lds_barrier();
             f4 O[NT][2];
+            if (p.o) {
 #pragma unroll
-            for (int x = 0; x < NT; ++x) O[x][0] = O[x][1] = zero;
-            if (p.o)
+                for (int x = 0; x < NT; ++x) O[x][0] = O[x][1] = zero;
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s)
+                for (int x = 0; x < NT; ++x) {
+                    u4 a[kSteps][2];
 #pragma unroll
-                    for (int x = 0; x < NT; ++x) {
-                        O[x][0] = mfma(o.q[s], sf[s][0][x][lane], O[x][0]);
-                        O[x][1] = mfma(o.q[s], sf[s][1][x][lane], O[x][1]);
+                    for (int s = 0; s < kSteps; ++s) a[s][0] = sf[s][0][x][lane], a[s][1] = sf[s][1][x][lane];
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int s = 0; s < kSteps; ++s) {
+                        O[x][0] = mfma(q[s], a[s][0], O[x][0]);
+                        O[x][1] = mfma(q[s], a[s][1], O[x][1]);
                     }
+                }
+                fetch_q();
+            }
             lds_barrier();
             lds_barrier();
             if (p.o) {
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
-                    f4 y = (O[x][0] + O[x][1]) * o.gamma;
+                    f4 y = (O[x][0] + O[x][1]) * gamma;
 #pragma unroll
                     for (int half = 0; half < 2; ++half)
                         if (half == 0 || two) {
-                            const u4 a = df[half][0][x][lane], b = df[half][1][x][lane];
-                            y = mfma(o.b[half][1], a, y);
-                            y = mfma(o.b[half][0], b, y);
-                            y = mfma(o.b[half][0], a, y);
+                            const u4 d = df[half][0][x][lane], e = df[half][1][x][lane];
+                            y = mfma(b[half][1], d, y);
+                            y = mfma(b[half][0], e, y);
+                            y = mfma(b[half][0], d, y);
                         }
+                    const int t0 = c * kChunk + token_of(wave, 4 * quad);
+                    uint16_t* const to = p.o + (first + t0) * p.o_stride + ((int64_t)h * p.V + col0 + 16 * x + col);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int t = chunk * kChunk + token_of(wave, 4 * quad + r);
-                        if (t < len) p.o[(first + t) * p.o_stride + (int64_t)h * p.V + col0 + 16 * x + col] = wkv7::f32_to_bf16(y[r]);
-                    }
+                    for (int r = 0; r < 4; ++r)
+                        if (t0 + r < len) to[r * p.o_stride] = wkv7::f32_to_bf16(y[r]);
                 }
-            }
-            lds_barrier();
-        };
-        lds_barrier();
-        OutputOperands<K> even, odd;
-        if (chunks > 0) fetch(0, even);
-        for (int c = 0; c < chunks; c += 2) {
-            fetch(min(c + 1, chunks - 1), odd);
-            step(c, even);
-            if (c + 1 < chunks) {
-                fetch(min(c + 2, chunks - 1), even);
-                step(c + 1, odd);
+                fetch_b();
             }
         }
         return;
     }
 
+    __builtin_amdgcn_s_setprio(2);  // the chain goes first where both have something to issue
     // rows of the state in tile 2b + j, row r of a lane: 32 b + 8 quad + 4 j + r
     const float* const from = initial(p, n, h);
     float* const to = final_state(p, n, h);
@@ -435,146 +429,186 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(const Params p, cons
 #pragma unroll
             for (int r = 0; r < 4; ++r) S[t][x][r] = from ? from[state_at(t, r) + 16 * x] : 0.f;
 
-    const auto fetch = [&](int chunk, StateOperands<K, NT>& o) {
-        const int64_t t0 = first + (int64_t)chunk * kChunk;
-        const int most = min(len - chunk * kChunk, kChunk) - 1;
-        const char* const rec = record(chunk);
-        const char *const k = heads(chunk) + wave * (kSteps * 1024), *const kt = heads(chunk) + (8 * kSteps + 2 * kTiles * wave) * 1024;
-        const uint16_t* const vp = wkv7::uniform_ptr(p.v + t0 * p.v_stride + (int64_t)h * p.V + col0);
+    constexpr bool kHalf = kTiles == 1;  // its rows are half an MFMA step: the other half is zeros
+    const int my_step = kHalf ? wave >> 1 : wave;
+    u4 k[4], tri[2][3], kt[kTiles][2];
+    f4 beta, seen, left;
+    float keep;
+    uint16_t v[NT][4];
+    const char *head = operands, *rec = records;
+    const uint16_t* vp = wkv7::uniform_ptr(p.v + first * p.v_stride + (int64_t)h * p.V + col0);
+    uint32_t v_at[4];
+    const auto tokens_of_v = [&](int most) {  // past the last token: it again, with factors of 0
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-            o.k[s] = *reinterpret_cast<const u4*>(k + s * 1024 + lane * 16u);
-        const char* const f = rec + kRecordFactors;
-        const uint32_t at = token_of(wave, 4 * quad) * 4u;
-        o.beta = *reinterpret_cast<const f4*>(f + at);
-        o.seen = *reinterpret_cast<const f4*>(f + 256 + at);
-        o.left = *reinterpret_cast<const f4*>(f + 512 + at);
-        o.keep = *reinterpret_cast<const float*>(f + 1024);
+        for (int r = 0; r < 4; ++r) v_at[r] = (uint32_t)min(token_of(wave, 4 * quad + r), most) * (uint32_t)p.v_stride + col;
+    };
+    const auto fetch_k = [&] {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t v_at = (uint32_t)min(token_of(wave, 4 * quad + r), most) * (uint32_t)p.v_stride + col;
+        for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const u4*>(head + (my_step + i * kSteps) * 1024 + at);
+    };
+    const auto fetch_v = [&] {
+        beta = *reinterpret_cast<const f4*>(rec + kRecordFactors + tokens_at);
+        seen = *reinterpret_cast<const f4*>(rec + kRecordFactors + 256 + tokens_at);
 #pragma unroll
-            for (int x = 0; x < NT; ++x) o.v[x][r] = vp[v_at + 16 * x];
-        }
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int x = 0; x < NT; ++x) v[x][r] = vp[v_at[r] + 16 * x];
+    };
+    const auto fetch_t = [&] {
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
             for (int m = 0; m < 3; ++m)
-                o.t[half][m] = *reinterpret_cast<const u4*>(rec + kRecordT + (block_of(wave, two ? half : 0) * 3 + m) * 1024 + lane * 16u);
+                tri[half][m] = *reinterpret_cast<const u4*>(rec + kRecordT + (block_of(wave, two ? half : 0) * 3 + m) * 1024 + at);
+        left = *reinterpret_cast<const f4*>(rec + kRecordFactors + 512 + tokens_at);
+    };
+    const auto fetch_kt = [&] {
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) o.kt[t][half] = *reinterpret_cast<const u4*>(kt + (t * 2 + half) * 1024 + lane * 16u);
+            for (int half = 0; half < 2; ++half)
+                kt[t][half] = *reinterpret_cast<const u4*>(head + (8 * kSteps + 2 * kTiles * wave + t * 2 + half) * 1024 + at);
+        keep = *reinterpret_cast<const float*>(rec + kRecordFactors + 1024);
     };
-    const auto share_state = [&] {
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-            for (int x = 0; x < NT; ++x) {
-                const int tile = wave * kTiles + t;
-                u2 a, b, c;
-#pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    uint32_t i, j, k;
-                    split3(S[t][x][2 * m], S[t][x][2 * m + 1], i, j, k);
-                    a[m] = i, b[m] = j, c[m] = k;
-                }
-                reinterpret_cast<u2*>(&sf[tile >> 1][0][x][lane])[tile & 1] = a;
-                reinterpret_cast<u2*>(&sf[tile >> 1][1][x][lane])[tile & 1] = b;
-                reinterpret_cast<u2*>(&sf[tile >> 1][2][x][lane])[tile & 1] = c;
-            }
-    };
-    const auto step = [&](const StateOperands<K, NT>& o) {
-        f4 P[NT][3];
-#pragma unroll
-        for (int x = 0; x < NT; ++x) P[x][0] = P[x][1] = P[x][2] = zero;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int x = 0; x < NT; ++x)
-#pragma unroll
-                for (int m = 0; m < 3; ++m) P[x][m] = mfma(o.k[s], sf[s][m][x][lane], P[x][m]);
+    // the state to the other wavefronts (two parts), and this one's share of S^T k (all three)
+    const auto hand_on = [&] {
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
-            f4 R;
-            u2 a, b, c;
+            u4 part[3] = {u4{0, 0, 0, 0}, u4{0, 0, 0, 0}, u4{0, 0, 0, 0}};
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                R[r] = fmaf(-o.seen[r], P[x][0][r] + (P[x][1][r] + P[x][2][r]), o.beta[r] * wkv7::bf16_to_f32(o.v[x][r]));
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    uint32_t i, j, l;
+                    split3(S[t][x][2 * m], S[t][x][2 * m + 1], i, j, l);
+                    part[0][2 * t + m] = i, part[1][2 * t + m] = j, part[2][2 * t + m] = l;
+                }
+            if constexpr (kHalf) {
+#pragma unroll
+                for (int m = 0; m < 2; ++m) reinterpret_cast<u2*>(&sf[my_step][m][x][lane])[wave & 1] = u2{part[m][0], part[m][1]};
+                if (wave & 1)
+#pragma unroll
+                    for (int m = 0; m < 3; ++m) part[m] = u4{0, 0, part[m][0], part[m][1]};
+            } else {
+#pragma unroll
+                for (int m = 0; m < 2; ++m) sf[my_step][m][x][lane] = part[m];
+            }
+            f4 P[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) P[i] = mfma(k[i], part[2], zero);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) P[i] = mfma(k[i], part[1], P[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) P[i] = mfma(k[i], part[0], P[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pf[wave][i][x][lane] = P[i];
+        }
+    };
+    if (chunks > 0) {
+        tokens_of_v(min(len, kChunk) - 1);
+        fetch_k();
+        fetch_v();
+        fetch_t();
+        fetch_kt();
+        hand_on();
+    }
+    for (int c = 0; c < chunks; ++c) {
+        const bool more = c + 1 < chunks;
+        head += more ? operand_size : 0;  // behind the last chunk: it again
+        rec += more ? record_size : 0;
+        vp += more ? kChunk * p.v_stride : 0;
+        if (more && len - (c + 1) * kChunk < kChunk) tokens_of_v(len - (c + 1) * kChunk - 1);
+        lds_barrier();
+        // Operands that were used last before are asked for here and below while the answers of LDS are awaited.
+        f4 share[4][NT];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int x = 0; x < NT; ++x) share[i][x] = pf[i][wave][x][lane];
+        fetch_k();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+            const f4 P = (share[0][x] + share[1][x]) + (share[2][x] + share[3][x]);
+            f4 R;
+            u2 a, b, d;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) R[r] = fmaf(-seen[r], P[r], beta[r] * wkv7::bf16_to_f32(v[x][r]));
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                uint32_t i, j, k;
-                split3(R[2 * m], R[2 * m + 1], i, j, k);
-                a[m] = i, b[m] = j, c[m] = k;
+                uint32_t i, j, l;
+                split3(R[2 * m], R[2 * m + 1], i, j, l);
+                a[m] = i, b[m] = j, d[m] = l;
             }
             reinterpret_cast<u2*>(&rf[wave >> 1][0][x][lane])[wave & 1] = a;
             reinterpret_cast<u2*>(&rf[wave >> 1][1][x][lane])[wave & 1] = b;
-            reinterpret_cast<u2*>(&rf[wave >> 1][2][x][lane])[wave & 1] = c;
+            reinterpret_cast<u2*>(&rf[wave >> 1][2][x][lane])[wave & 1] = d;
         }
         lds_barrier();
         f4 D[NT][3];
 #pragma unroll
         for (int x = 0; x < NT; ++x) D[x][0] = D[x][1] = D[x][2] = zero;
+        u4 y[2][3][NT];
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int m = 0; m < 3; ++m)
+#pragma unroll
+                for (int x = 0; x < NT; ++x) y[half][m][x] = rf[half][m][x][lane];
+        fetch_v();
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int half = 0; half < 2; ++half)
             if (half == 0 || two)
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
-                    const u4 a = rf[half][0][x][lane], b = rf[half][1][x][lane], c = rf[half][2][x][lane];
-                    D[x][2] = mfma(o.t[half][2], a, D[x][2]);
-                    D[x][1] = mfma(o.t[half][1], a, D[x][1]);
-                    D[x][0] = mfma(o.t[half][0], a, D[x][0]);
-                    D[x][2] = mfma(o.t[half][0], c, D[x][2]);
-                    D[x][1] = mfma(o.t[half][0], b, D[x][1]);
-                    D[x][2] = mfma(o.t[half][1], b, D[x][2]);
+                    D[x][2] = mfma(tri[half][2], y[half][0][x], D[x][2]);
+                    D[x][1] = mfma(tri[half][1], y[half][0][x], D[x][1]);
+                    D[x][0] = mfma(tri[half][0], y[half][0][x], D[x][0]);
+                    D[x][2] = mfma(tri[half][0], y[half][2][x], D[x][2]);
+                    D[x][1] = mfma(tri[half][0], y[half][1][x], D[x][1]);
+                    D[x][2] = mfma(tri[half][1], y[half][1][x], D[x][2]);
                 }
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
             const f4 d = D[x][0] + (D[x][1] + D[x][2]);
-            u2 a, b, c, g, e;
+            u2 part[5];
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                uint32_t i, j, k;
-                split3(d[2 * m] * o.left[2 * m], d[2 * m + 1] * o.left[2 * m + 1], i, j, k);
-                c[m] = i, g[m] = j, e[m] = k;
+                uint32_t i, j, l;
+                split3(d[2 * m] * left[2 * m], d[2 * m + 1] * left[2 * m + 1], i, j, l);
+                part[0][m] = i, part[1][m] = j, part[2][m] = l;
                 wkv7::split_pair(d[2 * m], d[2 * m + 1], i, j);
-                a[m] = i, b[m] = j;
+                part[3][m] = i, part[4][m] = j;
             }
-            reinterpret_cast<u2*>(&ef[wave >> 1][0][x][lane])[wave & 1] = c;
-            reinterpret_cast<u2*>(&ef[wave >> 1][1][x][lane])[wave & 1] = g;
-            reinterpret_cast<u2*>(&ef[wave >> 1][2][x][lane])[wave & 1] = e;
-            reinterpret_cast<u2*>(&df[wave >> 1][0][x][lane])[wave & 1] = a;
-            reinterpret_cast<u2*>(&df[wave >> 1][1][x][lane])[wave & 1] = b;
+#pragma unroll
+            for (int m = 0; m < 3; ++m) reinterpret_cast<u2*>(&ef[wave >> 1][m][x][lane])[wave & 1] = part[m];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) reinterpret_cast<u2*>(&df[wave >> 1][m][x][lane])[wave & 1] = part[3 + m];
         }
         lds_barrier();
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-            for (int x = 0; x < NT; ++x) S[t][x] *= o.keep;
 #pragma unroll
         for (int part = 2; part >= 0; --part)
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int x = 0; x < NT; ++x) {
-                    const u4 e = ef[half][part][x][lane];
+                for (int x = 0; x < NT; ++x) y[half][part][x] = ef[half][part][x][lane];
+        fetch_t();
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int t = 0; t < kTiles; ++t) S[t][x] = mfma(o.kt[t][half], e, S[t][x]);
-                }
-        share_state();
-        lds_barrier();
-    };
-    share_state();
-    StateOperands<K, NT> even, odd;
-    if (chunks > 0) fetch(0, even);
-    lds_barrier();
-    for (int c = 0; c < chunks; c += 2) {
-        fetch(min(c + 1, chunks - 1), odd);
-        step(even);
-        if (c + 1 < chunks) {
-            fetch(min(c + 2, chunks - 1), even);
-            step(odd);
-        }
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int x = 0; x < NT; ++x) S[t][x] *= keep;
+#pragma unroll
+        for (int part = 2; part >= 0; --part)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int x = 0; x < NT; ++x)
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) S[t][x] = mfma(kt[t][half], y[half][part][x], S[t][x]);
+        fetch_kt();
+        if (more) hand_on();
     }
     if (to)
 #pragma unroll
