@@ -71,6 +71,41 @@ __device__ __forceinline__ void split3(float x0, float x1, uint32_t& a, uint32_t
     wkv7::split_pair(y[0], y[1], b, c);
 }
 
+// The ragged rows that run by chunks into w.order, longest first (to a chunk, and up to kOrders of them): a scan that begins with its
+// longest rows ends together, and workgroups without a row come last, where they hold nothing up.  Which of two rows as long comes
+// first is left to chance; results do not depend on it.
+constexpr int kOrders = 256;
+__device__ void order_rows(const Params& p, const Work& w, int32_t* count) {
+    const int tid = threadIdx.x;
+    const auto place = [&](int n) {  // -1: runs by tokens
+        int64_t first;
+        int len;
+        extent(p, n, first, len);
+        return len <= p.token_len ? -1 : kOrders - 1 - min(kOrders - 1, len / kChunk);
+    };
+    for (int i = tid; i < kOrders; i += 256) count[i] = 0;
+    __syncthreads();
+    for (int n = tid; n < p.num_seqs; n += 256) {
+        const int at = place(n);
+        if (at >= 0) atomicAdd(&count[at], 1);
+    }
+    __syncthreads();
+    if (tid == 0) {
+        int sum = 0;
+        for (int i = 0; i < kOrders; ++i) {
+            const int c = count[i];
+            count[i] = sum;
+            sum += c;
+        }
+        w.order[0] = sum;
+    }
+    __syncthreads();
+    for (int n = tid; n < p.num_seqs; n += 256) {
+        const int at = place(n);
+        if (at >= 0) w.order[1 + atomicAdd(&count[at], 1)] = n;
+    }
+}
+
 // One workgroup: a chunk of a query/key head, then each of the value heads that share it.
 template <int K>
 __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, const Work w) {
@@ -83,6 +118,10 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, cons
     static_assert(64 * kPitch * 2 <= (int)sizeof(bm), "");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int row = lane & 15, quad = lane >> 4;
+    if (p.cu && blockIdx.x == gridDim.x - 1) {
+        order_rows(p, w, reinterpret_cast<int32_t*>(am));
+        return;
+    }
     const int64_t slot = blockIdx.x / (uint32_t)p.Hk;
     const int hk = (int)(blockIdx.x % (uint32_t)p.Hk);
     int n, len, chunk;
@@ -330,12 +369,11 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(const Params p, cons
     const uint32_t slices = (uint32_t)(p.V / (16 * NT)), each = slices * (uint32_t)w.together;
     const uint32_t group = blockIdx.x / 8 / each * 8 + blockIdx.x % 8, in = blockIdx.x / 8 % each;
     const int64_t unit = (int64_t)group * w.together + in / slices;
-    if (unit >= (int64_t)p.num_seqs * p.Hv) return;
-    const int n = (int)(unit / p.Hv), h = (int)(unit % p.Hv), hk = h / p.share, col0 = (int)(in % slices) * 16 * NT;
+    if (unit >= (int64_t)(p.cu ? w.order[0] : p.num_seqs) * p.Hv) return;
+    const int n = p.cu ? w.order[1 + (int)(unit / p.Hv)] : (int)(unit / p.Hv), h = (int)(unit % p.Hv), hk = h / p.share, col0 = (int)(in % slices) * 16 * NT;
     int64_t first;
     int len;
     extent(p, n, first, len);
-    if (p.cu && len <= p.token_len) return;
     const int chunks = (len + kChunk - 1) / kChunk;
     const int64_t slot = first_slot(p, n, first);
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -621,10 +659,12 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(const Params p, cons
 
 template <int K>
 hipError_t launch(const Params& p, const Work& w, int64_t slots, bool wide, hipStream_t stream) {
-    hipLaunchKernelGGL(delta_prep_kernel<K>, dim3((unsigned)(slots * p.Hk)), dim3(256), 0, stream, p, w);
+    hipLaunchKernelGGL(delta_prep_kernel<K>, dim3((unsigned)(slots * p.Hk + (p.cu ? 1 : 0))), dim3(256), 0, stream, p, w);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const int64_t groups = ((int64_t)p.num_seqs * p.Hv / w.together + 7) / 8 * 8;
+    int64_t rows = p.num_seqs;  // at most so many are longer than token_len
+    if (p.cu) rows = rows < p.total_tokens / (p.token_len + 1) ? rows : p.total_tokens / (p.token_len + 1);
+    const int64_t groups = (rows * p.Hv / w.together + 7) / 8 * 8;
     if (wide)
         hipLaunchKernelGGL((delta_scan_kernel<K, 2>), dim3((unsigned)(groups * w.together * (p.V / 32))), dim3(512), 0, stream, p, w);
     else
@@ -638,8 +678,8 @@ int64_t chunk_slots(int32_t num_seqs, int32_t T, int64_t total_tokens, bool ragg
     return ragged ? total_tokens / kChunk + num_seqs : (int64_t)num_seqs * ((T + kChunk - 1) / kChunk);
 }
 int64_t chunk_groups(int32_t num_seqs, int32_t Hv, int32_t V) { return ((int64_t)num_seqs + 7) / 8 * 8 * Hv * (V / 16); }
-size_t chunk_workspace(int64_t slots, int32_t Hk, int32_t Hv, int32_t K) {
-    return (size_t)slots * (Hk * (size_t)(3 * K * kChunk * 2) + Hv * (size_t)kRecord);
+size_t chunk_workspace(int64_t slots, int32_t num_seqs, int32_t Hk, int32_t Hv, int32_t K) {
+    return (size_t)slots * (Hk * (size_t)(3 * K * kChunk * 2) + Hv * (size_t)kRecord) + (size_t)(num_seqs + 1) * 4;
 }
 
 hipError_t launch_chunks(const Params& p, int cus, hipStream_t stream) {
@@ -647,6 +687,7 @@ hipError_t launch_chunks(const Params& p, int cus, hipStream_t stream) {
     Work w;
     w.kq = p.workspace;
     w.rec = p.workspace + slots * p.Hk * (int64_t)(3 * p.K * kChunk * 2);
+    w.order = reinterpret_cast<int32_t*>(w.rec + slots * p.Hv * kRecord);
     w.together = (int64_t)p.num_seqs * p.Hk >= 8 ? p.share : 1;
     const bool wide = p.V % 32 == 0 && (int64_t)p.num_seqs * p.Hv * (p.V / 32) >= 2 * cus;
     return p.K == 64 ? launch<64>(p, w, slots, wide, stream) : launch<128>(p, w, slots, wide, stream);

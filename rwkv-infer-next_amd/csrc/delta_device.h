@@ -81,11 +81,12 @@ constexpr int kChunk = 64;
 constexpr int64_t kRecordT = 0, kRecordB = 18 * 1024, kRecordFactors = 30 * 1024, kRecord = 30 * 1024 + 1280;
 struct Work {
     char *kq, *rec;
+    int32_t* order;    // ragged rows: how many run by chunks, then their numbers
     int32_t together;  // heads whose workgroups follow each other on one XCD
 };
 int64_t chunk_slots(int32_t num_seqs, int32_t T, int64_t total_tokens, bool ragged);
 int64_t chunk_groups(int32_t num_seqs, int32_t Hv, int32_t V);  // most workgroups of the chunks' scan
-size_t chunk_workspace(int64_t slots, int32_t Hk, int32_t Hv, int32_t K);
+size_t chunk_workspace(int64_t slots, int32_t num_seqs, int32_t Hk, int32_t Hv, int32_t K);
 
 // All rows (ragged: those longer than token_len) by chunks; by tokens (ragged: those up to token_len).
 hipError_t launch_chunks(const Params& p, int cus, hipStream_t stream);
