@@ -27,6 +27,7 @@ extern "C" {
 #define DELTA_STATUS_NKEEP 8192     /* negative n_keep: taken as 0 */
 #define DELTA_STATUS_CLASH 16384    /* two rows store to one slot (calls of at most 1024 rows) */
 
+#define DELTA_TOKEN_LEN 16          /* the library's choice of token_len */
 #define DELTA_MAX_STRIDE (1 << 24)  /* elements between tokens of an operand */
 
 typedef struct delta_args {

@@ -7,8 +7,6 @@ namespace delta {
 namespace {
 
 constexpr int kClashRows = 1024;
-// Rows of at most so many tokens run token by token.
-constexpr int kTokenLen = 16;
 
 struct Plan {
     bool tokens, chunks;
@@ -18,7 +16,7 @@ struct Plan {
 };
 Plan make_plan(const delta_args* a) {
     Plan pl{};
-    pl.token_len = a->token_len >= 0 ? a->token_len : kTokenLen;
+    pl.token_len = a->token_len >= 0 ? a->token_len : DELTA_TOKEN_LEN;
     const int64_t longest = a->cu_seqlens ? a->total_tokens : a->T;
     pl.chunks = !a->snapshots && longest > pl.token_len;
     pl.tokens = !pl.chunks || a->cu_seqlens;

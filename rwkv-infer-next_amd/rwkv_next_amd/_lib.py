@@ -86,6 +86,7 @@ DELTA_STATUS_SLOT = 2048
 DELTA_STATUS_SEQLENS = 4096
 DELTA_STATUS_NKEEP = 8192
 DELTA_STATUS_CLASH = 16384
+DELTA_TOKEN_LEN = 16
 DELTA_MAX_STRIDE = 1 << 24
 SLOTS_EXPORTED = ("slots_cache_size", "slots_copy", "slots_free", "slots_compact")
 SLOTS_MAX_CACHES = 16

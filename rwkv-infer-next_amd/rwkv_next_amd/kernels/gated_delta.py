@@ -27,66 +27,73 @@ from ._workspace import on_device, stream_handle
 from .wkv7 import _index_tensor, _require
 
 
-def _tokens(t, dtype, shape, align, name):
-    """`t` (B, T, ...) as it is where its tokens follow each other at one stride and each is contiguous, else a contiguous copy;
-    with that stride in elements."""
+def _tokens(t, dtype, shape, inner, align, name):
+    """`t` (B, T, ...) as it is where its tokens, `inner` contiguous elements each, follow each other at one stride, else a contiguous
+    copy; with that stride in elements and its address."""
     if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype} (got {t.dtype})")
     if t.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)} (got {tuple(t.shape)})")
-    B, T = shape[:2]
-    inner = 1
-    for n in shape[2:]:
-        inner *= n
-    st = t.stride()
-    token = st[1] if T > 1 else st[0] if B > 1 else inner
-    ok = (B == 1 or T == 1 or st[0] == T * st[1]) and inner <= token <= _lib.DELTA_MAX_STRIDE
-    want = 1
-    for n, s in zip(reversed(shape[2:]), reversed(st[2:])):
-        ok = ok and (n == 1 or s == want)
-        want *= n
-    if not ok or token % align or t.data_ptr() % (16 if align > 1 else 4):
-        # (a copy has its own memory, aligned)
-        return t.clone(memory_format=torch.contiguous_format), inner
-    return t, token
+    ptr = t.data_ptr()
+    if ptr % (16 if align > 1 else 4) == 0:
+        if t.is_contiguous():
+            return t, inner, ptr
+        B, T = shape[:2]
+        st = t.stride()
+        token = st[1] if T > 1 else st[0] if B > 1 else inner
+        ok = (B == 1 or T == 1 or st[0] == T * st[1]) and inner <= token <= _lib.DELTA_MAX_STRIDE and token % align == 0
+        want = 1
+        for n, s in zip(reversed(shape[2:]), reversed(st[2:])):
+            ok = ok and (n == 1 or s == want)
+            want *= n
+        if ok:
+            return t, token, ptr
+    t = t.detach().clone(memory_format=torch.contiguous_format)  # its own memory, aligned
+    return t, inner, t.data_ptr()
 
 
 def _launch(q, k, v, g, beta, *, o, h0=None, h0_idx=None, ht=None, ht_idx=None, fresh=None, cu=None, n_keep=None,
             snapshots=None, status=None, scale, qk_norm, token_len):
-    if q.dim() != 4 or v.dim() != 4:
-        raise ValueError(f"q, k must be (B, T, Hk, K) and v (B, T, Hv, V) (got {tuple(q.shape)}, {tuple(v.shape)})")
-    B, T, Hk, K = q.shape
-    Hv, V = v.shape[2:]
+    qs, vs = q.shape, v.shape
+    if len(qs) != 4 or len(vs) != 4:
+        raise ValueError(f"q, k must be (B, T, Hk, K) and v (B, T, Hv, V) (got {tuple(qs)}, {tuple(vs)})")
+    B, T, Hk, K = qs
+    Hv, V = vs[2], vs[3]
     if K not in (64, 128) or V % 16 or not 16 <= V <= 256:
         raise ValueError(f"head sizes must be K in (64, 128) and V a multiple of 16 up to 256 (got K={K}, V={V})")
     if Hk < 1 or Hv < Hk or Hv % Hk:
         raise ValueError(f"value heads must be a multiple of the query/key heads (got Hk={Hk}, Hv={Hv})")
-    dev = q.device
-    if dev.type != "cuda":
+    dev, index = q.device, q.get_device()
+    if index < 0:
         raise ValueError(f"operands must be on a GPU (got {dev})")
     for t, name in ((k, "k"), (v, "v"), (g, "g"), (beta, "beta"), (h0, "state"), (h0_idx, "slots"), (fresh, "fresh"),
                     (cu, "cu_seqlens"), (n_keep, "n_keep"), (snapshots, "snapshots"), (status, "status")):
-        if t is not None and t.device != dev:
+        if t is not None and t.get_device() != index:
             raise ValueError(f"{name} must be on {dev} (got {t.device})")
-    q, q_s = _tokens(q, torch.bfloat16, (B, T, Hk, K), 8, "q")
-    k, k_s = _tokens(k, torch.bfloat16, (B, T, Hk, K), 8, "k")
-    v, v_s = _tokens(v, torch.bfloat16, (B, T, Hv, V), 8, "v")
-    g, g_s = _tokens(g, torch.float32, (B, T, Hv), 1, "g")
-    beta, b_s = _tokens(beta, torch.float32, (B, T, Hv), 1, "beta")
-    N = B if cu is None else cu.numel() - 1
-    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    rows = lambda t: 0 if t is None else t.shape[0]  # noqa: E731
-    fields = [q.data_ptr(), k.data_ptr(), v.data_ptr(), q_s, k_s, v_s, g.data_ptr(), beta.data_ptr(), g_s, b_s,
-              ptr(o), Hv * V, ptr(h0), ptr(h0_idx), rows(h0), ptr(ht), ptr(ht_idx), rows(ht), ptr(fresh), ptr(cu),
-              ptr(n_keep), ptr(snapshots), ptr(status), 0, 0, B * T, N, 0 if cu is not None else T, Hk, Hv, K, V,
-              K ** -0.5 if scale is None else float(scale), int(qk_norm), token_len]  # in the order of the fields
-    lib, size = _lib.load(), ctypes.c_size_t(0)
+    q, q_s, q_p = _tokens(q, torch.bfloat16, qs, Hk * K, 8, "q")
+    k, k_s, k_p = _tokens(k, torch.bfloat16, qs, Hk * K, 8, "k")
+    v, v_s, v_p = _tokens(v, torch.bfloat16, (B, T, Hv, V), Hv * V, 8, "v")
+    heads = (B, T, Hv)
+    g, g_s, g_p = _tokens(g, torch.float32, heads, Hv, 1, "g")
+    beta, b_s, b_p = _tokens(beta, torch.float32, heads, Hv, 1, "beta")
+    h_p = 0 if h0 is None else h0.data_ptr()
+    fields = [q_p, k_p, v_p, q_s, k_s, v_s, g_p, b_p, g_s, b_s, 0 if o is None else o.data_ptr(), Hv * V,
+              h_p, 0 if h0_idx is None else h0_idx.data_ptr(), 0 if h0 is None else h0.shape[0],
+              0 if ht is None else h_p if ht is h0 else ht.data_ptr(), 0 if ht_idx is None else ht_idx.data_ptr(),
+              0 if ht is None else ht.shape[0], 0 if fresh is None else fresh.data_ptr(), 0 if cu is None else cu.data_ptr(),
+              0 if n_keep is None else n_keep.data_ptr(), 0 if snapshots is None else snapshots.data_ptr(),
+              0 if status is None else status.data_ptr(), 0, 0, B * T, B if cu is None else cu.numel() - 1,
+              T if cu is None else 0, Hk, Hv, K, V, K ** -0.5 if scale is None else float(scale), int(qk_norm),
+              token_len]  # in the order of the fields
+    lib = _lib.load()
     args = _lib.pack_delta(*fields)
-    _lib.check(lib.delta_workspace_size(args, ctypes.byref(size)))
-    if size.value:  # what it holds does not matter: from the caching allocator, in the stream's order
-        workspace = torch.empty(size.value, dtype=torch.uint8, device=dev)
-        fields[23:25] = workspace.data_ptr(), size.value
-        args = _lib.pack_delta(*fields)
+    if cu is not None or T > (_lib.DELTA_TOKEN_LEN if token_len < 0 else token_len):  # else token by token, without a workspace
+        size = ctypes.c_size_t(0)
+        _lib.check(lib.delta_workspace_size(args, ctypes.byref(size)))
+        if size.value:  # what it holds does not matter: from the caching allocator, in the stream's order
+            workspace = torch.empty(size.value, dtype=torch.uint8, device=dev)
+            fields[23:25] = workspace.data_ptr(), size.value
+            args = _lib.pack_delta(*fields)
     with on_device(dev):
         _lib.check(lib.delta_run(args, stream_handle(dev)))
 
@@ -132,15 +139,9 @@ def gated_delta(q, k, v, g, beta, state=None, *, cu_seqlens=None, scale=None, qk
     return o, ht
 
 
-@torch.library.custom_op("rwkv_next_amd::gated_delta_pool_", mutates_args=("pool", "snapshots", "status"))
-def gated_delta_pool_op(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, pool: Tensor, slots: Tensor,
-                        cu_seqlens: Optional[Tensor], n_keep: Optional[Tensor], fresh: Optional[Tensor],
-                        scale: Optional[float], qk_norm: bool, final: bool, store_o: bool, snapshots: Optional[Tensor],
-                        status: Optional[Tensor], token_len: int) -> Tensor:
-    """The slot-pool recurrence as a registered op (indices int64, cu_seqlens int32, fresh uint8).  Returns o, or an empty tensor
-    when store_o is False."""
+def _pool(q, k, v, g, beta, pool, slots, cu_seqlens, n_keep, fresh, scale, qk_norm, final, store_o, snapshots, status, token_len):
     N = q.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1
-    K, (Hv, V) = q.shape[3], v.shape[2:]
+    K, Hv, V = q.shape[3], v.shape[2], v.shape[3]
     _require(pool, "pool", torch.float32, (None, Hv, K, V))
     _require(slots, "slots", torch.int64, (N,))
     if cu_seqlens is not None:
@@ -164,6 +165,17 @@ def gated_delta_pool_op(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor
     return o
 
 
+@torch.library.custom_op("rwkv_next_amd::gated_delta_pool_", mutates_args=("pool", "snapshots", "status"))
+def gated_delta_pool_op(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, pool: Tensor, slots: Tensor,
+                        cu_seqlens: Optional[Tensor], n_keep: Optional[Tensor], fresh: Optional[Tensor],
+                        scale: Optional[float], qk_norm: bool, final: bool, store_o: bool, snapshots: Optional[Tensor],
+                        status: Optional[Tensor], token_len: int) -> Tensor:
+    """The slot-pool recurrence as a registered op (indices int64, cu_seqlens int32, fresh uint8).  Returns o, or an empty tensor
+    when store_o is False."""
+    return _pool(q, k, v, g, beta, pool, slots, cu_seqlens, n_keep, fresh, scale, qk_norm, final, store_o, snapshots, status,
+                 token_len)
+
+
 @gated_delta_pool_op.register_fake
 def _(q, k, v, g, beta, pool, slots, cu_seqlens, n_keep, fresh, scale, qk_norm, final, store_o, snapshots, status, token_len):
     return v.new_empty(v.shape if store_o else (0,))
@@ -180,7 +192,9 @@ def gated_delta_pool_(q, k, v, g, beta, pool, slots, *, cu_seqlens=None, n_keep=
     to the first n tokens is SlotCaches((snapshots.flatten(0, 1), 0)).copy_slots(row * T + n - 1, slots,
     into=SlotCaches((pool, 0))), or, on the pool as it was before, a call with n_keep=n, store_o=False on the same operands: where
     token by token, the same bits.
-    Returns o like v (None when store_o is False).  Runs as the registered op rwkv_next_amd::gated_delta_pool_."""
+    Returns o like v (None when store_o is False).  Under torch.compile or another tracer it is the registered op
+    rwkv_next_amd::gated_delta_pool_; an eager call goes straight to the library, as dense_matmul's (the dispatch of an op took 15 of
+    a single token's 27 us)."""
     cu, N = _rows(q, cu_seqlens)
     dev = q.device
     sl = _index_tensor(slots, dev, torch.int64, "slots")
@@ -191,6 +205,11 @@ def gated_delta_pool_(q, k, v, g, beta, pool, slots, *, cu_seqlens=None, n_keep=
         if fr.dtype == torch.bool:
             fr = fr.view(torch.uint8)
         fr = (fr if fr.dtype == torch.uint8 else fr.to(torch.uint8)).contiguous()
-    o = gated_delta_pool_op(q, k, v, g, beta, pool, sl, cu, nk, fr, scale, bool(qk_norm), final, store_o, snapshots, status,
-                            int(token_len))
+    traced = torch.compiler.is_compiling() or type(pool) is not Tensor or torch._C._len_torch_dispatch_stack() > 0
+    o = (gated_delta_pool_op if traced else _pool)(q, k, v, g, beta, pool, sl, cu, nk, fr, scale, bool(qk_norm), final, store_o,
+                                                   snapshots, status, int(token_len))
+    if not traced:
+        for t in (pool if final else None, snapshots, status):
+            if t is not None and not t.is_inference():
+                torch.autograd.graph.increment_version(t)  # written in place
     return o if store_o else None
