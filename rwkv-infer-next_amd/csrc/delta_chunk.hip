@@ -71,6 +71,15 @@ __device__ __forceinline__ void split3(float x0, float x1, uint32_t& a, uint32_t
     wkv7::split_pair(y[0], y[1], b, c);
 }
 
+// x of the lane that DPP control `kCtrl` names, 0 where there is none or the row of 16 lanes is not in `kRows`
+template <int kCtrl, int kRows>
+__device__ __forceinline__ double moved(double x) {
+    const u2 w = __builtin_bit_cast(u2, x);
+    const uint32_t lo = w[0], hi = w[1];
+    return __builtin_bit_cast(double, u2{(uint32_t)__builtin_amdgcn_update_dpp(0, (int)lo, kCtrl, kRows, 0xF, false),
+                                         (uint32_t)__builtin_amdgcn_update_dpp(0, (int)hi, kCtrl, kRows, 0xF, false)});
+}
+
 // The ragged rows that run by chunks into w.order, longest first (to a chunk, and up to kOrders of them): a scan that begins with its
 // longest rows ends together, and workgroups without a row come last, where they hold nothing up.  Which of two rows as long comes
 // first is left to chance; results do not depend on it.
@@ -111,10 +120,10 @@ template <int K>
 __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, const Work w) {
     constexpr int kSteps = K / 32, kPitch = K + 8;
     __shared__ __attribute__((aligned(16))) float am[64 * kRow];   // K's tile, then A, then T
-    __shared__ __attribute__((aligned(16))) float bm[64 * kRow];   // Q's tile, then B
-    __shared__ __attribute__((aligned(16))) float mm[32 * kRow];
-    __shared__ double cs[64];
-    __shared__ float rk[64], rq[64], be[64];
+    __shared__ __attribute__((aligned(16))) float bm[64 * kRow];   // Q's tile, then products on the way to T
+    __shared__ __attribute__((aligned(16))) double cs[64];
+    __shared__ __attribute__((aligned(16))) float rk[64], rq[64], be[64];
+    float* const mm = bm;
     static_assert(64 * kPitch * 2 <= (int)sizeof(bm), "");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int row = lane & 15, quad = lane >> 4;
@@ -154,31 +163,37 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, cons
         }
     }
     __syncthreads();
-    const auto rows = [&](const uint16_t* x, int block, u4* f) {
+    const auto rows = [&](const uint16_t* x, int token, u4* f) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) f[s] = *reinterpret_cast<const u4*>(x + (16 * block + row) * kPitch + 32 * s + 8 * quad);
+        for (int s = 0; s < kSteps; ++s) f[s] = *reinterpret_cast<const u4*>(x + token * kPitch + 32 * s + 8 * quad);
     };
-    f4 kk[4], qk[4];
+    const bool two = wave >= 2;
+    f4 kk[4], kq[4];  // K K^T by rows of this wavefront's 16 tokens in a row; K Q^T by columns of its dealt out ones
     char* const operands = w.kq + (slot * p.Hk + hk) * (3 * K * kChunk * 2);
     {
-        u4 kf[kSteps], qf[kSteps];
-        rows(k_tile, wave, kf);
-        rows(q_tile, wave, qf);
+        u4 kf[kSteps], of[kSteps];
+        rows(k_tile, 16 * wave + row, kf);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            kk[j] = qk[j] = f4{0.f, 0.f, 0.f, 0.f};
+            kk[j] = kq[j] = f4{0.f, 0.f, 0.f, 0.f};
             if (j <= wave) {
-                u4 of[kSteps];
-                rows(k_tile, j, of);
+                rows(k_tile, 16 * j + row, of);
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s) {
-                    kk[j] = mfma(kf[s], of[s], kk[j]);
-                    qk[j] = mfma(qf[s], of[s], qk[j]);
-                }
+                for (int s = 0; s < kSteps; ++s) kk[j] = mfma(kf[s], of[s], kk[j]);
             }
         }
+        u4 qf[kSteps];
+        const int mine = token_of(wave, row);
+        rows(q_tile, mine, qf);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < 2 || two) {
+                rows(k_tile, token_of(j, row), of);
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) kq[j] = mfma(of[s], qf[s], kq[j]);
+            }
+        rows(k_tile, mine, kf);
         float nk = 0.f, nq = 0.f;
-        const int t = 16 * wave + row, tile = 2 * (t >> 5) + (t >> 2 & 1), to = 16 * quad + 4 * (t >> 3 & 3) + (t & 3);  // token_of(tile, to) = t
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
@@ -187,14 +202,14 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, cons
                 nk = fmaf(x, x, nk);
                 nq = fmaf(y, y, nq);
             }
-            *reinterpret_cast<u4*>(operands + ((tile * kSteps + s) * 64 + to) * 16) = kf[s];
-            *reinterpret_cast<u4*>(operands + K * kChunk * 2 + ((tile * kSteps + s) * 64 + to) * 16) = qf[s];
+            *reinterpret_cast<u4*>(operands + ((wave * kSteps + s) * 64 + lane) * 16) = kf[s];
+            *reinterpret_cast<u4*>(operands + K * kChunk * 2 + ((wave * kSteps + s) * 64 + lane) * 16) = qf[s];
         }
         nk += __shfl_xor(nk, 16), nq += __shfl_xor(nq, 16);
         nk += __shfl_xor(nk, 32), nq += __shfl_xor(nq, 32);
         if (quad == 0) {
-            rk[16 * wave + row] = p.qk_norm ? 1.f / sqrtf(nk + kNormEps) : 1.f;
-            rq[16 * wave + row] = p.qk_norm ? p.scale / sqrtf(nq + kNormEps) : p.scale;
+            rk[mine] = p.qk_norm ? 1.f / sqrtf(nk + kNormEps) : 1.f;
+            rq[mine] = p.qk_norm ? p.scale / sqrtf(nq + kNormEps) : p.scale;
         }
     }
     // K^T in operand order: tile of 16 rows of the state, half of the tokens, lane
@@ -220,11 +235,12 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, cons
         const int64_t token = first + min(lane, len - 1);
         const float g = p.g[token * p.g_stride + h], b = p.beta[token * p.beta_stride + h];
         double c = lane < len ? (double)(g < kLeast ? kLeast : g) * 1.4426950408889634 : 0.0;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const double other = __shfl_up(c, d);
-            c += lane >= d ? other : 0.0;
-        }
+        c += moved<0x111, 0xF>(c);  // row_shr by 1, 2, 4, 8
+        c += moved<0x112, 0xF>(c);
+        c += moved<0x114, 0xF>(c);
+        c += moved<0x118, 0xF>(c);
+        c += moved<0x142, 0xA>(c);  // the rows' sums: lane 15 to row 1, 47 to row 3, then 31 to rows 2 and 3
+        c += moved<0x143, 0xC>(c);
         const double last = __shfl(c, 63);
         const float beta = lane < len ? b : 0.f;
         __syncthreads();  // the tiles are read; the head before is written
@@ -247,11 +263,36 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, cons
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int i = 16 * wave + 4 * quad + r;
-                    const float decay = i >= col ? __builtin_amdgcn_exp2f((float)(cs[i] - cs[col])) * rk[col] : 0.f;
+                    const float decay = i > col ? __builtin_amdgcn_exp2f((float)(cs[i] - cs[col])) * rk[col] : 0.f;
                     am[i * kRow + col] = i > col ? kk[j][r] * (be[i] * rk[i]) * decay : 0.f;
-                    bm[i * kRow + col] = qk[j][r] * rq[i] * decay;
                 }
             }
+        {  // B, in two bf16 parts: the rows of a K Q^T that a lane has are its operand of B D
+            const int i = token_of(wave, row);
+            const double ci = cs[i];
+            const float scale = rq[i];
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                if (half == 0 || two) {
+                    u4 hi, lo;
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {
+                        float x[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int j = 32 * half + 8 * quad + 2 * m + e;
+                            const float decay = __builtin_amdgcn_exp2f((float)(ci - cs[j])) * rk[j];
+                            x[e] = i >= j ? kq[2 * half + (m >> 1)][2 * (m & 1) + e] * scale * decay : 0.f;
+                        }
+                        uint32_t a, b;
+                        wkv7::split_pair(x[0], x[1], a, b);
+                        hi[m] = a, lo[m] = b;
+                    }
+                    char* const to = rec + kRecordB + block_of(wave, half) * 2048 + lane * 16;
+                    *reinterpret_cast<u4*>(to) = hi;
+                    *reinterpret_cast<u4*>(to + 1024) = lo;
+                }
+        }
         wkv7::wave_lds_sync();
         // the inverse of this wavefront's 16 x 16 block, a column a lane, by forward substitution
         {
@@ -317,33 +358,27 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, cons
             put(am, 2 + i, j, -x);
         }
         __syncthreads();
-        // T in three bf16 parts and B in two, in operand order
+        // T in three bf16 parts, in operand order
         for (int e = tid; e < 6 * 64; e += 256) {
             const int block = e >> 6, l = e & 63;
             const int t = block < 2 ? block : (block + 2) >> 1, half = block < 2 ? 0 : block & 1;
             const int i = token_of(t, l & 15), at = 32 * half + 8 * (l >> 4);
-            f4 x[2], y[2];
+            u4 part[3];
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                x[m] = *reinterpret_cast<const f4*>(am + i * kRow + at + 4 * m);
-                y[m] = *reinterpret_cast<const f4*>(bm + i * kRow + at + 4 * m);
+                f4 x = *reinterpret_cast<const f4*>(am + i * kRow + at + 4 * m);
 #pragma unroll
                 for (int r = 0; r < 4; ++r)  // above the diagonal nothing was computed
-                    if (at + 4 * m + r > i) x[m][r] = y[m][r] = 0.f;
-            }
-            u4 hi, lo, part[3];
+                    if (at + 4 * m + r > i) x[r] = 0.f;
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                uint32_t a, b, c;
-                wkv7::split_pair(y[m >> 1][2 * (m & 1)], y[m >> 1][2 * (m & 1) + 1], a, b);
-                hi[m] = a, lo[m] = b;
-                split3(x[m >> 1][2 * (m & 1)], x[m >> 1][2 * (m & 1) + 1], a, b, c);
-                part[0][m] = a, part[1][m] = b, part[2][m] = c;
+                for (int o = 0; o < 2; ++o) {
+                    uint32_t a, b, c;
+                    split3(x[2 * o], x[2 * o + 1], a, b, c);
+                    part[0][2 * m + o] = a, part[1][2 * m + o] = b, part[2][2 * m + o] = c;
+                }
             }
 #pragma unroll
             for (int m = 0; m < 3; ++m) *reinterpret_cast<u4*>(rec + kRecordT + ((block * 3 + m) * 64 + l) * 16) = part[m];
-            *reinterpret_cast<u4*>(rec + kRecordB + ((block * 2) * 64 + l) * 16) = hi;
-            *reinterpret_cast<u4*>(rec + kRecordB + ((block * 2 + 1) * 64 + l) * 16) = lo;
         }
     }
 }
