@@ -53,7 +53,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void dense_tile_kernel(const Param
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {  // past the last row: it again, not stored
         const int base = min(row0 + kThreads / 8 * i, p.M - 1);
-        ap[i] = wkv7::uniform_ptr(reinterpret_cast<const char*>(p.a + base * p.a_row_stride) + from_step * 64);
+        ap[i] = wkv7::uniform_ptr(reinterpret_cast<const char*>(p.a + base * p.a_row_stride) + (int64_t)from_step * 64);
         at_a[i] = (uint32_t)min(tid >> 3, p.M - 1 - base) * (uint32_t)(p.a_row_stride * 2);  // at most 63 rows: below 2^31
     }
     const int row = tid >> 3;

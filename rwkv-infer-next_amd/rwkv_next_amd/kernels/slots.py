@@ -17,6 +17,30 @@ from .. import _lib
 from ._workspace import on_device, stream_handle
 
 
+def _apart(a, slots_a, b, slots_b):
+    """Whether no slot of cache `a` shares memory with one of cache `b`, each (tensor, layer, slot, row, layers) with strides in bytes:
+    their extents are apart, or both lie in one grid of slots (two ranges of a tensor's slots, or two parts of its rows)."""
+    (t, layer, slot, row, layers), (u, layer_u, slot_u, row_u, layers_u) = a, b
+    if not (row and layers and slots_a and row_u and layers_u and slots_b):
+        return True
+    end = t.data_ptr() + (layers - 1) * layer + (slots_a - 1) * slot + row
+    end_u = u.data_ptr() + (layers_u - 1) * layer_u + (slots_b - 1) * slot_u + row_u
+    if end <= u.data_ptr() or end_u <= t.data_ptr():
+        return True
+    if slots_a == 1 and layers == 1 or slots_b == 1 and layers_u == 1:
+        return False
+    inner, outer = (slot, layer) if layers == 1 or slot <= layer else (layer, slot)
+    if {slot, layer if layers > 1 else 0} != {slot_u, layer_u if layers_u > 1 else 0}:
+        return False
+    far = u.data_ptr() - t.data_ptr()
+    if outer % inner == 0 and row <= far % inner and far % inner + row_u <= inner:
+        return True  # beside each other within every row of the grid
+    if far % inner or not outer or (slot, layer) != (slot_u, layer_u) or slot > layer:
+        return False
+    first = far % outer // slot  # a layer's slots of `b` begin so many after those of `a`
+    return slots_a <= first and (first + slots_b) * slot <= outer
+
+
 class SlotCaches:
     """A model's cache tensors that share their slots.  Each argument is a tensor (layers, slots, ..) or (tensor, dim) with dim 0 for
     (slots, ..) and 1 for (layers, slots, ..); a slot's part of a layer is contiguous.  At most 16 tensors, of any types."""
@@ -24,7 +48,7 @@ class SlotCaches:
     def __init__(self, *caches):
         if not 1 <= len(caches) <= _lib.SLOTS_MAX_CACHES:
             raise ValueError(f"SlotCaches takes 1 to {_lib.SLOTS_MAX_CACHES} tensors (got {len(caches)})")
-        self._rows, self.slots, self.device = [], None, None
+        self._rows, self.slots, self.device, self._shared = [], None, None, False
         for x in caches:
             t, dim = x if isinstance(x, tuple) else (x, 1)
             if dim not in (0, 1) or t.dim() <= dim:
@@ -50,6 +74,7 @@ class SlotCaches:
             if row and layers > 1 and self.slots > 1 and layer < self.slots * slot and slot < layers * layer:
                 raise ValueError(f"slots of a cache must not share memory (got {tuple(t.shape)}, strides {strides})")
             self._rows.append((t, layer, slot, row, layers))
+            self._shared |= not all(_apart(self._rows[-1], self.slots, x, self.slots) for x in self._rows[:-1])
         self._own = self._pairs(self)
 
     def _pairs(self, other):
@@ -70,6 +95,10 @@ class SlotCaches:
             raise ValueError(f"{name} must be an int64 tensor of one dimension (got {x.dtype} {tuple(x.shape)})")
         return x.contiguous()
 
+    def _require_apart(self):
+        if self._shared:
+            raise ValueError("caches whose slots move must not share memory with each other")
+
     def _status(self, status):
         if status is None:
             return None
@@ -78,7 +107,7 @@ class SlotCaches:
         return status.data_ptr()
 
     def copy_slots(self, src, dst, *, into: "SlotCaches | None" = None, status=None) -> None:
-        """into's slot dst[i] = this one's slot src[i] (into: these caches themselves where None), as if all sources were read
+        """into's slot dst[i] = this one's slot src[i] (into: these caches themselves where None, or caches apart from them), as if all sources were read
         before any destination is written: swaps and chains are exact.  A source may be named any number of times; of equal
         destinations the last one counts.  A negative index leaves its entry out, one past the slots does too and sets
         SLOTS_STATUS_SLOT in `status`.  At most 1024 entries."""
@@ -89,9 +118,15 @@ class SlotCaches:
         if n > _lib.SLOTS_MAX_PAIRS:
             raise ValueError(f"at most {_lib.SLOTS_MAX_PAIRS} copies per call (got {n})")
         a, to = self._own, self.slots
+        self._require_apart()
         if into is not None and into is not self:
+            into._require_apart()
             if into.device != self.device or len(into._rows) != len(self._rows):
                 raise ValueError(f"into must be {len(self._rows)} caches on {self.device}")
+            for x in self._rows:
+                for y in into._rows:
+                    if not _apart(x, self.slots, y, into.slots):
+                        raise ValueError("into must not share memory with these caches, but for being the same")
             a, to = self._pairs(into), into.slots
         with on_device(self.device):
             _lib.check(_lib.load().slots_copy(a, len(a), src.data_ptr(), dst.data_ptr(), n, self.slots, to,
@@ -113,6 +148,7 @@ class SlotCaches:
         if not isinstance(live, torch.Tensor) or live.device != self.device or live.dtype not in (torch.bool, torch.uint8) or \
                 live.shape != (self.slots,):
             raise ValueError(f"live must be a bool ({self.slots},) tensor on {self.device}")
+        self._require_apart()
         if self.slots > _lib.SLOTS_MAX_COMPACT:
             raise ValueError(f"at most {_lib.SLOTS_MAX_COMPACT} slots are compacted (got {self.slots})")
         live = live.contiguous()
