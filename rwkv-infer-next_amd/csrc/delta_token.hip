@@ -3,7 +3,9 @@
 // A wavefront holds 32 columns of one head's state in registers, K / 8 rows by 4 columns a lane, and walks the row's tokens.  With
 // r = S_{t-1}^T k and u = S_{t-1}^T q from one pass over the state,
 //     d = beta (v - a r),   S_t = a S_{t-1} + k d^T,   o = scale (a u + (q . k) d)
-// so a token costs one sum over the lanes.  For one token the reading and writing of the states, 8 K V bytes a head, bounds it.
+// so a token costs one sum over the lanes.  For one token the reading and writing of the states, 8 K V bytes a head, bounds it: 64
+// sequences, 32 heads of 128 x 128, 44 to 47 us, 5.7 to 6.1 TB/s in place where a large copy moves 4.9; one sequence 5.6 us.  Each
+// lane has its 16-byte pieces of 16 rows in flight at once, so nothing needs LDS or a barrier.
 #include "delta_device.h"
 
 namespace delta {

@@ -2,7 +2,8 @@
 //
 // All three move bytes: rows are read once and written once, and HBM bounds them.  A workgroup owns a range of a row's bytes in one
 // layer of one cache, for all the slots that the call names, so that sources which are also destinations are read before they are
-// written, and a source that goes to many slots comes from memory once.
+// written, and a source that goes to many slots comes from memory once.  Measured, where a large copy moves 4.9 TB/s: four states of 2.7 MB
+// to 28 slots 19.9 us, 4.3 TB/s; 17 slots of 21 MB moved 148 us, 4.9 TB/s.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
