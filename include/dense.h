@@ -35,6 +35,8 @@ extern "C" {
 #define DENSE_GELU 6     /* x (1 + erf(x / sqrt 2)) / 2 */
 
 #define DENSE_MAX_ROW_STRIDE (1 << 24)  /* elements between rows of activations */
+#define DENSE_UNSPLIT_ROWS 16           /* products of at most so many rows .. */
+#define DENSE_UNSPLIT_K 6112            /* .. and of a shorter K than this need no workspace on any device */
 
 typedef struct dense_args {
     const uint16_t *a;             /* activations [M][K], 16-byte aligned */

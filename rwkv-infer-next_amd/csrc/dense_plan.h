@@ -18,17 +18,22 @@ inline size_t weight_bytes(int32_t K, int32_t N) { return (size_t)(strips(N) * s
 constexpr int64_t sums_row(int32_t N) { return ((int64_t)N + 3) / 4 * 4; }  // floats of a row of a split product's sums
 
 // The tile of a workgroup, rows x columns, and among how many groups of wavefronts it shares K.
-enum Shape { k16x16, k32x16, k64x16, k16x64, k32x64, k64x64, k128x128, k128x256, kShapes };
+enum Shape { k16x16, k16x64, k32x64, k64x64, k128x128, k128x256, kShapes };
 struct Tile {
     int rows, columns, k_groups, threads;
 };
-constexpr Tile kTiles[kShapes] = {{16, 16, 8, 512}, {32, 16, 8, 512}, {64, 16, 6, 384}, {16, 64, 4, 512},
-                                  {32, 64, 4, 512}, {64, 64, 4, 512}, {128, 128, 1, 256}, {128, 256, 1, 256}};
+constexpr Tile kTiles[kShapes] = {{16, 16, 8, 512}, {16, 64, 4, 512}, {32, 64, 4, 512},
+                                  {64, 64, 4, 512}, {128, 128, 1, 256}, {128, 256, 1, 256}};
 constexpr int kPanelSteps = 2;  // K is shared in panels of so many steps
+constexpr int kPartPanels = 6;  // the least of a part's panels that a group has
+// Weights of so many bytes that one row of tiles reads pass by the caches: 64 rows, 4096 x 16384, 31.2 us against 32.6, 16 rows 25.3
+// against 26.8; but 13 MB, 2560 x 2560, 7.7 against 7.1.
+constexpr size_t kStreamBytes = (size_t)64 << 20;
 
 struct Plan {
     Shape shape;
-    int parts;  // of K, among workgroups; more than one are added by a second launch
+    int parts;    // of K, among workgroups; more than one are added by a second launch
+    bool stream;  // weights by loads that leave nothing in the caches
     int64_t row_groups, strip_groups, grid;
     size_t workspace;
 };
@@ -37,45 +42,49 @@ inline Plan plan_of(int32_t M, int32_t N, int32_t K, Shape shape, int64_t parts)
     Plan p{};
     const int64_t panels = (steps(K) + kPanelSteps - 1) / kPanelSteps;
     p.shape = shape;
-    p.parts = (int)std::max<int64_t>(1, std::min<int64_t>({parts, panels / (4 * kTiles[shape].k_groups), 16}));
+    p.parts = (int)std::max<int64_t>(1, std::min<int64_t>({parts, panels / (kPartPanels * kTiles[shape].k_groups), 16}));
     p.row_groups = ((int64_t)M + kTiles[shape].rows - 1) / kTiles[shape].rows;
     p.strip_groups = ((int64_t)N + kTiles[shape].columns - 1) / kTiles[shape].columns;
+    p.stream = kTiles[shape].columns == 64 && p.row_groups == 1 && weight_bytes(K, N) >= kStreamBytes;
     p.workspace = p.parts > 1 ? (size_t)p.parts * M * sums_row(N) * sizeof(float) : 0;
     p.grid = (p.row_groups * p.strip_groups * p.parts + 7) / 8 * 8;
     return p;
 }
 
 // Measured with weights cycled past the caches, bf16, us.
-// Up to 16 rows bytes count: columns of 16 while two workgroups a CU hold them all (one row, K = N = 4096 9.5 against 10.4 by columns of 64
-// in four parts; N = 8192 15.0 / 16.9), else of 64 (N = 16384 26 / 36 by 32 x 16).
-// Up to 64 rows: columns of 16 while every CU gets one tile at most, their rows 32 where that holds, else 64 (K = N = 4096, 32 rows 10.3 /
-// 13.3 by 32 x 64 in four parts; 64 rows 12.8 / 15.5, by 32 x 16 18.7; 64 rows, N = 6144 22.3 / 19.3); else of 64, K in as many parts as
-// CUs are left for (N = 16384, 64 rows 33 / 37 by 128 x 256 in three parts).
-// More rows: the same while tiles are that few and, for those of 64, K is short (192 rows, K = N = 2560 13.7 / 17.3 by 128 x 128; K = 4096
-// 25.7 / 21.7), else the cheaper of 128 x 128 and 128 x 256 by what a step of one takes and what adding the parts does (K = N = 4096, 256 rows
-// 23.1 / 25.5, 1000 rows 49 / 44.6; K = 10240, N = 2560, 500 rows 45 / 41).
+// Little work, of any number of rows: tiles of 16 x 16 while two workgroups a CU hold them all (of more than 16 rows and long K, one on
+// every other CU), in parts where there are fewer and K is long (one row, K = N = 4096 10.7 / 12.3 by 32 x 64 in parts; 16 rows, N =
+// 8192 16.3 / 18.3 by 16 x 64; 64 rows, K = N = 768 4.3 / 5.5; 256 rows, K = 4096, N = 320 8.5 / 9.6; but 16 rows, K = 2560, N = 10240,
+// 640 tiles, 16.2 / 14.2).
+// Up to 64 rows: of the tiles of 64 columns the one of fewest rows of which every CU gets one at most (32 rows, K = 4096, N = 8192 17.8
+// by 16 / 19.2 by 32; N = 16384 30.9 / 29.0; 64 rows 37.2 by 32 / 32.4 by 64); of long K, where A's and the weight's bytes count for
+// more, as many rows as there are, in parts (K = 10240, N = 2560, 64 rows 20.0 by 64 / 26.6 by 16).
+// More rows, short K, few tiles: the same (192 rows, K = N = 2560 13.3 / 17.1 by 128 x 128; but K = N = 4096 25.2 / 21.8).
+// Else 128 x 128 or 128 x 256: up to 128 rows or K = 1024 the former (K = 4096, N = 16384, 128 rows 38.0 / 41.1; K = 768, 512 rows 26.9 /
+// 33.7), of more the cheaper by what a step of one takes, alone on a CU or not, and what adding the parts does (K = N = 4096, 256 rows
+// 23.2 / 25.7, 1000 rows 49.0 / 44.1; K = 10240, N = 2560, 512 rows 45.1 / 40.5; K = 2560, N = 10240, 2048 rows 107 / 127; K = 4096, N =
+// 16384, 2048 rows 253 / 240).
 inline Plan plan(int32_t M, int32_t N, int32_t K, int cus) {
     const auto tiles = [&](Shape s) {
         return ((int64_t)M + kTiles[s].rows - 1) / kTiles[s].rows * (((int64_t)N + kTiles[s].columns - 1) / kTiles[s].columns);
     };
-    if (M <= 16) return plan_of(M, N, K, tiles(k16x16) <= 2 * cus ? k16x16 : k16x64, 1);
-    for (Shape s : {k32x16, k64x16})
-        if (tiles(s) <= cus) return plan_of(M, N, K, s, 1);
-    if (M <= 64) {
+    if (tiles(k16x16) <= (M <= 16 || K <= 4096 ? 2 * cus : cus / 2)) return plan_of(M, N, K, k16x16, 2 * cus / tiles(k16x16));
+    if (M <= 16) return plan_of(M, N, K, k16x64, cus / tiles(k16x64));
+    if (M <= 64 && K > 4096) {
         const Shape s = M <= 32 ? k32x64 : k64x64;
         return plan_of(M, N, K, s, cus / tiles(s));
     }
-    if (K <= 2560)
-        for (Shape s : {k32x64, k64x64})
-            if (tiles(s) <= cus) return plan_of(M, N, K, s, 1);
+    for (Shape s : {k16x64, k32x64, k64x64})
+        if (tiles(s) <= cus && (M <= 64 || K <= 2560 || (s == k16x64 && K <= 4096))) return plan_of(M, N, K, s, cus / tiles(s));
+    if (M <= 64) return plan_of(M, N, K, M <= 32 ? k32x64 : k64x64, 1);
     Plan best{};
     double least = 0;
-    for (Shape s : {k128x128, k128x256}) {
+    for (Shape s : {k128x256, k128x128}) {
         const Plan p = plan_of(M, N, K, s, cus / tiles(s));
         const int64_t rounds = (tiles(s) * p.parts + cus - 1) / cus;
-        const double us = (double)rounds * steps(K) / p.parts * (s == k128x128 ? 0.36 : 0.45) +
-                          (p.parts > 1 ? 3 + 8e-6 * p.parts * M * N / 6 : 0);
-        if (s == k128x128 || us < least) best = p, least = us;
+        const double step = s == k128x256 ? (rounds > 1 ? 0.48 : 0.45) : (rounds > 1 ? 0.28 : 0.38);
+        const double us = (double)rounds * steps(K) / p.parts * step + (p.parts > 1 ? 3 + 2e-6 * p.parts * M * N : 0);
+        if (s == k128x256 || us < least || M <= 128 || K <= 1024) best = p, least = us;
     }
     return best;
 }

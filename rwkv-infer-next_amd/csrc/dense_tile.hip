@@ -5,8 +5,8 @@
 // registers, D - 1 steps ahead.  The operands of a row tile are read while those before it multiply, over the barrier between
 // panels, so that neither LDS nor the barrier is waited for.  Products are taken as out^T = w^T a^T: a lane then has four columns
 // of a row.  Measured: 4096 rows, 4096 x 16384, 443 to 476 us by 128 x 256 (two workgroups of four wavefronts a CU; by 256 x 256, eight
-// wavefronts, 600), 1.16 to 1.24 PFLOP/s where a large library product reaches 1.22; the matrix cores work 58 % of the time.  64 rows 35 us,
-// 3.9 TB/s of weight: bound by memory, and by the first and last of 16 panels that nothing covers; a deeper D changed nothing.  500
+// wavefronts, 600), 1.16 to 1.24 PFLOP/s where a large library product reaches 1.22; the matrix cores work 58 % of the time.  64 rows 31 us,
+// 4.4 TB/s of weight: bound by memory, and by the first and last of 16 panels that nothing covers; a deeper D changed nothing.  500
 // rows, 10240 x 2560, 33 us and 7 for adding the parts: one wavefront a SIMD (27 %).  Which tile a product takes, and the
 // measured sides of the rules: dense_plan.h.
 #include "dense_device.h"
@@ -14,7 +14,7 @@
 namespace dense {
 namespace {
 
-template <int AT, int MT, int NT, int WN, int WK, int D>
+template <int AT, int MT, int NT, int WN, int WK, int D, bool STREAM>
 __global__ __launch_bounds__(64 * WN * WK, 2) void dense_tile_kernel(const Params p) {
     constexpr int kThreads = 64 * WN;                  // of a group that shares K with others
     constexpr int kPanel = MT * kPanelSteps * 1024;    // bytes
@@ -78,7 +78,10 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void dense_tile_kernel(const Param
     const auto load_w = [&](int step, u4* w) {
         const int64_t at = (int64_t)min(step, last) * kBlockBytes;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) w[t] = *reinterpret_cast<const u4*>(wp[t] + at + (uint32_t)lane * 16);
+        for (int t = 0; t < NT; ++t) {
+            const u4* const x = reinterpret_cast<const u4*>(wp[t] + at + (uint32_t)lane * 16);
+            w[t] = STREAM ? __builtin_nontemporal_load(x) : *x;
+        }
     };
     u4 a[kAhead], w[D][NT];
     const auto read = [&](int slot, int step, int i) {
@@ -194,14 +197,18 @@ template <int AT, Shape S, int MT, int NT, int WN, int D>
 void launch(const Params& p, const Plan& pl, hipStream_t s) {
     constexpr Tile t = kTiles[S];
     static_assert(t.rows == 16 * MT && t.columns == 16 * NT * WN && t.threads == 64 * WN * t.k_groups, "");
-    hipLaunchKernelGGL((dense_tile_kernel<AT, MT, NT, WN, t.k_groups, D>), dim3((unsigned)pl.grid), dim3(t.threads), 0, s, p);
+    const dim3 grid((unsigned)pl.grid), block(t.threads);
+    if constexpr (t.columns == 64)
+        if (pl.stream) {
+            hipLaunchKernelGGL((dense_tile_kernel<AT, MT, NT, WN, t.k_groups, D, true>), grid, block, 0, s, p);
+            return;
+        }
+    hipLaunchKernelGGL((dense_tile_kernel<AT, MT, NT, WN, t.k_groups, D, false>), grid, block, 0, s, p);
 }
 template <int AT>
 void launch_shape(const Params& p, const Plan& pl, hipStream_t s) {
     switch (pl.shape) {
         case k16x16: return launch<AT, k16x16, 1, 1, 1, 6>(p, pl, s);
-        case k32x16: return launch<AT, k32x16, 2, 1, 1, 6>(p, pl, s);
-        case k64x16: return launch<AT, k64x16, 4, 1, 1, 6>(p, pl, s);
         case k16x64: return launch<AT, k16x64, 1, 2, 2, 6>(p, pl, s);
         case k32x64: return launch<AT, k32x64, 2, 2, 2, 6>(p, pl, s);
         case k64x64: return launch<AT, k64x64, 4, 2, 2, 6>(p, pl, s);

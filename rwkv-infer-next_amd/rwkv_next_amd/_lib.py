@@ -80,6 +80,8 @@ DENSE_TANH = 3
 DENSE_SIGMOID = 4
 DENSE_SILU = 5
 DENSE_GELU = 6
+DENSE_UNSPLIT_ROWS = 16
+DENSE_UNSPLIT_K = 6112
 DENSE_MAX_ROW_STRIDE = 1 << 24
 DELTA_EXPORTED = ("delta_args_size", "delta_workspace_size", "delta_run")
 DELTA_STATUS_SLOT = 2048

@@ -113,7 +113,7 @@ def dense_matmul(a, packed: DensePacked, *, bias=None, activation: Optional[str]
         row, ptr = K, x.data_ptr()
     lib, sums, sums_p, size = _lib.load(), None, 0, 0
     with on_device(dev):
-        if M > 16:  # fewer rows are not split
+        if M > _lib.DENSE_UNSPLIT_ROWS or K >= _lib.DENSE_UNSPLIT_K:
             need = ctypes.c_size_t(0)
             _lib.check(lib.dense_workspace_size(M, N, K, ctypes.byref(need)))
             size = need.value

@@ -30,8 +30,9 @@ static void check(int32_t M, int32_t N, int32_t K, int cus) {
     if (p.row_groups * t.rows < M || (p.row_groups - 1) * t.rows >= M) fail("rows");
     if (p.strip_groups * t.columns < N || (p.strip_groups - 1) * t.columns >= N) fail("columns");
     const int64_t panels = (steps(K) + kPanelSteps - 1) / kPanelSteps;
-    if (p.parts < 1 || p.parts > 16 || (p.parts > 1 && p.parts * t.k_groups * 4 > panels)) fail("parts");
+    if (p.parts < 1 || p.parts > 16 || (p.parts > 1 && p.parts * t.k_groups * kPartPanels > panels)) fail("parts");
     if (p.parts > 1 ? p.workspace < (size_t)p.parts * M * N * 4 : p.workspace != 0) fail("the workspace");
+    if (M <= DENSE_UNSPLIT_ROWS && K < DENSE_UNSPLIT_K && p.workspace) fail("a workspace that nobody asks for");
     // offsets of 32 bits: the rows of A among which a wavefront group's lanes choose
     if ((uint64_t)(t.threads / t.k_groups / 8 - 1) * DENSE_MAX_ROW_STRIDE * 2 + (uint64_t)DENSE_MAX_ROW_STRIDE * 2 > 0xFFFFFFFFu) fail("an offset in A");
     if (p.grid % 8 || p.grid < p.row_groups * p.strip_groups * p.parts) fail("the grid");
@@ -65,13 +66,13 @@ int main(int argc, char** argv) {
     if (argc > 1) {
         for (int i = 1; i + 2 < argc; i += 3) {
             const Plan p = plan(atoi(argv[i]), atoi(argv[i + 2]), atoi(argv[i + 1]), 256);
-            printf("%d/%d\n", (int)p.shape, p.parts);
+            printf("%d/%d%s\n", (int)p.shape, p.parts, p.stream ? "s" : "");
         }
         return 0;
     }
     const int32_t rows[] = {1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 100, 128, 129, 255, 257, 500, 1000, 2049, 4096, 10000, 65536};
     const int32_t cols[] = {1, 15, 16, 17, 63, 64, 65, 96, 255, 256, 257, 768, 1000, 2560, 4096, 4099, 8192, 8193, 16384, 65536, 151936};
-    const int32_t ks[] = {32, 64, 96, 768, 2560, 2592, 4096, 10240, 16384, 65536};
+    const int32_t ks[] = {32, 64, 96, 768, 2560, 2592, 4096, 6080, 6112, 6144, 10240, 16384, 65536};
     for (int cus : {1, 64, 256, 304})
         for (int32_t M : rows)
             for (int32_t N : cols)
@@ -105,6 +106,8 @@ def test_the_gpu_tests_reach_every_tile(program):
     args = [str(x) for shape in SHAPES for x in shape]
     got = subprocess.run([program, *args], capture_output=True, text=True, check=True).stdout.split()
     assert len(got) == len(SHAPES)
-    assert {int(x.split("/")[0]) for x in got} == set(range(8))
-    # by 64 columns or more also in parts
-    assert {int(x.split("/")[0]) for x in got if not x.endswith("/1")} == {4, 5, 6, 7}, got
+    assert {int(x.split("/")[0]) for x in got} == set(range(6))
+    # in parts too, but for 16 x 64: more than two tiles of 16 x 16 a CU are more than half a one of 16 x 64
+    assert {int(x.split("/")[0]) for x in got if x.rstrip("s").split("/")[1] != "1"} == {0, 2, 3, 4, 5}, got
+    streams = {int(x.split("/")[0]) for x in got if x.endswith("s")}
+    assert streams == {1, 2, 3}, got

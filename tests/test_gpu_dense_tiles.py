@@ -14,14 +14,16 @@ U = 2.0 ** -24
 
 # rows, K, columns: what the rule takes them to on 256 CUs
 SHAPES = [
-    (1, 32, 16), (9, 64, 33), (16, 1056, 8192), (16, 544, 700),                # 16 x 16
-    (3, 96, 8209), (16, 1120, 8704),                                           # 16 x 64
-    (17, 32, 1), (31, 992, 4096), (100, 416, 500), (40, 2080, 1000),           # 32 x 16
-    (64, 32, 4096), (60, 864, 4000), (200, 800, 768), (300, 1600, 700),        # 64 x 16
-    (17, 64, 16400), (32, 2080, 4200), (32, 4128, 5000), (96, 608, 2576),      # 32 x 64, its K in 1 to 3 parts
-    (64, 64, 16385), (50, 2080, 6160), (64, 4128, 4160), (190, 96, 4100),      # 64 x 64
-    (128, 3104, 4112), (257, 2592, 2100), (129, 32, 33000), (70, 10272, 300),  # 128 x 128
-    (1024, 2624, 4096), (400, 10272, 2564), (2050, 96, 8193), (513, 2720, 4104),  # 128 x 256
+    (1, 32, 16), (9, 64, 33), (16, 1056, 8192), (100, 416, 500), (300, 1600, 400), (17, 32, 1), (40, 2080, 1000),  # 16 x 16
+    (7, 10272, 300), (16, 10272, 2560), (33, 6176, 640),                                             # .. in parts
+    (3, 96, 8209), (16, 1120, 8704), (64, 416, 2600), (30, 4096, 4200), (300, 3104, 700),           # 16 x 64
+    (17, 64, 16400), (130, 800, 2600), (33, 96, 8100),                            # 32 x 64
+    (32, 10272, 5000),                                                            # .. in parts
+    (64, 64, 16385), (50, 2080, 16000), (190, 96, 4100),                          # 64 x 64
+    (64, 10272, 4160),                                                            # .. in parts
+    (5, 4128, 8300), (32, 2080, 16160), (60, 4128, 8700),                         # the three by loads past the caches
+    (70, 10272, 2000), (128, 3104, 4112), (257, 2592, 2100), (129, 32, 33000),    # 128 x 128, whole and in parts
+    (1024, 2624, 4096), (400, 10272, 2564), (2050, 96, 8193), (513, 2720, 4104),  # 128 x 256, whole and in parts
 ]
 
 
@@ -53,7 +55,8 @@ def test_tiles(M, K, N, dtype):
         assert torch.equal(dense_matmul(a, p, bias=b, residual=res), z.to(dtype))
 
 
-@pytest.mark.parametrize("M,K,N", [(5, 192, 100), (33, 1056, 300), (64, 4128, 4160), (128, 3104, 4112), (400, 10272, 2564)])
+@pytest.mark.parametrize("M,K,N", [(5, 192, 100), (33, 6176, 640), (64, 10272, 4160), (64, 4128, 4160), (128, 3104, 4112),
+                                   (400, 10272, 2564)])
 def test_values_that_are_not_finite_behind_the_last_step(M, K, N):
     """The last step of K, an odd one, is multiplied once: an infinity there stays one."""
     from rwkv_next_amd.kernels import dense_matmul, prepack_dense
@@ -66,7 +69,7 @@ def test_values_that_are_not_finite_behind_the_last_step(M, K, N):
     assert torch.equal(y[:, :N - 1], clean[:, :N - 1]) and (y[:, N - 1] == float("inf")).all()
 
 
-@pytest.mark.parametrize("M,K,N", [(32, 4128, 5000), (128, 3104, 4112), (400, 10272, 2564)])
+@pytest.mark.parametrize("M,K,N", [(7, 10272, 300), (32, 10272, 5000), (128, 3104, 4112), (400, 10272, 2564)])
 def test_split_products_on_two_streams_and_in_a_graph(M, K, N):
     """Parts of K in a workspace of the call's own."""
     from rwkv_next_amd.kernels import dense_matmul, prepack_dense
