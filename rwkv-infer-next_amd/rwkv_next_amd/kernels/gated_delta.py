@@ -27,6 +27,9 @@ from ._workspace import on_device, stream_handle
 from .wkv7 import _index_tensor, _require
 
 
+_increment_version = torch.autograd.graph.increment_version
+
+
 def _tokens(t, dtype, shape, inner, align, name):
     """`t` (B, T, ...) as it is where its tokens, `inner` contiguous elements each, follow each other at one stride, else a contiguous
     copy; with that stride in elements and its address."""
@@ -66,10 +69,9 @@ def _launch(q, k, v, g, beta, *, o, h0=None, h0_idx=None, ht=None, ht_idx=None, 
     dev, index = q.device, q.get_device()
     if index < 0:
         raise ValueError(f"operands must be on a GPU (got {dev})")
-    for t, name in ((k, "k"), (v, "v"), (g, "g"), (beta, "beta"), (h0, "state"), (h0_idx, "slots"), (fresh, "fresh"),
-                    (cu, "cu_seqlens"), (n_keep, "n_keep"), (snapshots, "snapshots"), (status, "status")):
+    for t in (k, v, g, beta, h0, h0_idx, fresh, cu, n_keep, snapshots, status):
         if t is not None and t.get_device() != index:
-            raise ValueError(f"{name} must be on {dev} (got {t.device})")
+            raise ValueError(f"all operands must be on {dev} (got {tuple(t.shape)} {t.dtype} on {t.device})")
     q, q_s, q_p = _tokens(q, torch.bfloat16, qs, Hk * K, 8, "q")
     k, k_s, k_p = _tokens(k, torch.bfloat16, qs, Hk * K, 8, "k")
     v, v_s, v_p = _tokens(v, torch.bfloat16, (B, T, Hv, V), Hv * V, 8, "v")
@@ -142,8 +144,10 @@ def gated_delta(q, k, v, g, beta, state=None, *, cu_seqlens=None, scale=None, qk
 def _pool(q, k, v, g, beta, pool, slots, cu_seqlens, n_keep, fresh, scale, qk_norm, final, store_o, snapshots, status, token_len):
     N = q.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1
     K, Hv, V = q.shape[3], v.shape[2], v.shape[3]
-    _require(pool, "pool", torch.float32, (None, Hv, K, V))
-    _require(slots, "slots", torch.int64, (N,))
+    if pool.dtype is not torch.float32 or pool.shape[1:] != (Hv, K, V) or not pool.is_contiguous():
+        _require(pool, "pool", torch.float32, (None, Hv, K, V))
+    if slots.dtype is not torch.int64 or slots.shape != (N,) or not slots.is_contiguous():
+        _require(slots, "slots", torch.int64, (N,))
     if cu_seqlens is not None:
         _require(cu_seqlens, "cu_seqlens", torch.int32, (None,))
     if n_keep is not None:
@@ -193,12 +197,14 @@ def gated_delta_pool_(q, k, v, g, beta, pool, slots, *, cu_seqlens=None, n_keep=
     into=SlotCaches((pool, 0))), or, on the pool as it was before, a call with n_keep=n, store_o=False on the same operands: where
     token by token, the same bits.
     Returns o like v (None when store_o is False).  Under torch.compile or another tracer it is the registered op
-    rwkv_next_amd::gated_delta_pool_; an eager call goes straight to the library, as dense_matmul's (the dispatch of an op took 15 of
+    rwkv_next_amd::gated_delta_pool_; an eager call goes straight to the library, as dense_matmul's (the dispatch of an op took 12 of
     a single token's 27 us)."""
     cu, N = _rows(q, cu_seqlens)
     dev = q.device
-    sl = _index_tensor(slots, dev, torch.int64, "slots")
-    nk = _index_tensor(n_keep, dev, torch.int64, "n_keep")
+    sl = slots
+    if type(slots) is not Tensor or slots.dtype is not torch.int64 or slots.device != dev or not slots.is_contiguous():
+        sl = _index_tensor(slots, dev, torch.int64, "slots")
+    nk = None if n_keep is None else _index_tensor(n_keep, dev, torch.int64, "n_keep")
     fr = None
     if fresh is not None:
         fr = fresh if isinstance(fresh, Tensor) and fresh.device == dev else torch.as_tensor(fresh, device=dev)
@@ -208,8 +214,10 @@ def gated_delta_pool_(q, k, v, g, beta, pool, slots, *, cu_seqlens=None, n_keep=
     traced = torch.compiler.is_compiling() or type(pool) is not Tensor or torch._C._len_torch_dispatch_stack() > 0
     o = (gated_delta_pool_op if traced else _pool)(q, k, v, g, beta, pool, sl, cu, nk, fr, scale, bool(qk_norm), final, store_o,
                                                    snapshots, status, int(token_len))
-    if not traced:
-        for t in (pool if final else None, snapshots, status):
+    if not traced:  # written in place, as autograd is told
+        if final and not pool.is_inference():
+            _increment_version(pool)
+        for t in (snapshots, status):
             if t is not None and not t.is_inference():
-                torch.autograd.graph.increment_version(t)  # written in place
+                _increment_version(t)
     return o if store_o else None

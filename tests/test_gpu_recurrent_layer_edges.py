@@ -128,6 +128,19 @@ def test_an_eager_call_is_the_op(T):
     assert not got.requires_grad and _same(got, o) and _same(four, one)
 
 
+def test_indices_of_any_kind():
+    """Slots as a list, of another type, strided: taken as they are meant."""
+    from rwkv_next_amd.kernels import gated_delta_pool_
+    ops = [x.reshape(2, 3, *x.shape[2:]) for x in _inputs(6, 1, 2, 64, 64, 1)]
+    was = torch.randn(4, 2, 64, 64, device=DEV)
+    want = was.clone()
+    o = gated_delta_pool_(*ops, want, torch.tensor([3, 1], device=DEV), qk_norm=True, n_keep=torch.tensor([2, 3], device=DEV))
+    for slots in ([3, 1], torch.tensor([3, 1]), torch.tensor([3, 1], device=DEV, dtype=torch.int32),
+                  torch.tensor([3, 7, 1, 7], device=DEV)[::2]):
+        pool = was.clone()
+        assert torch.equal(gated_delta_pool_(*ops, pool, slots, qk_norm=True, n_keep=[2, 3])[1], o[1]) and torch.equal(pool, want)
+
+
 def test_caches_that_share_memory():
     from rwkv_next_amd.kernels import SlotCaches
     gen = torch.Generator(device=DEV).manual_seed(3)
