@@ -85,13 +85,6 @@ __device__ __forceinline__ f4 load4(const void* x, int dtype, int64_t at) {
     return f4{(float)x16[0], (float)x16[1], (float)x16[2], (float)x16[3]};
 }
 __device__ __forceinline__ void finish4(const Params& p, int64_t row, int64_t n, f4 x) {
-    if (!p.fours) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (n + r < p.N) finish(p, row, n + r, x[r]);
-        return;
-    }
-    if (n >= p.N) return;
     if (p.bias) x += load4(p.bias, p.bias_dtype, n);
     if (p.activation != DENSE_NONE)
 #pragma unroll

@@ -167,27 +167,47 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void dense_tile_kernel(const Param
                 for (int t = 0; t < NT; ++t)
                     *reinterpret_cast<f4*>(mine + (i % kAtOnce * 16 + col) * kPitch + 16 * t + 4 * quad) = acc[i][t];
         wkv7::wave_lds_sync();
-#pragma unroll 1
+        if (p.parts == 1 && !p.fours) {  // a column a lane
+#pragma unroll 4
+            for (int e = lane; e < kAtOnce * 256 * NT; e += 64) {
+                const int r = e / (16 * NT), c = e % (16 * NT);
+                const int64_t m = row0 + 16 * g * kAtOnce + r, n = (int64_t)strip0 * kStrip + c;
+                if (m < p.M && n < p.N) finish(p, m, n, mine[r * kPitch + c]);
+            }
+            continue;
+        }
+#pragma unroll 2
         for (int e = lane; e < kAtOnce * 64 * NT; e += 64) {
             const int r = e / (4 * NT), c = e % (4 * NT) * 4;
             const int64_t m = row0 + 16 * g * kAtOnce + r, n = (int64_t)strip0 * kStrip + c;
             const f4 x = *reinterpret_cast<const f4*>(mine + r * kPitch + c);
-            if (m < p.M) {
+            if (m < p.M && n < p.N) {
                 if (p.parts == 1)
                     finish4(p, m, n, x);
-                else if (n < p.N)
+                else
                     *reinterpret_cast<f4*>(p.sums + (part * (int64_t)p.M + m) * sums_row(p.N) + n) = x;
             }
         }
     }
 }
 
-// The parts of a split product, added in their order, four columns a thread.
+// The parts of a split product, added in their order, four columns a thread, or one.
 __global__ __launch_bounds__(256) void dense_join_kernel(const Params p) {
     const int64_t pitch = sums_row(p.N), fours = pitch / 4, all = p.M * fours;
+    if (!p.fours) {
+        for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < (int64_t)p.M * p.N; e += (int64_t)gridDim.x * 256) {
+            const int64_t m = e / p.N, n = e % p.N;
+            float x = 0.f;
+#pragma unroll 4
+            for (int i = 0; i < p.parts; ++i) x += p.sums[(i * (int64_t)p.M + m) * pitch + n];
+            finish(p, m, n, x);
+        }
+        return;
+    }
     for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < all; e += (int64_t)gridDim.x * 256) {
         const float* const at = p.sums + e * 4;
         f4 x = *reinterpret_cast<const f4*>(at);
+#pragma unroll 4
         for (int i = 1; i < p.parts; ++i) x += *reinterpret_cast<const f4*>(at + (int64_t)i * p.M * pitch);
         finish4(p, e / fours, e % fours * 4, x);
     }
