@@ -409,7 +409,8 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(const Params p, cons
     const uint32_t group = blockIdx.x / 8 / each * 8 + blockIdx.x % 8, in = blockIdx.x / 8 % each;
     const int64_t unit = (int64_t)group * w.together + in / slices;
     if (unit >= (int64_t)(p.cu ? w.order[0] : p.num_seqs) * p.Hv) return;
-    const int n = p.cu ? w.order[1 + (int)(unit / p.Hv)] : (int)(unit / p.Hv), h = (int)(unit % p.Hv), hk = h / p.share, col0 = (int)(in % slices) * 16 * NT;
+    const int n = p.cu ? w.order[1 + (int)(unit / p.Hv)] : (int)(unit / p.Hv), h = (int)(unit % p.Hv), hk = h / p.share;
+    const int col0 = (int)(in % slices) * 16 * NT;
     int64_t first;
     int len;
     extent(p, n, first, len);

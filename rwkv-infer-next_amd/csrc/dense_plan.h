@@ -54,19 +54,19 @@ inline Plan plan_of(int32_t M, int32_t N, int32_t K, Shape shape, int64_t parts)
 }
 
 // Measured with weights cycled past the caches, bf16, us.
-// Little work, of any number of rows: tiles of 16 x 16 while two workgroups a CU hold them all (and, of more
-// than 16 rows, read little), in parts where there are fewer and K is long (one row, K = N = 4096 10.7 / 12.3 by 32 x 64 in parts; 16 rows, N =
-// 8192 16.3 / 18.3 by 16 x 64; 64 rows, K = N = 768 4.3 / 5.5; 256 rows, K = 4096, N = 320 8.5 / 9.6; but 16 rows, K = 2560, N = 10240,
-// 640 tiles, 16.2 / 14.2).
+// Little work, of any number of rows: tiles of 16 x 16 while two workgroups a CU hold them all (and, of more than 16 rows, read little),
+// in parts where there are fewer and K is long (one row, K = N = 4096 10.7 / 12.3 by 32 x 64 in parts; 16 rows, N = 8192 16.3 / 18.3 by
+// 16 x 64; 64 rows, K = N = 768 4.3 / 5.5; 256 rows, K = 4096, N = 320 8.5 / 9.6; but 16 rows, K = 2560, N = 10240, 640 tiles, 16.2 /
+// 14.2; 64 rows, K = 10240, N = 2560 36.9 / 20.0 by 64 x 64).
 // Up to 64 rows: of the tiles of 64 columns the one of fewest rows of which every CU gets one at most (32 rows, K = 4096, N = 8192 17.8
 // by 16 / 19.2 by 32; N = 16384 30.9 / 29.0; 64 rows 37.2 by 32 / 32.4 by 64); of long K, where A's and the weight's bytes count for
 // more, as many rows as there are, in parts (K = 10240, N = 2560, 64 rows 20.0 by 64 / 26.6 by 16).
 // More rows, short K, few tiles: the same (192 rows, K = N = 2560 13.3 / 17.1 by 128 x 128; but K = N = 4096 25.2 / 21.8).
-// Else 128 x 128 or 128 x 256, and 64 x 64 for narrow products of long K (413 rows, K = 6400, N = 586 19.8 / 30.9 by 128 x 128): up to
-// 128 rows or K = 1024 not 128 x 256 (K = 4096, N = 16384, 128 rows 38.0 / 41.1; K = 768, 512 rows 26.9 /
-// 33.7), of more the cheaper by what a step of one takes, alone on a CU or not, and what adding the parts does (K = N = 4096, 256 rows
-// 23.2 / 25.7, 1000 rows 49.0 / 44.1; K = 5952, N = 1588, 2459 rows 97.7 whole, 65.6 in three parts; K = 10240, N = 2560, 512 rows 45.1 / 40.5; K = 2560, N = 10240, 2048 rows 107 / 127; K = 4096, N =
-// 16384, 2048 rows 253 / 240).
+// Else 128 x 128 or 128 x 256, and 64 x 64 for narrow products of long K (75 rows, K = 7872, N = 1003 19.4 / 21.7 by 128 x 128): up to 128
+// rows or K = 1024 not 128 x 256 (K = 4096, N = 16384, 128 rows 38.0 / 41.1; K = 768, 512 rows 26.9 / 33.7), else the cheapest by what a
+// step of one takes, alone on a CU or not, and what adding the parts does (K = N = 4096, 256 rows 23.2 / 25.7, 1000 rows 49.0 / 44.1;
+// K = 5952, N = 1588, 2459 rows 97.7 whole, 65.6 in three parts; K = 10240, N = 2560, 512 rows 45.1 / 40.5; K = 2560, N = 10240, 2048
+// rows 107 / 127; K = 4096, N = 16384, 2048 rows 253 / 240).
 inline Plan plan(int32_t M, int32_t N, int32_t K, int cus) {
     const auto tiles = [&](Shape s) {
         return ((int64_t)M + kTiles[s].rows - 1) / kTiles[s].rows * (((int64_t)N + kTiles[s].columns - 1) / kTiles[s].columns);
