@@ -6,6 +6,8 @@
  *   S_t = a_t S_{t-1} + k_t d_t^T,   d_t = beta_t (v_t - a_t S_{t-1}^T k_t),   a_t = exp(g_t)
  *   o_t = scale S_t^T q_t
  * With qk_norm, q and k are divided by sqrt(sum of squares + 1e-6) first.  States and sums are fp32.
+ * A value of token t that is not finite makes o from t on and the final state not finite, in its column (v) or head (k, g, beta); in q,
+ * o of t alone.  Tokens before t, other columns, heads and sequences have the results that they have without it.
  *
  * Return codes are the WKV7_* codes of wkv7.h.  No call allocates or synchronises; all can be recorded into a HIP graph.
  */

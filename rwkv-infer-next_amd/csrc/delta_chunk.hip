@@ -8,6 +8,10 @@
 // Two launches: one makes T, B and the tokens' factors of every chunk, all chunks at once; the other goes through a row's chunks in
 // order.  Norms, decays and beta are factors of rows, kept apart from the products, whose one operand is so the caller's bf16, exact.
 // The other, fp32, is split into three bf16 parts, 24 bits, wherever it leads to the state; the outputs, bf16, take two parts.
+// A product with a triangle multiplies the zeros above its diagonal too, and 0 times an infinity or NaN of a later token is NaN for an
+// earlier one.  So on the way to T 0 goes in the place of what is out of range, and from the first token that had such a value, R is
+// NaN.  In the scan the state of R's column is then NaN, as it is token by token; outputs that came out of range are made again, by the
+// wavefronts which make them, without the tokens that cannot have a part in them.
 // Measured, 4096 tokens, 16 query/key and 32 value heads of 128: 35 to 38 us and 95 us (token by token 5.4 ms).
 #include "delta_device.h"
 
@@ -29,6 +33,7 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 constexpr int kRow = 68;           // floats between rows of a matrix in LDS: 16-byte reads of 16 rows meet no bank twice
+constexpr float kMost = 3.3895314e38f;  // the largest bf16: no part of what is within is infinite
 constexpr float kLeast = -1e4f;    // decays below e^-10000 are 0 all the same, and differences of their sums stay finite
 
 // Of a 64 x 64 lower triangle in blocks of 16 x 32: tile t = 0, 1 has one, tile 2, 3 have two.
@@ -70,6 +75,31 @@ __device__ __forceinline__ void split3(float x0, float x1, uint32_t& a, uint32_t
     const f2 y = {__builtin_amdgcn_fdot2_f32_bf16(h, m0, x0, false), __builtin_amdgcn_fdot2_f32_bf16(h, m1, x1, false)};
     a = __builtin_bit_cast(uint32_t, h);
     wkv7::split_pair(y[0], y[1], b, c);
+}
+
+// split3 of two tokens' values, of which the later, x1, reaches no part of x0: where it is infinite or NaN, split3's products with 0 do.
+__device__ __forceinline__ void split3_in_order(float x0, float x1, uint32_t& a, uint32_t& b, uint32_t& c) {
+    typedef wkv7::f2_t f2;
+    const wkv7::bf16x2_t m1 = wkv7::bf16_pair_in_register(0xBF800000u);
+    const auto rest = [&](f2 x, uint32_t& part) {
+        const wkv7::bf16x2_t h = __builtin_convertvector(x, wkv7::bf16x2_t);
+        part = __builtin_bit_cast(uint32_t, h);
+        return f2{x[0] - __uint_as_float(part << 16), __builtin_amdgcn_fdot2_f32_bf16(h, m1, x[1], false)};
+    };
+    const f2 z = rest(rest(f2{x0, x1}, a), b);
+    c = wkv7::pack_bf16x2(z[0], z[1]);
+}
+
+__device__ __forceinline__ bool within(float x) { return fabsf(x) <= kMost; }  // false for NaN
+__device__ __forceinline__ bool within(f4 x) { return within(x[0]) && within(x[1]) && within(x[2]) && within(x[3]); }
+// x, whose elements belong to the tokens from `token` on, with 0 for what is not within, whose first token *first learns.
+__device__ __forceinline__ f4 kept(f4 x, int token, int* first) {
+    if (!within(x)) {
+        atomicMin(first, token + (!within(x[0]) ? 0 : !within(x[1]) ? 1 : !within(x[2]) ? 2 : 3));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = within(x[r]) ? x[r] : 0.f;
+    }
+    return x;
 }
 
 // x of the lane that DPP control `kCtrl` names, 0 where there is none or the row of 16 lanes is not in `kRows`
@@ -125,6 +155,7 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, cons
     __shared__ __attribute__((aligned(16))) float bm[64 * kRow];   // Q's tile, then products on the way to T
     __shared__ __attribute__((aligned(16))) double cs[64];
     __shared__ __attribute__((aligned(16))) float rk[64], rq[64], be[64];
+    __shared__ int lost;  // the first token whose row of A or T is not within
     float* const mm = bm;
     static_assert(64 * kPitch * 2 <= (int)sizeof(bm), "");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -255,19 +286,23 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, cons
             f[64 + lane] = beta * gamma * rk[lane];
             f[128 + lane] = __builtin_amdgcn_exp2f((float)(last - c)) * rk[lane];
             f[192 + lane] = gamma * rq[lane];
-            if (lane == 0) f[256] = __builtin_amdgcn_exp2f((float)last);
+            if (lane == 0) f[256] = __builtin_amdgcn_exp2f((float)last), lost = kChunk;
         }
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (j <= wave) {
-                const int col = 16 * j + row;
+                const int col = 16 * j + row, i0 = 16 * wave + 4 * quad;
+                f4 x;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * wave + 4 * quad + r;
+                    const int i = i0 + r;
                     const float decay = i > col ? __builtin_amdgcn_exp2f((float)(cs[i] - cs[col])) * rk[col] : 0.f;
-                    am[i * kRow + col] = i > col ? kk[j][r] * (be[i] * rk[i]) * decay : 0.f;
+                    x[r] = i > col ? kk[j][r] * (be[i] * rk[i]) * decay : 0.f;
                 }
+                x = kept(x, i0, &lost);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) am[(i0 + r) * kRow + col] = x[r];
             }
         {  // B, in two bf16 parts: the rows of a K Q^T that a lane has are its operand of B D
             const int i = token_of(wave, row);
@@ -313,6 +348,13 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, cons
                 x[i] = s0 + s1;
                 if (i == 7 || i == 11) __builtin_amdgcn_sched_barrier(0);  // a few rows of A at a time: all of them are 144 registers
             }
+            if (!within(x[15])) {  // an infinity or NaN makes all rows behind it so too
+                int first = 16 * wave + 15;
+#pragma unroll
+                for (int i = 15; i >= 0; --i)
+                    if (!within(x[i])) x[i] = 0.f, first = 16 * wave + i;
+                atomicMin(&lost, first);
+            }
             wkv7::wave_lds_sync();
 #pragma unroll
             for (int i = 0; i < 16; ++i)
@@ -342,24 +384,27 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, cons
         const f4 zero = {0.f, 0.f, 0.f, 0.f};
         // [[P, 0], [X, Q]]^-1 = [[P^-1, 0], [-Q^-1 X P^-1, Q^-1]], for blocks of 16, then of 32
         if (wave < 2) {
-            const f4 m = times(left(am, 2 * wave + 1, 2 * wave), right(am, 2 * wave, 2 * wave), zero);
-            const f4 x = times(left(am, 2 * wave + 1, 2 * wave + 1), m, zero);
+            const int token0 = 16 * (2 * wave + 1) + 4 * quad;
+            const f4 m = kept(times(left(am, 2 * wave + 1, 2 * wave), right(am, 2 * wave, 2 * wave), zero), token0, &lost);
+            const f4 x = kept(times(left(am, 2 * wave + 1, 2 * wave + 1), m, zero), token0, &lost);
             put(am, 2 * wave + 1, 2 * wave, -x);
         }
         __syncthreads();
-        const int i = wave >> 1, j = wave & 1;
+        const int i = wave >> 1, j = wave & 1, token0 = 16 * (2 + i) + 4 * quad;
         {
             f4 m = zero;
             for (int k = j; k < 2; ++k) m = times(left(am, 2 + i, k), right(am, k, j), m);
-            put(mm, i, j, m);
+            put(mm, i, j, kept(m, token0, &lost));
         }
         __syncthreads();
         {
             f4 x = zero;
             for (int k = 0; k <= i; ++k) x = times(left(am, 2 + i, 2 + k), right(mm, k, j), x);
-            put(am, 2 + i, j, -x);
+            put(am, 2 + i, j, -kept(x, token0, &lost));
         }
         __syncthreads();
+        // R of the tokens from `lost` on is NaN by its factor
+        if (wave == 0 && lane >= lost) reinterpret_cast<float*>(rec + kRecordFactors)[lane] = __builtin_nanf("");
         // T in three bf16 parts, in operand order
         for (int e = tid; e < 6 * 64; e += 256) {
             const int block = e >> 6, l = e & 63;
@@ -421,7 +466,8 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(const Params p, cons
     const char* const operands = wkv7::uniform_ptr(w.kq + (slot * p.Hk + hk) * (3 * K * kChunk * 2));
     const int64_t record_size = p.Hv * kRecord, operand_size = (int64_t)p.Hk * (3 * K * kChunk * 2);
     const bool two = wave >= 2;  // these rows of the lower triangles have a second half
-    const uint32_t at = lane * 16u, tokens_at = token_of(wave, 4 * quad) * 4u;
+    const int token0 = token_of(wave, 4 * quad);     // the first of a lane's four
+    const uint32_t at = lane * 16u, tokens_at = token0 * 4u;
 
     if (role == 1) {
         u4 q[kSteps], b[2][2];
@@ -470,16 +516,74 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(const Params p, cons
             if (p.o) {
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
-                    f4 y = (O[x][0] + O[x][1]) * gamma;
+                    u4 d[2][2];
 #pragma unroll
                     for (int half = 0; half < 2; ++half)
-                        if (half == 0 || two) {
-                            const u4 d = df[half][0][x][lane], e = df[half][1][x][lane];
-                            y = mfma(b[half][1], d, y);
-                            y = mfma(b[half][0], e, y);
-                            y = mfma(b[half][0], d, y);
+                        if (half == 0 || two) d[half][0] = df[half][0][x][lane], d[half][1] = df[half][1][x][lane];
+                    const auto output = [&] {
+                        f4 y = (O[x][0] + O[x][1]) * gamma;
+#pragma unroll
+                        for (int half = 0; half < 2; ++half)
+                            if (half == 0 || two) {
+                                y = mfma(b[half][1], d[half][0], y);
+                                y = mfma(b[half][0], d[half][1], y);
+                                y = mfma(b[half][0], d[half][0], y);
+                            }
+                        return y;
+                    };
+                    f4 y = output();
+                    if (__ballot(!within(y))) {  // D once more, from R and of D what is within; NaN from the first token that is not
+                        int lost = kChunk;
+                        const char* const t = records + c * record_size + kRecordT + at;
+                        u4 r[2][3];
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                            for (int m = 0; m < 3; ++m) r[half][m] = rf[half][m][x][lane];
+#pragma unroll
+                            for (int i = 7; i >= 0; --i)
+                                if (!within(bf16_at(r[half][0], i)) || !within(bf16_at(r[half][1], i)) || !within(bf16_at(r[half][2], i))) {
+                                    lost = min(lost, 32 * half + 8 * quad + i);
+#pragma unroll
+                                    for (int m = 0; m < 3; ++m) r[half][m][i / 2] &= i & 1 ? 0xFFFFu : 0xFFFF0000u;
+                                }
                         }
-                    const int t0 = c * kChunk + token_of(wave, 4 * quad);
+#pragma unroll
+                        for (int tile = 0; tile < 4; ++tile) {
+                            f4 D[3] = {zero, zero, zero};
+#pragma unroll
+                            for (int half = 0; half < 2; ++half)
+                                if (half == 0 || tile >= 2) {
+                                    u4 tri[3];
+#pragma unroll
+                                    for (int m = 0; m < 3; ++m)
+                                        tri[m] = *reinterpret_cast<const u4*>(t + (block_of(tile, half) * 3 + m) * 1024);
+                                    D[2] = mfma(tri[2], r[half][0], D[2]);
+                                    D[1] = mfma(tri[1], r[half][0], D[1]);
+                                    D[0] = mfma(tri[0], r[half][0], D[0]);
+                                    D[2] = mfma(tri[0], r[half][2], D[2]);
+                                    D[1] = mfma(tri[0], r[half][1], D[1]);
+                                    D[2] = mfma(tri[1], r[half][1], D[2]);
+                                }
+                            f4 z = D[0] + (D[1] + D[2]);
+#pragma unroll
+                            for (int i = 3; i >= 0; --i)
+                                if (!within(z[i])) z[i] = 0.f, lost = min(lost, token_of(tile, 4 * quad) + i);
+#pragma unroll
+                            for (int m = 0; m < 2; ++m) {
+                                uint32_t i, j;
+                                wkv7::split_pair(z[2 * m], z[2 * m + 1], i, j);
+                                d[tile >> 1][0][2 * (tile & 1) + m] = i, d[tile >> 1][1][2 * (tile & 1) + m] = j;
+                            }
+                        }
+                        lost = min(lost, __shfl_xor(lost, 16));
+                        lost = min(lost, __shfl_xor(lost, 32));
+                        y = output();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (token0 + i >= lost) y[i] = __builtin_nanf("");
+                    }
+                    const int t0 = c * kChunk + token0;
                     uint16_t* const to = p.o + (first + t0) * p.o_stride + ((int64_t)h * p.V + col0 + 16 * x + col);
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
@@ -615,7 +719,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(const Params p, cons
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 uint32_t i, j, l;
-                split3(R[2 * m], R[2 * m + 1], i, j, l);
+                split3_in_order(R[2 * m], R[2 * m + 1], i, j, l);
                 a[m] = i, b[m] = j, d[m] = l;
             }
             reinterpret_cast<u2*>(&rf[wave >> 1][0][x][lane])[wave & 1] = a;

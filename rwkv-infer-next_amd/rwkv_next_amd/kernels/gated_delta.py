@@ -11,7 +11,8 @@ Per value head h, with query/key head h // (Hv // Hk) and the state S (K x V, fp
 
 Layouts: q, k (B, T, Hk, K) and v (B, T, Hv, V) bfloat16, parts of one projection's result or tensors of their own (the strides
 between tokens are free); g (B, T, Hv) log decays <= 0 and beta (B, T, Hv), float32; states (N, Hv, K, V) float32; o like v.
-K is 64 or 128, V a multiple of 16 up to 256, Hv a multiple of Hk.  Inference only: there is no backward pass.  Every call runs on
+K is 64 or 128, V a multiple of 16 up to 256, Hv a multiple of Hk.  A value that is not finite reaches its own token and later ones of
+its column (v) or head (k, g, beta), nothing else.  Inference only: there is no backward pass.  Every call runs on
 the current stream, no host sync, and can be recorded into a HIP graph.
 """
 from __future__ import annotations
