@@ -43,14 +43,29 @@ def _apart(a, slots_a, b, slots_b):
 
 class SlotCaches:
     """A model's cache tensors that share their slots.  Each argument is a tensor (layers, slots, ..) or (tensor, dim) with dim 0 for
-    (slots, ..) and 1 for (layers, slots, ..); a slot's part of a layer is contiguous.  At most 16 tensors, of any types."""
+    (slots, ..) and 1 for (layers, slots, ..); a slot's part of a layer is contiguous.  At most 16 tensors, of any types.  A tensor that
+    is given other memory or another shape later (t.data = .., set_, resize_) is taken as it is at a call."""
 
     def __init__(self, *caches):
         if not 1 <= len(caches) <= _lib.SLOTS_MAX_CACHES:
             raise ValueError(f"SlotCaches takes 1 to {_lib.SLOTS_MAX_CACHES} tensors (got {len(caches)})")
+        self._caches = [x if isinstance(x, tuple) else (x, 1) for x in caches]
+        self._lay_out()
+
+    def _places(self):
+        """What the layout follows from, of every tensor."""
+        return [(t.data_ptr(), t.shape, t.stride(), t.dtype, t.get_device()) for t, _ in self._caches]
+
+    def _current(self):
+        """Before every call: addresses are those that the tensors have now."""
+        if self._places() != self._laid:
+            self._lay_out()
+
+    def _lay_out(self):
+        places = self._places()
+        self._laid = None  # until all is found right
         self._rows, self.slots, self.device, self._shared = [], None, None, False
-        for x in caches:
-            t, dim = x if isinstance(x, tuple) else (x, 1)
+        for t, dim in self._caches:
             if dim not in (0, 1) or t.dim() <= dim:
                 raise ValueError(f"the slots are dimension 0 or 1 of a cache (got dimension {dim} of {tuple(t.shape)})")
             if not t.is_cuda:
@@ -76,6 +91,7 @@ class SlotCaches:
             self._rows.append((t, layer, slot, row, layers))
             self._shared |= not all(_apart(self._rows[-1], self.slots, x, self.slots) for x in self._rows[:-1])
         self._own = self._pairs(self)
+        self._laid = places
 
     def _pairs(self, other):
         a = (_lib.SlotsCache * len(self._rows))()
@@ -111,6 +127,7 @@ class SlotCaches:
         before any destination is written: swaps and chains are exact.  A source may be named any number of times; of equal
         destinations the last one counts.  A negative index leaves its entry out, one past the slots does too and sets
         SLOTS_STATUS_SLOT in `status`.  At most 1024 entries."""
+        self._current()
         src, dst = self._index(src, "src"), self._index(dst, "dst")
         n = src.numel()
         if n != dst.numel():
@@ -120,6 +137,7 @@ class SlotCaches:
         a, to = self._own, self.slots
         self._require_apart()
         if into is not None and into is not self:
+            into._current()
             into._require_apart()
             if into.device != self.device or len(into._rows) != len(self._rows):
                 raise ValueError(f"into must be {len(self._rows)} caches on {self.device}")
@@ -134,6 +152,7 @@ class SlotCaches:
 
     def free_slots(self, idx, *, status=None) -> None:
         """Slot idx[i] = 0 in every cache, indices as in copy_slots.  At most 65535."""
+        self._current()
         idx = self._index(idx, "idx")
         if idx.numel() > 65535:
             raise ValueError(f"at most 65535 slots per call (got {idx.numel()})")
@@ -145,6 +164,7 @@ class SlotCaches:
         """Moves the live slots to the front: with k the number of live ones (live (S,) bool), those at k and behind go, in their
         order, to the free ones before k, in theirs.  Returns (where, count): where (S,) int64 a slot's place after, -1 for a free
         one, count (1,) int32 k, both on the device.  Slots that nothing moves to keep what they hold (free_slots zeroes)."""
+        self._current()
         if not isinstance(live, torch.Tensor) or live.device != self.device or live.dtype not in (torch.bool, torch.uint8) or \
                 live.shape != (self.slots,):
             raise ValueError(f"live must be a bool ({self.slots},) tensor on {self.device}")

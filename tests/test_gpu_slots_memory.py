@@ -1,0 +1,105 @@
+"""SlotCaches whose tensors are given other memory or another shape after it was made: every call takes them as they are."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+def _idx(*x):
+    return torch.tensor(x, device=DEV)
+
+
+def _fresh(*n):
+    return torch.arange(1, torch.Size(n).numel() + 1, device=DEV, dtype=torch.float32).view(n)
+
+
+@pytest.mark.parametrize("how", ["data", "set_", "resize_", "storage"])
+def test_other_memory_is_followed(how):
+    from rwkv_next_amd.kernels import SlotCaches
+    t, u = _fresh(3, 6, 8), _fresh(6, 5)
+    caches = SlotCaches(t, (u, 0))
+    keep = t.detach()  # the old memory stays, so that a write to it would show
+    was = keep.clone()
+    if how == "data":
+        t.data = _fresh(3, 6, 8) * 2
+    elif how == "set_":
+        t.set_(_fresh(3, 6, 8) * 2)
+    elif how == "resize_":
+        keep, was = None, None
+        t.resize_(4, 6, 8)  # more layers: memory of its own, larger
+        t.copy_(_fresh(4, 6, 8))
+    else:
+        keep, was = None, None
+        t.untyped_storage().resize_(2 * t.untyped_storage().nbytes())
+        t.copy_(_fresh(3, 6, 8))
+    want, other = t.clone(), u.clone()
+    want[:, 1], other[1] = t[:, 4], u[4]
+    caches.copy_slots(_idx(4), _idx(1))
+    assert torch.equal(t, want) and torch.equal(u, other)
+    want[:, 5], other[5] = 0, 0
+    caches.free_slots(_idx(5))
+    assert torch.equal(t, want) and torch.equal(u, other)
+    live = torch.tensor([False, True, True, True, True, False], device=DEV)
+    want[:, 0], other[0] = t[:, 4], u[4]
+    where, count = caches.compact_slots(live)
+    assert torch.equal(t, want) and torch.equal(u, other) and int(count) == 4 and where.tolist() == [-1, 1, 2, 3, 0, -1]
+    assert keep is None or torch.equal(keep, was)
+
+
+def test_other_memory_of_into_is_followed():
+    from rwkv_next_amd.kernels import SlotCaches
+    t, u = _fresh(3, 6, 8), _fresh(3, 9, 8)
+    here, there = SlotCaches(t), SlotCaches(u)
+    keep = u.detach()
+    was = keep.clone()
+    u.data = _fresh(3, 20, 8) * 2  # more slots too
+    want = u.clone()
+    want[:, 17] = t[:, 2]
+    here.copy_slots(_idx(2), _idx(17), into=there)
+    assert torch.equal(u, want) and torch.equal(keep, was) and there.slots == 20
+
+
+def test_what_no_longer_fits_is_refused():
+    from rwkv_next_amd.kernels import SlotCaches
+    t, u = _fresh(3, 6, 8), _fresh(6, 5)
+    caches = SlotCaches(t, (u, 0))
+    live = torch.ones(6, dtype=torch.bool, device=DEV)
+    calls = (lambda: caches.copy_slots(_idx(0), _idx(1)), lambda: caches.free_slots(_idx(0)), lambda: caches.compact_slots(live))
+    for bad in (_fresh(3, 7, 8), _fresh(3, 6, 16)[..., ::2], torch.zeros(3, 6, 8), _fresh(1, 6, 8).expand(3, 6, 8)):
+        t.data = bad
+        was, other = t.clone(), u.clone()
+        for call in calls:  # again and again, not the first time alone
+            with pytest.raises(ValueError):
+                call()
+        assert torch.equal(t, was) and torch.equal(u, other)
+    t.data = u.view(1, 6, 5)  # the other cache's memory
+    for call in (calls[0], calls[2]):
+        with pytest.raises(ValueError, match="share memory"):
+            call()
+    t.data = _fresh(3, 6, 8)
+    for call in calls:
+        call()
+    assert not t[:, 0].any() and not u[0].any() and torch.equal(t[:, 1], _fresh(3, 6, 8)[:, 0])
+
+
+def test_a_captured_call_keeps_the_memory_of_its_capture():
+    """A graph holds addresses, as torch's own do: later memory is taken by later calls."""
+    from rwkv_next_amd.kernels import SlotCaches
+    t = _fresh(2, 4, 8)
+    caches = SlotCaches(t)
+    src, dst = _idx(0), _idx(3)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        caches.copy_slots(src, dst)
+    keep = t.detach()
+    t.data = _fresh(2, 4, 8) * 3
+    new = t.clone()
+    for _ in range(3):
+        keep.copy_(_fresh(2, 4, 8))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(keep[:, 3], keep[:, 0]) and torch.equal(t, new)
+    caches.copy_slots(src, dst)
+    assert torch.equal(t[:, 3], new[:, 0])
