@@ -41,6 +41,9 @@ def _apart(a, slots_a, b, slots_b):
     return slots_a <= first and (first + slots_b) * slot <= outer
 
 
+_increment_version = torch.autograd.graph.increment_version
+
+
 class SlotCaches:
     """A model's cache tensors that share their slots.  Each argument is a tensor (layers, slots, ..) or (tensor, dim) with dim 0 for
     (slots, ..) and 1 for (layers, slots, ..); a slot's part of a layer is contiguous.  At most 16 tensors, of any types.  A tensor that
@@ -111,6 +114,12 @@ class SlotCaches:
             raise ValueError(f"{name} must be an int64 tensor of one dimension (got {x.dtype} {tuple(x.shape)})")
         return x.contiguous()
 
+    def _written(self):
+        """In place, as autograd is told."""
+        for t, _ in self._caches:
+            if not t.is_inference():
+                _increment_version(t)
+
     def _require_apart(self):
         if self._shared:
             raise ValueError("caches whose slots move must not share memory with each other")
@@ -149,6 +158,7 @@ class SlotCaches:
         with on_device(self.device):
             _lib.check(_lib.load().slots_copy(a, len(a), src.data_ptr(), dst.data_ptr(), n, self.slots, to,
                                               self._status(status), stream_handle(self.device)))
+        (self if into is None else into)._written()
 
     def free_slots(self, idx, *, status=None) -> None:
         """Slot idx[i] = 0 in every cache, indices as in copy_slots.  At most 65535."""
@@ -159,6 +169,7 @@ class SlotCaches:
         with on_device(self.device):
             _lib.check(_lib.load().slots_free(self._own, len(self._own), idx.data_ptr(), idx.numel(), self.slots,
                                               self._status(status), stream_handle(self.device)))
+        self._written()
 
     def compact_slots(self, live):
         """Moves the live slots to the front: with k the number of live ones (live (S,) bool), those at k and behind go, in their
@@ -177,4 +188,5 @@ class SlotCaches:
         with on_device(self.device):
             _lib.check(_lib.load().slots_compact(self._own, len(self._own), live.data_ptr(), self.slots, where.data_ptr(),
                                                  count.data_ptr(), stream_handle(self.device)))
+        self._written()
         return where, count

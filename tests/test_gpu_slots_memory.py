@@ -103,3 +103,25 @@ def test_a_captured_call_keeps_the_memory_of_its_capture():
         assert torch.equal(keep[:, 3], keep[:, 0]) and torch.equal(t, new)
     caches.copy_slots(src, dst)
     assert torch.equal(t[:, 3], new[:, 0])
+
+
+def test_autograd_is_told_of_what_is_written():
+    from rwkv_next_amd.kernels import SlotCaches
+    t, u, v = _fresh(2, 4, 8), _fresh(4, 3), _fresh(2, 9, 8)
+    caches, other = SlotCaches(t, (u, 0)), SlotCaches(v, (_fresh(9, 3), 0))
+    live = torch.tensor([False, True, True, False], device=DEV)
+    for call in (lambda: caches.copy_slots(_idx(0), _idx(1)), lambda: caches.free_slots(_idx(3)), lambda: caches.compact_slots(live)):
+        w = torch.ones(2, 4, 8, device=DEV, requires_grad=True)
+        versions = t._version, u._version
+        y = (w * t).sum()
+        call()
+        assert t._version > versions[0] and u._version > versions[1]
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    versions = t._version, u._version, v._version
+    caches.copy_slots(_idx(0), _idx(8), into=other)  # read alone
+    assert (t._version, u._version) == versions[:2] and v._version > versions[2]
+    with torch.inference_mode():  # inference tensors have no counter
+        SlotCaches(_fresh(2, 4, 8)).copy_slots(_idx(0), _idx(1))
+        caches.free_slots(_idx(0))
+    assert not t[:, 0].any()
