@@ -11,7 +11,7 @@ constexpr int kClashRows = 1024;
 struct Plan {
     bool tokens, chunks;
     int32_t token_len;
-    int64_t slots;
+    int64_t slots, rows;  // of the workspace; that can run by chunks
     size_t bytes;
 };
 Plan make_plan(const delta_args* a) {
@@ -21,7 +21,8 @@ Plan make_plan(const delta_args* a) {
     pl.chunks = !a->snapshots && longest > pl.token_len;
     pl.tokens = !pl.chunks || a->cu_seqlens;
     if (pl.chunks) {
-        pl.slots = delta::chunk_slots(a->num_seqs, a->T, a->total_tokens, a->cu_seqlens != nullptr);
+        pl.slots = delta::chunk_slots(a->num_seqs, a->T, a->total_tokens, pl.token_len, a->cu_seqlens != nullptr).count;
+        pl.rows = a->cu_seqlens ? delta::long_rows(a->num_seqs, a->total_tokens, pl.token_len) : a->num_seqs;
         pl.bytes = delta::chunk_workspace(pl.slots, a->num_seqs, a->Hk, a->Hv, a->K);
     }
     return pl;
@@ -104,7 +105,7 @@ int delta_run(const delta_args* a, void* stream) {
     const delta::Plan pl = delta::make_plan(a);
     if (pl.bytes && (!a->workspace || a->workspace_bytes < pl.bytes)) return WKV7_ERR_WORKSPACE;
     if (pl.bytes && !delta::aligned(a->workspace, 256)) return WKV7_ERR_ALIGN;
-    if (pl.chunks && (pl.slots * a->Hk >= 0xFFFFFF || delta::chunk_groups(a->num_seqs, a->Hv, a->V) > 0x7FFFFF))
+    if (pl.chunks && (pl.slots * a->Hk >= 0xFFFFFF || delta::chunk_groups(pl.rows, a->Hv, a->V) > 0x7FFFFF))
         return WKV7_ERR_SHAPE;  // work-items of a launch below 2^32
     delta::Params p;
     p.q = a->q, p.k = a->k, p.v = a->v, p.q_stride = a->q_stride, p.k_stride = a->k_stride, p.v_stride = a->v_stride;

@@ -42,26 +42,25 @@ __device__ __forceinline__ constexpr int block_of(int tile, int half) { return t
 // are eight tokens in a row: a result is the next product's operand without an exchange between lanes.  Rows of the state too.
 __device__ __forceinline__ int token_of(int tile, int row) { return 32 * (tile >> 1) + 8 * (row >> 2) + 4 * (tile & 1) + (row & 3); }
 
-// Which row and chunk a slot of the workspace holds; false for a slot that holds none.  Ragged rows begin at slot
-// cu[n] / 64 + n, which leaves each one room enough.
-__device__ __forceinline__ int64_t first_slot(const Params& p, int n, int64_t first) {
-    return p.cu ? first / kChunk + n : (int64_t)n * ((p.T + kChunk - 1) / kChunk);
+// Which row and chunk a slot of the workspace holds; false for a slot that holds none.
+__device__ __forceinline__ int64_t first_slot(const Params& p, const Work& w, int n, int64_t first) {
+    return p.cu ? ragged_slot(w.shift, w.rows, n, first) : (int64_t)n * ((p.T + kChunk - 1) / kChunk);
 }
-__device__ __forceinline__ bool locate(const Params& p, int64_t slot, int& n, int64_t& first, int& len, int& chunk) {
+__device__ __forceinline__ bool locate(const Params& p, const Work& w, int64_t slot, int& n, int64_t& first, int& len, int& chunk) {
     if (p.cu) {
         int lo = 0, hi = p.num_seqs;
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
             int64_t s = p.cu[mid];
             s = s < 0 ? 0 : s > p.total_tokens ? p.total_tokens : s;
-            if (s / kChunk + mid <= slot) lo = mid; else hi = mid;
+            if (ragged_slot(w.shift, w.rows, mid, s) <= slot) lo = mid; else hi = mid;
         }
         n = lo;
     } else {
         n = (int)(slot / ((p.T + kChunk - 1) / kChunk));
     }
     extent(p, n, first, len);
-    const int64_t c = slot - first_slot(p, n, first);
+    const int64_t c = slot - first_slot(p, w, n, first);
     chunk = (int)c;
     return c >= 0 && c * kChunk < len && !(p.cu && len <= p.token_len);
 }
@@ -168,7 +167,7 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, cons
     const int hk = (int)(blockIdx.x % (uint32_t)p.Hk);
     int n, len, chunk;
     int64_t first;
-    if (!locate(p, slot, n, first, len, chunk)) return;
+    if (!locate(p, w, slot, n, first, len, chunk)) return;
     first += (int64_t)chunk * kChunk;
     len = min(len - chunk * kChunk, kChunk);  // tokens of this chunk
 
@@ -460,7 +459,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(const Params p, cons
     int len;
     extent(p, n, first, len);
     const int chunks = (len + kChunk - 1) / kChunk;
-    const int64_t slot = first_slot(p, n, first);
+    const int64_t slot = first_slot(p, w, n, first);
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
     const char* const records = wkv7::uniform_ptr(w.rec + (slot * p.Hv + h) * kRecord);
     const char* const operands = wkv7::uniform_ptr(w.kq + (slot * p.Hk + hk) * (3 * K * kChunk * 2));
@@ -806,8 +805,7 @@ hipError_t launch(const Params& p, const Work& w, int64_t slots, bool wide, hipS
     hipLaunchKernelGGL(delta_prep_kernel<K>, dim3((unsigned)(slots * p.Hk + (p.cu ? 1 : 0))), dim3(256), 0, stream, p, w);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    int64_t rows = p.num_seqs;  // at most so many are longer than token_len
-    if (p.cu) rows = rows < p.total_tokens / (p.token_len + 1) ? rows : p.total_tokens / (p.token_len + 1);
+    const int64_t rows = p.cu ? long_rows(p.num_seqs, p.total_tokens, p.token_len) : p.num_seqs;
     const int64_t groups = (rows * p.Hv / w.together + 7) / 8 * 8;
     if (wide)
         hipLaunchKernelGGL((delta_scan_kernel<K, 2>), dim3((unsigned)(groups * w.together * (p.V / 32))), dim3(512), 0, stream, p, w);
@@ -818,17 +816,19 @@ hipError_t launch(const Params& p, const Work& w, int64_t slots, bool wide, hipS
 
 }  // namespace
 
-int64_t chunk_slots(int32_t num_seqs, int32_t T, int64_t total_tokens, bool ragged) {
-    return ragged ? total_tokens / kChunk + num_seqs : (int64_t)num_seqs * ((T + kChunk - 1) / kChunk);
+Slots chunk_slots(int32_t num_seqs, int32_t T, int64_t total_tokens, int32_t token_len, bool ragged) {
+    return ragged ? ragged_slots(num_seqs, total_tokens, token_len) : row_slots(num_seqs, T);
 }
-int64_t chunk_groups(int32_t num_seqs, int32_t Hv, int32_t V) { return ((int64_t)num_seqs + 7) / 8 * 8 * Hv * (V / 16); }
+int64_t chunk_groups(int64_t rows, int32_t Hv, int32_t V) { return (rows + 7) / 8 * 8 * Hv * (V / 16); }
 size_t chunk_workspace(int64_t slots, int32_t num_seqs, int32_t Hk, int32_t Hv, int32_t K) {
     return (size_t)slots * (Hk * (size_t)(3 * K * kChunk * 2) + Hv * (size_t)kRecord) + (size_t)(num_seqs + 1) * 4;
 }
 
 hipError_t launch_chunks(const Params& p, int cus, hipStream_t stream) {
-    const int64_t slots = chunk_slots(p.num_seqs, p.T, p.total_tokens, p.cu != nullptr);
+    const Slots of = chunk_slots(p.num_seqs, p.T, p.total_tokens, p.token_len, p.cu != nullptr);
+    const int64_t slots = of.count;
     Work w;
+    w.shift = of.shift, w.rows = of.rows;
     w.kq = p.workspace;
     w.rec = p.workspace + slots * p.Hk * (int64_t)(3 * p.K * kChunk * 2);
     w.order = reinterpret_cast<int32_t*>(w.rec + slots * p.Hv * kRecord);

@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include "delta.h"
+#include "delta_plan.h"
 #include "wkv7_device.h"
 
 namespace delta {
@@ -77,15 +78,15 @@ __device__ __forceinline__ float bf16_at(u4 x, int i) {  // element i of eight
 
 // The workspace of the chunks' kernels.  For each slot (a chunk's place) and query/key head K, Q and K^T in operand order, and for each slot and
 // value head a record: T (three bf16 parts) and B (two) of the lower triangle's blocks, six each, and the tokens' factors.
-constexpr int kChunk = 64;
 constexpr int64_t kRecordT = 0, kRecordB = 18 * 1024, kRecordFactors = 30 * 1024, kRecord = 30 * 1024 + 1280;
 struct Work {
     char *kq, *rec;
     int32_t* order;    // ragged rows: how many run by chunks, then their numbers
+    int32_t shift, rows;  // ragged rows: where their slots begin (ragged_slot)
     int32_t together;  // heads whose workgroups follow each other on one XCD
 };
-int64_t chunk_slots(int32_t num_seqs, int32_t T, int64_t total_tokens, bool ragged);
-int64_t chunk_groups(int32_t num_seqs, int32_t Hv, int32_t V);  // most workgroups of the chunks' scan
+Slots chunk_slots(int32_t num_seqs, int32_t T, int64_t total_tokens, int32_t token_len, bool ragged);
+int64_t chunk_groups(int64_t rows, int32_t Hv, int32_t V);  // most workgroups of the chunks' scan
 size_t chunk_workspace(int64_t slots, int32_t num_seqs, int32_t Hk, int32_t Hv, int32_t K);
 
 // All rows (ragged: those longer than token_len) by chunks; by tokens (ragged: those up to token_len).

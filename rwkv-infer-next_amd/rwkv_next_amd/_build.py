@@ -28,7 +28,7 @@ SOURCES = ("wkv7_recurrent.hip", "wkv7_chunked.hip", "wkv7_seg.hip", "wkv7_gener
            "dense.hip", "dense_tile.hip", "delta_token.hip", "delta_chunk.hip", "delta_capi.hip", "slots.hip", "wkv7_capi.hip")
 NOALLOC_SOURCE = "wkv7_noalloc.hip"
 NOALLOC_LIB_PATH = os.path.join(PKG_DIR, "librwkv7_noalloc.so")
-HEADERS = ("delta_device.h", "dense_device.h", "dense_plan.h", "logits_device.h", "w4a16_plan.h", "w6a16_grid.h", "w6a16_plan.h",
+HEADERS = ("delta_device.h", "delta_plan.h", "dense_device.h", "dense_plan.h", "logits_device.h", "w4a16_plan.h", "w6a16_grid.h", "w6a16_plan.h",
            "wkv7_device.h", "wkv7_launch.h", "wkv7_token.h")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
