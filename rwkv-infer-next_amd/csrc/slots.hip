@@ -40,7 +40,7 @@ struct Call {
     int64_t from_slots, to_slots;
     int32_t n, num_caches;
     int32_t shift;   // copy: a range has 2^shift units; free, compact: kThreads * kUnits units
-    int32_t groups;  // compact: workgroups that share a range's moves
+    int32_t groups;  // compact, free: workgroups that share a range's moves or slots
 };
 
 // The cache, layer and range of workgroup `b`.
@@ -131,23 +131,25 @@ __global__ __launch_bounds__(kThreads) void slots_copy_kernel(const Call p) {
     });
 }
 
-// Workgroup (x, y): range x for slot idx[y].
+// Workgroup (x, y): range x for slots idx[y], idx[y + groups], ..
 __global__ __launch_bounds__(kThreads) void slots_free_kernel(const Call p) {
     const Place at = place(p, blockIdx.x);
     const Cache c = p.c[at.cache];
-    const int64_t s = p.dst[blockIdx.y];
-    if (p.status && blockIdx.x == 0 && threadIdx.x == 0 && s >= p.to_slots) report(p.status);
-    if (s < 0 || s >= p.to_slots) return;
-    char* const row = c.to + at.layer * c.to_layer + s * c.to_slot;
     const int64_t first = (int64_t)at.range * (kThreads * kUnits);
-    with_unit(c.unit, [&](auto zero) {
-        typedef decltype(zero) T;
+    for (int i = blockIdx.y; i < p.n; i += p.groups) {
+        const int64_t s = p.dst[i];
+        if (p.status && blockIdx.x == 0 && threadIdx.x == 0 && s >= p.to_slots) report(p.status);
+        if (s < 0 || s >= p.to_slots) continue;
+        char* const row = c.to + at.layer * c.to_layer + s * c.to_slot;
+        with_unit(c.unit, [&](auto zero) {
+            typedef decltype(zero) T;
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-            const int64_t q = first + u * kThreads + threadIdx.x;
-            if (q < c.units) __builtin_nontemporal_store(T{}, reinterpret_cast<T*>(row) + q);
-        }
-    });
+            for (int u = 0; u < kUnits; ++u) {
+                const int64_t q = first + u * kThreads + threadIdx.x;
+                if (q < c.units) __builtin_nontemporal_store(T{}, reinterpret_cast<T*>(row) + q);
+            }
+        });
+    }
 }
 
 // Workgroup (x, y): range x for the moves y, y + groups, ..  Each makes the plan for itself: it is a scan of `slots` bytes.
@@ -306,9 +308,9 @@ int slots_free(const slots_cache* caches, int32_t num_caches, const int64_t* idx
     if (rc != WKV7_OK) return rc;
     if (n == 0 || blocks == 0) return WKV7_OK;
     if (!idx) return WKV7_ERR_NULL;
-    if (blocks * n > slots::kMaxGrid) return WKV7_ERR_SHAPE;
+    p.groups = (int32_t)std::min<int64_t>(n, std::max<int64_t>(1, slots::kMaxGrid / blocks));  // a slot each where a launch holds them
     p.dst = idx, p.n = n, p.to_slots = slots, p.status = status;
-    hipLaunchKernelGGL(slots::slots_free_kernel, dim3((unsigned)blocks, (unsigned)n), dim3(slots::kThreads), 0,
+    hipLaunchKernelGGL(slots::slots_free_kernel, dim3((unsigned)blocks, (unsigned)p.groups), dim3(slots::kThreads), 0,
                        static_cast<hipStream_t>(stream), p);
     return static_cast<int>(hipGetLastError());
 }

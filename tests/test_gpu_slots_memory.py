@@ -125,3 +125,18 @@ def test_autograd_is_told_of_what_is_written():
         SlotCaches(_fresh(2, 4, 8)).copy_slots(_idx(0), _idx(1))
         caches.free_slots(_idx(0))
     assert not t[:, 0].any()
+
+
+def test_as_many_slots_are_freed_as_a_call_may_name():
+    """65535 slots in three caches of 61 layers: more than a launch has workgroups for, were each to have one slot."""
+    from rwkv_next_amd.kernels import SlotCaches, new_status
+    S, n = 70000, 65535
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    caches = [torch.randint(1, 100, (61, S, w), device=DEV, generator=gen, dtype=torch.uint8) for w in (1, 2, 16)]
+    idx = torch.randperm(S + 500, device=DEV, generator=gen)[:n]
+    idx[5::1000] = -1
+    want, status = [t.clone() for t in caches], new_status(DEV)
+    for t in want:
+        t[:, idx[(idx >= 0) & (idx < S)]] = 0
+    SlotCaches(*caches).free_slots(idx, status=status)
+    assert int(status) == 1024 and all(torch.equal(t, w) for t, w in zip(caches, want))
