@@ -5,7 +5,8 @@ them with torch operations), beside int4_matmul and int6_matmul.
     prepack_dense(w)                                     -> DensePacked, made once when the weights are loaded
     dense_matmul(a, packed, bias=None, activation=None, residual=None, out_dtype=None)
                                                          -> act(a @ w + bias) + residual
-    dense_matmul_op(a, weight, K, N, bias, activation, residual)   op rwkv_next_amd::dense_matmul, the fields of a DensePacked
+    dense_matmul_op(a, weight, K, N, bias, activation, residual, out_dtype=None)
+                                                         op rwkv_next_amd::dense_matmul, the fields of a DensePacked
 
 Activations and weights are both bfloat16 or both float16; sums and the epilogue are fp32, the result is rounded once.  K is a
 multiple of 32, N is any.  Every call runs on the current stream, no host sync, and can be recorded into a HIP graph.
@@ -128,11 +129,11 @@ def dense_matmul(a, packed: DensePacked, *, bias=None, activation: Optional[str]
 
 @torch.library.custom_op("rwkv_next_amd::dense_matmul", mutates_args=())
 def dense_matmul_op(a: torch.Tensor, weight: torch.Tensor, K: int, N: int, bias: Optional[torch.Tensor], activation: str,
-                    residual: Optional[torch.Tensor]) -> torch.Tensor:
+                    residual: Optional[torch.Tensor], out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """dense_matmul as a registered op, for torch.compile: the fields of a DensePacked."""
-    return dense_matmul(a, DensePacked(weight, K, N), bias=bias, activation=activation, residual=residual)
+    return dense_matmul(a, DensePacked(weight, K, N), bias=bias, activation=activation, residual=residual, out_dtype=out_dtype)
 
 
 @dense_matmul_op.register_fake
-def _(a, weight, K, N, bias, activation, residual):
-    return a.new_empty((*a.shape[:-1], N))
+def _(a, weight, K, N, bias, activation, residual, out_dtype=None):
+    return a.new_empty((*a.shape[:-1], N), dtype=a.dtype if out_dtype is None else out_dtype)
