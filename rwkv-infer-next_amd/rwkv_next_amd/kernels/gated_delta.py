@@ -58,11 +58,9 @@ def _tokens(t, dtype, shape, inner, align, name):
 
 def _launch(q, k, v, g, beta, *, o, h0=None, h0_idx=None, ht=None, ht_idx=None, fresh=None, cu=None, n_keep=None,
             snapshots=None, status=None, scale, qk_norm, token_len):
-    qs, vs = q.shape, v.shape
-    if len(qs) != 4 or len(vs) != 4:
-        raise ValueError(f"q, k must be (B, T, Hk, K) and v (B, T, Hv, V) (got {tuple(qs)}, {tuple(vs)})")
+    qs = q.shape
     B, T, Hk, K = qs
-    Hv, V = vs[2], vs[3]
+    Hv, V = v.shape[2:]
     if K not in (64, 128) or V % 16 or not 16 <= V <= 256:
         raise ValueError(f"head sizes must be K in (64, 128) and V a multiple of 16 up to 256 (got K={K}, V={V})")
     if Hk < 1 or Hv < Hk or Hv % Hk:
@@ -124,6 +122,14 @@ def _rows(q, cu_seqlens):
     return cu, cu.numel() - 1
 
 
+def _heads(q, v):
+    """K, Hv, V"""
+    qs, vs = q.shape, v.shape
+    if len(qs) != 4 or len(vs) != 4:
+        raise ValueError(f"q, k must be (B, T, Hk, K) and v (B, T, Hv, V) (got {tuple(qs)}, {tuple(vs)})")
+    return qs[3], vs[2], vs[3]
+
+
 @torch.no_grad()
 def gated_delta(q, k, v, g, beta, state=None, *, cu_seqlens=None, scale=None, qk_norm: bool = False, final: bool = True,
                 token_len: int = -1):
@@ -133,7 +139,7 @@ def gated_delta(q, k, v, g, beta, state=None, *, cu_seqlens=None, scale=None, qk
     scale: K ** -0.5 where None.  qk_norm: q and k are divided by sqrt(sum of squares + 1e-6) first.  token_len: rows of at most
     so many tokens run token by token instead of by chunks (-1: the library's choice)."""
     cu, N = _rows(q, cu_seqlens)
-    K, (Hv, V) = q.shape[3], v.shape[2:]
+    K, Hv, V = _heads(q, v)
     h0 = _state(state, N, Hv, K, V, "state")
     h0 = None if h0 is None else h0.contiguous()
     o = torch.empty(v.shape, dtype=torch.bfloat16, device=v.device)
@@ -144,7 +150,7 @@ def gated_delta(q, k, v, g, beta, state=None, *, cu_seqlens=None, scale=None, qk
 
 def _pool(q, k, v, g, beta, pool, slots, cu_seqlens, n_keep, fresh, scale, qk_norm, final, store_o, snapshots, status, token_len):
     N = q.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1
-    K, Hv, V = q.shape[3], v.shape[2], v.shape[3]
+    K, Hv, V = _heads(q, v)
     if pool.dtype is not torch.float32 or pool.shape[1:] != (Hv, K, V) or not pool.is_contiguous():
         _require(pool, "pool", torch.float32, (None, Hv, K, V))
     if slots.dtype is not torch.int64 or slots.shape != (N,) or not slots.is_contiguous():
