@@ -29,6 +29,7 @@ from .wkv7 import _index_tensor, _require
 
 
 _increment_version = torch.autograd.graph.increment_version
+_MOST_TOKENS = 1 << 30  # of a call: a longer token_len is no other
 
 
 def _tokens(t, dtype, shape, inner, align, name):
@@ -65,6 +66,7 @@ def _launch(q, k, v, g, beta, *, o, h0=None, h0_idx=None, ht=None, ht_idx=None, 
         raise ValueError(f"head sizes must be K in (64, 128) and V a multiple of 16 up to 256 (got K={K}, V={V})")
     if Hk < 1 or Hv < Hk or Hv % Hk:
         raise ValueError(f"value heads must be a multiple of the query/key heads (got Hk={Hk}, Hv={Hv})")
+    token_len = min(token_len, _MOST_TOKENS)
     dev, index = q.device, q.get_device()
     if index < 0:
         raise ValueError(f"operands must be on a GPU (got {dev})")

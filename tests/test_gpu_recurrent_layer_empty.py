@@ -1,0 +1,49 @@
+"""The delta rule and the slot operators where there is nothing: no rows, no tokens, no slots, no entries; and limits past every size."""
+import sys
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+def _ops(B, T, Hk=1, Hv=2, K=64, V=32):
+    r = lambda *n: torch.randn(*n, device=DEV)  # noqa: E731
+    return [r(B, T, Hk, K).bfloat16(), r(B, T, Hk, K).bfloat16(), r(B, T, Hv, V).bfloat16(), -torch.rand(B, T, Hv, device=DEV),
+            torch.rand(B, T, Hv, device=DEV)]
+
+
+@pytest.mark.parametrize("B,T", [(0, 0), (0, 5), (0, 100), (3, 0)])
+def test_no_rows_or_no_tokens(B, T):
+    from rwkv_next_amd.kernels import gated_delta, gated_delta_pool_
+    state = torch.randn(B, 2, 64, 32, device=DEV)
+    o, ht = gated_delta(*_ops(B, T), state)
+    assert o.shape == (B, T, 2, 32) and torch.equal(ht, state)
+    assert not gated_delta(*_ops(B, T))[1].any()
+    pool = torch.randn(4, 2, 64, 32, device=DEV)
+    was = pool.clone()
+    assert gated_delta_pool_(*_ops(B, T), pool, torch.arange(B, device=DEV)).shape == (B, T, 2, 32) and torch.equal(pool, was)
+    fresh = torch.ones(B, dtype=torch.bool, device=DEV)
+    gated_delta_pool_(*_ops(B, T), pool, torch.arange(B, device=DEV), fresh=fresh)
+    assert not pool[:B].any() and torch.equal(pool[B:], was[B:])
+
+
+def test_no_ragged_rows():
+    from rwkv_next_amd.kernels import gated_delta_pool_, new_status
+    pool = torch.randn(4, 2, 64, 32, device=DEV)
+    was, status = pool.clone(), new_status(DEV)
+    for total in (0, 50):
+        gated_delta_pool_(*_ops(1, total), pool, torch.arange(0, device=DEV), cu_seqlens=torch.tensor([0], device=DEV), status=status)
+        gated_delta_pool_(*_ops(1, total), pool, torch.arange(3, device=DEV), cu_seqlens=torch.tensor([0] * 4, device=DEV), status=status)
+    assert torch.equal(pool, was) and int(status) == 0
+
+
+@pytest.mark.parametrize("token_len", [1 << 31, sys.maxsize])
+@pytest.mark.parametrize("T", [1, 40])
+def test_a_token_len_past_every_length(T, token_len):
+    from rwkv_next_amd.kernels import gated_delta
+    ops = _ops(2, T)
+    want, got = gated_delta(*ops, token_len=1 << 30), gated_delta(*ops, token_len=token_len)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
