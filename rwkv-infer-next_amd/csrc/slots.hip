@@ -74,6 +74,11 @@ __global__ __launch_bounds__(kThreads) void slots_copy_kernel(const Call p) {
     __shared__ int32_t from[SLOTS_MAX_PAIRS], to[SLOTS_MAX_PAIRS];
     __shared__ int32_t key[kTable], last[kTable];
     const int tid = threadIdx.x;
+    if (p.num_caches == 0) {  // the indices alone
+        for (int i = tid; i < p.n; i += kThreads)
+            if (p.src[i] >= p.from_slots || p.dst[i] >= p.to_slots) report(p.status);
+        return;
+    }
     const Place at = place(p, blockIdx.x);
     const Cache c = p.c[at.cache];
     int table = 2;  // at most half full
@@ -133,6 +138,11 @@ __global__ __launch_bounds__(kThreads) void slots_copy_kernel(const Call p) {
 
 // Workgroup (x, y): range x for slots idx[y], idx[y + groups], ..
 __global__ __launch_bounds__(kThreads) void slots_free_kernel(const Call p) {
+    if (p.num_caches == 0) {  // the indices alone
+        for (int i = threadIdx.x; i < p.n; i += kThreads)
+            if (p.dst[i] >= p.to_slots) report(p.status);
+        return;
+    }
     const Place at = place(p, blockIdx.x);
     const Cache c = p.c[at.cache];
     const int64_t first = (int64_t)at.range * (kThreads * kUnits);
@@ -241,8 +251,9 @@ __global__ __launch_bounds__(kThreads) void slots_compact_kernel(const Call p) {
 
 constexpr int64_t kMaxGrid = 0x7FFFFF;  // workgroups of one launch: with 256 threads below 2^32 work-items
 
-// The caches with their units and workgroups; a range has `range` units.  A negative code for what is refused.
-int fill(Call& p, const slots_cache* caches, int32_t num, bool copies, int64_t range, int64_t* blocks) {
+// The caches that hold something (in `slots` slots), with their units and workgroups; a range has `range` units.  A negative code for
+// what is refused.
+int fill(Call& p, const slots_cache* caches, int32_t num, bool copies, int64_t slots, int64_t range, int64_t* blocks) {
     if (num < 0 || num > SLOTS_MAX_CACHES) return WKV7_ERR_SHAPE;
     if (num && !caches) return WKV7_ERR_NULL;
     *blocks = 0;
@@ -250,7 +261,7 @@ int fill(Call& p, const slots_cache* caches, int32_t num, bool copies, int64_t r
     for (int i = 0; i < num; ++i) {
         const slots_cache& x = caches[i];
         if (x.row_bytes < 0 || x.layers < 0) return WKV7_ERR_SHAPE;
-        if (x.row_bytes == 0 || x.layers == 0) continue;
+        if (x.row_bytes == 0 || x.layers == 0 || slots == 0) continue;
         if (!x.to || (copies && !x.from)) return WKV7_ERR_NULL;
         if (x.to_slot_stride < x.row_bytes || x.to_layer_stride < 0 ||
             (copies && (x.from_slot_stride < x.row_bytes || x.from_layer_stride < 0)))
@@ -289,10 +300,11 @@ int slots_copy(const slots_cache* caches, int32_t num_caches, const int64_t* src
     int shift = 0;  // as many units of a row as the registers hold for n slots
     while (shift < 12 && (n << (shift + 1)) <= slots::kThreads * slots::kUnits) ++shift;
     int64_t blocks;
-    const int rc = slots::fill(p, caches, num_caches, true, (int64_t)1 << shift, &blocks);
+    const int rc = slots::fill(p, caches, num_caches, true, std::min(from_slots, to_slots), (int64_t)1 << shift, &blocks);
     if (rc != WKV7_OK) return rc;
-    if (n == 0 || blocks == 0) return WKV7_OK;
+    if (n == 0 || (blocks == 0 && !status)) return WKV7_OK;
     if (!src || !dst) return WKV7_ERR_NULL;
+    if (blocks == 0) blocks = 1;  // looks at the indices alone
     p.src = src, p.dst = dst, p.n = n, p.from_slots = from_slots, p.to_slots = to_slots, p.status = status, p.shift = shift;
     hipLaunchKernelGGL(slots::slots_copy_kernel, dim3((unsigned)blocks), dim3(slots::kThreads), 0,
                        static_cast<hipStream_t>(stream), p);
@@ -304,11 +316,13 @@ int slots_free(const slots_cache* caches, int32_t num_caches, const int64_t* idx
     if (n < 0 || n > 65535 || slots < 0) return WKV7_ERR_SHAPE;
     slots::Call p{};
     int64_t blocks;
-    const int rc = slots::fill(p, caches, num_caches, false, slots::kThreads * slots::kUnits, &blocks);
+    const int rc = slots::fill(p, caches, num_caches, false, slots, slots::kThreads * slots::kUnits, &blocks);
     if (rc != WKV7_OK) return rc;
-    if (n == 0 || blocks == 0) return WKV7_OK;
+    if (n == 0 || (blocks == 0 && !status)) return WKV7_OK;
     if (!idx) return WKV7_ERR_NULL;
-    p.groups = (int32_t)std::min<int64_t>(n, std::max<int64_t>(1, slots::kMaxGrid / blocks));  // a slot each where a launch holds them
+    // a slot each where a launch holds them; without caches one workgroup looks at the indices alone
+    p.groups = blocks == 0 ? 1 : (int32_t)std::min<int64_t>(n, std::max<int64_t>(1, slots::kMaxGrid / blocks));
+    if (blocks == 0) blocks = 1;
     p.dst = idx, p.n = n, p.to_slots = slots, p.status = status;
     hipLaunchKernelGGL(slots::slots_free_kernel, dim3((unsigned)blocks, (unsigned)p.groups), dim3(slots::kThreads), 0,
                        static_cast<hipStream_t>(stream), p);
@@ -320,7 +334,7 @@ int slots_compact(const slots_cache* caches, int32_t num_caches, const uint8_t* 
     if (slots < 0 || slots > SLOTS_MAX_COMPACT) return WKV7_ERR_SHAPE;
     slots::Call p{};
     int64_t blocks;
-    const int rc = slots::fill(p, caches, num_caches, false, slots::kThreads * 4, &blocks);
+    const int rc = slots::fill(p, caches, num_caches, false, slots, slots::kThreads * 4, &blocks);
     if (rc != WKV7_OK) return rc;
     if (slots > 0 && !live) return WKV7_ERR_NULL;
     if (blocks == 0) blocks = 1;  // the plan alone

@@ -47,3 +47,24 @@ def test_a_token_len_past_every_length(T, token_len):
     ops = _ops(2, T)
     want, got = gated_delta(*ops, token_len=1 << 30), gated_delta(*ops, token_len=token_len)
     assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
+def test_no_slots():
+    from rwkv_next_amd.kernels import SlotCaches, new_status
+    none = torch.zeros(0, dtype=torch.int64, device=DEV)
+    empty = SlotCaches(torch.zeros(2, 0, 8, device=DEV), (torch.zeros(0, 3, device=DEV), 0))
+    empty.copy_slots(none, none)
+    empty.free_slots(none)
+    where, count = empty.compact_slots(torch.zeros(0, dtype=torch.bool, device=DEV))
+    assert where.shape == (0,) and int(count) == 0
+    t, u = torch.randn(2, 5, 8, device=DEV), torch.randn(5, 3, device=DEV)
+    was, other = t.clone(), u.clone()
+    some = SlotCaches(t, (u, 0))
+    one = torch.tensor([0], device=DEV)
+    for call in (lambda s: empty.copy_slots(one, one, status=s), lambda s: empty.free_slots(one, status=s),
+                 lambda s: empty.copy_slots(one, one, into=some, status=s), lambda s: some.copy_slots(one, one, into=empty, status=s),
+                 lambda s: SlotCaches(torch.zeros(2, 5, 0, device=DEV)).free_slots(one + 5, status=s)):  # past the slots, of which there are none
+        status = new_status(DEV)
+        call(status)
+        assert int(status) == 1024
+    assert torch.equal(t, was) and torch.equal(u, other)
