@@ -12,7 +12,7 @@
 // earlier one.  So on the way to T 0 goes in the place of what is out of range, and from the first token that had such a value, R is
 // NaN.  In the scan the state of R's column is then NaN, as it is token by token; outputs that came out of range are made again, by the
 // wavefronts which make them, without the tokens that cannot have a part in them.
-// Measured, 4096 tokens, 16 query/key and 32 value heads of 128: 35 to 38 us and 95 us (token by token 5.4 ms).
+// Measured, 4096 tokens, 16 query/key and 32 value heads of 128: 31 to 34 us and 95 us (token by token 5.4 ms).
 #include "delta_device.h"
 
 namespace delta {
@@ -146,7 +146,7 @@ __device__ void order_rows(const Params& p, const Work& w, int32_t* count) {
 }
 
 // One workgroup: a chunk of a query/key head, then each of the value heads that share it.  Bound by its bytes: 48 KiB of operands a
-// query/key head and 31 KiB a value head are written for each chunk, 150 MB with what is read for 4096 tokens in 35 to 38 us.
+// query/key head and 31 KiB a value head are written for each chunk, 139 MB with what is read for 4096 tokens in 31 to 34 us.
 template <int K>
 __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, const Work w) {
     constexpr int kSteps = K / 32, kPitch = K + 8;
@@ -435,8 +435,9 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(const Params p, cons
 // with barriers between.  Wavefronts 4 to 7 have a quarter of the tokens each and make the outputs beside it.  Operands of the next
 // chunk are asked for as soon as those of this one are used, while LDS is waited for, so the loads, 78 KiB a chunk, are spread over
 // it: asked for together, at its begin, they held the chain up for a third of its time (4096 tokens 133 us then, 95 now, 1.5 us a chunk).
-// By 32 columns a chunk takes 2.8 us, half the loads for each: taken where 16 would leave every CU two workgroups or more (8 rows of 1276
-// tokens on average 225 us; by 16 columns 359).
+// By 32 columns a chunk takes 2.8 us, half the loads for each: taken where 16 would leave every CU two workgroups or more, were all rows
+// to run by chunks (8 rows of 1276 tokens on average 227 us; by 16 columns 359).  Which of a ragged call's rows do is the device's
+// knowledge, and little hangs on it: one row of 2048 tokens among 63 of one, 32 heads of 128, 76 us by 32 columns, 75 by 16.
 template <int K, int NT>
 __global__ __launch_bounds__(512, 2) void delta_scan_kernel(const Params p, const Work w) {
     constexpr int kSteps = K / 32, kTiles = K / 64;  // of the state's rows: MFMA steps, tiles of a wavefront

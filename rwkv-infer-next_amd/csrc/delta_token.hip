@@ -4,7 +4,9 @@
 // r = S_{t-1}^T k and u = S_{t-1}^T q from one pass over the state,
 //     d = beta (v - a r),   S_t = a S_{t-1} + k d^T,   o = scale (a u + (q . k) d)
 // so a token costs one sum over the lanes.  For one token the reading and writing of the states, 8 K V bytes a head, bounds it: 64
-// sequences, 32 heads of 128 x 128, 44 to 47 us, 5.7 to 6.1 TB/s in place where a large copy moves 4.9; one sequence 5.6 us.  Each
+// sequences, 32 heads of 128 x 128, 49 us with states from memory (eight pools in turn), 5.5 TB/s in place where a large copy moves 4.9;
+// 44 to 47 with one pool, half of which the caches hold; one sequence 5.3 to 5.6 us.  Blocks of 2, 4, 8 tokens 51, 56, 70 us; with a
+// snapshot of each token 78, 138, 253 (4.8 TB/s).  Each
 // lane has its 16-byte pieces of 16 rows in flight at once, so nothing needs LDS or a barrier.
 #include "delta_device.h"
 

@@ -7,7 +7,7 @@
 // of a row.  Measured: 4096 rows, 4096 x 16384, 443 to 476 us by 128 x 256 (two workgroups of four wavefronts a CU; by 256 x 256, eight
 // wavefronts, 600), 1.16 to 1.24 PFLOP/s where a large library product reaches 1.22; the matrix cores work 58 % of the time.  64 rows
 // 31 us, 4.4 TB/s of weight: bound by memory, and by the first and last of 16 panels that nothing covers; a deeper D changed nothing.
-// 500 rows, 10240 x 2560, 33 us and 7 for adding the parts: one wavefront a SIMD (27 %).  A width that four does not divide stores a column a
+// 500 rows, 10240 x 2560, 33 to 36 us and 7 for adding the parts: one wavefront a SIMD (27 %).  A width that four does not divide stores a column a
 // lane: 22 us against 16 (1175 rows, K = 64, N = 5665, 5664).  Which tile a product takes, and the measured sides of the rules: dense_plan.h.
 #include "dense_device.h"
 

@@ -58,7 +58,7 @@ int main() {
     std::mt19937 rng(7);
     const auto pick = [&](int64_t below) { return (int64_t)(rng() % (uint64_t)below); };
     const int32_t lens[] = {0, 1, 2, 3, 7, 14, 15, 16, 17, 30, 31, 32, 33, 62, 63, 64, 65, 200};
-    for (int round = 0; round < 60000; ++round) {
+    for (int pass = 0; pass < 60000; ++pass) {
         const int32_t token_len = lens[pick(18)];
         const int kind = (int)pick(4), n = 1 + (int)pick(kind == 3 ? 300 : 20);
         std::vector<int64_t> cu{pick(3) ? 0 : pick(100)};

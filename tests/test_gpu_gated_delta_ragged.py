@@ -97,3 +97,36 @@ def test_many_rows_of_many_heads():
         assert _rel(o[0, n:n + 1], want) <= O_TOL
         if state is not None:
             assert _rel(pool[slots[n]], states[-1]) <= (K / 8 + 12) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("rows,total", [(40, 300), (4, 700)])
+def test_a_captured_call_follows_its_offsets(rows, total):
+    """One graph, other rows at every replay: which of them run by chunks, and where these lie, is found on the device."""
+    from rwkv_next_amd.kernels import gated_delta_pool_
+    Hk, Hv, K, V = 1, 2, 64, 32
+    ops = _inputs(total, Hk, Hv, K, V, rows)
+    rng = np.random.default_rng(rows)
+    pool = torch.randn(rows, Hv, K, V, device=DEV)
+    mine, slots = pool.clone(), torch.randperm(rows, device=DEV)
+    cu = torch.zeros(rows + 1, dtype=torch.int32, device=DEV)
+    keep = torch.full((rows,), 1000, device=DEV)
+    gated_delta_pool_(*ops, mine, slots, cu_seqlens=cu, n_keep=keep, qk_norm=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = gated_delta_pool_(*ops, mine, slots, cu_seqlens=cu, n_keep=keep, qk_norm=True)
+    for replay in range(6):
+        ends = np.sort(rng.integers(0, total + 1, rows - 1)) if replay % 2 else np.minimum(np.arange(1, rows) + (total - rows if replay else 0), total)
+        cu.copy_(torch.tensor([0, *ends, total], dtype=torch.int32))
+        keep.copy_(torch.from_numpy(rng.integers(0, 200, rows)))
+        mine.copy_(pool)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = pool.clone()
+        want = gated_delta_pool_(*ops, eager, slots, cu_seqlens=cu, n_keep=keep, qk_norm=True)
+        assert torch.equal(mine, eager), replay
+        for n, (a, b) in enumerate(zip(cu.tolist(), cu.tolist()[1:])):
+            b = min(b, a + int(keep[n]))
+            assert torch.equal(o[0, a:b], want[0, a:b]), (replay, n)
+            ref, states = oracle.delta_ref.gated_delta_ref(*(_np(x[0, a:b]) for x in ops), _np(pool[slots[n]]), qk_norm=True)
+            assert b == a or _rel(o[0, a:b], ref) <= O_TOL, (replay, n)
+            assert _rel(mine[slots[n]], states[-1]) <= max(1.0, b - a) ** 0.5 * (K / 8 + 12) * 2.0 ** -24, (replay, n)
