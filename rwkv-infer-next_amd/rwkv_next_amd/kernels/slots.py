@@ -65,18 +65,17 @@ class SlotCaches:
             self._lay_out()
 
     def _lay_out(self):
-        places = self._places()
-        self._laid = None  # until all is found right
-        self._rows, self.slots, self.device, self._shared = [], None, None, False
+        """All of it, taken when it is found right."""
+        places, rows, slots, device, shared = self._places(), [], None, None, False
         for t, dim in self._caches:
             if dim not in (0, 1) or t.dim() <= dim:
                 raise ValueError(f"the slots are dimension 0 or 1 of a cache (got dimension {dim} of {tuple(t.shape)})")
             if not t.is_cuda:
                 raise ValueError(f"caches must be on a GPU (got {t.device})")
-            if self.device is None:
-                self.device, self.slots = t.device, t.shape[dim]
-            if t.device != self.device or t.shape[dim] != self.slots:
-                raise ValueError(f"caches must have {self.slots} slots on {self.device} (got {t.shape[dim]} on {t.device})")
+            if device is None:
+                device, slots = t.device, t.shape[dim]
+            if t.device != device or t.shape[dim] != slots:
+                raise ValueError(f"caches must have {slots} slots on {device} (got {t.shape[dim]} on {t.device})")
             layers, shape, strides, size = t.shape[0] if dim else 1, t.shape[dim + 1:], t.stride(), t.element_size()
             row = 1
             for n, s in zip(reversed(shape), reversed(strides[dim + 1:])):
@@ -84,17 +83,17 @@ class SlotCaches:
                     raise ValueError(f"a slot's part of a cache must be contiguous (got {tuple(t.shape)}, strides {strides})")
                 row *= n
             row *= size
-            slot = strides[dim] * size if self.slots > 1 else row
+            slot = strides[dim] * size if slots > 1 else row
             layer = strides[0] * size if dim and layers > 1 else 0
             if row and (slot < row or (layers > 1 and layer < row)):
                 raise ValueError(f"slots of a cache must not share memory (got {tuple(t.shape)}, strides {strides})")
             # layers outside slots or within them, but not interlocked
-            if row and layers > 1 and self.slots > 1 and layer < self.slots * slot and slot < layers * layer:
+            if row and layers > 1 and slots > 1 and layer < slots * slot and slot < layers * layer:
                 raise ValueError(f"slots of a cache must not share memory (got {tuple(t.shape)}, strides {strides})")
-            self._rows.append((t, layer, slot, row, layers))
-            self._shared |= not all(_apart(self._rows[-1], self.slots, x, self.slots) for x in self._rows[:-1])
-        self._own = self._pairs(self)
-        self._laid = places
+            rows.append((t, layer, slot, row, layers))
+            shared |= not all(_apart(rows[-1], slots, x, slots) for x in rows[:-1])
+        self._rows, self.slots, self.device, self._shared = rows, slots, device, shared
+        self._own, self._laid = self._pairs(self), places
 
     def _pairs(self, other):
         a = (_lib.SlotsCache * len(self._rows))()

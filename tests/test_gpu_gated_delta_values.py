@@ -92,13 +92,14 @@ def test_a_state_reaches_its_column(by):
         _check(got[1], want[1], clean)
 
 
-def test_many_ragged_rows():
+@pytest.mark.parametrize("K,V", [(128, 128), (64, 160)])
+def test_many_ragged_rows(K, V):
     """By 32 columns a workgroup; several tokens of a row, of which the first counts; rows beside it."""
     from rwkv_next_amd.kernels import gated_delta
     lens = [70 + 3 * i for i in range(40)]
     at = np.cumsum([0] + lens)
-    ops, _ = _inputs(1, int(at[-1]), 2, 16, 128, 128, 3)
-    state = torch.randn(40, 16, 128, 128, device=DEV)
+    ops, _ = _inputs(1, int(at[-1]), 2, 16, K, V, 3)
+    state = torch.randn(40, 16, K, V, device=DEV)
     cu = torch.tensor(at, device=DEV).int()
     want = gated_delta(*ops, state, cu_seqlens=cu, token_len=0)
     out, fin = torch.ones_like(want[0], dtype=torch.bool), torch.ones_like(want[1], dtype=torch.bool)

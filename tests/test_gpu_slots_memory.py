@@ -73,7 +73,7 @@ def test_what_no_longer_fits_is_refused():
         for call in calls:  # again and again, not the first time alone
             with pytest.raises(ValueError):
                 call()
-        assert torch.equal(t, was) and torch.equal(u, other)
+        assert torch.equal(t, was) and torch.equal(u, other) and caches.slots == 6 and caches.device == u.device
     t.data = u.view(1, 6, 5)  # the other cache's memory
     for call in (calls[0], calls[2]):
         with pytest.raises(ValueError, match="share memory"):
